@@ -40,6 +40,9 @@ enum {
   XRMM_I64 = 7,
   XRMM_BOOL = 8,
   XRMM_UNSPECIFIED = 9,
+  /* beyond the reference's list: the types of the MX4 and kv8 operators */
+  XRMM_BF16 = 16,
+  XRMM_E4M3 = 17, /* 8-bit float, 4 exponent and 3 mantissa bits, no infinities */
 };
 
 /* Fused activation kinds of MatMulNBitsMlp; the codes are those of
@@ -416,6 +419,84 @@ int xrmm_matmul_nbits_int8a(const void* A, const void* B, const void* scales, co
 int xrmm_matmul_nbits_int8a_noalloc(const void* A, const void* B, const void* scales, const void* zero_points,
                                     int32_t zp_dtype, const void* bias, void* Y, int64_t M, int64_t K, int64_t N,
                                     int32_t bits, int32_t block_size, int32_t dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit values (MX4; no counterpart in the reference). Blocks of
+ * 32 values along K share one E8M0 scale byte s, 2^(s - 127) (255: NaN); a value
+ * is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign) times its block's scale.
+ * Codes are [rows, kb, 16] bytes, low nibble first, scales [rows, kb] bytes,
+ * kb = ceil(K / 32); codes past K are 0. dtype is XRMM_F32, XRMM_F16 or XRMM_BF16.
+ *
+ * xrmm_mx4_quantize: s = max(floor(log2 max|x|) + 127 - 2, 0), codes to nearest,
+ * ties to even, saturated at 6, sign kept. A block that holds a NaN or an
+ * infinity gets s = 255 and codes 0. codes 4-byte aligned. */
+int xrmm_mx4_quantize(const void* x, void* codes, void* scales, int64_t rows, int64_t K, int32_t dtype, void* stream);
+
+/* Y [M, N] = A [M, K] W^T (+ bias [N]) with W as MX4 codes [N, kb, 16] and scales
+ * [N, kb]; sums in float32, one rounding to out_dtype (XRMM_F32, XRMM_F16,
+ * XRMM_BF16; bias has that type). a_dtype: XRMM_F16 or XRMM_BF16 (A_scales NULL), or
+ * XRMM_U8: A holds MX4 codes [M, kb, 16] with A_scales [M, kb]. Codes are 16-byte
+ * aligned; K at most 2^23. Weights past float32's range (scale bytes 253 and 254)
+ * are infinite. The workspace, at least xrmm_matmul_mx4_workspace_bytes (0: none
+ * used), is optional and has the form of xrmm_matmul_nbits_ws's: 256-byte
+ * aligned, its first 4096 bytes zero before its first use and after every call. With it,
+ * geometries with few output tiles split K across workgroups (added in a fixed order). */
+int64_t xrmm_matmul_mx4_workspace_bytes(int64_t M, int64_t K, int64_t N, int32_t a_dtype);
+int xrmm_matmul_mx4(const void* A, const void* A_scales, int32_t a_dtype, const void* B, const void* scales,
+                    const void* bias, void* Y, int32_t out_dtype, int64_t M, int64_t K, int64_t N, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
+/* Kernel family xrmm_matmul_mx4 picks for 16-byte aligned operands and a workspace,
+ * NULL for an invalid geometry. No device work. */
+const char* xrmm_matmul_mx4_kernel(int64_t M, int64_t K, int64_t N, int32_t a_dtype);
+
+/* ---------------------------------------------------------------------------
+ * Attention over a paged 8-bit cache (no counterpart in the reference). k_cache and
+ * v_cache: [pages, kv_heads, page_size, head_dim] of XRMM_I8 or XRMM_E4M3 codes
+ * (16-byte aligned), k_scales and v_scales [pages, kv_heads] float32: a value is its
+ * code times its page's and head's scale. Token t of sequence b lies in page
+ * block_table[b, t / page_size] (int32 [batch, table_width]; entries past a
+ * sequence's tokens are not read), slot t % page_size. lengths [batch] int32: tokens
+ * of each sequence, the call's own among them. The call's own tensors hold `rows`
+ * tokens, sequence b's from starts[b] to starts[b + 1] (int32 [batch + 1]), or
+ * rows / batch each when starts is NULL; they are the sequence's last ones. max_new:
+ * at least the most tokens a sequence has in the call (0: not known). head_dim 64,
+ * 96, 128 or 256; page_size a power of two from 16 to 256. A page outside [0, pages), a
+ * position below 0 or past the table, or `starts` outside the rows is left out and
+ * raises `status` (a device uint32, or NULL) to 55.
+ *
+ * xrmm_kv8_append writes the call's tokens (k, v [rows, kv_heads, head_dim] of dtype,
+ * token strides in elements). Let e(r) be the smallest integer >= -126 with
+ * r <= qmax 2^e (qmax 127, e4m3: 448), and max the largest magnitude entering a page and
+ * head. If the page's first slot is among them, or its scale is 0, its scale becomes
+ * 2^e(max) (0 for max 0); else it is multiplied by 2^max(0, e(max / scale)) and
+ * the codes before the new ones are rounded to it. Codes: x / scale to nearest, ties to even. A
+ * NaN or infinity among them makes the scale NaN and the new codes 0. Pages that sequences
+ * share must not be among those written. */
+int xrmm_kv8_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t dtype, void* k_cache,
+                    void* v_cache, void* k_scales, void* v_scales, int32_t cache_dtype, const void* block_table,
+                    const void* lengths, const void* starts, void* status, int64_t rows, int32_t max_new, int32_t batch,
+                    int32_t table_width, int64_t pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, void* stream);
+
+/* output [rows, q_heads, head_dim] (contiguous) = softmax(scale q k^T) v in float32,
+ * rounded once; q [rows, q_heads, head_dim] of dtype XRMM_F16 or XRMM_BF16, token
+ * stride in elements; query head h reads key head h / (q_heads / kv_heads). Query i of a
+ * sequence's n stands at p = length - n + i and sees tokens 0 <= t < length, t <= p if
+ * causal, t > p - window if window > 0; a row that sees none is 0. Cache scales are any
+ * float32. e4m3 NaN codes must not occur (xrmm_kv8_append writes none): rows that do not
+ * see such a token may be NaN too. The workspace, at least
+ * xrmm_kv8_attention_workspace_bytes (0: none used), is optional, of the same form as
+ * xrmm_matmul_mx4's; with it, long contexts of few rows are split across
+ * workgroups and joined in a fixed order. */
+int64_t xrmm_kv8_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
+                                           int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                           int32_t causal, int32_t window);
+int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
+                       const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
+                       const void* block_table, const void* lengths, const void* starts, void* status, int64_t rows,
+                       int32_t max_new, int32_t batch, int32_t table_width, int64_t pages, int32_t page_size,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal, int32_t window,
+                       void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Measurement (no counterpart in the reference, which publishes no throughput

@@ -17,6 +17,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "xrmm.h")
 
 XRMM_OK, XRMM_EINVAL, XRMM_EDEVICE = 0, 1, 2
 F32, F16, I32, U32, I16, I8, U8, I64, BOOL, UNSPECIFIED = range(10)
+BF16, E4M3 = 16, 17
 ACT = {"none": 0, "": 0, "identity": 0, "relu": 1, "silu": 2, "swish": 2, "gelu": 3,
        "tanh": 4, "sigmoid": 5, "swiglu": 6}
 
@@ -76,6 +77,15 @@ def _sig(lib):
       _i32, _i32, _vp)
     s("xrmm_matmul_nbits_int8a_noalloc", ctypes.c_int, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _i64, _i32,
       _i32, _i32, _vp)
+    s("xrmm_mx4_quantize", ctypes.c_int, _vp, _vp, _vp, _i64, _i64, _i32, _vp)
+    s("xrmm_matmul_mx4_workspace_bytes", _i64, _i64, _i64, _i64, _i32)
+    s("xrmm_matmul_mx4", ctypes.c_int, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp)
+    s("xrmm_matmul_mx4_kernel", ctypes.c_char_p, _i64, _i64, _i64, _i32)
+    s("xrmm_kv8_append", ctypes.c_int, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
+      _i32, _i32, _i32, _i64, _i32, _i32, _i32, _vp)
+    s("xrmm_kv8_attention_workspace_bytes", _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32)
+    s("xrmm_kv8_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32,
+      _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
     s("xrmm_stream_read", ctypes.c_int, _vp, ctypes.c_uint64, _vp, _i32, _vp)
     s("xrmm_stream_read_ex", ctypes.c_int, _vp, ctypes.c_uint64, _vp, _i32, _i32, _i32, _vp)
     s("xrmm_mfma_peak_operand_bytes", _i64)

@@ -668,3 +668,222 @@ def mfma_peak(operands, clocks, *, workgroups, waves=4, accumulators=4, iters, s
     nat.check(nat.lib().xrmm_mfma_peak(_ptr(operands), _ptr(sink), _ptr(clocks), int(workgroups), int(waves),
                                        int(accumulators), int(iters), _stream(stream, dev)))
     return clocks
+
+
+# ---------------------------------------------------------------------------
+# Microscaled 4-bit values (MX4) and attention over an 8-bit paged cache
+
+_LT = {torch.float32: nat.F32, torch.float16: nat.F16, torch.bfloat16: nat.BF16}
+_CACHE = {torch.int8: nat.I8, torch.float8_e4m3fn: nat.E4M3}
+
+
+def _empty(shape, dtype, device, stream):
+    """An output in the memory of the stream that writes it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _take_workspace(need, workspace, ref, dev, s, stream):
+    """(workspace or None, bytes): the caller's, checked, else this module's for the stream; none under graph
+    capture, where the call then runs unsplit."""
+    if need <= 0:
+        return None, 0
+    if workspace is not None:
+        if (workspace.dtype != torch.uint8 or workspace.numel() < need or workspace.get_device() != dev
+                or not workspace.is_contiguous()):
+            raise nat.XrmmInvalid(f"workspace must be contiguous uint8 with at least {need} bytes on the call's device")
+        return workspace, workspace.numel()
+    if torch.cuda.is_current_stream_capturing():
+        return None, 0
+    ws = _workspace(ref.device, s, need, stream)
+    return ws, ws.numel()
+
+
+def mx4_quantize(x, *, stream=None):
+    """Values to microscaled 4-bit (MX4): ``(codes, scales)``, uint8 ``[..., kb, 16]`` (low nibble first) and
+    uint8 ``[..., kb]``, ``kb = ceil(K / 32)``.
+
+    x ``[..., K]`` float32, float16 or bfloat16. A block of 32 has the scale ``2^(byte - 127)`` with
+    ``byte = max(floor(log2 max|x|) + 125, 0)``; codes are E2M1 to nearest, ties to even, saturated at 6. A block
+    that holds a NaN or an infinity has byte 255 (NaN)."""
+    if x.dtype not in _LT:
+        raise nat.XrmmInvalid("x must be float32, float16 or bfloat16")
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise nat.XrmmInvalid("x must be [..., K] with K positive")
+    K = int(x.shape[-1])
+    lead, kb = tuple(x.shape[:-1]), (K + 31) // 32
+    dev = _check_dev(x)
+    codes = _empty(lead + (kb, 16), torch.uint8, x.device, stream)
+    scales = _empty(lead + (kb,), torch.uint8, x.device, stream)
+    nat.check(nat.lib().xrmm_mx4_quantize(_ptr(x), _ptr(codes), _ptr(scales), x.numel() // K, K, _LT[x.dtype],
+                                          _stream(stream, dev)))
+    return codes, scales
+
+
+def matmul_mx4(A, B, scales, bias=None, *, A_scales=None, out_dtype=None, out=None, workspace=None, stream=None):
+    """``Y = A @ W.T (+ bias)`` with W in MX4: codes uint8 ``[N, kb, 16]``, scales uint8 ``[N, kb]`` (mx4_quantize's).
+
+    A is float16 or bfloat16 ``[..., K]`` (the output's type), or MX4 codes uint8 ``[..., kb, 16]`` with ``A_scales``
+    ``[..., kb]`` (output ``out_dtype``: float16 unless given, or bfloat16, float32). bias ``[N]`` has the output's
+    type. Sums are float32, rounded once. Geometries with few output tiles split K across workgroups on a workspace
+    (``matmul_mx4_workspace_bytes``; see ``matmul_nbits`` for whose it is and for graph capture)."""
+    if B.dtype != torch.uint8 or B.dim() != 3 or B.shape[2] != 16:
+        raise nat.XrmmInvalid(f"B must be uint8 [N, kb, 16], got {B.dtype} {tuple(B.shape)}")
+    N, kb = int(B.shape[0]), int(B.shape[1])
+    if scales.dtype != torch.uint8 or tuple(scales.shape) != (N, kb):
+        raise nat.XrmmInvalid(f"scales must be uint8 [{N}, {kb}], got {scales.dtype} {tuple(scales.shape)}")
+    if A.dtype == torch.uint8:
+        if A_scales is None:
+            raise nat.XrmmInvalid("MX4 codes as A need A_scales")
+        if A.dim() < 2 or tuple(A.shape[-2:]) != (kb, 16):
+            raise nat.XrmmInvalid(f"A must be uint8 [..., {kb}, 16], got {tuple(A.shape)}")
+        lead, K, at = tuple(A.shape[:-2]), kb * 32, nat.U8
+        if A_scales.dtype != torch.uint8 or tuple(A_scales.shape) != lead + (kb,):
+            raise nat.XrmmInvalid(f"A_scales must be uint8 {list(lead + (kb,))}, got {A_scales.dtype} {tuple(A_scales.shape)}")
+        dt = out_dtype if out_dtype is not None else out.dtype if out is not None else torch.float16
+        if dt not in _LT:
+            raise nat.XrmmInvalid("out_dtype must be float32, float16 or bfloat16")
+    else:
+        if A.dtype not in (torch.float16, torch.bfloat16):
+            raise nat.XrmmInvalid("A must be float16, bfloat16 or MX4 codes (uint8)")
+        if A_scales is not None:
+            raise nat.XrmmInvalid("A_scales belong to MX4 codes")
+        if A.dim() < 1 or A.shape[-1] == 0 or (int(A.shape[-1]) + 31) // 32 != kb:
+            raise nat.XrmmInvalid(f"A's last dimension must have {kb} blocks of 32, got {tuple(A.shape)}")
+        lead, K, at, dt = tuple(A.shape[:-1]), int(A.shape[-1]), _LT[A.dtype], A.dtype
+        if out_dtype not in (None, dt):
+            raise nat.XrmmInvalid("out_dtype must be A's dtype")
+    if bias is not None and (bias.dtype != dt or tuple(bias.shape) != (N,)):
+        raise nat.XrmmInvalid("bias must be [N] of the output's dtype")
+    _check_out(out, lead + (N,), dt)
+    dev = _check_dev(A, A_scales, B, scales, bias, out)
+    M = _numel(lead)
+    lib = nat.lib()
+    s = _stream(stream, dev)
+    ws, nws = _take_workspace(int(lib.xrmm_matmul_mx4_workspace_bytes(M, K, N, at)), workspace, A, dev, s, stream)
+    if out is None:
+        out = _empty(lead + (N,), dt, A.device, stream)
+    nat.check(lib.xrmm_matmul_mx4(_ptr(A), _ptr(A_scales), at, _ptr(B), _ptr(scales), _ptr(bias), _ptr(out), _LT[dt],
+                                  M, K, N, _ptr(ws), nws, s))
+    return out
+
+
+def matmul_mx4_workspace_bytes(M, K, N, dtype=torch.float16):
+    """Bytes of the split-K workspace of a matmul_mx4 geometry (0: none); dtype is A's (uint8: MX4 codes)."""
+    return int(nat.lib().xrmm_matmul_mx4_workspace_bytes(int(M), int(K), int(N),
+                                                          nat.U8 if dtype == torch.uint8 else _LT[dtype]))
+
+
+def matmul_mx4_kernel(M, K, N, dtype=torch.float16) -> str:
+    r = nat.lib().xrmm_matmul_mx4_kernel(int(M), int(K), int(N), nat.U8 if dtype == torch.uint8 else _LT[dtype])
+    if r is None:
+        raise nat.XrmmInvalid(nat.last_error())
+    return r.decode()
+
+
+def _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status):
+    if k_cache.dtype not in _CACHE or v_cache.dtype != k_cache.dtype:
+        raise nat.XrmmInvalid("k_cache and v_cache must both be int8 or float8_e4m3fn")
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise nat.XrmmInvalid("k_cache and v_cache must share a shape [pages, kv_heads, page_size, head_dim]")
+    P, H = int(k_cache.shape[0]), int(k_cache.shape[1])
+    for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        if t.dtype != torch.float32 or tuple(t.shape) != (P, H):
+            raise nat.XrmmInvalid(f"{name} must be float32 [{P}, {H}], got {t.dtype} {tuple(t.shape)}")
+    if lengths.dtype != torch.int32 or lengths.dim() != 1:
+        raise nat.XrmmInvalid("lengths must be int32 [batch]")
+    B = int(lengths.shape[0])
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
+        raise nat.XrmmInvalid(f"block_table must be int32 [{B}, width]")
+    if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (B + 1,)):
+        raise nat.XrmmInvalid(f"starts must be int32 [{B + 1}]")
+    if status is not None and (status.dtype not in (torch.int32, torch.uint32) or status.numel() < 1):
+        raise nat.XrmmInvalid("status must be an int32 or uint32 tensor of at least one element")
+    return B, P, H, int(k_cache.shape[2]), int(k_cache.shape[3])
+
+
+def _token_rows(t, heads, dim, name):
+    """A ``[tokens, heads, head_dim]`` tensor whose tokens may lie apart (a slice of a wider buffer): its token stride."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
+        raise nat.XrmmInvalid(f"{name} must be [tokens, {heads}, {dim}], got {tuple(t.shape)}")
+    if t.shape[0] and ((dim > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != dim)
+                       or (t.shape[0] > 1 and t.stride(0) < heads * dim)):
+        raise nat.XrmmInvalid(f"{name}: a token's heads must be contiguous, and tokens must not overlap")
+    return int(t.stride(0)) if t.shape[0] > 1 else heads * dim
+
+
+def _same_device(dev, *ts):
+    if any(t.get_device() != dev for t in ts):
+        raise nat.XrmmInvalid("tensors must share one device")
+
+
+def kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths, *, starts=None, max_new=None,
+               status=None, stream=None):
+    """Write new tokens into a paged 8-bit cache, in place.
+
+    k, v ``[T, kv_heads, head_dim]`` float32, float16 or bfloat16 (token stride free): sequence b's new tokens are rows
+    ``starts[b] .. starts[b + 1]`` (int32 ``[batch + 1]``; without it every sequence has ``T / batch``) and its last ones:
+    positions ``lengths[b] - n .. lengths[b] - 1``. k_cache, v_cache ``[pages, kv_heads, page_size, head_dim]`` int8 or
+    float8_e4m3fn, k_scales, v_scales float32 ``[pages, kv_heads]``, block_table int32 ``[batch, width]``, lengths int32
+    ``[batch]``. A page and head has one scale: a power of two that covers what entered, from the first slot on; a larger
+    value multiplies it by a power of two and the codes already there are rounded to it. A NaN or an infinity makes the
+    scale NaN. ``max_new``: at least the most tokens of one sequence (a bound on the work; T when not given). Pages
+    outside the cache, positions past the table and rows outside T are left out and raise the device word
+    ``status`` (int32) to 55."""
+    B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
+    if k.dtype not in _LT or v.dtype != k.dtype:
+        raise nat.XrmmInvalid("k and v must both be float32, float16 or bfloat16")
+    ks, vs = _token_rows(k, H, D, "k"), _token_rows(v, H, D, "v")
+    if k.shape[0] != v.shape[0]:
+        raise nat.XrmmInvalid("k and v must hold the same tokens")
+    dev = _check_dev(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
+    _same_device(dev, k, v)
+    nat.check(nat.lib().xrmm_kv8_append(
+        _ptr(k), _ptr(v), ks, vs, _LT[k.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+        _CACHE[k_cache.dtype], _ptr(block_table), _ptr(lengths), _ptr(starts), _ptr(status), int(k.shape[0]),
+        int(max_new or 0), B, int(block_table.shape[1]), P, page, H, D, _stream(stream, dev)))
+
+
+def kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, *, starts=None, max_new=None, scale=None,
+                  causal=True, window=0, out=None, workspace=None, status=None, stream=None):
+    """Softmax attention of new tokens over a paged 8-bit cache (kv8_append's layout, any float32 scales).
+
+    q ``[T, q_heads, head_dim]`` float16 or bfloat16 (token stride free), q_heads a multiple of the cache's heads; the
+    queries are each sequence's last tokens, as in kv8_append, whose keys and values are already in the cache.
+    Query at position p sees tokens t < lengths[b], t <= p if ``causal``, t > p - window if ``window``. A row that sees none
+    is 0. ``scale``: head_dim^-0.5 when not given. Returns ``[T, q_heads, head_dim]`` of q's dtype. Long contexts of few rows
+    are split across workgroups on a workspace (``kv8_attention_workspace_bytes``; see ``matmul_nbits`` for whose it is and
+    for graph capture)."""
+    B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise nat.XrmmInvalid("q must be float16 or bfloat16")
+    if q.dim() != 3 or q.shape[1] == 0 or H == 0 or q.shape[1] % H != 0:
+        raise nat.XrmmInvalid("q must be [tokens, q_heads, head_dim] with q_heads a multiple of the cache's heads")
+    T, Hq = int(q.shape[0]), int(q.shape[1])
+    qs = _token_rows(q, Hq, D, "q")
+    _check_out(out, (T, Hq, D), q.dtype)
+    dev = _check_dev(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status, out)
+    _same_device(dev, q)
+    W, most = int(block_table.shape[1]), int(max_new or 0)
+    lib = nat.lib()
+    s = _stream(stream, dev)
+    need = int(lib.xrmm_kv8_attention_workspace_bytes(T, most, int(starts is not None), B, W, page, Hq, H, D, int(causal),
+                                                      int(window)))
+    ws, nws = _take_workspace(need, workspace, q, dev, s, stream)
+    if out is None:
+        out = _empty((T, Hq, D), q.dtype, q.device, stream)
+    nat.check(lib.xrmm_kv8_attention(
+        _ptr(q), qs, _ptr(out), _LT[q.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+        _CACHE[k_cache.dtype], _ptr(block_table), _ptr(lengths), _ptr(starts), _ptr(status), T, most, B, W, P, page, Hq, H,
+        D, float(D ** -0.5 if scale is None else scale), int(causal), int(window), _ptr(ws), nws, s))
+    return out
+
+
+def kv8_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batch, table_width, page_size, max_new=0, ragged=False,
+                                  causal=True, window=0):
+    """Bytes of the split workspace of a kv8_attention call (0: none); ``ragged``: the call has ``starts``."""
+    return int(nat.lib().xrmm_kv8_attention_workspace_bytes(int(T), int(max_new), int(ragged), int(batch), int(table_width),
+                                                            int(page_size), int(q_heads), int(kv_heads), int(head_dim),
+                                                            int(causal), int(window)))
