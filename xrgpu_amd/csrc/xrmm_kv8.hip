@@ -77,11 +77,9 @@ __global__ __launch_bounds__(KVA_T) void k_kv8_append(KvAppendArgs a, uint32_t t
   int first, count;
   const bool rows = kv_rows(c, b, a.max_new, first, count);
   if (!rows && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
-  const int len = c.lengths[b], begin = len - count;  // positions begin .. len - 1 enter the cache
+  const int64_t len = c.lengths[b], begin = len - count;  // positions begin .. len - 1 enter the cache
   if (count <= 0) return;
-  const int page0 = begin >= 0 ? begin >> c.page_log2 : -((-begin + c.page - 1) >> c.page_log2);
-  const int pi = page0 + i;                            // page of the sequence
-  const int64_t base = static_cast<int64_t>(pi) << c.page_log2;
+  const int64_t base = ((begin >> c.page_log2) + i) * c.page;  // first position of the page
   if (base >= len) return;
   const int32_t page = base < 0 || base > 0x7FFFFFFF ? -1 : kv_page(c, b, static_cast<int>(base));
   if (page < 0) {
@@ -239,7 +237,10 @@ __global__ __launch_bounds__(64 * KVR_WAVES) void k_kv8_rows(KvAttnArgs a, uint3
   if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
   const int nrows = count * G, r0 = tile * 16 * NT;
   if (r0 >= nrows) return;
-  const int len = c.lengths[b] > 0 ? c.lengths[b] : 0, past = c.lengths[b] - count;
+  // positions past the table are left out: the walk over tokens ends with the table
+  const int span = c.width << c.page_log2, all = c.lengths[b], past = all - count;
+  const int len = all < 0 ? 0 : all < span ? all : span;
+  if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   // this lane's rows: their queries as binary16 (scaled by a power of two for bfloat16), what they see
   f16x8 q[NT][KD / 8];
