@@ -56,6 +56,7 @@ UNITS = [
     ("xrmm_bnb4_gemm.hip", [], "bnb4_gemm.o"),
     ("xrmm_int8a_gemm.hip", [], "int8a_gemm.o"),
     ("xrmm_mx4.hip", [], "mx4.o"),
+    ("xrmm_mx4_gemm.hip", [], "mx4_gemm.o"),
     ("xrmm_kv8.hip", [], "kv8.o"),
     ("xrmm_lowbit_api.cpp", [], "lowbit_api.o"),
     ("xrmm_probe.hip", [], "probe.o"),

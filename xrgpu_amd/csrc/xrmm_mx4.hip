@@ -3,12 +3,10 @@
 //   quantise: E = floor(log2 max|x|), scale byte max(E + 127 - 2, 0), code = the E2M1 value
 //             nearest x / 2^(byte - 127), ties to even, saturated at 6, sign kept
 //   product:  Y[m, n] = sum_k A[m, k] e2m1(code[n, k]) 2^(byte[n, k / 32] - 127) (+ bias[n])
-#include "xrmm_lowbit.h"
+#include "xrmm_mx4.h"
 
 namespace xrmm {
 namespace {
-
-constexpr uint32_t OOB = 0x80000000u;  // past every buffer bound here: loads return zero
 
 // ---------------------------------------------------------------------------
 // Quantisation. A lane holds eight consecutive values, so four lanes hold a block: the
@@ -93,40 +91,6 @@ hipError_t quantize_for(const MxQuantArgs& a, hipStream_t st) {
 
 constexpr int MXR_WAVES = 8;
 
-template <int AT>
-struct MxFrag { typedef bf16x8 t; };
-template <>
-struct MxFrag<LT_F16> { typedef f16x8 t; };
-
-template <int AT>
-__device__ __forceinline__ typename MxFrag<AT>::t mx_dq8(uint32_t w, float s) {
-  if constexpr (AT == LT_F16) {
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 1);
-    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, 3);
-    return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-  } else {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3);
-    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-  }
-}
-
-// x = hi + lo with both terms bfloat16: the upper eight significant bits and the rest (a binary16 has
-// eleven). An infinity or NaN stays in hi alone.
-__device__ __forceinline__ void split_f16(f16x8 x, bf16x8& hi, bf16x8& lo) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = static_cast<float>(x[i]);
-    const uint32_t b = __builtin_bit_cast(uint32_t, f);
-    const float h = __builtin_bit_cast(float, b & 0xFFFF0000u);
-    const bool fin = (b & 0x7F800000u) != 0x7F800000u;
-    hi[i] = __builtin_bit_cast(bf16, static_cast<uint16_t>(b >> 16));
-    lo[i] = static_cast<bf16>(fin ? f - h : 0.f);
-  }
-}
-
-__device__ __forceinline__ bool mx_f16_fits(uint32_t byte) { return byte - 104u <= 36u; }  // 2^-23 .. 2^13
-
 template <int AT, int NT, int CT, bool AL>
 __global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t col_tiles) {
   constexpr bool MX = AT < 0;
@@ -159,8 +123,8 @@ __global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t 
       for (int u = 0; u < 2; ++u) {
         const uint32_t b = it * 8 + g * 2 + u, r = i * 16 + c;
         const bool ok = b < kb && r < rowsB;
-        w[i][u] = bld16_nt(rB, ok ? (r * kb + b) * MX_BLOB : OOB, 0);
-        s[i][u] = bld_u8(rS, ok ? r * kb + b : OOB, 0);
+        w[i][u] = bld16_nt(rB, ok ? (r * kb + b) * MX_BLOB : MX_OOB, 0);
+        s[i][u] = bld_u8(rS, ok ? r * kb + b : MX_OOB, 0);
       }
     if constexpr (MX) {
 #pragma unroll
@@ -169,14 +133,11 @@ __global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t 
         for (int u = 0; u < 2; ++u) {
           const uint32_t b = it * 8 + g * 2 + u, r = j * 16 + c;
           const bool ok = b < kb && r < rowsA;
-          const u32x4 x = bld16(rA, ok ? (r * kb + b) * MX_BLOB : OOB, 0);
-          const int xs = static_cast<int>(bld_u8(rAs, ok ? r * kb + b : OOB, 0));
-          const i32x8 xv = {static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3]), 0, 0, 0, 0};
+          const u32x4 x = bld16(rA, ok ? (r * kb + b) * MX_BLOB : MX_OOB, 0);
+          const int xs = static_cast<int>(bld_u8(rAs, ok ? r * kb + b : MX_OOB, 0));
 #pragma unroll
           for (int i = 0; i < CT; ++i) {
-            const u32x4 y = w[i][u];
-            const i32x8 wv = {static_cast<int>(y[0]), static_cast<int>(y[1]), static_cast<int>(y[2]), static_cast<int>(y[3]), 0, 0, 0, 0};
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[i][j], 4, 4, 0, static_cast<int>(s[i][u]), 0, xs);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_fp4(w[i][u]), mx_fp4(x), acc[i][j], 4, 4, 0, static_cast<int>(s[i][u]), 0, xs);
           }
         }
     } else {
@@ -190,14 +151,14 @@ __global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t 
           for (int q = 0; q < 4; ++q) {
             const uint32_t k = (it * 8 + g * 2 + u) * MX_BLOCK + q * 8, r = j * 16 + c;
             if constexpr (AL) {  // K a multiple of 8: a piece is whole or absent
-              x[j][q] = __builtin_bit_cast(frag, bld16(rA, (k < K && r < rowsA) ? (r * K + k) * 2u : OOB, 0));
+              x[j][q] = __builtin_bit_cast(frag, bld16(rA, (k < K && r < rowsA) ? (r * K + k) * 2u : MX_OOB, 0));
             } else {
               u32x4 v;
 #pragma unroll
               for (uint32_t d = 0; d < 4; ++d) {
                 const uint32_t k2 = k + 2 * d;
-                const uint32_t lo = bld_u16(rA, (k2 < K && r < rowsA) ? (r * K + k2) * 2u : OOB, 0);
-                const uint32_t hi = bld_u16(rA, (k2 + 1 < K && r < rowsA) ? (r * K + k2 + 1) * 2u : OOB, 0);
+                const uint32_t lo = bld_u16(rA, (k2 < K && r < rowsA) ? (r * K + k2) * 2u : MX_OOB, 0);
+                const uint32_t hi = bld_u16(rA, (k2 + 1 < K && r < rowsA) ? (r * K + k2 + 1) * 2u : MX_OOB, 0);
                 v[d] = lo | (hi << 16);
               }
               x[j][q] = __builtin_bit_cast(frag, v);
@@ -208,9 +169,7 @@ __global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t 
           const float sf = e8m0(s[i][u]);
           bool wide = false;
           if constexpr (AT == LT_F16) {
-            const u32x4 y = w[i][u];
-            const bool zero = ((y[0] | y[1] | y[2] | y[3]) & 0x77777777u) == 0u;
-            wide = __any(!mx_f16_fits(s[i][u]) && !(zero && s[i][u] != 255u));
+            wide = __any(!mx_f16_fits(s[i][u], w[i][u]));
           }
           if (wide) {
             if constexpr (AT == LT_F16) {
@@ -285,12 +244,22 @@ hipError_t launch_mx4_quantize(const MxQuantArgs& a, hipStream_t st) {
   }
 }
 
-int64_t mx4_workspace_bytes(int64_t, int64_t, int64_t, int) { return 0; }
+int64_t mx4_workspace_bytes(int64_t M, int64_t K, int64_t N, int a_type) { return mx4_gemm_plan(M, K, N, a_type, true).ws_bytes; }
 
-const char* mx4_kernel_name(const MxArgs&) { return "mx4_rows"; }
+const char* mx4_kernel_name(const MxArgs& a) {
+  switch (mx4_gemm_plan(a.M, a.K, a.N, a.a_type, true).t) {
+    case 4: return "mx4_gemm_256";
+    case 2: return "mx4_gemm_128";
+    case 1: return "mx4_gemm_64";
+  }
+  return "mx4_rows";
+}
 
 hipError_t launch_matmul_mx4(const MxArgs& a, hipStream_t st) {
   if (a.M == 0) return hipSuccess;
+  MxPlan p = mx4_gemm_plan(a.M, a.K, a.N, a.a_type, a.ws != nullptr);
+  if (p.ws_bytes > a.ws_bytes) p = mx4_gemm_plan(a.M, a.K, a.N, a.a_type, false);
+  if (p.t != 0) return launch_mx4_gemm(a, p, st);
   switch (a.a_type) {
     case LT_F16: return rows_for<LT_F16, 1, 1>(a, st);
     case LT_BF16: return rows_for<LT_BF16, 1, 1>(a, st);

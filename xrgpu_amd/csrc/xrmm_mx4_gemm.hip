@@ -1,0 +1,518 @@
+// MX4 product, many rows: Y = A W^T (+ bias) on tiles of 32 WM TM rows by 64 TN columns.
+//
+// WM x 2 waves, each with TM x TN accumulators of 32 x 32. A K step stages 128 bytes of every row: 64 values of 16-bit
+// activations and of the weights, converted on the way into LDS, or 256 codes where both operands are
+// MX4 (v_mfma_scale takes them and their scales as they are). Either way a row is eight pieces of 16 bytes; piece p of row r lies
+// in slot p ^ (r % 8), which spreads a fragment's rows over all banks without padding.
+//
+// Two stages. While step s computes, the pieces of step s + 1 go from registers to the other
+// stage, a quarter beside each K slice, and each is loaded anew for step s + 2 at once, so a load has a whole step to
+// arrive. The barrier stands before the last slice's MFMAs: the next stage's first fragments are
+// read behind them.
+//
+// The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
+#include <atomic>
+
+#include "xrmm_mx4.h"
+
+namespace xrmm {
+
+int device_cus();
+
+namespace {
+
+template <int AT, int WM, int TM, int TN>
+struct MxTile {
+  static constexpr bool MX = AT < 0;
+  static constexpr int T = 128 * WM, RA = 32 * WM * TM, RB = 64 * TN;
+  static constexpr int CODES = (RA + RB) * 128;                    // bytes of a stage's rows
+  static constexpr int STAGE = CODES + (MX ? (RA + RB + T - 1) / T * T * 8 : 0);  // and of its scales, one row a thread
+  static constexpr int STRIP = 32 * (32 * TN * 4 + 16);            // of a wave's rows on their way out
+  static constexpr int LDS = 2 * STAGE > 2 * WM * STRIP ? 2 * STAGE : 2 * WM * STRIP;
+  static constexpr int BLOCKS = MX ? 8 : 2;                        // blocks of 32 along K in a step
+};
+
+struct MxGrid {
+  uint32_t mt, nb, ns, nbig, splits, per;
+};
+
+template <int AT, int WM, int TM, int TN, bool AL>
+__device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n0, const MxGrid& g, uint32_t tile, uint32_t split) {
+  typedef MxTile<AT, WM, TM, TN> Ti;
+  constexpr bool MX = Ti::MX;
+  constexpr int T = Ti::T, RA = Ti::RA, RB = Ti::RB, NA = RA * 8 / T, NB = MX ? RB * 8 / T : (2 * RB + T - 1) / T;
+  constexpr int NS = MX ? (RA + RB + T - 1) / T : NB, TR = T / 8;  // TR: rows that the threads cover with one piece each
+  typedef typename MxFrag<AT>::t half8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int64_t m0 = static_cast<int64_t>(row) * RA;
+  const uint32_t kb = static_cast<uint32_t>(a.kb), K = static_cast<uint32_t>(a.K);
+  const uint32_t rowsA = static_cast<uint32_t>(a.M - m0 < RA ? a.M - m0 : RA);
+  const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < RB ? a.N - n0 : RB);
+  const uint32_t s0 = split * g.per, s1 = s0 + g.per;  // an even number of steps
+  // the split's end along K, in blocks and values: what lies past it loads as zeros
+  const uint32_t kbe = s1 * Ti::BLOCKS < kb ? s1 * Ti::BLOCKS : kb, Ke = kbe * MX_BLOCK < K ? kbe * MX_BLOCK : K;
+
+  const uint32_t rowA = MX ? kb * MX_BLOB : K * 2u, rowB = kb * MX_BLOB;
+  // an unaligned A: its resource starts at the dword that holds its first byte
+  const uint8_t* pA = static_cast<const uint8_t*>(a.A) + m0 * rowA;
+  const uint32_t misA = AL ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(pA)) & 3u;
+  const rsrc_t rA = mk_rsrc(pA - misA, (rowsA * rowA + misA + 3u) & ~3u);
+  const rsrc_t rB = mk_rsrc(a.B + n0 * rowB, rowsB * rowB);
+  // scales: a wave's threads hold rows of one operand each; MX4 scales at any alignment start at a dword
+  rsrc_t rS[NS];
+  uint32_t sbase[NS];  // byte offset of the thread's row (MX) or block (16-bit activations)
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    if constexpr (MX) {
+      const bool isA = wave * 64 + T * i < RA;
+      const uint8_t* ps = isA ? a.As + m0 * a.kb : a.S + n0 * a.kb;
+      const uint32_t mis = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ps)) & 3u, rows = isA ? rowsA : rowsB;
+      rS[i] = mk_rsrc(ps - mis, (rows * kb + mis + 3u) & ~3u);
+      const uint32_t r = static_cast<uint32_t>(tid + T * i) - (isA ? 0u : RA);
+      sbase[i] = r < rows ? r * kb + mis : MX_OOB;
+    } else {
+      const uint32_t c = static_cast<uint32_t>(tid + T * i), r = c >> 1;
+      rS[i] = mk_rsrc(a.S + n0 * a.kb, rowsB * kb);
+      sbase[i] = r < rowsB && r < RB ? r * kb + (c & 1u) : MX_OOB;
+    }
+  }
+
+  // ---- staging registers
+  struct Wide {           // loaded at a step's start for the step after the next: two sets
+    u32x4 b[MX ? 1 : NB];
+    uint32_t s[NS][MX ? 3 : 1];
+  };
+  u32x4 ra[NA], rb[MX ? NB : 1];
+  uint32_t rx[AL ? 1 : NA];
+  bool misfit = false;
+
+  const uint32_t srow = static_cast<uint32_t>(tid >> 3), spiece = static_cast<uint32_t>((tid & 7) ^ (srow & 7u));
+  auto load_a = [&](int i, uint32_t s) {
+    const uint32_t r = srow + TR * i;
+    if constexpr (MX) {
+      const uint32_t b = s * 8u + spiece;
+      ra[i] = bld16(rA, (r < rowsA && b < kbe) ? r * rowA + b * MX_BLOB : MX_OOB, 0);
+    } else {
+      const uint32_t k = s * 64u + spiece * 8u;
+      const bool ok = r < rowsA && k < Ke;
+      if constexpr (AL) {
+        ra[i] = bld16(rA, ok ? r * rowA + k * 2u : MX_OOB, 0);
+      } else {
+        const uint32_t off = r * rowA + k * 2u + misA;
+        ra[i] = bld16(rA, ok ? off & ~3u : MX_OOB, 0);
+        rx[i] = bld_u32(rA, ok ? (off & ~3u) + 16u : MX_OOB, 0);
+      }
+    }
+  };
+  auto load_b = [&](int i, uint32_t s) {  // MX4 operands
+    const uint32_t r = srow + TR * i, b = s * 8u + spiece;
+    rb[MX ? i : 0] = bld16(rB, (r < rowsB && b < kbe) ? r * rowB + b * MX_BLOB : MX_OOB, 0);
+  };
+  auto load_wide = [&](Wide& w, uint32_t s) {
+    if constexpr (MX) {
+      // eight scale bytes a row: three dwords
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const uint32_t at = s * 8u < kbe ? (sbase[i] + s * 8u) & ~3u : MX_OOB;
+#pragma unroll
+        for (int d = 0; d < 3; ++d) w.s[i][MX ? d : 0] = bld_u32(rS[i], at + 4u * d, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t c = static_cast<uint32_t>(tid + T * i), r = c >> 1, b = s * 2u + (c & 1u);
+        const bool ok = r < rowsB && b < kbe && c < 2u * RB;
+        w.b[MX ? 0 : i] = bld16(rB, ok ? r * rowB + b * MX_BLOB : MX_OOB, 0);
+        w.s[i][0] = bld_u8(rS[i], b < kbe ? sbase[i] + s * 2u : MX_OOB, 0);
+      }
+    }
+  };
+  // Quarter d of the pieces of step s to LDS stage `st`, and each piece's load for step s + 1
+  auto part = [&](int d, uint32_t s, int st, const Wide& w) {
+    unsigned char* base = smem + st * Ti::STAGE;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      if (i * 4 / NA != d) continue;
+      u32x4 v = ra[i];
+      if constexpr (!MX && !AL) {
+        const uint32_t k = s * 64u + spiece * 8u, r = srow + TR * i;
+        const uint32_t sh = (r * rowA + k * 2u + misA) & 3u;
+        const u32x4 x = v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(e < 3 ? x[e + 1] : rx[AL ? 0 : i], x[e], sh);
+        if (k + 8u > K) {  // the row's last piece: what lies past it is the next row's
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t ke = k + 2u * e;
+            v[e] = ke + 1u < K ? v[e] : ke < K ? v[e] & 0xFFFFu : 0u;
+          }
+        }
+      }
+      *reinterpret_cast<u32x4*>(base + (srow + TR * i) * 128 + (tid & 7) * 16) = v;
+      load_a(i, s + 1);
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        if (i * 4 / NB != d) continue;
+        *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = rb[MX ? i : 0];
+        load_b(i, s + 1);
+      }
+      if (d == 0) {
+        const uint32_t b0 = s * 8u, n = b0 < kbe ? kbe - b0 : 0u;  // scales of blocks past K are 2^-127 on both sides: products of 0
+        const uint32_t k0 = n >= 4u ? ~0u : (1u << (8u * n)) - 1u, k1 = n >= 8u ? ~0u : n <= 4u ? 0u : (1u << (8u * (n - 4u))) - 1u;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const int r = tid + T * i;
+          const uint32_t sh = (sbase[i] + b0) & 3u;
+          u32x2 v;
+          v[0] = __builtin_amdgcn_alignbyte(w.s[i][MX ? 1 : 0], w.s[i][0], sh) & k0;
+          v[1] = __builtin_amdgcn_alignbyte(w.s[i][MX ? 2 : 0], w.s[i][MX ? 1 : 0], sh) & k1;
+          *reinterpret_cast<u32x2*>(base + Ti::CODES + r * 8) = v;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int c = tid + T * i, r = c >> 1;
+        const u32x4 wb = w.b[MX ? 0 : i];
+        if (AT == LT_F16 && d == 0) misfit |= !mx_f16_fits(w.s[i][0], wb);
+        if (NB * T == 2 * RB || c < 2 * RB)
+          *reinterpret_cast<half8*>(base + (RA + r) * 128 + ((((c & 1) * 4 + d) ^ (r & 7)) * 16)) = mx_dq8<AT>(wb[d], e8m0(w.s[i][0]));
+      }
+    }
+  };
+
+  f32x16 acc[TN][TM];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+
+  // ---- fragments: lane (r, h) = (lane % 32, lane / 32) reads piece 2 kk + h of row r
+  constexpr bool TWO = !(MX && WM == 4);  // fragments of the next slice beside the current one's; else two waves a SIMD cover the reads
+  u32x4 fa[2][TM], fb[2][TN];
+  u32x2 ta[MX ? TM : 1], tb[MX ? TN : 1];  // scales of the step, moved so that byte 2 kk is this half's
+  const int fr = lane & 31, fh = lane >> 5;
+  auto read = [&](int st, int kk) {
+    const int buf = TWO ? kk & 1 : 0;
+    const unsigned char* base = smem + st * Ti::STAGE + (((2 * kk + fh) ^ (fr & 7)) * 16) + fr * 128;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) fa[buf][i] = *reinterpret_cast<const u32x4*>(base + (wm * TM + i) * 4096);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[buf][j] = *reinterpret_cast<const u32x4*>(base + RA * 128 + (wn * TN + j) * 4096);
+  };
+  auto read_scales = [&](int st) {
+    if constexpr (MX) {
+      const unsigned char* base = smem + st * Ti::STAGE + Ti::CODES + fr * 8;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        ta[i] = *reinterpret_cast<const u32x2*>(base + (wm * TM + i) * 256);
+        ta[i] >>= fh * 8;
+      }
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        tb[j] = *reinterpret_cast<const u32x2*>(base + RA * 8 + (wn * TN + j) * 256);
+        tb[j] >>= fh * 8;
+      }
+    }
+  };
+  auto mfmas = [&](auto kkc) {
+    constexpr int kk = decltype(kkc)::value, buf = TWO ? kk & 1 : 0;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        if constexpr (MX)
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_fp4(fb[buf][j]), mx_fp4(fa[buf][i]), acc[j][i], 4, 4, (kk & 1) * 2,
+                                                                       static_cast<int>(tb[j][kk >> 1]), (kk & 1) * 2, static_cast<int>(ta[i][kk >> 1]));
+        else if constexpr (AT == LT_F16)
+          acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fb[buf][j]), __builtin_bit_cast(f16x8, fa[buf][i]), acc[j][i], 0, 0, 0);
+        else
+          acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fb[buf][j]), __builtin_bit_cast(bf16x8, fa[buf][i]), acc[j][i], 0, 0, 0);
+      }
+  };
+  auto step = [&](uint32_t s, int st, Wide& nxt, Wide& fill) {
+    load_wide(fill, s + 2);
+    if (TWO) read(st, 1);
+    part(0, s + 1, st ^ 1, nxt);
+    mfmas(std::integral_constant<int, 0>{});
+    read(st, TWO ? 2 : 1);
+    part(1, s + 1, st ^ 1, nxt);
+    mfmas(std::integral_constant<int, 1>{});
+    read(st, TWO ? 3 : 2);
+    part(2, s + 1, st ^ 1, nxt);
+    part(3, s + 1, st ^ 1, nxt);
+    mfmas(std::integral_constant<int, 2>{});
+    if (!TWO) {
+      read(st, 3);
+      mfmas(std::integral_constant<int, 3>{});
+    }
+    __syncthreads();
+    read(st ^ 1, 0);
+    if (TWO) mfmas(std::integral_constant<int, 3>{});
+    read_scales(st ^ 1);
+  };
+
+  {
+    Wide w0, w1;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) load_a(i, s0);
+    if constexpr (MX)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) load_b(i, s0);
+    load_wide(w0, s0);
+    load_wide(w1, s0 + 1);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) part(d, s0, 0, w0);
+    __syncthreads();
+    read(0, 0);
+    read_scales(0);
+    for (uint32_t s = s0; s < s1; s += 2) {
+      step(s, 0, w1, w0);
+      step(s + 1, 1, w0, w1);
+    }
+  }
+
+  if constexpr (AT == LT_F16) {
+    // A block of the tile has a scale that binary16 cannot hold (or NaN): the tile again, slowly, with weights in
+    // bfloat16 and each activation as the sum of two bfloat16 terms, exact for every scale.
+    if (__syncthreads_or(misfit)) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+      for (uint32_t q = s0 * 4u; q < kbe * 2u; ++q) {  // 16 values of K
+        const uint32_t b = q >> 1, k = q * 16u + fh * 8u;
+        bf16x8 wf[TN];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const uint32_t r = (wn * TN + j) * 32 + fr;
+          const uint32_t w = bld_u32(rB, r < rowsB ? r * rowB + b * MX_BLOB + ((q & 1u) * 2u + fh) * 4u : MX_OOB, 0);
+          wf[j] = mx_dq8<LT_BF16>(w, e8m0(bld_u8(rS[0], r < rowsB ? r * kb + b : MX_OOB, 0)));
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          const uint32_t r = (wm * TM + i) * 32 + fr;
+          f16x8 x;
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e)
+            x[e] = __builtin_bit_cast(f16, static_cast<uint16_t>(bld_u16(rA, (r < rowsA && k + e < K) ? r * rowA + (k + e) * 2u + misA : MX_OOB, 0)));
+          bf16x8 hi, lo;
+          split_f16(x, hi, lo);
+#pragma unroll
+          for (int j = 0; j < TN; ++j) {
+            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[j], hi, acc[j][i], 0, 0, 0);
+            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[j], lo, acc[j][i], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+
+  if (g.splits > 1) {
+    // The splits' float32 parts meet in the workspace: coherent stores (sc0 sc1), one relaxed arrival count a
+    // workgroup, and the last one adds them in split order.
+    constexpr int COHERENT = 1 | 16;
+    constexpr uint32_t BYTES = RA * RB * 4;  // of a tile's part
+    __shared__ int s_last;
+    uint32_t* cnt = static_cast<uint32_t*>(a.ws);
+    const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + MX_COUNTERS + static_cast<int64_t>(tile) * g.splits * BYTES, g.splits * BYTES);
+    const uint32_t at = static_cast<uint32_t>(wave) * (TM * TN * 4096u) + lane * 16u;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rW, split * BYTES + at + ((j * TM + i) * 4 + q) * 1024u, 0, COHERENT);
+        }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) s_last = __hip_atomic_fetch_add(cnt + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.splits - 1;
+    __syncthreads();
+    if (!s_last) return;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+    for (uint32_t sp = 0; sp < g.splits; ++sp)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, sp * BYTES + at + ((j * TM + i) * 4 + q) * 1024u, 0, COHERENT));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][i][4 * q + e] += v[e];
+          }
+    if (tid == 0) __hip_atomic_store(cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+
+  // ---- output: 32 rows at a time through the wave's part of LDS, so that rows are written in whole pieces of 16 bytes
+  __syncthreads();
+  const int osz = a.out == LT_F32 ? 4 : 2;
+  const int pitch = 32 * TN * osz + 16;
+  unsigned char* strip = smem + wave * Ti::STRIP;
+  const int64_t nw = n0 + wn * 32 * TN, mw = m0 + wm * 32 * TM;
+  const bool vec = (a.N * osz & 15) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 15u) == 0;
+  const int per = 16 / osz, ppr = 32 * TN / per;  // values of a piece, pieces of a strip's row
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * j + 8 * q + 4 * fh;
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = acc[j][i][4 * q + e];
+          if (a.bias != nullptr && nw + c + e < a.N) v[e] += ld_lt(a.bias, nw + c + e, a.out);
+        }
+        unsigned char* at = strip + fr * pitch + c * osz;
+        if (a.out == LT_F32) *reinterpret_cast<f32x4*>(at) = v;
+        else if (a.out == LT_F16) *reinterpret_cast<f16x4*>(at) = f16x4{static_cast<f16>(v[0]), static_cast<f16>(v[1]), static_cast<f16>(v[2]), static_cast<f16>(v[3])};
+        else *reinterpret_cast<bf16x4*>(at) = bf16x4{static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int x = lane; x < 32 * ppr; x += 64) {
+      const int r = x / ppr, p = x % ppr;
+      const int64_t m = mw + 32 * i + r, n = nw + p * per;
+      if (m >= a.M || n >= a.N) continue;
+      const unsigned char* src = strip + r * pitch + p * 16;
+      unsigned char* dst = static_cast<unsigned char*>(a.Y) + (m * a.N + n) * osz;
+      if (vec) {
+        *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
+      } else if (osz == 4) {
+        for (int e = 0; e < 4 && n + e < a.N; ++e) reinterpret_cast<uint32_t*>(dst)[e] = reinterpret_cast<const uint32_t*>(src)[e];
+      } else {
+        for (int e = 0; e < 8 && n + e < a.N; ++e) reinterpret_cast<uint16_t*>(dst)[e] = reinterpret_cast<const uint16_t*>(src)[e];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// Tile l of a raster in groups of four row tiles, row fastest inside a group: the tiles that one XCD
+// runs at once share few row and column panels in its L2.
+__device__ __forceinline__ void mx_raster(uint32_t l, uint32_t mt, uint32_t nc, uint32_t& row, uint32_t& col) {
+  constexpr uint32_t G = 4;
+  const uint32_t q = l / (G * nc), rows = mt - q * G < G ? mt - q * G : G, r = l - q * G * nc;
+  row = q * G + r % rows;
+  col = r / rows;
+}
+
+template <int AT, int WM, int TM, int TN, bool AL>
+__global__ __launch_bounds__(128 * WM, TM == 1 ? 4 : 2) void k_mx4_gemm(MxArgs a, MxGrid g) {
+  uint32_t row, col;
+  const uint32_t bid = blockIdx.x;
+  if (TN < 4 || bid < g.nbig) {
+    const uint32_t n = g.mt * g.nb * g.splits, l = xcd_slot(bid, n), split = l % g.splits;
+    mx_raster(l / g.splits, g.mt, g.nb, row, col);
+    mx_tile<AT, WM, TM, TN, AL>(a, row, static_cast<int64_t>(col) * (64 * TN), g, l / g.splits, split);
+  } else if constexpr (TN == 4) {
+    const uint32_t n = g.mt * g.ns, l = xcd_slot(bid - g.nbig, n);
+    mx_raster(l, g.mt, g.ns, row, col);
+    mx_tile<AT, WM, TM, 3, AL>(a, row, static_cast<int64_t>(g.nb) * 256 + static_cast<int64_t>(col) * 192, g, 0, 0);
+  }
+}
+
+template <int AT, int WM, int TM, int TN, bool AL>
+hipError_t gemm_al(const MxArgs& a, const MxPlan& p, hipStream_t st) {
+  auto kern = k_mx4_gemm<AT, WM, TM, TN, AL>;
+  constexpr int lds = MxTile<AT, WM, TM, TN>::LDS;
+  static std::atomic<int> done[kMaxDevices];
+  if (lds > 65536) {
+    const hipError_t e = raise_lds_cap(reinterpret_cast<const void*>(kern), lds, done);
+    if (e != hipSuccess) return e;
+  }
+  const MxGrid g{p.mt, p.nb, p.ns, p.mt * p.nb * p.splits, p.splits, p.per};
+  const int64_t n = static_cast<int64_t>(p.mt) * p.nb * p.splits + static_cast<int64_t>(p.mt) * p.ns;
+  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  kern<<<dim3(static_cast<uint32_t>(n)), 128 * WM, lds, st>>>(a, g);
+  return hipGetLastError();
+}
+
+template <int AT, int WM, int TM, int TN>
+hipError_t gemm_for(const MxArgs& a, const MxPlan& p, hipStream_t st) {
+  if (AT < 0 || (a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15u) == 0)) return gemm_al<AT, WM, TM, TN, true>(a, p, st);
+  if constexpr (AT >= 0) return gemm_al<AT, WM, TM, TN, false>(a, p, st);
+  return hipErrorInvalidValue;
+}
+
+template <int AT>
+hipError_t gemm_at(const MxArgs& a, const MxPlan& p, hipStream_t st) {
+  if (p.t == 4) return gemm_for<AT, 4, 2, 4>(a, p, st);
+  if (p.t == 2) return gemm_for<AT, 2, 2, 2>(a, p, st);
+  return gemm_for<AT, 2, 1, 1>(a, p, st);
+}
+
+}  // namespace
+
+MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) {
+  MxPlan p{};
+  const int64_t kb = (K + MX_BLOCK - 1) / MX_BLOCK;
+  if (M <= 16 || K > (int64_t(1) << 21)) return p;  // 256 rows of 16-bit values stay below 2^31 bytes
+  const int64_t cus = device_cus() > 0 ? device_cus() : 256;
+  const int64_t steps = (kb + (a_type < 0 ? 7 : 1)) / (a_type < 0 ? 8 : 2);
+  auto tiles = [&](int64_t t) { return ((M + 64 * t - 1) / (64 * t)) * ((N + 64 * t - 1) / (64 * t)); };
+  int t = tiles(4) >= cus ? 4 : tiles(2) >= cus ? 2 : 1;
+  p.t = t;
+  p.mt = static_cast<uint32_t>((M + 64 * t - 1) / (64 * t));
+  p.nb = static_cast<uint32_t>((N + 64 * t - 1) / (64 * t));
+  p.splits = 1;
+  p.per = static_cast<uint32_t>((steps + 1) / 2 * 2);
+  if (t == 4 && static_cast<int64_t>(p.mt) * p.nb > cus && cus % p.mt == 0) {
+    // wide and narrow (192) columns mixed, where that makes fewer rounds of the CUs
+    const int64_t per = cus / p.mt;
+    double best = static_cast<double>((static_cast<int64_t>(p.mt) * p.nb + cus - 1) / cus);
+    for (int64_t j = 1; j <= 16; ++j) {
+      const int64_t rest = N - 192 * j * per, k = rest > 0 ? (rest + 256 * per - 1) / (256 * per) : 0;
+      const double time = static_cast<double>(k) + 0.75 * static_cast<double>(j);
+      if (time < best - 0.05) {
+        best = time;
+        p.nb = static_cast<uint32_t>(k * per);
+        p.ns = static_cast<uint32_t>(j * per);
+      }
+    }
+  }
+  int64_t splits = 1;
+  const int64_t n = static_cast<int64_t>(p.mt) * p.nb;
+  if (have_ws && p.ns == 0 && n * 2 <= cus && n <= MX_COUNTERS / 4) {
+    splits = cus / n;
+    splits = splits < 8 ? splits : 8;
+    splits = splits < steps / 4 ? splits : steps / 4;
+  }
+  if (splits > 1) {
+    p.per = static_cast<uint32_t>((steps + 2 * splits - 1) / (2 * splits) * 2);
+    p.splits = static_cast<uint32_t>((steps + p.per - 1) / p.per);
+    p.ws_bytes = MX_COUNTERS + n * p.splits * t * t * 16384;
+  }
+  return p;
+}
+
+hipError_t launch_mx4_gemm(const MxArgs& a, const MxPlan& p, hipStream_t st) {
+  switch (a.a_type) {
+    case LT_F16: return gemm_at<LT_F16>(a, p, st);
+    case LT_BF16: return gemm_at<LT_BF16>(a, p, st);
+    default: return gemm_at<-1>(a, p, st);
+  }
+}
+
+}  // namespace xrmm
