@@ -226,6 +226,30 @@ def test_other_stream_workspace_and_graph(gpu, M):
             ops().matmul_mx4(A, codes, scales)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 8, 40, 150])
+@pytest.mark.parametrize("dt,center", [("f16", 139), ("bf16", 245)])
+def test_subnormal_activations(gpu, M, dt, center):
+    """Activations below the smallest normal value count in full."""
+    N, K = 70, 224
+    codes, scales = weights(N, K, M, spread=1, center=center)
+    t = DT[dt]
+    step = torch.finfo(t).tiny * torch.finfo(t).eps
+    A = (torch.randint(-30, 31, (M, K), generator=torch.Generator().manual_seed(M)).double() * step).to(t)
+    y = ops().matmul_mx4(A.cuda(), codes, scales)
+    check_product(A.double().numpy(), codes, scales, None, y)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 16])
+@pytest.mark.parametrize("K,N", [(1, 1), (31, 17), (2048, 5), (2080, 33), (4097, 130), (20000, 40), (70000, 3)])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_product_few_rows(gpu, M, K, N, dt):
+    codes, scales = weights(N, K, M + K + N)
+    A = torch.randn(M, K, generator=torch.Generator().manual_seed(K)).to(DT[dt])
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(N)).to(DT[dt]).cuda()
+    y = ops().matmul_mx4(A.cuda(), codes, scales, bias)
+    check_product(A.double().numpy(), codes, scales, bias, y)
+
+
 def test_kernel_names(gpu):
     assert ops().matmul_mx4_kernel(1, 4096, 4096).startswith("mx4_")
     with pytest.raises(ValueError):

@@ -55,7 +55,7 @@ struct MxPlan {
   uint32_t mt;         // row tiles
   uint32_t nb, ns;     // column tiles of 64 t columns, and of 192 behind them (t 4 only)
   uint32_t splits;     // of K
-  uint32_t per;        // K steps of a split, even
+  uint32_t per;        // K steps of a split
   int64_t ws_bytes;
 };
 MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws);

@@ -3,9 +3,14 @@
 //   quantise: E = floor(log2 max|x|), scale byte max(E + 127 - 2, 0), code = the E2M1 value
 //             nearest x / 2^(byte - 127), ties to even, saturated at 6, sign kept
 //   product:  Y[m, n] = sum_k A[m, k] e2m1(code[n, k]) 2^(byte[n, k / 32] - 127) (+ bias[n])
+#include <type_traits>
+
 #include "xrmm_mx4.h"
 
 namespace xrmm {
+
+int device_cus();
+
 namespace {
 
 // ---------------------------------------------------------------------------
@@ -78,159 +83,265 @@ hipError_t quantize_for(const MxQuantArgs& a, hipStream_t st) {
 
 // ---------------------------------------------------------------------------
 // Product, few rows. The weights are the MFMA's first operand: lane (c, g) = (lane % 16,
-// lane / 16) loads blocks 8 it + 2 g + {0, 1} of column c, 32 consecutive bytes, straight
+// lane / 16) loads block 4 it + g of column c, 16 consecutive bytes, straight
 // into the fragment (the order of k inside an MFMA is free as long as both operands agree),
-// and the second operand's lane (c, g) holds the same blocks of row c. float16 / bfloat16
-// activations: each byte pair of codes becomes two 16-bit values with its block's scale in one
+// and the second operand's lane (c, g) holds the same block of row c. float16 / bfloat16
+// activations: each byte of codes becomes two 16-bit values times its block's scale in one
 // conversion instruction, v_mfma_f32_16x16x32 four times a block. MX4 activations: one
-// v_mfma_scale_f32_16x16x128 for four blocks, scales applied by the instruction.
+// v_mfma_scale_f32_16x16x128 for the four blocks, scales applied by the instruction.
+//
+// A wave takes every WV-th group of four blocks, with nothing in LDS until the waves' sums meet, so no wave waits
+// for another; sixteen waves a CU keep the loads in flight. The loop is short on purpose: the kernel
+// lives for a few microseconds, and code that is run once or twice is fetched slower than it runs (unrolled by four, loads
+// of the next four groups ahead: 21 us at 1 x 4096 x 14336 for 15 here; 8 x 4096 x 4096 8.6 for 7.6).
 //
 // A bfloat16 holds every E2M1 value times 2^(byte - 127) exactly. A binary16 does for scales in
-// [2^-23, 2^13]; a wave that meets another scale takes that block's weights in bfloat16 and the
+// [2^-23, 2^13]; a workgroup that met another scale sums its share again, with weights in bfloat16 and the
 // activations as the sum of two bfloat16 terms (8 and 3 bits: exact), so every scale is right.
 
-constexpr int MXR_WAVES = 8;
-
-template <int AT, int NT, int CT, bool AL>
-__global__ __launch_bounds__(64 * MXR_WAVES) void k_mx4_rows(MxArgs a, uint32_t col_tiles) {
+template <int AT, int WV, bool AL>
+__global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a) {
   constexpr bool MX = AT < 0;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x % col_tiles) * (16 * CT);
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x / col_tiles) * (16 * NT);
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
   const uint32_t kb = static_cast<uint32_t>(a.kb), K = static_cast<uint32_t>(a.K);
-  const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < 16 * CT ? a.N - n0 : 16 * CT);
-  const uint32_t rowsA = static_cast<uint32_t>(a.M - m0 < 16 * NT ? a.M - m0 : 16 * NT);
+  const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < 16 ? a.N - n0 : 16), rowsA = static_cast<uint32_t>(a.M);  // at most 16
+  const uint32_t rowA = MX ? kb * MX_BLOB : K * 2u;
+  const uint32_t mis = AL ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.A)) & 3u;
+  const rsrc_t rA = mk_rsrc(static_cast<const uint8_t*>(a.A) - mis, (rowsA * rowA + mis + 3u) & ~3u);
   const rsrc_t rB = mk_rsrc(a.B + n0 * a.kb * MX_BLOB, rowsB * kb * MX_BLOB);
   const rsrc_t rS = mk_rsrc(a.S + n0 * a.kb, rowsB * kb);
-  const rsrc_t rA = MX ? mk_rsrc(static_cast<const uint8_t*>(a.A) + m0 * a.kb * MX_BLOB, rowsA * kb * MX_BLOB)
-                       : mk_rsrc(static_cast<const uint16_t*>(a.A) + m0 * a.K, rowsA * K * 2u);
-  const rsrc_t rAs = mk_rsrc(MX ? a.As + m0 * a.kb : a.S, MX ? rowsA * kb : 0u);
+  const rsrc_t rT = mk_rsrc(MX ? a.As : a.S, MX ? rowsA * kb : 0u);
+  const uint32_t cb = static_cast<uint32_t>(c) < rowsB ? c * kb : MX_OOB / 16, ca = static_cast<uint32_t>(c);
+  const bool oka = ca < rowsA, okb = static_cast<uint32_t>(c) < rowsB;
+  typedef typename MxFrag<AT>::t frag;
 
-  f32x4 acc[CT][NT];
-#pragma unroll
-  for (int i = 0; i < CT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const uint32_t its = (kb + 7) / 8;
-  for (uint32_t it = static_cast<uint32_t>(wave); it < its; it += MXR_WAVES) {
-    u32x4 w[CT][2];
-    uint32_t s[CT][2];
-#pragma unroll
-    for (int i = 0; i < CT; ++i)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t b = it * 8 + g * 2 + u, r = i * 16 + c;
-        const bool ok = b < kb && r < rowsB;
-        w[i][u] = bld16_nt(rB, ok ? (r * kb + b) * MX_BLOB : MX_OOB, 0);
-        s[i][u] = bld_u8(rS, ok ? r * kb + b : MX_OOB, 0);
-      }
-    if constexpr (MX) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint32_t b = it * 8 + g * 2 + u, r = j * 16 + c;
-          const bool ok = b < kb && r < rowsA;
-          const u32x4 x = bld16(rA, ok ? (r * kb + b) * MX_BLOB : MX_OOB, 0);
-          const int xs = static_cast<int>(bld_u8(rAs, ok ? r * kb + b : MX_OOB, 0));
-#pragma unroll
-          for (int i = 0; i < CT; ++i) {
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_fp4(w[i][u]), mx_fp4(x), acc[i][j], 4, 4, 0, static_cast<int>(s[i][u]), 0, xs);
-          }
-        }
+  // Piece d (eight values of K) of block b of the lane's row
+  auto piece = [&](uint32_t b, uint32_t d) {
+    const uint32_t k = b * MX_BLOCK + 8 * d, at = ca * rowA + k * 2u + mis;
+    if constexpr (AL) {  // K a multiple of 8: a piece is whole or absent
+      return bld16(rA, oka && b < kb && k < K ? at : MX_OOB, 0);
     } else {
-      typedef typename MxFrag<AT>::t frag;
+      const bool ok = oka && b < kb && k < K;
+      u32x4 v = bld16(rA, ok ? at & ~3u : MX_OOB, 0);
+      const uint32_t x = bld_u32(rA, ok ? (at & ~3u) + 16u : MX_OOB, 0);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        frag x[NT][4];
+      for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t ke = k + 2 * e, y = __builtin_amdgcn_alignbyte(e < 3 ? v[e + 1] : x, v[e], at & 3u);
+        v[e] = ke + 1 < K ? y : ke < K ? y & 0xFFFFu : 0u;
+      }
+      return v;
+    }
+  };
+
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  bool misfit = false;
+#pragma unroll 1
+  for (uint32_t b = wave * 4 + g; b - g < kb; b += WV * 4) {
+    const bool ok = okb && b < kb;
+    const u32x4 w = bld16_nt(rB, ok ? (cb + b) * MX_BLOB : MX_OOB, 0);
+    const uint32_t s = bld_u8(rS, ok ? cb + b : MX_OOB, 0);
+    if constexpr (MX) {
+      const bool have = oka && b < kb;
+      const u32x4 x = bld16(rA, have ? (ca * kb + b) * MX_BLOB : MX_OOB, 0);
+      const uint32_t t = bld_u8(rT, have ? ca * kb + b : MX_OOB, 0);
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_fp4(w), mx_fp4(x), acc, 4, 4, 0, static_cast<int>(s), 0, static_cast<int>(t));
+    } else {
+      u32x4 x[4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+      for (uint32_t d = 0; d < 4; ++d) x[d] = piece(b, d);
+      if (AT == LT_F16) misfit |= !mx_f16_fits(s, w);
+      const float sf = e8m0(s);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t k = (it * 8 + g * 2 + u) * MX_BLOCK + q * 8, r = j * 16 + c;
-            if constexpr (AL) {  // K a multiple of 8: a piece is whole or absent
-              x[j][q] = __builtin_bit_cast(frag, bld16(rA, (k < K && r < rowsA) ? (r * K + k) * 2u : MX_OOB, 0));
-            } else {
-              u32x4 v;
-#pragma unroll
-              for (uint32_t d = 0; d < 4; ++d) {
-                const uint32_t k2 = k + 2 * d;
-                const uint32_t lo = bld_u16(rA, (k2 < K && r < rowsA) ? (r * K + k2) * 2u : MX_OOB, 0);
-                const uint32_t hi = bld_u16(rA, (k2 + 1 < K && r < rowsA) ? (r * K + k2 + 1) * 2u : MX_OOB, 0);
-                v[d] = lo | (hi << 16);
-              }
-              x[j][q] = __builtin_bit_cast(frag, v);
-            }
-          }
-#pragma unroll
-        for (int i = 0; i < CT; ++i) {
-          const float sf = e8m0(s[i][u]);
-          bool wide = false;
-          if constexpr (AT == LT_F16) {
-            wide = __any(!mx_f16_fits(s[i][u], w[i][u]));
-          }
-          if (wide) {
-            if constexpr (AT == LT_F16) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const bf16x8 wf = mx_dq8<LT_BF16>(w[i][u][q], sf);
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                  bf16x8 hi, lo;
-                  split_f16(x[j][q], hi, lo);
-                  acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, hi, acc[i][j], 0, 0, 0);
-                  acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, lo, acc[i][j], 0, 0, 0);
-                }
-              }
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const frag wf = mx_dq8<AT>(w[i][u][q], sf);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                if constexpr (AT == LT_F16) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, x[j][q], acc[i][j], 0, 0, 0);
-                else acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, x[j][q], acc[i][j], 0, 0, 0);
-              }
-            }
-          }
-        }
+      for (int d = 0; d < 4; ++d) {
+        const frag wf = mx_dq8<AT>(w[d], sf);
+        if constexpr (AT == LT_F16) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(f16x8, x[d]), acc, 0, 0, 0);
+        else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, __builtin_bit_cast(bf16x8, x[d]), acc, 0, 0, 0);
+      }
+    }
+  }
+  if constexpr (AT == LT_F16) {
+    if (__syncthreads_or(misfit)) {
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (uint32_t q = (wave * 4 + g) * 4; (q >> 2) - g < kb; q += (q & 3u) == 3u ? WV * 16 - 3 : 1) {
+        const uint32_t b = q >> 2, d = q & 3u;
+        const bool ok = okb && b < kb;
+        const float sf = e8m0(bld_u8(rS, ok ? cb + b : MX_OOB, 0));
+        const bf16x8 wf = mx_dq8<LT_BF16>(bld_u32(rB, ok ? (cb + b) * MX_BLOB + 4 * d : MX_OOB, 0), sf);
+        bf16x8 hi, lo;
+        split_f16(__builtin_bit_cast(f16x8, piece(b, d)), hi, lo);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, hi, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, lo, acc, 0, 0, 0);
       }
     }
   }
 
   // The waves' sums meet in LDS and are added in wave order.
-  __shared__ f32x4 red[MXR_WAVES][CT * NT][64];
-#pragma unroll
-  for (int i = 0; i < CT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) red[wave][i * NT + j][lane] = acc[i][j];
+  __shared__ f32x4 red[WV][64];
+  red[wave][lane] = acc;
   __syncthreads();
-  for (int p = tid; p < CT * NT * 64; p += 64 * MXR_WAVES) {
-    const int t = p >> 6, l = p & 63;
-    f32x4 v = red[0][t][l];
+  if (wave != 0 || c >= a.M) return;
+  f32x4 v = red[0][lane];
 #pragma unroll
-    for (int w = 1; w < MXR_WAVES; ++w) v += red[w][t][l];
-    const int64_t m = m0 + (t % NT) * 16 + (l & 15), n = n0 + (t / NT) * 16 + (l >> 4) * 4;
-    if (m >= a.M) continue;
+  for (int w = 1; w < WV; ++w) v += red[w][lane];
+  const int64_t n = n0 + g * 4;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < a.N) st_lt(a.Y, m * a.N + n + e, v[e] + (a.bias ? ld_lt(a.bias, n + e, a.out) : 0.f), a.out);
+  for (int e = 0; e < 4; ++e)
+    if (n + e < a.N) st_lt(a.Y, c * a.N + n + e, v[e] + (a.bias ? ld_lt(a.bias, n + e, a.out) : 0.f), a.out);
+}
+
+// ---------------------------------------------------------------------------
+// Product, one or two rows of 16-bit activations. A wave holds 64 blocks of K, one a lane, of every row in
+// registers and walks over columns: a column's 64 blocks are one load of 1 KB. A lane sums its block
+// from the codes as they are (exact in 16 bits whatever the scale; two products and a float32 sum in one v_dot2) and
+// then applies the scale, so no scale is out of range. The lanes' sums meet by DPP, the chunks of K in LDS,
+// in order. Nothing but the loop over columns repeats, and it is short: the kernel lives for a few microseconds, and
+// unrolled code is fetched slower than it runs.
+
+template <int AT>
+__device__ __forceinline__ float mx_dot2(uint32_t a, uint32_t b, float c) {
+  if constexpr (AT == LT_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+  else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, a), __builtin_bit_cast(bf16x2, b), c, false);
+}
+
+__device__ __forceinline__ float mx_wave_total(float v) {
+  auto dpp = [](float x, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v += dpp(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v += dpp(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v += dpp(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  auto at = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+  return (at(0) + at(16)) + (at(32) + at(48));
+}
+
+constexpr int MXD_MAX_WAVES = 16, MXD_MAX_COLS = 64;
+
+template <int AT, int R, bool AL>
+__global__ __launch_bounds__(64 * MXD_MAX_WAVES) void k_mx4_dot(MxArgs a, uint32_t ncols, uint32_t chunk_waves, uint32_t col_waves) {
+  constexpr int P = 2;  // columns whose loads are in flight together
+  __shared__ float part[MXD_MAX_WAVES][MXD_MAX_COLS][R];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(tid >> 6));
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * ncols;
+  const uint32_t kb = static_cast<uint32_t>(a.kb), K = static_cast<uint32_t>(a.K), M = static_cast<uint32_t>(a.M);
+  const uint32_t cols = a.N - n0 < ncols ? static_cast<uint32_t>(a.N - n0) : ncols;
+  const uint32_t mis = AL ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.A)) & 3u;
+  const rsrc_t rA = mk_rsrc(static_cast<const uint8_t*>(a.A) - mis, (M * K * 2u + mis + 3u) & ~3u);
+  const rsrc_t rB = mk_rsrc(a.B + n0 * a.kb * MX_BLOB, cols * kb * MX_BLOB);
+  const rsrc_t rS = mk_rsrc(a.S + n0 * a.kb, cols * kb);
+  const uint32_t cw = wave % chunk_waves, gw = wave / chunk_waves;
+  for (uint32_t c = gw; c < cols; c += col_waves)
+    if (lane < R) part[wave][c][lane] = 0.f;
+#pragma unroll 1
+  for (uint32_t chunk = cw; chunk * 64 < kb; chunk += chunk_waves) {
+    const uint32_t b = chunk * 64 + lane, k = b * MX_BLOCK;
+    const bool in = b < kb;
+    u32x4 x[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint32_t off = (r * K + k) * 2u + mis;
+#pragma unroll
+      for (uint32_t d = 0; d < 4; ++d)  // pieces past K are absent; unaligned, the last value may lie in the next piece's first dword
+        x[r][d] = bld16(rA, in && static_cast<uint32_t>(r) < M && k + 8 * d < (AL ? K : K + 1) ? (off & ~3u) + 16 * d : MX_OOB, 0);
+      if constexpr (!AL) {
+        const uint32_t last = bld_u32(rA, in && static_cast<uint32_t>(r) < M ? (off & ~3u) + 64u : MX_OOB, 0), sh = off & 3u;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t next = e < 3 ? x[r][d][e + 1] : d < 3 ? x[r][d < 3 ? d + 1 : 0][0] : last;
+            const uint32_t ke = k + 8 * d + 2 * e, y = __builtin_amdgcn_alignbyte(next, x[r][d][e], sh);
+            x[r][d][e] = ke + 1 < K ? y : ke < K ? y & 0xFFFFu : 0u;
+          }
+      }
+    }
+#pragma unroll 1
+    for (uint32_t c = gw; c < cols; c += P * col_waves) {
+      u32x4 w[P];
+      uint32_t s[P];
+#pragma unroll
+      for (uint32_t p = 0; p < P; ++p) {
+        const uint32_t cp = c + p * col_waves;
+        const bool ok = in && cp < cols;
+        w[p] = bld16_nt(rB, ok ? (cp * kb + b) * MX_BLOB : MX_OOB, 0);
+        s[p] = bld_u8(rS, ok ? cp * kb + b : MX_OOB, 0);
+      }
+#pragma unroll
+      for (uint32_t p = 0; p < P; ++p) {
+        const uint32_t cp = c + p * col_waves;
+        float sum[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) sum[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const u32x4 wv = __builtin_bit_cast(u32x4, mx_dq8<AT>(w[p][d], 1.f));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int r = 0; r < R; ++r) sum[r] = mx_dot2<AT>(wv[e], x[r][d][e], sum[r]);
+        }
+        const float sc = e8m0(s[p]);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float t = mx_wave_total(in ? sum[r] * sc : 0.f);
+          if (lane == r && cp < cols) part[wave][cp][r] += t;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  for (uint32_t x = tid; x < cols * M; x += blockDim.x) {
+    const uint32_t c = x % cols, r = x / cols, w0 = (c % col_waves) * chunk_waves;
+    float v = part[w0][c][r];
+    for (uint32_t w = 1; w < chunk_waves; ++w) v += part[w0 + w][c][r];
+    const int64_t n = n0 + c;
+    st_lt(a.Y, r * a.N + n, v + (a.bias ? ld_lt(a.bias, n, a.out) : 0.f), a.out);
   }
 }
 
-template <int AT, int NT, int CT>
-hipError_t rows_for(const MxArgs& a, hipStream_t st) {
-  const int64_t ct = (a.N + 16 * CT - 1) / (16 * CT), mt = (a.M + 16 * NT - 1) / (16 * NT);
-  if (ct * mt > 0x7FFFFFFF) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<uint32_t>(ct * mt));
+template <int AT, int R>
+hipError_t dot_r(const MxArgs& a, hipStream_t st) {
+  const int64_t chunks = (a.kb + 63) / 64, cus = device_cus() > 0 ? device_cus() : 256;
+  // a wave for each chunk of K, and as many times that as fit eight waves
+  const uint32_t cw = static_cast<uint32_t>(chunks < MXD_MAX_WAVES ? chunks : MXD_MAX_WAVES), gw = cw < 8 ? 8 / cw : 1;
+  // columns of a workgroup: about 20 waves a CU (4 to 64 columns at 1 x 4096 x 14336: 9.1 us at 8, 8.9 at 16, 9.4 at 32, 11.7 at
+  // 64; at 1 x 14336 x 4096: 12.3 us at 2, 10.6 at 4, 10.0 at 8, 11.8 at 16)
+  int64_t cols = (a.N * cw * gw + 20 * cus - 1) / (20 * cus);
+  cols = (cols + gw - 1) / gw * gw;
+  cols = cols < MXD_MAX_COLS ? cols : MXD_MAX_COLS;
+  const dim3 grid(static_cast<uint32_t>((a.N + cols - 1) / cols)), block(64 * cw * gw);
   const bool al = a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15u) == 0;
-  if (AT < 0 || al) k_mx4_rows<AT, NT, CT, true><<<grid, 64 * MXR_WAVES, 0, st>>>(a, static_cast<uint32_t>(ct));
-  else k_mx4_rows<AT, NT, CT, false><<<grid, 64 * MXR_WAVES, 0, st>>>(a, static_cast<uint32_t>(ct));
+  if (al) k_mx4_dot<AT, R, true><<<grid, block, 0, st>>>(a, static_cast<uint32_t>(cols), cw, gw);
+  else k_mx4_dot<AT, R, false><<<grid, block, 0, st>>>(a, static_cast<uint32_t>(cols), cw, gw);
   return hipGetLastError();
 }
+
+template <int AT>
+hipError_t dot_for(const MxArgs& a, hipStream_t st) {
+  switch (a.M) {
+    case 1: return dot_r<AT, 1>(a, st);
+    default: return dot_r<AT, 2>(a, st);
+  }
+}
+
+constexpr int MXR_WAVES = 8;
+
+template <int AT>
+hipError_t rows_for(const MxArgs& a, hipStream_t st) {
+  const dim3 grid(static_cast<uint32_t>((a.N + 15) / 16)), block(64 * MXR_WAVES);
+  const bool al = a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15u) == 0;
+  if (AT < 0 || al) k_mx4_rows<AT, MXR_WAVES, true><<<grid, block, 0, st>>>(a);
+  else if constexpr (AT >= 0) k_mx4_rows<AT, MXR_WAVES, false><<<grid, block, 0, st>>>(a);
+  return hipGetLastError();
+}
+
+// Rows that k_mx4_dot takes: at 4096 x 14336 one row takes 8.9 us there and 15 in k_mx4_rows, two 11.8, four 19 and 18
+// (a wave's activations are loaded anew for every few columns, and outgrow the weights).
+bool use_dot(int64_t M, int a_type) { return M <= 2 && a_type >= 0; }
 
 }  // namespace
 
@@ -244,7 +355,9 @@ hipError_t launch_mx4_quantize(const MxQuantArgs& a, hipStream_t st) {
   }
 }
 
-int64_t mx4_workspace_bytes(int64_t M, int64_t K, int64_t N, int a_type) { return mx4_gemm_plan(M, K, N, a_type, true).ws_bytes; }
+int64_t mx4_workspace_bytes(int64_t M, int64_t K, int64_t N, int a_type) {
+  return mx4_gemm_plan(M, K, N, a_type, true).ws_bytes;
+}
 
 const char* mx4_kernel_name(const MxArgs& a) {
   switch (mx4_gemm_plan(a.M, a.K, a.N, a.a_type, true).t) {
@@ -252,7 +365,7 @@ const char* mx4_kernel_name(const MxArgs& a) {
     case 2: return "mx4_gemm_128";
     case 1: return "mx4_gemm_64";
   }
-  return "mx4_rows";
+  return use_dot(a.M, a.a_type) ? "mx4_dot" : "mx4_rows";
 }
 
 hipError_t launch_matmul_mx4(const MxArgs& a, hipStream_t st) {
@@ -260,10 +373,11 @@ hipError_t launch_matmul_mx4(const MxArgs& a, hipStream_t st) {
   MxPlan p = mx4_gemm_plan(a.M, a.K, a.N, a.a_type, a.ws != nullptr);
   if (p.ws_bytes > a.ws_bytes) p = mx4_gemm_plan(a.M, a.K, a.N, a.a_type, false);
   if (p.t != 0) return launch_mx4_gemm(a, p, st);
+  if (use_dot(a.M, a.a_type)) return a.a_type == LT_F16 ? dot_for<LT_F16>(a, st) : dot_for<LT_BF16>(a, st);
   switch (a.a_type) {
-    case LT_F16: return rows_for<LT_F16, 1, 1>(a, st);
-    case LT_BF16: return rows_for<LT_BF16, 1, 1>(a, st);
-    default: return rows_for<-1, 1, 1>(a, st);
+    case LT_F16: return rows_for<LT_F16>(a, st);
+    case LT_BF16: return rows_for<LT_BF16>(a, st);
+    default: return rows_for<-1>(a, st);
   }
 }
 

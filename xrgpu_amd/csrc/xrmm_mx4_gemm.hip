@@ -21,6 +21,8 @@ int device_cus();
 
 namespace {
 
+constexpr int MXG_AHEAD = 2;  // K steps that loads run ahead (four: 26.6 for 26.7 us at 37 x 14336 x 4096)
+
 template <int AT, int WM, int TM, int TN>
 struct MxTile {
   static constexpr bool MX = AT < 0;
@@ -41,6 +43,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   typedef MxTile<AT, WM, TM, TN> Ti;
   constexpr bool MX = Ti::MX;
   constexpr int T = Ti::T, RA = Ti::RA, RB = Ti::RB, NA = RA * 8 / T, NB = MX ? RB * 8 / T : (2 * RB + T - 1) / T;
+  constexpr int D = MXG_AHEAD;
+  constexpr bool ONE = TN > 2;  // one set of pieces: see part
   constexpr int NS = MX ? (RA + RB + T - 1) / T : NB, TR = T / 8;  // TR: rows that the threads cover with one piece each
   typedef typename MxFrag<AT>::t half8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -51,7 +55,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   const uint32_t kb = static_cast<uint32_t>(a.kb), K = static_cast<uint32_t>(a.K);
   const uint32_t rowsA = static_cast<uint32_t>(a.M - m0 < RA ? a.M - m0 : RA);
   const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < RB ? a.N - n0 : RB);
-  const uint32_t s0 = split * g.per, s1 = s0 + g.per;  // an even number of steps
+  const uint32_t s0 = split * g.per, s1 = s0 + g.per;  // a multiple of D steps
   // the split's end along K, in blocks and values: what lies past it loads as zeros
   const uint32_t kbe = s1 * Ti::BLOCKS < kb ? s1 * Ti::BLOCKS : kb, Ke = kbe * MX_BLOCK < K ? kbe * MX_BLOCK : K;
 
@@ -81,16 +85,18 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   }
 
   // ---- staging registers
-  struct Wide {           // loaded at a step's start for the step after the next: two sets
-    u32x4 b[MX ? 1 : NB];
+  struct Set {
+    u32x4 b[NB];  // 16-bit activations: blocks of weights; MX4: pieces
     uint32_t s[NS][MX ? 3 : 1];
+    u32x4 a[ONE ? 1 : NA];
+    uint32_t x[ONE || AL ? 1 : NA];
   };
-  u32x4 ra[NA], rb[MX ? NB : 1];
-  uint32_t rx[AL ? 1 : NA];
+  u32x4 oa[NA], ob[NB];
+  uint32_t ox[AL ? 1 : NA];
   bool misfit = false;
 
   const uint32_t srow = static_cast<uint32_t>(tid >> 3), spiece = static_cast<uint32_t>((tid & 7) ^ (srow & 7u));
-  auto load_a = [&](int i, uint32_t s) {
+  auto load_a = [&](int i, uint32_t s, u32x4* ra, uint32_t* rx) {
     const uint32_t r = srow + TR * i;
     if constexpr (MX) {
       const uint32_t b = s * 8u + spiece;
@@ -107,11 +113,18 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
       }
     }
   };
-  auto load_b = [&](int i, uint32_t s) {  // MX4 operands
+  auto load_b = [&](int i, uint32_t s, u32x4* rb) {  // MX4 operands
     const uint32_t r = srow + TR * i, b = s * 8u + spiece;
-    rb[MX ? i : 0] = bld16(rB, (r < rowsB && b < kbe) ? r * rowB + b * MX_BLOB : MX_OOB, 0);
+    rb[i] = bld16(rB, (r < rowsB && b < kbe) ? r * rowB + b * MX_BLOB : MX_OOB, 0);
   };
-  auto load_wide = [&](Wide& w, uint32_t s) {
+  auto load_set = [&](Set& w, uint32_t s) {
+    if constexpr (!ONE) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) load_a(i, s, w.a, w.x);
+      if constexpr (MX)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) load_b(i, s, w.b);
+    }
     if constexpr (MX) {
       // eight scale bytes a row: three dwords
 #pragma unroll
@@ -125,24 +138,24 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
       for (int i = 0; i < NB; ++i) {
         const uint32_t c = static_cast<uint32_t>(tid + T * i), r = c >> 1, b = s * 2u + (c & 1u);
         const bool ok = r < rowsB && b < kbe && c < 2u * RB;
-        w.b[MX ? 0 : i] = bld16(rB, ok ? r * rowB + b * MX_BLOB : MX_OOB, 0);
+        w.b[i] = bld16(rB, ok ? r * rowB + b * MX_BLOB : MX_OOB, 0);
         w.s[i][0] = bld_u8(rS[i], b < kbe ? sbase[i] + s * 2u : MX_OOB, 0);
       }
     }
   };
-  // Quarter d of the pieces of step s to LDS stage `st`, and each piece's load for step s + 1
-  auto part = [&](int d, uint32_t s, int st, const Wide& w) {
+  // Quarter d of the pieces of step s to LDS stage `st`; with one set of pieces, each piece's load for step s + 1
+  auto part = [&](int d, uint32_t s, int st, const Set& w) {
     unsigned char* base = smem + st * Ti::STAGE;
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       if (i * 4 / NA != d) continue;
-      u32x4 v = ra[i];
+      u32x4 v = ONE ? oa[i] : w.a[ONE ? 0 : i];
       if constexpr (!MX && !AL) {
         const uint32_t k = s * 64u + spiece * 8u, r = srow + TR * i;
         const uint32_t sh = (r * rowA + k * 2u + misA) & 3u;
         const u32x4 x = v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(e < 3 ? x[e + 1] : rx[AL ? 0 : i], x[e], sh);
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(e < 3 ? x[e + 1] : ONE ? ox[AL ? 0 : i] : w.x[ONE || AL ? 0 : i], x[e], sh);
         if (k + 8u > K) {  // the row's last piece: what lies past it is the next row's
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -152,14 +165,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
         }
       }
       *reinterpret_cast<u32x4*>(base + (srow + TR * i) * 128 + (tid & 7) * 16) = v;
-      load_a(i, s + 1);
+      if (ONE) load_a(i, s + 1, oa, ox);
     }
     if constexpr (MX) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         if (i * 4 / NB != d) continue;
-        *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = rb[MX ? i : 0];
-        load_b(i, s + 1);
+        *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = ONE ? ob[i] : w.b[i];
+        if (ONE) load_b(i, s + 1, ob);
       }
       if (d == 0) {
         const uint32_t b0 = s * 8u, n = b0 < kbe ? kbe - b0 : 0u;  // scales of blocks past K are 2^-127 on both sides: products of 0
@@ -178,7 +191,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int c = tid + T * i, r = c >> 1;
-        const u32x4 wb = w.b[MX ? 0 : i];
+        const u32x4 wb = w.b[i];
         if (AT == LT_F16 && d == 0) misfit |= !mx_f16_fits(w.s[i][0], wb);
         if (NB * T == 2 * RB || c < 2 * RB)
           *reinterpret_cast<half8*>(base + (RA + r) * 128 + ((((c & 1) * 4 + d) ^ (r & 7)) * 16)) = mx_dq8<AT>(wb[d], e8m0(w.s[i][0]));
@@ -195,12 +208,12 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
       for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
 
   // ---- fragments: lane (r, h) = (lane % 32, lane / 32) reads piece 2 kk + h of row r
-  constexpr bool TWO = !(MX && WM == 4);  // fragments of the next slice beside the current one's; else two waves a SIMD cover the reads
+
   u32x4 fa[2][TM], fb[2][TN];
   u32x2 ta[MX ? TM : 1], tb[MX ? TN : 1];  // scales of the step, moved so that byte 2 kk is this half's
   const int fr = lane & 31, fh = lane >> 5;
   auto read = [&](int st, int kk) {
-    const int buf = TWO ? kk & 1 : 0;
+    const int buf = kk & 1;
     const unsigned char* base = smem + st * Ti::STAGE + (((2 * kk + fh) ^ (fr & 7)) * 16) + fr * 128;
 #pragma unroll
     for (int i = 0; i < TM; ++i) fa[buf][i] = *reinterpret_cast<const u32x4*>(base + (wm * TM + i) * 4096);
@@ -223,7 +236,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     }
   };
   auto mfmas = [&](auto kkc) {
-    constexpr int kk = decltype(kkc)::value, buf = TWO ? kk & 1 : 0;
+    constexpr int kk = decltype(kkc)::value, buf = kk & 1;
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -237,46 +250,42 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
           acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fb[buf][j]), __builtin_bit_cast(bf16x8, fa[buf][i]), acc[j][i], 0, 0, 0);
       }
   };
-  auto step = [&](uint32_t s, int st, Wide& nxt, Wide& fill) {
-    load_wide(fill, s + 2);
-    if (TWO) read(st, 1);
+  auto step = [&](uint32_t s, int st, Set& nxt, Set& fill) {
+    load_set(fill, s + D);
+    read(st, 1);
     part(0, s + 1, st ^ 1, nxt);
     mfmas(std::integral_constant<int, 0>{});
-    read(st, TWO ? 2 : 1);
+    read(st, 2);
     part(1, s + 1, st ^ 1, nxt);
     mfmas(std::integral_constant<int, 1>{});
-    read(st, TWO ? 3 : 2);
+    read(st, 3);
     part(2, s + 1, st ^ 1, nxt);
     part(3, s + 1, st ^ 1, nxt);
     mfmas(std::integral_constant<int, 2>{});
-    if (!TWO) {
-      read(st, 3);
-      mfmas(std::integral_constant<int, 3>{});
-    }
     __syncthreads();
     read(st ^ 1, 0);
-    if (TWO) mfmas(std::integral_constant<int, 3>{});
+    mfmas(std::integral_constant<int, 3>{});
     read_scales(st ^ 1);
   };
 
-  {
-    Wide w0, w1;
+  Set w[D];
+  if constexpr (ONE) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) load_a(i, s0);
+    for (int i = 0; i < NA; ++i) load_a(i, s0, oa, ox);
     if constexpr (MX)
 #pragma unroll
-      for (int i = 0; i < NB; ++i) load_b(i, s0);
-    load_wide(w0, s0);
-    load_wide(w1, s0 + 1);
+      for (int i = 0; i < NB; ++i) load_b(i, s0, ob);
+  }
 #pragma unroll
-    for (int d = 0; d < 4; ++d) part(d, s0, 0, w0);
-    __syncthreads();
-    read(0, 0);
-    read_scales(0);
-    for (uint32_t s = s0; s < s1; s += 2) {
-      step(s, 0, w1, w0);
-      step(s + 1, 1, w0, w1);
-    }
+  for (int i = 0; i < D; ++i) load_set(w[i], s0 + i);
+#pragma unroll
+  for (int d = 0; d < 4; ++d) part(d, s0, 0, w[0]);
+  __syncthreads();
+  read(0, 0);
+  read_scales(0);
+  for (uint32_t s = s0; s < s1; s += D) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) step(s + i, i & 1, w[(i + 1) % D], w[i]);
   }
 
   if constexpr (AT == LT_F16) {
@@ -317,96 +326,114 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     }
   }
 
-  if (g.splits > 1) {
-    // The splits' float32 parts meet in the workspace: coherent stores (sc0 sc1), one relaxed arrival count a
-    // workgroup, and the last one adds them in split order.
-    constexpr int COHERENT = 1 | 16;
-    constexpr uint32_t BYTES = RA * RB * 4;  // of a tile's part
-    __shared__ int s_last;
-    uint32_t* cnt = static_cast<uint32_t*>(a.ws);
-    const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + MX_COUNTERS + static_cast<int64_t>(tile) * g.splits * BYTES, g.splits * BYTES);
-    const uint32_t at = static_cast<uint32_t>(wave) * (TM * TN * 4096u) + lane * 16u;
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rW, split * BYTES + at + ((j * TM + i) * 4 + q) * 1024u, 0, COHERENT);
-        }
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (tid == 0) s_last = __hip_atomic_fetch_add(cnt + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.splits - 1;
-    __syncthreads();
-    if (!s_last) return;
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
-    for (uint32_t sp = 0; sp < g.splits; ++sp)
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const f32x4 v = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, sp * BYTES + at + ((j * TM + i) * 4 + q) * 1024u, 0, COHERENT));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][i][4 * q + e] += v[e];
-          }
-    if (tid == 0) __hip_atomic_store(cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-
-  // ---- output: 32 rows at a time through the wave's part of LDS, so that rows are written in whole pieces of 16 bytes
-  __syncthreads();
-  const int osz = a.out == LT_F32 ? 4 : 2;
-  const int pitch = 32 * TN * osz + 16;
-  unsigned char* strip = smem + wave * Ti::STRIP;
+  // ---- output: 32 rows at a time through the wave's part of LDS as float32, then in a loop of few instructions (a
+  // workgroup passes here once, and code that is fetched for one pass costs more than it does) eight columns a lane.
+  // Split K: the parts meet in the workspace as float32, with coherent stores (sc0 sc1) and one relaxed
+  // arrival count a workgroup; the last one adds them in split order.
+  constexpr int COHERENT = 1 | 16, PITCH = 32 * TN + 4, PPR = 4 * TN;  // values of a strip's row, pieces of eight
+  constexpr uint32_t BYTES = RA * RB * 4;
+  const rsrc_t rW = g.splits > 1 ? mk_rsrc(static_cast<uint8_t*>(a.ws) + MX_COUNTERS + static_cast<int64_t>(tile) * g.splits * BYTES, g.splits * BYTES)
+                                 : mk_rsrc(a.A, 0);
+  float* strip = reinterpret_cast<float*>(smem + wave * Ti::STRIP);
+  const uint32_t at = static_cast<uint32_t>(wave) * (TM * TN * 4096u);
   const int64_t nw = n0 + wn * 32 * TN, mw = m0 + wm * 32 * TM;
+  const int osz = a.out == LT_F32 ? 4 : 2;
   const bool vec = (a.N * osz & 15) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 15u) == 0;
-  const int per = 16 / osz, ppr = 32 * TN / per;  // values of a piece, pieces of a strip's row
+  auto finish = [&](int r, int p, float (&v)[8]) {  // eight values of row r of the wave's rows, from column 8 p on
+    const int64_t m = mw + r, n = nw + 8 * p;
+    if (m >= a.M || n >= a.N) return;
+    const int left = a.N - n < 8 ? static_cast<int>(a.N - n) : 8;
+    if (a.bias != nullptr) {
+      if (a.out == LT_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += static_cast<const float*>(a.bias)[e < left ? n + e : n];
+      } else {
+        uint16_t b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = static_cast<const uint16_t*>(a.bias)[e < left ? n + e : n];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          v[e] += a.out == LT_F16 ? static_cast<float>(__builtin_bit_cast(f16, b[e])) : static_cast<float>(__builtin_bit_cast(bf16, b[e]));
+      }
+    }
+    const int64_t o = m * a.N + n;
+    if (a.out == LT_F32) {
+      float* y = static_cast<float*>(a.Y) + o;
+      if (vec) {
+        *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
+        if (left > 4) *reinterpret_cast<f32x4*>(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        return;
+      }
+    } else if (vec && left == 8) {
+      u32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = a.out == LT_F16 ? __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(v[2 * e]), static_cast<f16>(v[2 * e + 1])})
+                               : __builtin_bit_cast(uint32_t, bf16x2{static_cast<bf16>(v[2 * e]), static_cast<bf16>(v[2 * e + 1])});
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.Y) + o) = x;
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) st_lt(a.Y, o + e, v[e], a.out);
+  };
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * j + 8 * q + 4 * fh;
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = acc[j][i][4 * q + e];
-          if (a.bias != nullptr && nw + c + e < a.N) v[e] += ld_lt(a.bias, nw + c + e, a.out);
-        }
-        unsigned char* at = strip + fr * pitch + c * osz;
-        if (a.out == LT_F32) *reinterpret_cast<f32x4*>(at) = v;
-        else if (a.out == LT_F16) *reinterpret_cast<f16x4*>(at) = f16x4{static_cast<f16>(v[0]), static_cast<f16>(v[1]), static_cast<f16>(v[2]), static_cast<f16>(v[3])};
-        else *reinterpret_cast<bf16x4*>(at) = bf16x4{static_cast<bf16>(v[0]), static_cast<bf16>(v[1]), static_cast<bf16>(v[2]), static_cast<bf16>(v[3])};
-      }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(strip + fr * PITCH + 32 * j + 8 * q + 4 * fh) =
+            f32x4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    for (int x = lane; x < 32 * ppr; x += 64) {
-      const int r = x / ppr, p = x % ppr;
-      const int64_t m = mw + 32 * i + r, n = nw + p * per;
-      if (m >= a.M || n >= a.N) continue;
-      const unsigned char* src = strip + r * pitch + p * 16;
-      unsigned char* dst = static_cast<unsigned char*>(a.Y) + (m * a.N + n) * osz;
-      if (vec) {
-        *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
-      } else if (osz == 4) {
-        for (int e = 0; e < 4 && n + e < a.N; ++e) reinterpret_cast<uint32_t*>(dst)[e] = reinterpret_cast<const uint32_t*>(src)[e];
+#pragma unroll 1
+    for (int x = lane; x < 32 * PPR; x += 64) {
+      const int r = x / PPR, p = x % PPR;
+      const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + 8 * p), hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + 8 * p + 4);
+      if (g.splits > 1) {
+        const uint32_t o = split * BYTES + at + (static_cast<uint32_t>(i) * 32 * PPR + x) * 32u;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rW, o, 0, COHERENT);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rW, o + 16, 0, COHERENT);
       } else {
-        for (int e = 0; e < 8 && n + e < a.N; ++e) reinterpret_cast<uint16_t*>(dst)[e] = reinterpret_cast<const uint16_t*>(src)[e];
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        finish(32 * i + r, p, v);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   }
+  if (g.splits == 1) return;
+  __shared__ int s_last;
+  uint32_t* cnt = static_cast<uint32_t*>(a.ws);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) s_last = __hip_atomic_fetch_add(cnt + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.splits - 1;
+  __syncthreads();
+  if (!s_last) return;
+#pragma unroll 1
+  for (int x = lane; x < TM * 32 * PPR; x += 64) {
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll 1
+    for (uint32_t s4 = 0; s4 < g.splits; s4 += 4) {  // four splits' loads in flight; past the last one zeros
+      f32x4 pl[4], ph[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t o = s4 + i < g.splits ? (s4 + i) * BYTES + at + x * 32u : MX_OOB;
+        pl[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, COHERENT));
+        ph[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, 0, COHERENT));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo += pl[i];
+        hi += ph[i];
+      }
+    }
+    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    finish(x / PPR, x % PPR, v);
+  }
+  if (tid == 0) __hip_atomic_store(cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // Tile l of a raster in groups of four row tiles, row fastest inside a group: the tiles that one XCD
@@ -419,7 +446,7 @@ __device__ __forceinline__ void mx_raster(uint32_t l, uint32_t mt, uint32_t nc, 
 }
 
 template <int AT, int WM, int TM, int TN, bool AL>
-__global__ __launch_bounds__(128 * WM, TM == 1 ? 4 : 2) void k_mx4_gemm(MxArgs a, MxGrid g) {
+__global__ __launch_bounds__(128 * WM, TM == 1 ? 3 : 2) void k_mx4_gemm(MxArgs a, MxGrid g) {
   uint32_t row, col;
   const uint32_t bid = blockIdx.x;
   if (TN < 4 || bid < g.nbig) {
@@ -465,46 +492,65 @@ hipError_t gemm_at(const MxArgs& a, const MxPlan& p, hipStream_t st) {
 
 }  // namespace
 
+// The plan with the least estimated time. A tile size costs a CU so much for a K step: what one workgroup alone takes,
+// or the work of all its workgroups at the rate of a full CU (units of 64 x 64; us measured at 2.4 GHz):
+//   16-bit activations, steps of 64:  64-tiles 0.45, 3.3 units a us; 128-tiles 0.75, 6; 256-tiles 1.8, 8.9
+//   both MX4, steps of 256:           64-tiles 0.60, 2.7 units a us; 128-tiles 1.0, 5.1; 256-tiles 2.1, 7
+// and a start of 3, 5 or 12 us; a split exchange costs 5 us and what its parts weigh. It places 512 x 4096 x 4096 on 64- or 128-tiles
+// (35 to 42 us; 256-tiles 55), 128 rows on 64-tiles with K split (17; 128-tiles 24), the prefills on 256-tiles (237; 128-tiles 281).
 MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) {
-  MxPlan p{};
+  MxPlan best{};
+  const bool mx = a_type < 0;
   const int64_t kb = (K + MX_BLOCK - 1) / MX_BLOCK;
-  if (M <= 16 || K > (int64_t(1) << 21)) return p;  // 256 rows of 16-bit values stay below 2^31 bytes
+  if (M <= 16 || K > (int64_t(1) << 21)) return best;  // 256 rows of 16-bit values stay below 2^31 bytes
   const int64_t cus = device_cus() > 0 ? device_cus() : 256;
-  const int64_t steps = (kb + (a_type < 0 ? 7 : 1)) / (a_type < 0 ? 8 : 2);
-  auto tiles = [&](int64_t t) { return ((M + 64 * t - 1) / (64 * t)) * ((N + 64 * t - 1) / (64 * t)); };
-  int t = tiles(4) >= cus ? 4 : tiles(2) >= cus ? 2 : 1;
-  p.t = t;
-  p.mt = static_cast<uint32_t>((M + 64 * t - 1) / (64 * t));
-  p.nb = static_cast<uint32_t>((N + 64 * t - 1) / (64 * t));
-  p.splits = 1;
-  p.per = static_cast<uint32_t>((steps + 1) / 2 * 2);
-  if (t == 4 && static_cast<int64_t>(p.mt) * p.nb > cus && cus % p.mt == 0) {
-    // wide and narrow (192) columns mixed, where that makes fewer rounds of the CUs
-    const int64_t per = cus / p.mt;
-    double best = static_cast<double>((static_cast<int64_t>(p.mt) * p.nb + cus - 1) / cus);
-    for (int64_t j = 1; j <= 16; ++j) {
-      const int64_t rest = N - 192 * j * per, k = rest > 0 ? (rest + 256 * per - 1) / (256 * per) : 0;
-      const double time = static_cast<double>(k) + 0.75 * static_cast<double>(j);
-      if (time < best - 0.05) {
-        best = time;
-        p.nb = static_cast<uint32_t>(k * per);
-        p.ns = static_cast<uint32_t>(j * per);
+  const int64_t steps = (kb + (mx ? 7 : 1)) / (mx ? 8 : 2);
+  struct Cost {
+    int t;
+    double alone, rate, start;
+  };
+  static constexpr Cost kCost[2][3] = {{{1, 0.45, 3.3, 3}, {2, 0.75, 6.0, 5}, {4, 1.8, 8.9, 12}},
+                                       {{1, 0.60, 2.7, 3}, {2, 1.0, 5.1, 5}, {4, 2.1, 7.0, 12}}};
+  double least = 0;
+  for (const Cost& c : kCost[mx ? 1 : 0]) {
+    const int64_t mt = (M + 64 * c.t - 1) / (64 * c.t), nt = (N + 64 * c.t - 1) / (64 * c.t), n = mt * nt;
+    if (n > 0x3FFFFFFF) continue;
+    for (int64_t s = 1; s <= 8; ++s) {
+      if (s > 1 && (!have_ws || n > MX_COUNTERS / 4 || n * s > 2 * cus || steps < 4 * s)) break;
+      MxPlan p{};
+      p.t = c.t;
+      p.mt = static_cast<uint32_t>(mt);
+      p.nb = static_cast<uint32_t>(nt);
+      p.per = static_cast<uint32_t>((steps + MXG_AHEAD * s - 1) / (MXG_AHEAD * s) * MXG_AHEAD);
+      p.splits = static_cast<uint32_t>((steps + p.per - 1) / p.per);
+      if (p.splits != s) continue;
+      double rounds = static_cast<double>((n * s + cus - 1) / cus);  // tiles of the fullest CU
+      if (c.t == 4 && s == 1 && rounds > 1 && cus % mt == 0) {
+        // columns of wide tiles and narrow ones (192) mixed, where that makes fewer rounds of the CUs
+        const int64_t per = cus / mt;
+        for (int64_t j = 1; j <= 16; ++j) {
+          const int64_t rest = N - 192 * j * per, k = rest > 0 ? (rest + 256 * per - 1) / (256 * per) : 0;
+          const double r = static_cast<double>(k) + 0.75 * static_cast<double>(j);
+          if (r < rounds - 0.05) {
+            rounds = r;
+            p.nb = static_cast<uint32_t>(k * per);
+            p.ns = static_cast<uint32_t>(j * per);
+          }
+        }
+      }
+      const double units = static_cast<double>(c.t * c.t), step = units * rounds / c.rate;
+      double time = c.start * (c.t == 4 ? rounds : 1.0) + static_cast<double>(p.per) * (step > c.alone ? step : c.alone);
+      if (s > 1) {
+        p.ws_bytes = MX_COUNTERS + n * s * c.t * c.t * 16384;
+        time += 5.0 + static_cast<double>(p.ws_bytes) * 0.5e-6;  // written and read back at about 4 TB/s
+      }
+      if (best.t == 0 || time < least) {
+        best = p;
+        least = time;
       }
     }
   }
-  int64_t splits = 1;
-  const int64_t n = static_cast<int64_t>(p.mt) * p.nb;
-  if (have_ws && p.ns == 0 && n * 2 <= cus && n <= MX_COUNTERS / 4) {
-    splits = cus / n;
-    splits = splits < 8 ? splits : 8;
-    splits = splits < steps / 4 ? splits : steps / 4;
-  }
-  if (splits > 1) {
-    p.per = static_cast<uint32_t>((steps + 2 * splits - 1) / (2 * splits) * 2);
-    p.splits = static_cast<uint32_t>((steps + p.per - 1) / p.per);
-    p.ws_bytes = MX_COUNTERS + n * p.splits * t * t * 16384;
-  }
-  return p;
+  return best;
 }
 
 hipError_t launch_mx4_gemm(const MxArgs& a, const MxPlan& p, hipStream_t st) {
