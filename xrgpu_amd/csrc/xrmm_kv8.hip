@@ -1,7 +1,12 @@
 // The 8-bit paged cache: appending tokens, and attention over it.
+#include <atomic>
+
 #include "xrmm_lowbit.h"
 
 namespace xrmm {
+
+int device_cus();
+
 namespace {
 
 // ---------------------------------------------------------------------------
@@ -40,7 +45,6 @@ __device__ __forceinline__ uint32_t kv_code4(float a, float b, float c, float d)
 template <bool FP8>
 __device__ __forceinline__ void kv_value4(uint32_t x, float (&v)[4]) {
   if constexpr (FP8) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
     const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x), false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(x), true);
     v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
   } else {
@@ -220,51 +224,104 @@ __device__ __forceinline__ KvBytes<N> kv_bytes(const uint8_t* p) {
   return r;
 }
 
-constexpr int KVR_WAVES = 4;
+// Few rows: the cache's bytes bound the call. A workgroup takes 16 rows of one sequence and key head and `chunk`
+// tokens; its waves take turns at steps of 32 tokens, with the next step's codes in flight and the
+// page after that looked up. Workgroups of one (sequence, head, rows) leave their
+// unnormalised outputs, maxima and sums in the workspace, and the last to arrive joins them in
+// token order.
+constexpr int KVR_WAVES = 8;
+constexpr int KVR_PASS = KVR_WAVES * KVT;  // tokens of a step of all waves
+constexpr int64_t KV_COUNTERS = 4096;      // bytes of arrival counters at the head of the workspace
 
-template <int D, bool FP8, int NT>
-__global__ __launch_bounds__(64 * KVR_WAVES) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles) {
+template <int D>
+constexpr int64_t kv_part_bytes() { return 16 * (D + 2) * 4; }  // [16][D] outputs, [16] (maximum, sum)
+
+template <int D>
+struct KvStep {
+  int32_t pg[2];  // the two 16-token tiles lie in one page each
+  float ks[2], vs[2];
+  KvBytes<D / 4> k[2];
+  KvBytes<D / 16> v[8];
+};
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
   constexpr int KD = D / 4, VD = D / 16;  // codes of a token that a lane holds
   const KvCache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  uint32_t id = blockIdx.x;
-  const int tile = static_cast<int>(id % row_tiles);
-  id /= row_tiles;
-  const int h = static_cast<int>(id % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(id / static_cast<uint32_t>(c.Hkv));
+  const uint32_t split = blockIdx.x % splits, unit = blockIdx.x / splits;
+  const int tile = static_cast<int>(unit % row_tiles);
+  const uint32_t bh = unit / row_tiles;
+  const int h = static_cast<int>(bh % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(bh / static_cast<uint32_t>(c.Hkv));
   const int G = a.Hq / c.Hkv;
   int first, count;
   if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
-  const int nrows = count * G, r0 = tile * 16 * NT;
+  const int nrows = count * G, r0 = tile * 16;
   if (r0 >= nrows) return;
   // positions past the table are left out: the walk over tokens ends with the table
   const int span = c.width << c.page_log2, all = c.lengths[b], past = all - count;
   const int len = all < 0 ? 0 : all < span ? all : span;
   if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
-  // this lane's rows: their queries as binary16 (scaled by a power of two for bfloat16), what they see
-  f16x8 q[NT][KD / 8];
-  float qs[NT];  // the factor of a score
-  int lo[NT], hi[NT];
+  // the tokens that any of the rows sees, and those that all of them see
+  const int last = r0 + 16 < nrows ? r0 + 15 : nrows - 1, i0 = r0 / G, i1 = last / G;
+  auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
+  auto row_lo = [&](int i) { return a.window > 0 && past + i - a.window + 1 > 0 ? past + i - a.window + 1 : 0; };
+  const int lo_all = row_lo(i0) / KVT * KVT, hi_all = row_hi(i1), full_lo = row_lo(i1), full_hi = row_hi(i0);
+  const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;  // at most `splits`
+  if (split >= parts) return;
+  const int tlo = lo_all + static_cast<int>(split * chunk);
+  const int thi = splits > 1 && split + 1 < parts ? tlo + static_cast<int>(chunk) : hi_all;
+
+  auto find = [&](int t0, int32_t (&pg)[2]) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int r = r0 + 16 * t + col;
+    for (int u = 0; u < 2; ++u) {
+      const int32_t p = kv_page(c, b, t0 + 16 * u);
+      pg[u] = t0 + 16 * u < thi ? p : -2;
+    }
+  };
+  auto load = [&](KvStep<D>& s, const int32_t (&pg)[2], int t0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = t0 + 16 * u;
+      s.pg[u] = pg[u];
+      const int64_t at = static_cast<int64_t>(pg[u] < 0 ? 0 : pg[u]) * c.Hkv + h;
+      s.ks[u] = c.ks[at];
+      s.vs[u] = c.vs[at];
+      const int64_t slot = (at * c.page + (t & (c.page - 1))) * D;
+      s.k[u] = kv_bytes<KD>(c.k + slot + col * D + g * KD);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s.v[4 * u + x] = kv_bytes<VD>(c.v + slot + (4 * g + x) * D + col * VD);
+    }
+  };
+  int32_t pg[2];
+  KvStep<D> cur;
+  find(tlo + wave * KVT, pg);
+  load(cur, pg, tlo + wave * KVT);
+  find(tlo + wave * KVT + KVR_PASS, pg);
+
+  // this lane's row: its query as binary16 (scaled by a power of two for bfloat16), what it sees
+  f16x8 q[KD / 8];
+  float qs = a.scale * 1.44269504088896340736f;  // the factor of a score
+  int lo, hi;
+  {
+    const int r = r0 + col;
     const bool ok = r < nrows;
     const int i = ok ? r / G : 0, hq = h * G + (ok ? r % G : 0);
     const int64_t at = (first + i) * a.q_stride + static_cast<int64_t>(hq) * D + g * KD;
-    const int p = past + i;
-    hi[t] = !ok ? 0 : a.causal && p + 1 < len ? p + 1 : len;
-    lo[t] = a.window > 0 && p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-    qs[t] = a.scale * 1.44269504088896340736f;
+    hi = ok ? row_hi(i) : 0;
+    lo = row_lo(i);
     if (a.dtype == LT_F16) {
 #pragma unroll
-      for (int e = 0; e < KD; ++e) q[t][e / 8][e % 8] = ok ? static_cast<const f16*>(a.q)[at + e] : static_cast<f16>(0.f);
+      for (int e = 0; e < KD; ++e) q[e / 8][e % 8] = ok ? static_cast<const f16*>(a.q)[at + e] : static_cast<f16>(0.f);
     } else {
       float v[KD];
+#pragma unroll
+      for (int e = 0; e < KD; ++e) v[e] = ok ? static_cast<float>(static_cast<const bf16*>(a.q)[at + e]) : 0.f;
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < KD; ++e) {
-        v[e] = ok ? static_cast<float>(static_cast<const bf16*>(a.q)[at + e]) : 0.f;
         const uint32_t m = __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu;
         top = top > m ? top : m;
       }
@@ -278,207 +335,745 @@ __global__ __launch_bounds__(64 * KVR_WAVES) void k_kv8_rows(KvAttnArgs a, uint3
       if (top >= 0x7F800000u || top < 0x00800000u) e2 = 0;
       const float s1 = two(-(e2 / 2)), s2 = two(-(e2 - e2 / 2));
 #pragma unroll
-      for (int e = 0; e < KD; ++e) q[t][e / 8][e % 8] = static_cast<f16>(v[e] * s1 * s2);
-      qs[t] = qs[t] * two(e2 / 2) * two(e2 - e2 / 2);
+      for (int e = 0; e < KD; ++e) q[e / 8][e % 8] = static_cast<f16>(v[e] * s1 * s2);
+      qs = qs * two(e2 / 2) * two(e2 - e2 / 2);
     }
   }
-  // the tokens that any of the rows sees, and those that all of them see
-  const int i0 = r0 / G, i1 = (r0 + 16 * NT < nrows ? r0 + 16 * NT - 1 : nrows - 1) / G;
-  auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
-  auto row_lo = [&](int i) { return a.window > 0 && past + i - a.window + 1 > 0 ? past + i - a.window + 1 : 0; };
-  const int tlo = row_lo(i0) / KVT * KVT, thi = row_hi(i1), full_lo = row_lo(i1), full_hi = row_hi(i0);
 
-  f32x4 o[NT][VD];
-  float m[NT], l[NT];
+  f32x4 o[VD];
+  float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    m[t] = -__builtin_inff();
-    l[t] = 0.f;
-#pragma unroll
-    for (int j = 0; j < VD; ++j) o[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int j = 0; j < VD; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float vref = 0.f;  // the value scale that the sums are in units of
   bool bad = false;
 
-  for (int t0 = tlo + wave * KVT; t0 < thi; t0 += KVR_WAVES * KVT) {
-    // the two 16-token tiles lie in one page each
-    int32_t pg[2];
-    float ks[2], vs[2];
-    const uint8_t *kp[2], *vp[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = t0 + 16 * u;
-      pg[u] = t < thi ? kv_page(c, b, t) : -2;
-      bad |= pg[u] == -1;
-      const int64_t at = static_cast<int64_t>(pg[u] < 0 ? 0 : pg[u]) * c.Hkv + h;
-      ks[u] = c.ks[at];
-      vs[u] = c.vs[at];
-      const int64_t slot = at * c.page + (t & (c.page - 1));
-      kp[u] = c.k + slot * D;
-      vp[u] = c.v + slot * D;
-    }
+#pragma unroll 1
+  for (int t0 = tlo + wave * KVT; t0 < thi; t0 += KVR_PASS) {
+    KvStep<D> nxt;
+    load(nxt, pg, t0 + KVR_PASS);
+    find(t0 + 2 * KVR_PASS, pg);
+    bad |= cur.pg[0] == -1 || cur.pg[1] == -1;
     // scores
-    f32x4 s[NT][2];
+    f32x4 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const KvBytes<KD> kc = kv_bytes<KD>(kp[u] + col * D + g * KD);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int x = 0; x < KD / 8; ++x) {
-        const f16x8 kf = cat8(kv_half4<FP8>(kc.w[2 * x]), kv_half4<FP8>(kc.w[2 * x + 1]));
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[t][x], s[t][u], 0, 0, 0);
+        const f16x8 kf = cat8(kv_half4<FP8>(cur.k[u].w[2 * x]), kv_half4<FP8>(cur.k[u].w[2 * x + 1]));
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[x], s[u], 0, 0, 0);
       }
     }
     // a page's value scale above all before it: the sums go into its units
+    const float ref = vref;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (pg[u] >= 0 && vs[u] > vref && vs[u] <= 3.4028235e38f) {
-        const float f = vref / vs[u];
-        vref = vs[u];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int j = 0; j < VD; ++j) o[t][j] *= f;
-      }
+      if (cur.pg[u] >= 0 && cur.vs[u] > vref && cur.vs[u] <= 3.4028235e38f) vref = cur.vs[u];
     const float inv = vref > 0.f ? 1.f / vref : 0.f;
-    const bool masked = t0 < full_lo || t0 + KVT > full_hi || pg[0] < 0 || pg[1] < 0;
-    f16x8 pf[NT];
+    const bool masked = t0 < full_lo || t0 + KVT > full_hi || cur.pg[0] < 0 || cur.pg[1] < 0;
+    float top = -__builtin_inff();
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float top = -__builtin_inff();
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = s[t][u][e] * (qs[t] * ks[u]);
-          if (masked) {
-            const int tok = t0 + 16 * u + 4 * g + e;
-            if (pg[u] < 0 || tok < lo[t] || tok >= hi[t]) v = -__builtin_inff();
-          }
-          s[t][u][e] = v;
-          top = fmaxf(top, v);
+      for (int e = 0; e < 4; ++e) {
+        float v = s[u][e] * (qs * cur.ks[u]);
+        if (masked) {
+          const int tok = t0 + 16 * u + 4 * g + e;
+          if (cur.pg[u] < 0 || tok < lo || tok >= hi) v = -__builtin_inff();
         }
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m[t], top);
-      const float base = mn == -__builtin_inff() ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m[t] - base);
-      m[t] = mn;
-      l[t] *= f;
+        s[u][e] = v;
+        top = fmaxf(top, v);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - base);
+    m = mn;
+    l *= f;
+    const float fo = ref < vref ? f * (ref / vref) : f;
 #pragma unroll
-      for (int j = 0; j < VD; ++j) o[t][j] *= f;
+    for (int j = 0; j < VD; ++j) o[j] *= fo;
+    f16x8 pf;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float w = vs[u] * inv * KV_P;
+    for (int u = 0; u < 2; ++u) {
+      const float w = cur.vs[u] * inv * KV_P;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = s[t][u][e], p = __builtin_amdgcn_exp2f(v - base);
-          l[t] += p;
-          // a masked token's weight is 0 whatever its page's scale holds
-          pf[t][4 * u + e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float v = s[u][e], p = __builtin_amdgcn_exp2f(v - base);
+        l += p;
+        // a masked token's weight is 0 whatever its page's scale holds
+        pf[4 * u + e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
       }
     }
     // values
-    KvBytes<VD> vc[8];
+    if (masked) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      vc[x] = kv_bytes<VD>(vp[x >> 2] + (4 * g + (x & 3)) * D + col * VD);
-      if (masked && (pg[x >> 2] < 0 || t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= thi)) {
+      for (int x = 0; x < 8; ++x)
+        if (cur.pg[x >> 2] < 0 || t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= thi) {
 #pragma unroll
-        for (int y = 0; y < (VD + 3) / 4; ++y) vc[x].w[y] = 0u;  // no token: its codes may be anything
-      }
+          for (int y = 0; y < (VD + 3) / 4; ++y) cur.v[x].w[y] = 0u;  // no token: its codes may be anything
+        }
     }
 #pragma unroll
     for (int y = 0; y < (VD + 3) / 4; ++y) {
       // words of four d, eight tokens -> four fragments of eight tokens
       f16x4 t4[8];
 #pragma unroll
-      for (int x = 0; x < 8; ++x) t4[x] = kv_half4<FP8>(vc[x].w[y]);
+      for (int x = 0; x < 8; ++x) t4[x] = kv_half4<FP8>(cur.v[x].w[y]);
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         if (4 * y + z >= VD) break;
         const f16x8 vf = {t4[0][z], t4[1][z], t4[2][z], t4[3][z], t4[4][z], t4[5][z], t4[6][z], t4[7][z]};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][4 * y + z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[t], o[t][4 * y + z], 0, 0, 0);
+        o[4 * y + z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf, o[4 * y + z], 0, 0, 0);
       }
     }
+    cur = nxt;
   }
   if (bad && lane == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   // The waves' parts meet in LDS. Sums of rows: over the four lanes of a column, then the waves.
-  __shared__ float wm[KVR_WAVES][NT][16], wl[KVR_WAVES][NT][16];
-  __shared__ f32x4 red[KVR_WAVES][4][64];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    l[t] += __shfl_xor(l[t], 16, 64);
-    l[t] += __shfl_xor(l[t], 32, 64);
-    if (g == 0) {
-      wm[wave][t][col] = m[t];
-      wl[wave][t][col] = l[t];
-    }
+  constexpr int JT = VD < 8 ? VD : 8;  // output tiles of a round
+  __shared__ float wm[KVR_WAVES][16], wl[KVR_WAVES][16];
+  __shared__ f32x4 red[KVR_WAVES][JT][64];
+  __shared__ float row[16][D];
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) {
+    wm[wave][col] = m;
+    wl[wave][col] = l;
   }
   __syncthreads();
+  float top = wm[0][col];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float top = wm[0][t][col];
+  for (int w = 1; w < KVR_WAVES; ++w) top = fmaxf(top, wm[w][col]);
+  const float base = top == -__builtin_inff() ? 0.f : top;
+  float sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < KVR_WAVES; ++w) top = fmaxf(top, wm[w][t][col]);
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    float sum = 0.f;
+  for (int w = 0; w < KVR_WAVES; ++w) sum += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - base);
+  const float mine = __builtin_amdgcn_exp2f(m - base) * vref * (1.f / KV_P);
 #pragma unroll
-    for (int w = 0; w < KVR_WAVES; ++w) sum += wl[w][t][col] * __builtin_amdgcn_exp2f(wm[w][t][col] - base);
-    const float mine = __builtin_amdgcn_exp2f(m[t] - base) * vref;
-    const float inv = sum != 0.f ? 1.f / (sum * KV_P) : 0.f;
-    const int r = r0 + 16 * t + col;
+  for (int j0 = 0; j0 < VD; j0 += JT) {
+    if (j0 > 0) __syncthreads();
 #pragma unroll
-    for (int j0 = 0; j0 < VD; j0 += 4) {
+    for (int j = 0; j < JT; ++j) red[wave][j][lane] = o[j0 + j] * mine;
+    __syncthreads();
+    if (wave < JT) {  // wave w finishes tile j0 + w
+      f32x4 v = red[0][wave][lane];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j0 + j < VD) red[wave][j][lane] = o[t][j0 + j] * mine;
-      __syncthreads();
-      // wave w finishes tile j0 + w
-      const int j = j0 + wave;
-      if (j < VD && r < nrows) {
-        f32x4 v = red[0][wave][lane];
+      for (int w = 1; w < KVR_WAVES; ++w) v += red[w][wave][lane];
 #pragma unroll
-        for (int w = 1; w < KVR_WAVES; ++w) v += red[w][wave][lane];
-        const int64_t at = (static_cast<int64_t>(first + r / G) * a.Hq + h * G + r % G) * D;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st_lt(a.o, at + VD * (4 * g + e) + j, v[e] * inv, a.dtype);
-      }
-      __syncthreads();
+      for (int e = 0; e < 4; ++e) row[col][VD * (4 * g + e) + j0 + wave] = v[e];
     }
+  }
+  // sums of this workgroup's tokens: the rows' outputs in `row`, maxima and sums where wave is 0 and g is 0
+  __shared__ float rm[16], rl[16];
+  if (tid < 16) {
+    rm[tid] = top;
+    rl[tid] = sum;
+  }
+  __syncthreads();
+  const int rows = nrows - r0 < 16 ? nrows - r0 : 16, pieces = rows * (D / 4);  // pieces of four values
+  auto put = [&](int p, f32x4 v, float lsum) {
+    const int r = r0 + p / (D / 4);
+    const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+    const int64_t at = (static_cast<int64_t>(first + r / G) * a.Hq + h * G + r % G) * D + p % (D / 4) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) st_lt(a.o, at + e, v[e] * inv, a.dtype);
+  };
+  if (parts == 1) {
+#pragma unroll 1
+    for (int p = tid; p < pieces; p += 64 * KVR_WAVES) put(p, *reinterpret_cast<const f32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]), rl[p / (D / 4)]);
+    return;
+  }
+  constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
+  constexpr uint32_t PART = static_cast<uint32_t>(kv_part_bytes<D>());
+  __shared__ int s_last;
+  uint32_t* cnt = static_cast<uint32_t*>(a.ws);
+  const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + KV_COUNTERS + static_cast<int64_t>(unit) * splits * PART, splits * PART);
+#pragma unroll 1
+  for (int p = tid; p < pieces; p += 64 * KVR_WAVES)
+    __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]), rW, split * PART + p * 16, 0, COHERENT);
+  if (tid < rows) {
+    const u32x2 ml = {__builtin_bit_cast(uint32_t, rm[tid]), __builtin_bit_cast(uint32_t, rl[tid])};
+    __builtin_amdgcn_raw_buffer_store_b64(ml, rW, split * PART + 16 * D * 4 + tid * 8, 0, COHERENT);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) s_last = __hip_atomic_fetch_add(cnt + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+  __syncthreads();
+  if (!s_last) return;
+  if (tid == 0) __hip_atomic_store(cnt + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // The join: `groups` groups of threads take every groups-th part each, four parts' loads in flight, then meet in LDS.
+  const int groups = pieces < 64 * KVR_WAVES ? 64 * KVR_WAVES / pieces : 1;
+  f32x4* jo = &red[0][0][0];                                                 // [512]
+  float *jm = reinterpret_cast<float*>(jo + 64 * KVR_WAVES), *jl = jm + 64 * KVR_WAVES;  // [512] each
+  static_assert(sizeof(red) >= 64 * KVR_WAVES * 24, "the join fits the waves' sums");
+#pragma unroll 1
+  for (int p0 = 0; p0 < pieces; p0 += 64 * KVR_WAVES) {
+    const int p = p0 + (groups > 1 ? tid % pieces : tid), grp = groups > 1 ? tid / pieces : 0;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    float vm = -__builtin_inff(), vl = 0.f;
+    if (p < pieces && grp < groups) {
+#pragma unroll 1
+      for (uint32_t s = grp; s < parts; s += 4 * groups) {
+        u32x4 x[4];
+        f32x2 ml[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t at = s + i * groups < parts ? (s + i * groups) * PART : 0x80000000u;  // past the last: zeros
+          x[i] = __builtin_amdgcn_raw_buffer_load_b128(rW, at + p * 16, 0, COHERENT);
+          ml[i] = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rW, at + 16 * D * 4 + p / (D / 4) * 8, 0, COHERENT));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          if (s + i * groups >= parts) break;
+          const float pm = ml[i][0], mn = fmaxf(vm, pm), bs = mn == -__builtin_inff() ? 0.f : mn;
+          const float f0 = __builtin_amdgcn_exp2f(vm - bs), f1 = __builtin_amdgcn_exp2f(pm - bs);
+          v = v * f0 + __builtin_bit_cast(f32x4, x[i]) * f1;
+          vl = vl * f0 + ml[i][1] * f1;
+          vm = mn;
+        }
+      }
+    }
+    if (groups > 1) {
+      jo[tid] = v;
+      jm[tid] = vm;
+      jl[tid] = vl;
+      __syncthreads();
+      if (grp == 0) {
+        float bs = vm;
+        for (int k = 1; k < groups; ++k) bs = fmaxf(bs, jm[tid + k * pieces]);
+        bs = bs == -__builtin_inff() ? 0.f : bs;
+        v = f32x4{0.f, 0.f, 0.f, 0.f};
+        vl = 0.f;
+        for (int k = 0; k < groups; ++k) {
+          const float f = __builtin_amdgcn_exp2f(jm[tid + k * pieces] - bs);
+          v += jo[tid + k * pieces] * f;
+          vl += jl[tid + k * pieces] * f;
+        }
+      }
+    }
+    if (p < pieces && grp == 0) put(p, v, vl);
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: products bound the call. A workgroup takes 128 rows (32 a wave) of one sequence and key head and walks over
+// tiles of TT tokens: their codes become binary16 in LDS once for all rows, K as it lies (tokens by d), V transposed (d
+// by tokens, the tokens of a piece in the order in which the scores leave the MFMA). The sums are those
+// above with v_mfma_f32_32x32x16: a row's maximum, sum and factor belong to a lane, and P goes from one product
+// into the next without leaving its lane. Pieces of 16 bytes are swizzled by their row, so that neither the
+// fragments' rows nor the transposing stores meet in a bank.
+//
+// Two stages: while tile i computes, tile i + 1 goes from registers to LDS, tile i + 2 is loaded and the
+// pages of tile i + 3 are looked up. One barrier a tile.
+//
+// A row's maximum may lag by up to 2^KV_LAG: the outputs are rescaled only when some row of the wave outgrows that
+// (KV_P 2^KV_LAG stays inside binary16). Workgroups of one key head follow each other on one XCD's L2 where heads and
+// sequences make a multiple of eight; the rows that see the most tokens come first. Few workgroups
+// and long contexts: tokens are split and joined as above.
+constexpr int KVM_WAVES = 4, KVM_ROWS = 32 * KVM_WAVES, KVM_T = 64 * KVM_WAVES;
+constexpr float KV_LAG = 5.f;
+
+template <int D>
+struct KvTile {
+  static constexpr int TT = D > 128 ? 32 : 64;                     // tokens of a tile
+  static constexpr int KP = D <= 64 ? 128 : D <= 128 ? 256 : 512;  // bytes of a token's K, of a d's V
+  static constexpr int VP = TT * 2;
+  static constexpr int STAGE = TT * KP + D * VP;
+  static constexpr int KN = (TT * D / 16 + KVM_T - 1) / KVM_T, VN = (TT * D / 32 + KVM_T - 1) / KVM_T;  // pieces a thread moves
+  static constexpr int64_t PART = KVM_ROWS * (D + 2) * 4;
+};
+
+template <int D>
+__device__ __forceinline__ int kv_vslot(int d, int piece) {
+  return KvTile<D>::TT == 64 ? piece ^ ((d ^ (d >> 3)) & 7) : piece ^ (((d >> 1) ^ (d >> 3)) & 3);
+}
+
 template <int D, bool FP8>
-hipError_t rows_for(const KvAttnArgs& a, hipStream_t st) {
-  constexpr int NT = 1;
-  const int64_t G = a.Hq / a.c.Hkv, tiles = (a.max_new * G + 16 * NT - 1) / (16 * NT);
-  const int64_t grid = tiles * a.c.Hkv * a.c.B;
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
-  k_kv8_rows<D, FP8, NT><<<dim3(static_cast<uint32_t>(grid)), 64 * KVR_WAVES, 0, st>>>(a, static_cast<uint32_t>(tiles));
+__global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+  typedef KvTile<D> Ti;
+  constexpr int TT = Ti::TT, KN = Ti::KN, VN = Ti::VN, JT = D / 32, GR = TT / 16;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const KvCache& c = a.c;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hf = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t nbh = static_cast<uint32_t>(c.Hkv) * static_cast<uint32_t>(c.B), bh = blockIdx.x % nbh, rest = blockIdx.x / nbh;
+  const uint32_t split = rest % splits;
+  const int tile = static_cast<int>(row_tiles - 1 - rest / splits);
+  const uint32_t unit = bh * row_tiles + static_cast<uint32_t>(tile);
+  const int h = static_cast<int>(bh % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(bh / static_cast<uint32_t>(c.Hkv));
+  const int G = a.Hq / c.Hkv;
+  int first, count;
+  if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  const int nrows = count * G, r0 = tile * KVM_ROWS;
+  if (r0 >= nrows) return;
+  const int span = c.width << c.page_log2, all = c.lengths[b], past = all - count;
+  const int len = all < 0 ? 0 : all < span ? all : span;
+  if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
+  auto row_lo = [&](int i) { return a.window > 0 && past + i - a.window + 1 > 0 ? past + i - a.window + 1 : 0; };
+  auto query = [&](int r) { return (r < nrows ? r : nrows - 1) / G; };  // of a row, the last one's past the end
+  const int lo_all = row_lo(query(r0)) / TT * TT, hi_all = row_hi(query(r0 + KVM_ROWS - 1));
+  const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;
+  if (split >= parts) return;
+  const int tlo = lo_all + static_cast<int>(split * chunk);
+  const int thi = splits > 1 && split + 1 < parts ? tlo + static_cast<int>(chunk) : hi_all;
+  // this wave's rows: the tokens that any sees, and those that all see
+  const int w0 = r0 + 32 * wave;
+  const bool live = w0 < nrows;
+  const int wlo = row_lo(query(w0)), whi = live ? row_hi(query(w0 + 31)) : 0, full_lo = row_lo(query(w0 + 31)), full_hi = row_hi(query(w0));
+
+  // ---- moving a tile: K pieces of 16 codes of a token, V pieces of four tokens by eight d
+  // Everything of a tile is loaded together, from pages looked up a tile before: one for each 16 tokens.
+  uint32_t kc[KN][4], vc[VN][8];
+  float ksn[GR], vsn[GR];     // the loaded tile's scales
+  uint32_t none_n = 0;        // and its 16-token groups in no page, a bit each
+  int32_t pg[GR];             // pages of the tile to be loaded next
+  bool bad = false;
+  auto find = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      const int32_t p = kv_page(c, b, t0 + 16 * u);
+      pg[u] = t0 + 16 * u < thi ? p : -2;
+    }
+  };
+  auto page_of = [&](int t) {  // of token t of the tile, page 0 where there is none
+    const int32_t p0 = pg[0], p1 = pg[1], p2 = pg[GR - 2], p3 = pg[GR - 1];
+    int32_t p = (t & 16) != 0 ? p1 : p0;
+    if (GR == 4 && (t & 32) != 0) p = (t & 16) != 0 ? p3 : p2;
+    return static_cast<uint32_t>(p < 0 ? 0 : p);
+  };
+  const uint32_t page_bytes = static_cast<uint32_t>(c.page) * D;  // of one head
+  auto code = [&](const uint8_t* base, int t0, int t, int d) {    // where d of token t0 + t lies
+    const uint64_t at = static_cast<uint64_t>(page_of(t)) * static_cast<uint32_t>(c.Hkv) + static_cast<uint32_t>(h);
+    return base + at * page_bytes + (static_cast<uint32_t>((t0 + t) & (c.page - 1)) * D + static_cast<uint32_t>(d));
+  };
+  auto load = [&](int t0) {
+    none_n = 0;
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      const int64_t at = static_cast<int64_t>(pg[u] < 0 ? 0 : pg[u]) * c.Hkv + h;
+      ksn[u] = c.ks[at];
+      vsn[u] = c.vs[at];
+      none_n |= pg[u] < 0 ? 1u << u : 0u;
+      bad |= pg[u] == -1;
+    }
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int x = tid + KVM_T * i;
+      const u32x4 v = ld16(code(c.k, t0, x / (D / 16), x % (D / 16) * 16));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kc[i][e] = v[e];
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int x = tid + KVM_T * i;
+      const uint8_t* src = code(c.v, t0, x / (D / 8) * 4, x % (D / 8) * 8);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(src + e * D);
+        vc[i][2 * e] = v[0];
+        vc[i][2 * e + 1] = v[1];
+      }
+    }
+  };
+  auto store = [&](int t0, int st) {
+    unsigned char* ks = smem + st * Ti::STAGE;
+    unsigned char* vs = ks + TT * Ti::KP;
+#pragma unroll
+    for (int i = 0; i < KN; ++i) {
+      const int x = tid + KVM_T * i, t = x / (D / 16), p = x % (D / 16);
+      if (KN * KVM_T > TT * (D / 16) && t >= TT) break;
+      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + ((2 * p) ^ (t & 7)) * 16) = cat8(kv_half4<FP8>(kc[i][0]), kv_half4<FP8>(kc[i][1]));
+      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + ((2 * p + 1) ^ (t & 7)) * 16) = cat8(kv_half4<FP8>(kc[i][2]), kv_half4<FP8>(kc[i][3]));
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int x = tid + KVM_T * i, q = x / (D / 8), d0 = x % (D / 8) * 8;
+      if (VN * KVM_T > TT * D / 32 && q >= TT / 4) break;
+      if (none_n != 0 || t0 + TT > thi) {  // tokens that are none: their codes may be anything
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((none_n >> (q >> 2) & 1u) != 0 || t0 + 4 * q + e >= thi) vc[i][2 * e] = vc[i][2 * e + 1] = 0u;
+      }
+      // tokens 4 q .. + 3 of a 32: piece 2 (q / 4) + q % 2, its half q / 2 % 2
+      const int piece = q / 8 * 4 + (q % 8) / 4 * 2 + (q & 1), half = (q >> 1) & 1;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t r0 = vc[i][y], r1 = vc[i][2 + y], r2 = vc[i][4 + y], r3 = vc[i][6 + y];
+        const uint32_t a0 = __builtin_amdgcn_perm(r1, r0, 0x05010400u), a1 = __builtin_amdgcn_perm(r1, r0, 0x07030602u);
+        const uint32_t b0 = __builtin_amdgcn_perm(r3, r2, 0x05010400u), b1 = __builtin_amdgcn_perm(r3, r2, 0x07030602u);
+        const uint32_t z[4] = {__builtin_amdgcn_perm(b0, a0, 0x05040100u), __builtin_amdgcn_perm(b0, a0, 0x07060302u),
+                               __builtin_amdgcn_perm(b1, a1, 0x05040100u), __builtin_amdgcn_perm(b1, a1, 0x07060302u)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = d0 + 4 * y + e;
+          *reinterpret_cast<f16x4*>(vs + d * Ti::VP + kv_vslot<D>(d, piece) * 16 + half * 8) = kv_half4<FP8>(z[e]);
+        }
+      }
+    }
+  };
+
+  // ---- the wave's queries as binary16 (scaled by a power of two for bfloat16): lane (row, half) holds d 16 x + 8 half .. + 7
+  f16x8 q[D / 16];
+  float qs = a.scale * 1.44269504088896340736f;  // the factor of a score
+  int lo = 0, hi = 0;
+  const int r = w0 + col;
+  find(tlo);
+  load(tlo);
+  {
+    const bool ok = r < nrows;
+    const int i = query(r), hq = h * G + (ok ? r % G : 0);
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (first + i) * a.q_stride + static_cast<int64_t>(hq) * D + 8 * hf;
+    const bool whole = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stride * 2)) & 15u) == 0;
+    hi = ok ? row_hi(i) : 0;
+    lo = row_lo(i);
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (ok) {
+        if (whole) v = ld16(src + 16 * x);
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = src[16 * x + 2 * e] | (static_cast<uint32_t>(src[16 * x + 2 * e + 1]) << 16);
+      }
+      q[x] = __builtin_bit_cast(f16x8, v);
+    }
+    if (a.dtype != LT_F16) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const u32x4 v = __builtin_bit_cast(u32x4, q[x]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t m0 = (v[e] << 16) & 0x7FFFFFFFu, m1 = v[e] & 0x7FFF0000u;
+          top = top > m0 ? top : m0;
+          top = top > m1 ? top : m1;
+        }
+      }
+      const uint32_t m2 = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64));
+      top = top > m2 ? top : m2;
+      // the largest magnitude comes to [2^14, 2^15): binary16 then holds what is 2^-28 of it exactly
+      int e2 = static_cast<int>(top >> 23) - 127 - 14;
+      if (top >= 0x7F800000u || top < 0x00800000u) e2 = 0;
+      const float s1 = two(-(e2 / 2)), s2 = two(-(e2 - e2 / 2));
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const bf16x8 v = __builtin_bit_cast(bf16x8, q[x]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[x][e] = static_cast<f16>(static_cast<float>(v[e]) * s1 * s2);
+      }
+      qs = qs * two(e2 / 2) * two(e2 - e2 / 2);
+    }
+  }
+
+  f32x16 o[JT];
+#pragma unroll
+  for (int j = 0; j < JT; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+  float vref = 0.f;  // the value scale that the sums are in units of
+  // scales and missing groups of the tile in LDS
+  float ksc[GR], vsc[GR];
+  uint32_t none;
+  auto take = [&] {
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      ksc[u] = ksn[u];
+      vsc[u] = vsn[u];
+    }
+    none = none_n;
+  };
+  store(tlo, 0);
+  take();
+  find(tlo + TT);
+  load(tlo + TT);
+  find(tlo + 2 * TT);
+  __syncthreads();
+
+  int st = 0;
+#pragma unroll 1
+  for (int t0 = tlo; t0 < thi; t0 += TT, st ^= 1) {
+    const unsigned char* ks = smem + st * Ti::STAGE;
+    const unsigned char* vs = ks + TT * Ti::KP;
+    auto move = [&] {  // the next tile to the other stage, the one after it to registers
+      if (t0 + TT < thi) {
+        store(t0 + TT, st ^ 1);
+        take();
+        load(t0 + 2 * TT);
+        find(t0 + 3 * TT);
+      }
+    };
+    if (t0 >= whi || t0 + TT <= wlo) {  // none of it is this wave's
+      move();
+      __syncthreads();
+      continue;
+    }
+    f32x16 s[TT / 32];
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+      for (int u = 0; u < TT / 32; ++u) {
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + (((2 * x + hf) ^ (col & 7)) * 16));
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], x == 0 ? f32x16{} : s[u], 0, 0, 0);
+      }
+    const uint32_t no = none;
+    float kq[GR], vw[GR];
+    const float ref = vref;
+    bool plain = true;  // factors of the usual kind: see below
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      kq[u] = qs * ksc[u];
+      vw[u] = vsc[u];
+      if ((no >> u & 1u) == 0 && vsc[u] > vref && vsc[u] <= 3.4028235e38f) vref = vsc[u];  // a wave's own: its sums alone are in these units
+    }
+    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+    for (int u = 0; u < GR; ++u) {
+      vw[u] *= inv * KV_P;
+      plain &= kq[u] >= 0.f && vw[u] >= 0x1p-8f && vw[u] <= KV_P;
+    }
+    move();
+    {
+      plain = __all(plain && !(t0 < full_lo || t0 + TT > full_hi || no != 0));
+      float top = -__builtin_inff();
+      if (plain) {
+        // no masks, key factors not negative: a group's largest score is its largest sum's
+#pragma unroll
+        for (int u = 0; u < GR; ++u) {
+          float x = s[u / 2][8 * (u & 1)];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) x = fmaxf(x, s[u / 2][8 * (u & 1) + e]);
+          top = fmaxf(top, x * kq[u]);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < TT / 32; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int tok = 32 * u + 8 * (e >> 2) + 4 * hf + (e & 3);
+            const bool out = (no >> (2 * u + (e >> 3)) & 1u) != 0 || t0 + tok < lo || t0 + tok >= hi;
+            s[u][e] = out ? -__builtin_inff() : s[u][e] * kq[2 * u + (e >> 3)];
+            top = fmaxf(top, s[u][e]);
+          }
+      }
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m + KV_LAG || ref < vref)) {
+        const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f(m - base);
+        m = mn;
+        l *= f;
+        const float fo = ref < vref ? f * (ref / vref) : f;
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[j][e] *= fo;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < TT / 32; ++u)
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl) {
+          const float w = vw[2 * u + sl];
+          f16x8 pf;
+          if (plain) {
+            // the exponential with the value's factor in its exponent: one multiply-add and one exponential a weight
+            const float kf = kq[2 * u + sl], lw = __builtin_amdgcn_logf(w) - base;  // log2
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * sl + e], kf, lw));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][8 * sl + e + 1], kf, lw));
+              sum += p0 + p1;
+              const f16x2 h2 = __builtin_convertvector((f32x2{p0, p1}), f16x2);
+              pf[e] = h2[0];
+              pf[e + 1] = h2[1];
+            }
+            l += sum * __builtin_amdgcn_rcpf(w);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float v = s[u][8 * sl + e], p = __builtin_amdgcn_exp2f(v - base);
+              l += p;
+              // a masked token's weight is 0 whatever its page's scale holds
+              pf[e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < JT; ++j) {
+            const int d = 32 * j + col;
+            const f16x8 vf = *reinterpret_cast<const f16x8*>(vs + d * Ti::VP + kv_vslot<D>(d, u * 4 + sl * 2 + hf) * 16);
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
+          }
+        }
+    }
+    __syncthreads();
+  }
+  if (__any(bad) && lane == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+
+  l += __shfl_xor(l, 32, 64);
+  const float unit_v = vref * (1.f / KV_P);
+  if (parts > 1) {
+    constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
+    constexpr uint32_t PART = static_cast<uint32_t>(Ti::PART), ML = KVM_ROWS * D * 4;
+    int* s_last = reinterpret_cast<int*>(smem);
+    uint32_t* cnt = static_cast<uint32_t*>(a.ws);
+    const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + KV_COUNTERS + static_cast<int64_t>(unit) * splits * PART, splits * PART);
+    const uint32_t at = (32 * wave + col) * (D * 4) + hf * 16, ml = ML + (32 * wave + col) * 8;
+    if (r < nrows) {
+#pragma unroll
+      for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const f32x4 v = {o[j][4 * y] * unit_v, o[j][4 * y + 1] * unit_v, o[j][4 * y + 2] * unit_v, o[j][4 * y + 3] * unit_v};
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rW, split * PART + at + j * 128 + y * 32, 0, COHERENT);
+        }
+      if (hf == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, l)}, rW, split * PART + ml, 0, COHERENT);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) *s_last = __hip_atomic_fetch_add(cnt + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    __syncthreads();
+    if (!*s_last) return;
+    __syncthreads();
+    if (tid == 0) __hip_atomic_store(cnt + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    m = -__builtin_inff();
+    l = 0.f;
+#pragma unroll
+    for (int j = 0; j < JT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
+    if (r < nrows) {
+#pragma unroll 1
+      for (uint32_t sp = 0; sp < parts; ++sp) {
+        const f32x2 x = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(rW, sp * PART + ml, 0, COHERENT));
+        f32x4 v[JT][4];
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            v[j][y] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, sp * PART + at + j * 128 + y * 32, 0, COHERENT));
+        const float pm = x[0], mn = fmaxf(m, pm), base = mn == -__builtin_inff() ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(pm - base);
+        m = mn;
+        l = l * f0 + x[1] * f1;
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * f0 + v[j][e >> 2][e & 3] * f1;
+      }
+    }
+  }
+  // 32 rows through the wave's part of LDS in the output's type, then whole pieces of 16 bytes
+  const float inv = (l != 0.f ? 1.f / l : 0.f) * (parts > 1 ? 1.f : unit_v);
+  constexpr int PITCH = D * 2 + 16;
+  unsigned char* strip = smem + wave * (32 * PITCH);
+#pragma unroll
+  for (int j = 0; j < JT; ++j)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      u32x2 v;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x0 = o[j][4 * y + 2 * e] * inv, x1 = o[j][4 * y + 2 * e + 1] * inv;
+        v[e] = a.dtype == LT_F16 ? __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(x0), static_cast<f16>(x1)})
+                                 : __builtin_bit_cast(uint32_t, bf16x2{static_cast<bf16>(x0), static_cast<bf16>(x1)});
+      }
+      *reinterpret_cast<u32x2*>(strip + col * PITCH + (32 * j + 8 * y + 4 * hf) * 2) = v;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const bool vec = (reinterpret_cast<uintptr_t>(a.o) & 15u) == 0;
+#pragma unroll 1
+  for (int x = lane; x < 32 * (D / 8); x += 64) {
+    const int rr = w0 + x / (D / 8), p = x % (D / 8);
+    if (rr >= nrows) continue;
+    const unsigned char* src = strip + x / (D / 8) * PITCH + p * 16;
+    uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<int64_t>(first + rr / G) * a.Hq + h * G + rr % G) * D + p * 8;
+    if (vec) *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(src);
+    else
+      for (int e = 0; e < 8; ++e) dst[e] = reinterpret_cast<const uint16_t*>(src)[e];
+  }
+}
+
+struct KvPlan {
+  bool tile;  // k_kv8_tile, else k_kv8_rows
+  int64_t row_tiles, splits, chunk, ws_bytes;
+};
+
+// Up to 16 rows of a key head take k_kv8_rows. Tokens are split only as far as the card has room for more
+// workgroups at once (a start, a join and the code's own fetch cost more than even shares gain): one of k_kv8_rows a CU, two of k_kv8_tile
+// (heads of 256: one). One sequence of 65000: 129 us in shares of 256 tokens, 83 of 512, 57 of 1024, 39 of 2048 (one a
+// CU); 48 of up to 8000: 227 us in shares of 1024, 170 of 2048, 108 unsplit; 8 of 4000: 35 of 512, 25 of 1024, 32 of 2048.
+KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
+  const int64_t G = a.Hq / a.c.Hkv, cus = device_cus() > 0 ? device_cus() : 256;
+  KvPlan p{};
+  p.tile = a.max_new * G > 16;
+  const int64_t rows = p.tile ? KVM_ROWS : 16;
+  p.row_tiles = (a.max_new * G + rows - 1) / rows;
+  const int64_t units = p.row_tiles * a.c.Hkv * a.c.B;
+  int64_t span = static_cast<int64_t>(a.c.width) << a.c.page_log2;
+  if (a.window > 0) {  // what the rows' windows cover, from a multiple of a tile's tokens on
+    const int64_t seen = static_cast<int64_t>(a.window) + (a.causal ? rows : a.max_new) + 64;
+    span = span < seen ? span : seen;
+  }
+  p.splits = 1;
+  p.chunk = span > 0 ? span : 1;
+  if (have_ws && units * 4 <= KV_COUNTERS && span > KVR_PASS) {
+    const int64_t room = p.tile && a.c.D <= 128 ? 2 * cus : cus, want = room / units > 1 ? room / units : 1;
+    int64_t chunk = ((span + want - 1) / want + KVR_PASS - 1) / KVR_PASS * KVR_PASS;
+    if (p.tile && chunk < 2 * KVR_PASS) chunk = 2 * KVR_PASS;
+    const int64_t s = (span + chunk - 1) / chunk;
+    if (s > 1) {
+      p.splits = s;
+      p.chunk = chunk;
+      p.ws_bytes = KV_COUNTERS + units * s * rows * (a.c.D + 2) * 4;
+    }
+  }
+  return p;
+}
+
+template <int D, bool FP8>
+hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
+  const int64_t n = p.row_tiles * p.splits * a.c.Hkv * a.c.B;
+  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<uint32_t>(n));
+  const uint32_t rt = static_cast<uint32_t>(p.row_tiles), sp = static_cast<uint32_t>(p.splits), ch = static_cast<uint32_t>(p.chunk);
+  if (!p.tile) {
+    k_kv8_rows<D, FP8><<<grid, 64 * KVR_WAVES, 0, st>>>(a, rt, sp, ch);
+    return hipGetLastError();
+  }
+  constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16), lds = 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
+  static std::atomic<int> done[kMaxDevices];
+  if (lds > 65536) {
+    const hipError_t e = raise_lds_cap(reinterpret_cast<const void*>(k_kv8_tile<D, FP8>), lds, done);
+    if (e != hipSuccess) return e;
+  }
+  k_kv8_tile<D, FP8><<<grid, KVM_T, lds, st>>>(a, rt, sp, ch);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t kv8_workspace_bytes(const KvAttnArgs&) { return 0; }
+int64_t kv8_workspace_bytes(const KvAttnArgs& a) {
+  return a.c.B == 0 || a.max_new == 0 ? 0 : attention_plan(a, true).ws_bytes;
+}
 
 hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st) {
   if (a.c.B == 0 || a.max_new == 0) return hipSuccess;
+  KvPlan p = attention_plan(a, a.ws != nullptr);
+  if (p.ws_bytes > a.ws_bytes) p = attention_plan(a, false);
   switch (a.c.D * 2 + (a.c.fp8 ? 1 : 0)) {
-    case 128: return rows_for<64, false>(a, st);
-    case 129: return rows_for<64, true>(a, st);
-    case 192: return rows_for<96, false>(a, st);
-    case 193: return rows_for<96, true>(a, st);
-    case 256: return rows_for<128, false>(a, st);
-    case 257: return rows_for<128, true>(a, st);
-    case 512: return rows_for<256, false>(a, st);
-    case 513: return rows_for<256, true>(a, st);
+    case 128: return attention_for<64, false>(a, p, st);
+    case 129: return attention_for<64, true>(a, p, st);
+    case 192: return attention_for<96, false>(a, p, st);
+    case 193: return attention_for<96, true>(a, p, st);
+    case 256: return attention_for<128, false>(a, p, st);
+    case 257: return attention_for<128, true>(a, p, st);
+    case 512: return attention_for<256, false>(a, p, st);
+    case 513: return attention_for<256, true>(a, p, st);
   }
   return hipErrorInvalidValue;
 }

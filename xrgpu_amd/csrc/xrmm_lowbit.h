@@ -13,6 +13,7 @@ typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int MX_BLOCK = 32;  // values per scale
@@ -118,12 +119,13 @@ __device__ __forceinline__ bool kv_rows(const KvCache& c, int b, int most, int& 
   return ok;
 }
 
-// The page that holds token t (inside the table's width) of sequence b, or -1 where there is none.
+// The page that holds token t of sequence b, or -1 where there is none. Reads the table in any case (the
+// host gives an empty one the address of the lengths), so that lookups need no branches.
 __device__ __forceinline__ int32_t kv_page(const KvCache& c, int b, int t) {
   const int i = t >> c.page_log2;
-  if (t < 0 || i >= c.width) return -1;
-  const int32_t p = c.table[static_cast<int64_t>(b) * c.width + i];
-  return p >= 0 && p < c.pages ? p : -1;
+  const bool in = t >= 0 && i < c.width;
+  const int32_t p = c.table[static_cast<int64_t>(b) * c.width + (in ? i : 0)];
+  return in && p >= 0 && p < c.pages ? p : -1;
 }
 
 constexpr uint32_t KV_BAD = 55u;  // the status code of a row that names what does not exist

@@ -62,7 +62,7 @@ int cache_of(xrmm::KvCache& c, void* k, void* v, void* ks, void* vs, const void*
   c.v = static_cast<uint8_t*>(v);
   c.ks = static_cast<float*>(ks);
   c.vs = static_cast<float*>(vs);
-  c.table = static_cast<const int32_t*>(table);
+  c.table = static_cast<const int32_t*>(width > 0 ? table : lengths);
   c.lengths = static_cast<const int32_t*>(lengths);
   c.starts = static_cast<const int32_t*>(starts);
   c.status = static_cast<uint32_t*>(status);

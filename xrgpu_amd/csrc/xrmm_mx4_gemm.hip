@@ -12,6 +12,7 @@
 //
 // The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
 #include <atomic>
+#include <cstdlib>
 
 #include "xrmm_mx4.h"
 
@@ -513,10 +514,16 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
                                        {{1, 0.60, 2.7, 3}, {2, 1.0, 5.1, 5}, {4, 2.1, 7.0, 12}}};
   double least = 0;
   for (const Cost& c : kCost[mx ? 1 : 0]) {
+#ifdef XRMM_TUNE
+    if (const char* e = getenv("MXT")) if (atoi(e) != c.t) continue;
+#endif
     const int64_t mt = (M + 64 * c.t - 1) / (64 * c.t), nt = (N + 64 * c.t - 1) / (64 * c.t), n = mt * nt;
     if (n > 0x3FFFFFFF) continue;
     for (int64_t s = 1; s <= 8; ++s) {
       if (s > 1 && (!have_ws || n > MX_COUNTERS / 4 || n * s > 2 * cus || steps < 4 * s)) break;
+#ifdef XRMM_TUNE
+      if (const char* e = getenv("MXS")) if (atoi(e) != s) continue;
+#endif
       MxPlan p{};
       p.t = c.t;
       p.mt = static_cast<uint32_t>(mt);
