@@ -12,15 +12,18 @@
 // return values and no exceptions: a throw costs 4 us, more than the checks (a float32
 // call on a workspace 17 x 1024 x 1024 took 18.7 us on the host with throws and every
 // check made twice, 15.8 without a front end).
-// Nothing is kept between calls. Measured, among other passes: Qkv 4 x 4096 x (4096 + 2 x
+// Nothing is kept between calls; the MX4 and kv8 calls look their workspace up in ops.py's own table (its
+// bytes come back as above where it is not there yet, too small, or a graph is being captured). Measured, among other passes: Qkv 4 x 4096 x (4096 + 2 x
 // 1024) 17.8 -> 7.6 us a call, MatMulNBits 1 x 4096 x 14336 8.4 -> 6.9.
 #include <Python.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/version.h>
 
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 
@@ -395,6 +398,282 @@ PyObject* gather(PyObject*, PyObject* const* v, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// MX4 and the 8-bit paged cache
+
+constexpr int I8 = 5, BF16 = 16, E4M3 = 17;  // xrmm_dtype
+
+using QuantizeFn = int (*)(const void*, void*, void*, int64_t, int64_t, int32_t, void*);
+using Mx4WsFn = int64_t (*)(int64_t, int64_t, int64_t, int32_t);
+using Mx4Fn = int (*)(const void*, const void*, int32_t, const void*, const void*, const void*, void*, int32_t, int64_t, int64_t,
+                      int64_t, void*, int64_t, void*);
+using AppendFn = int (*)(const void*, const void*, int64_t, int64_t, int32_t, void*, void*, void*, void*, int32_t, const void*,
+                         const void*, const void*, void*, int64_t, int32_t, int32_t, int32_t, int64_t, int32_t, int32_t,
+                         int32_t, void*);
+using AttendWsFn = int64_t (*)(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t);
+using AttendFn = int (*)(const void*, int64_t, void*, int32_t, const void*, const void*, const void*, const void*, int32_t,
+                         const void*, const void*, const void*, void*, int64_t, int32_t, int32_t, int32_t, int64_t, int32_t,
+                         int32_t, int32_t, int32_t, float, int32_t, int32_t, void*, int64_t, void*);
+
+QuantizeFn g_quantize;
+Mx4WsFn g_mx4_ws;
+Mx4Fn g_mx4;
+AppendFn g_append;
+AttendWsFn g_attend_ws;
+AttendFn g_attend;
+PyObject *g_workspaces, *g_capturing;  // {(device, stream): uint8 tensor} of ops.py; whether the current stream captures
+
+// The type of an activation or output, or -1.
+int lt(at::ScalarType t) { return t == at::kHalf ? F16 : t == at::kFloat ? F32 : t == at::kBFloat16 ? BF16 : -1; }
+
+// ops.py's workspace of the stream where it is large enough and no graph is captured; else none, and `need` is ops.py's to meet.
+bool kept_workspace(int dev, void* st, int64_t need, void*& ws, int64_t& bytes) {
+  PyObject* c = PyObject_CallNoArgs(g_capturing);
+  const bool eager = c == Py_False;
+  Py_XDECREF(c);
+  if (!eager) {
+    PyErr_Clear();
+    return false;
+  }
+  PyObject* key = Py_BuildValue("(iN)", dev, PyLong_FromVoidPtr(st));
+  PyObject* o = key ? PyDict_GetItem(g_workspaces, key) : nullptr;  // borrowed
+  Py_XDECREF(key);
+  if (o == nullptr || !THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  ws = t.data_ptr();
+  bytes = t.numel();
+  return bytes >= need;
+}
+
+// A tensor [tokens, heads, dim] whose tokens may lie apart.
+bool token_rows(PyObject* o, int& dev, int64_t heads, int64_t dim, const at::Tensor*& out, int64_t& stride) {
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  const auto ks = t.key_set();
+  if (!t.is_cuda() || t.layout() != at::kStrided || ks.has(c10::DispatchKey::Python) ||
+      ks.has_any(c10::functorch_transforms_ks) || t.is_conj() || t.is_neg() || t.dim() != 3 || t.size(0) == 0 ||
+      t.size(1) != heads || t.size(2) != dim || t.get_device() != dev || t.stride(2) != 1 || (heads > 1 && t.stride(1) != dim) ||
+      (t.size(0) > 1 && t.stride(0) < heads * dim))
+    return false;
+  stride = t.size(0) > 1 ? t.stride(0) : heads * dim;
+  out = &t;
+  return true;
+}
+
+struct Cache {
+  const at::Tensor *k, *v, *ks, *vs, *table, *lengths;
+  const void* starts = nullptr;
+  void* status = nullptr;
+  int64_t P = 0, H = 0, page = 0, D = 0, B = 0, W = 0;
+  int dt = I8;
+  bool set(PyObject* const* o, PyObject* st, PyObject* stat, int& dev) {
+    if (!plain(o[0], dev, k) || !plain(o[1], dev, v) || !plain(o[2], dev, ks) || !plain(o[3], dev, vs) ||
+        !plain(o[4], dev, table) || !plain(o[5], dev, lengths))
+      return false;
+    dt = k->scalar_type() == at::kChar ? I8 : k->scalar_type() == at::kFloat8_e4m3fn ? E4M3 : -1;
+    if (dt < 0 || v->scalar_type() != k->scalar_type() || k->dim() != 4 || v->sizes() != k->sizes()) return false;
+    P = k->size(0), H = k->size(1), page = k->size(2), D = k->size(3);
+    if (!shape(*ks, {P, H}) || !shape(*vs, {P, H}) || ks->scalar_type() != at::kFloat || vs->scalar_type() != at::kFloat ||
+        lengths->scalar_type() != at::kInt || lengths->dim() != 1 || table->scalar_type() != at::kInt || table->dim() != 2)
+      return false;
+    B = lengths->size(0), W = table->size(1);
+    if (table->size(0) != B || B > INT32_MAX || W > INT32_MAX || H > INT32_MAX || page > INT32_MAX || D > INT32_MAX) return false;
+    if (!none(st)) {
+      const at::Tensor* t;
+      if (!plain(st, dev, t) || t->scalar_type() != at::kInt || !shape(*t, {B + 1})) return false;
+      starts = t->data_ptr();
+    }
+    if (!none(stat)) {
+      const at::Tensor* t;
+      if (!plain(stat, dev, t) || !(t->scalar_type() == at::kInt || t->scalar_type() == at::kUInt32)) return false;
+      status = t->data_ptr();
+    }
+    return true;
+  }
+};
+
+// None or an integer of 32 bits
+bool small(PyObject* o, int32_t& v) {
+  int64_t x = 0;
+  if (!none(o) && !integer(o, x)) return false;
+  v = static_cast<int32_t>(x);
+  return x >= INT32_MIN && x <= INT32_MAX;
+}
+
+// (x)
+PyObject* mx4_quantize(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 1, [&]() -> PyObject* {
+    int dev = -1;
+    const at::Tensor* x;
+    void* st;
+    if (!plain(v[0], dev, x) || x->dim() < 1 || lt(x->scalar_type()) < 0 || !stream_of(dev, st)) Py_RETURN_NONE;
+    at::Tensor codes, scales;
+    int rc;
+    {
+      NoGil ng;
+      const int64_t K = x->size(-1);
+      at::DimVector s(x->sizes().slice(0, x->dim() - 1));
+      s.push_back((K + 31) / 32);
+      scales = at::empty(s, x->options().dtype(at::kByte));
+      s.push_back(16);
+      codes = at::empty(s, x->options().dtype(at::kByte));
+      rc = g_quantize(x->data_ptr(), codes.data_ptr(), scales.data_ptr(), x->numel() / K, K, lt(x->scalar_type()), st);
+    }
+    if (!checked(rc)) return nullptr;
+    PyObject *o0 = THPVariable_Wrap(codes), *o1 = THPVariable_Wrap(scales);
+    return Py_BuildValue("(NN)", o0, o1);
+  });
+}
+
+// (A, B, scales, bias, A_scales, out_dtype); an int: checked, needs a workspace of that many bytes
+PyObject* matmul_mx4(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    int dev = -1;
+    const at::Tensor *A, *B, *S, *T = nullptr;
+    if (!plain(v[0], dev, A) || !plain(v[1], dev, B) || !plain(v[2], dev, S) || B->scalar_type() != at::kByte || B->dim() != 3 ||
+        B->size(2) != 16 || S->scalar_type() != at::kByte)
+      Py_RETURN_NONE;
+    const int64_t N = B->size(0), kb = B->size(1);
+    if (!shape(*S, {N, kb})) Py_RETURN_NONE;
+    const bool mx = A->scalar_type() == at::kByte;
+    int64_t K = kb * 32, lead = A->dim() - (mx ? 2 : 1);
+    at::ScalarType out = A->scalar_type();
+    if (lead < 0 || !(none(v[5]) || THPDtype_Check(v[5]))) Py_RETURN_NONE;
+    if (mx) {
+      if (A->size(-1) != 16 || A->size(-2) != kb || !plain(v[4], dev, T) || T->scalar_type() != at::kByte ||
+          T->sizes() != A->sizes().slice(0, lead + 1))
+        Py_RETURN_NONE;
+      out = none(v[5]) ? at::kHalf : reinterpret_cast<THPDtype*>(v[5])->scalar_type;
+    } else {
+      K = A->size(-1);
+      if (!none(v[4]) || (K + 31) / 32 != kb || !(out == at::kHalf || out == at::kBFloat16) ||
+          !(none(v[5]) || reinterpret_cast<THPDtype*>(v[5])->scalar_type == out))
+        Py_RETURN_NONE;
+    }
+    const void* bias = nullptr;
+    if (lt(out) < 0) Py_RETURN_NONE;
+    if (!none(v[3])) {
+      const at::Tensor* b;
+      if (!plain(v[3], dev, b) || b->scalar_type() != out || !shape(*b, {N})) Py_RETURN_NONE;
+      bias = b->data_ptr();
+    }
+    const int64_t M = A->numel() / (mx ? kb * 16 : K);
+    const int at_ = mx ? U8 : lt(A->scalar_type());
+    void *st, *ws = nullptr;
+    if (!stream_of(dev, st)) Py_RETURN_NONE;
+    const int64_t need = g_mx4_ws(M, K, N, at_);
+    int64_t bytes = 0;
+    if (need > 0 && !kept_workspace(dev, st, need, ws, bytes)) return PyLong_FromLongLong(need);
+    at::Tensor y;
+    int rc;
+    {
+      NoGil ng;
+      at::DimVector s(A->sizes().slice(0, lead));
+      s.push_back(N);
+      y = at::empty(s, A->options().dtype(out));
+      rc = g_mx4(A->data_ptr(), T ? T->data_ptr() : nullptr, at_, B->data_ptr(), S->data_ptr(), bias, y.data_ptr(), lt(out), M, K,
+                 N, ws, bytes, st);
+    }
+    if (!checked(rc)) return nullptr;
+    return THPVariable_Wrap(y);
+  });
+}
+
+// (k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, max_new, status); True when done
+PyObject* kv8_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject* {
+    int dev = -1;
+    Cache c;
+    const at::Tensor *k, *w;
+    int64_t ks = 0, vs = 0;
+    int32_t most = 0;
+    void* st;
+    if (!c.set(v + 2, v[8], v[10], dev) || !small(v[9], most) || !token_rows(v[0], dev, c.H, c.D, k, ks) ||
+        !token_rows(v[1], dev, c.H, c.D, w, vs) || k->size(0) != w->size(0) || lt(k->scalar_type()) < 0 ||
+        w->scalar_type() != k->scalar_type() || !stream_of(dev, st))
+      Py_RETURN_NONE;
+    int rc;
+    {
+      NoGil ng;
+      rc = g_append(k->data_ptr(), w->data_ptr(), ks, vs, lt(k->scalar_type()), c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(),
+                    c.vs->data_ptr(), c.dt, c.table->data_ptr(), c.lengths->data_ptr(), c.starts, c.status, k->size(0), most,
+                    static_cast<int32_t>(c.B), static_cast<int32_t>(c.W), c.P, static_cast<int32_t>(c.page),
+                    static_cast<int32_t>(c.H), static_cast<int32_t>(c.D), st);
+    }
+    if (!checked(rc)) return nullptr;
+    Py_RETURN_TRUE;
+  });
+}
+
+// (q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, max_new, scale, causal, window, status); an int: checked,
+// needs a workspace of that many bytes
+PyObject* kv8_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 13, [&]() -> PyObject* {
+    int dev = -1;
+    Cache c;
+    const at::Tensor* q;
+    int64_t qs = 0;
+    int32_t most = 0, window = 0;
+    float scale;
+    void *st, *ws = nullptr;
+    if (!c.set(v + 1, v[7], v[12], dev) || !small(v[8], most) || !PyBool_Check(v[10]) || none(v[11]) || !small(v[11], window) ||
+        !THPVariable_CheckExact(v[0]) || THPVariable_Unpack(v[0]).dim() != 3)
+      Py_RETURN_NONE;
+    const int64_t Hq = THPVariable_Unpack(v[0]).size(1);
+    if (Hq == 0 || Hq > INT32_MAX || Hq % c.H != 0 || !token_rows(v[0], dev, Hq, c.D, q, qs) ||
+        !(q->scalar_type() == at::kHalf || q->scalar_type() == at::kBFloat16))
+      Py_RETURN_NONE;
+    if (none(v[9])) scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.D)));
+    else if (!real(v[9], scale)) Py_RETURN_NONE;
+    if (!stream_of(dev, st)) Py_RETURN_NONE;
+    const int32_t B = static_cast<int32_t>(c.B), W = static_cast<int32_t>(c.W), page = static_cast<int32_t>(c.page),
+                  H = static_cast<int32_t>(c.H), D = static_cast<int32_t>(c.D), causal = v[10] == Py_True;
+    const int64_t need = g_attend_ws(q->size(0), most, c.starts != nullptr, B, W, page, static_cast<int32_t>(Hq), H, D, causal, window);
+    int64_t bytes = 0;
+    if (need > 0 && !kept_workspace(dev, st, need, ws, bytes)) return PyLong_FromLongLong(need);
+    at::Tensor o;
+    int rc;
+    {
+      NoGil ng;
+      o = at::empty(q->sizes(), q->options());
+      rc = g_attend(q->data_ptr(), qs, o.data_ptr(), lt(q->scalar_type()), c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(),
+                    c.vs->data_ptr(), c.dt, c.table->data_ptr(), c.lengths->data_ptr(), c.starts, c.status, q->size(0), most, B, W,
+                    c.P, page, static_cast<int32_t>(Hq), H, D, scale, causal, window, ws, bytes, st);
+    }
+    if (!checked(rc)) return nullptr;
+    return THPVariable_Wrap(o);
+  });
+}
+
+// (workspace table, capture query, addresses of the six entry points)
+PyObject* bind_lowbit(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 8 || !PyDict_CheckExact(v[0])) {
+    PyErr_SetString(PyExc_TypeError, "bind_lowbit takes a dict, a function and six addresses");
+    return nullptr;
+  }
+  void* f[6];
+  for (int i = 0; i < 6; ++i) {
+    f[i] = PyLong_AsVoidPtr(v[2 + i]);
+    if (f[i] == nullptr) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
+      return nullptr;
+    }
+  }
+  Py_INCREF(v[0]);
+  Py_INCREF(v[1]);
+  Py_XDECREF(g_workspaces);
+  Py_XDECREF(g_capturing);
+  g_workspaces = v[0];
+  g_capturing = v[1];
+  g_quantize = reinterpret_cast<QuantizeFn>(f[0]);
+  g_mx4_ws = reinterpret_cast<Mx4WsFn>(f[1]);
+  g_mx4 = reinterpret_cast<Mx4Fn>(f[2]);
+  g_append = reinterpret_cast<AppendFn>(f[3]);
+  g_attend_ws = reinterpret_cast<AttendWsFn>(f[4]);
+  g_attend = reinterpret_cast<AttendFn>(f[5]);
+  Py_RETURN_NONE;
+}
+
 // (raw stream function, check function, addresses of the seven entry points)
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (n != 9) {
@@ -427,7 +706,8 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
 
 #define XRMM_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {XRMM_FN(bind), XRMM_FN(matmul), XRMM_FN(qkv), XRMM_FN(mlp),
-                          XRMM_FN(bnb4), XRMM_FN(gather), {nullptr, nullptr, 0, nullptr}};
+                          XRMM_FN(bnb4), XRMM_FN(gather), XRMM_FN(bind_lowbit), XRMM_FN(mx4_quantize),
+                          XRMM_FN(matmul_mx4), XRMM_FN(kv8_append), XRMM_FN(kv8_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_xrmm_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -72,6 +72,10 @@ def _load_front():
     mod.bind(_raw_stream, nat.check, *(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
         "xrmm_matmul_nbits", "xrmm_matmul_nbits_workspace_bytes", "xrmm_matmul_nbits_fused_workspace_bytes",
         "xrmm_matmul_nbits_qkv_ws", "xrmm_matmul_nbits_mlp_ws", "xrmm_matmul_bnb4", "xrmm_gather_block_quantized")))
+    mod.bind_lowbit(_WORKSPACES, torch._C._cuda_isCurrentStreamCapturing, *(
+        ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+            "xrmm_mx4_quantize", "xrmm_matmul_mx4_workspace_bytes", "xrmm_matmul_mx4", "xrmm_kv8_append",
+            "xrmm_kv8_attention_workspace_bytes", "xrmm_kv8_attention")))
     return mod
 
 
@@ -708,6 +712,10 @@ def mx4_quantize(x, *, stream=None):
     x ``[..., K]`` float32, float16 or bfloat16. A block of 32 has the scale ``2^(byte - 127)`` with
     ``byte = max(floor(log2 max|x|) + 125, 0)``; codes are E2M1 to nearest, ties to even, saturated at 6. A block
     that holds a NaN or an infinity has byte 255 (NaN)."""
+    if stream is None and _front():
+        r = _FRONT.mx4_quantize(x)
+        if r is not None:
+            return r
     if x.dtype not in _LT:
         raise nat.XrmmInvalid("x must be float32, float16 or bfloat16")
     if x.dim() < 1 or x.shape[-1] == 0:
@@ -729,6 +737,10 @@ def matmul_mx4(A, B, scales, bias=None, *, A_scales=None, out_dtype=None, out=No
     ``[..., kb]`` (output ``out_dtype``: float16 unless given, or bfloat16, float32). bias ``[N]`` has the output's
     type. Sums are float32, rounded once. Geometries with few output tiles split K across workgroups on a workspace
     (``matmul_mx4_workspace_bytes``; see ``matmul_nbits`` for whose it is and for graph capture)."""
+    if out is None and workspace is None and stream is None and _front():
+        r = _FRONT.matmul_mx4(A, B, scales, bias, A_scales, out_dtype)
+        if r is not None and type(r) is not int:
+            return r
     if B.dtype != torch.uint8 or B.dim() != 3 or B.shape[2] != 16:
         raise nat.XrmmInvalid(f"B must be uint8 [N, kb, 16], got {B.dtype} {tuple(B.shape)}")
     N, kb = int(B.shape[0]), int(B.shape[1])
@@ -832,6 +844,9 @@ def kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     scale NaN. ``max_new``: at least the most tokens of one sequence (a bound on the work; T when not given). Pages
     outside the cache, positions past the table and rows outside T are left out and raise the device word
     ``status`` (int32) to 55."""
+    if stream is None and _front() and _FRONT.kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
+                                                         starts, max_new, status):
+        return
     B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
     if k.dtype not in _LT or v.dtype != k.dtype:
         raise nat.XrmmInvalid("k and v must both be float32, float16 or bfloat16")
@@ -856,6 +871,11 @@ def kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     is 0. ``scale``: head_dim^-0.5 when not given. Returns ``[T, q_heads, head_dim]`` of q's dtype. Long contexts of few rows
     are split across workgroups on a workspace (``kv8_attention_workspace_bytes``; see ``matmul_nbits`` for whose it is and
     for graph capture)."""
+    if out is None and workspace is None and stream is None and _front():
+        r = _FRONT.kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, max_new, scale, causal,
+                                 window, status)
+        if r is not None and type(r) is not int:
+            return r
     B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise nat.XrmmInvalid("q must be float16 or bfloat16")
