@@ -12,7 +12,6 @@
 //
 // The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
 #include <atomic>
-#include <cstdlib>
 
 #include "xrmm_mx4.h"
 
@@ -96,64 +95,68 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   uint32_t ox[AL ? 1 : NA];
   bool misfit = false;
 
+  // A thread's place in each row it loads, past every bound where there is none; a step adds a scalar offset, and one
+  // comparison a step says whether the thread's piece lies before the split's end.
   const uint32_t srow = static_cast<uint32_t>(tid >> 3), spiece = static_cast<uint32_t>((tid & 7) ^ (srow & 7u));
-  auto load_a = [&](int i, uint32_t s, u32x4* ra, uint32_t* rx) {
+  uint32_t va[NA], vb[NB];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) {
     const uint32_t r = srow + TR * i;
+    va[i] = r < rowsA ? ((r * rowA + misA) & ~3u) + spiece * 16u : MX_OOB;
+  }
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
     if constexpr (MX) {
-      const uint32_t b = s * 8u + spiece;
-      ra[i] = bld16(rA, (r < rowsA && b < kbe) ? r * rowA + b * MX_BLOB : MX_OOB, 0);
+      const uint32_t r = srow + TR * i;
+      vb[i] = r < rowsB ? r * rowB + spiece * MX_BLOB : MX_OOB;
     } else {
-      const uint32_t k = s * 64u + spiece * 8u;
-      const bool ok = r < rowsA && k < Ke;
-      if constexpr (AL) {
-        ra[i] = bld16(rA, ok ? r * rowA + k * 2u : MX_OOB, 0);
-      } else {
-        const uint32_t off = r * rowA + k * 2u + misA;
-        ra[i] = bld16(rA, ok ? off & ~3u : MX_OOB, 0);
-        rx[i] = bld_u32(rA, ok ? (off & ~3u) + 16u : MX_OOB, 0);
-      }
+      const uint32_t c = static_cast<uint32_t>(tid + T * i), r = c >> 1;
+      vb[i] = r < rowsB && r < RB ? r * rowB + (c & 1u) * MX_BLOB : MX_OOB;
     }
+  }
+  auto inside = [&](uint32_t s) { return MX ? s * 8u + spiece < kbe : s * 64u + spiece * 8u < Ke; };
+  auto load_a = [&](int i, uint32_t s, bool in, u32x4* ra, uint32_t* rx) {
+    const uint32_t v = in ? va[i] : MX_OOB;
+    ra[i] = bld16(rA, v, s * 128u);
+    if constexpr (!MX && !AL) rx[i] = bld_u32(rA, v + 16u, s * 128u);
   };
-  auto load_b = [&](int i, uint32_t s, u32x4* rb) {  // MX4 operands
-    const uint32_t r = srow + TR * i, b = s * 8u + spiece;
-    rb[i] = bld16(rB, (r < rowsB && b < kbe) ? r * rowB + b * MX_BLOB : MX_OOB, 0);
-  };
+  auto load_b = [&](int i, uint32_t s, bool in, u32x4* rb) { rb[i] = bld16(rB, in ? vb[i] : MX_OOB, s * 128u); };  // MX4 operands
   auto load_set = [&](Set& w, uint32_t s) {
     if constexpr (!ONE) {
+      const bool in = inside(s);
 #pragma unroll
-      for (int i = 0; i < NA; ++i) load_a(i, s, w.a, w.x);
+      for (int i = 0; i < NA; ++i) load_a(i, s, in, w.a, w.x);
       if constexpr (MX)
 #pragma unroll
-        for (int i = 0; i < NB; ++i) load_b(i, s, w.b);
+        for (int i = 0; i < NB; ++i) load_b(i, s, in, w.b);
     }
     if constexpr (MX) {
       // eight scale bytes a row: three dwords
+      const bool in = s * 8u < kbe;
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const uint32_t at = s * 8u < kbe ? (sbase[i] + s * 8u) & ~3u : MX_OOB;
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int d = 0; d < 3; ++d) w.s[i][MX ? d : 0] = bld_u32(rS[i], at + 4u * d, 0);
-      }
+        for (int d = 0; d < 3; ++d) w.s[i][MX ? d : 0] = bld_u32(rS[i], (in ? sbase[i] & ~3u : MX_OOB) + 4u * d, s * 8u);
     } else {
+      const bool in = s * 2u + static_cast<uint32_t>(tid & 1) < kbe;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const uint32_t c = static_cast<uint32_t>(tid + T * i), r = c >> 1, b = s * 2u + (c & 1u);
-        const bool ok = r < rowsB && b < kbe && c < 2u * RB;
-        w.b[i] = bld16(rB, ok ? r * rowB + b * MX_BLOB : MX_OOB, 0);
-        w.s[i][0] = bld_u8(rS[i], b < kbe ? sbase[i] + s * 2u : MX_OOB, 0);
+        w.b[i] = bld16(rB, in ? vb[i] : MX_OOB, s * 32u);
+        w.s[i][0] = bld_u8(rS[i], in ? sbase[i] : MX_OOB, s * 2u);
       }
     }
   };
   // Quarter d of the pieces of step s to LDS stage `st`; with one set of pieces, each piece's load for step s + 1
   auto part = [&](int d, uint32_t s, int st, const Set& w) {
     unsigned char* base = smem + st * Ti::STAGE;
+    const bool in = inside(s + 1);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
       if (i * 4 / NA != d) continue;
       u32x4 v = ONE ? oa[i] : w.a[ONE ? 0 : i];
       if constexpr (!MX && !AL) {
         const uint32_t k = s * 64u + spiece * 8u, r = srow + TR * i;
-        const uint32_t sh = (r * rowA + k * 2u + misA) & 3u;
+        const uint32_t sh = (r * rowA + misA) & 3u;  // a step's pieces start at multiples of 16 bytes of a row
         const u32x4 x = v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_alignbyte(e < 3 ? x[e + 1] : ONE ? ox[AL ? 0 : i] : w.x[ONE || AL ? 0 : i], x[e], sh);
@@ -166,14 +169,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
         }
       }
       *reinterpret_cast<u32x4*>(base + (srow + TR * i) * 128 + (tid & 7) * 16) = v;
-      if (ONE) load_a(i, s + 1, oa, ox);
+      if (ONE) load_a(i, s + 1, in, oa, ox);
     }
     if constexpr (MX) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         if (i * 4 / NB != d) continue;
         *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = ONE ? ob[i] : w.b[i];
-        if (ONE) load_b(i, s + 1, ob);
+        if (ONE) load_b(i, s + 1, in, ob);
       }
       if (d == 0) {
         const uint32_t b0 = s * 8u, n = b0 < kbe ? kbe - b0 : 0u;  // scales of blocks past K are 2^-127 on both sides: products of 0
@@ -181,7 +184,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           const int r = tid + T * i;
-          const uint32_t sh = (sbase[i] + b0) & 3u;
+          const uint32_t sh = sbase[i] & 3u;
           u32x2 v;
           v[0] = __builtin_amdgcn_alignbyte(w.s[i][MX ? 1 : 0], w.s[i][0], sh) & k0;
           v[1] = __builtin_amdgcn_alignbyte(w.s[i][MX ? 2 : 0], w.s[i][MX ? 1 : 0], sh) & k1;
@@ -272,10 +275,10 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   Set w[D];
   if constexpr (ONE) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) load_a(i, s0, oa, ox);
+    for (int i = 0; i < NA; ++i) load_a(i, s0, inside(s0), oa, ox);
     if constexpr (MX)
 #pragma unroll
-      for (int i = 0; i < NB; ++i) load_b(i, s0, ob);
+      for (int i = 0; i < NB; ++i) load_b(i, s0, inside(s0), ob);
   }
 #pragma unroll
   for (int i = 0; i < D; ++i) load_set(w[i], s0 + i);
@@ -394,6 +397,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
       const int r = x / PPR, p = x % PPR;
       const f32x4 lo = *reinterpret_cast<const f32x4*>(strip + r * PITCH + 8 * p), hi = *reinterpret_cast<const f32x4*>(strip + r * PITCH + 8 * p + 4);
       if (g.splits > 1) {
+        if (mw + 32 * i + r >= a.M) continue;
         const uint32_t o = split * BYTES + at + (static_cast<uint32_t>(i) * 32 * PPR + x) * 32u;
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, lo), rW, o, 0, COHERENT);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, hi), rW, o + 16, 0, COHERENT);
@@ -413,26 +417,39 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   if (tid == 0) s_last = __hip_atomic_fetch_add(cnt + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.splits - 1;
   __syncthreads();
   if (!s_last) return;
+  // 32 loads in flight: each batch costs a trip past the caches
+  constexpr int XB = TM * 32 * PPR / 64 < 4 ? TM * 32 * PPR / 64 : 4, SB = 16 / XB;
 #pragma unroll 1
-  for (int x = lane; x < TM * 32 * PPR; x += 64) {
-    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+  for (int x0 = lane; x0 < TM * 32 * PPR; x0 += 64 * XB) {
+    f32x4 lo[XB], hi[XB];
+#pragma unroll
+    for (int k = 0; k < XB; ++k) lo[k] = hi[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-    for (uint32_t s4 = 0; s4 < g.splits; s4 += 4) {  // four splits' loads in flight; past the last one zeros
-      f32x4 pl[4], ph[4];
+    for (uint32_t sp = 0; sp < g.splits; sp += SB) {  // past the last split zeros
+      f32x4 pl[XB][SB], ph[XB][SB];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t o = s4 + i < g.splits ? (s4 + i) * BYTES + at + x * 32u : MX_OOB;
-        pl[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, COHERENT));
-        ph[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, 0, COHERENT));
-      }
+      for (int k = 0; k < XB; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        lo += pl[i];
-        hi += ph[i];
-      }
+        for (uint32_t i = 0; i < SB; ++i) {
+          const int x = x0 + 64 * k;
+          const uint32_t o = sp + i < g.splits && mw + x / PPR < a.M ? (sp + i) * BYTES + at + x * 32u : MX_OOB;
+          pl[k][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o, 0, COHERENT));
+          ph[k][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rW, o + 16, 0, COHERENT));
+        }
+#pragma unroll
+      for (int k = 0; k < XB; ++k)
+#pragma unroll
+        for (int i = 0; i < SB; ++i) {
+          lo[k] += pl[k][i];
+          hi[k] += ph[k][i];
+        }
     }
-    float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    finish(x / PPR, x % PPR, v);
+#pragma unroll
+    for (int k = 0; k < XB; ++k) {
+      const int x = x0 + 64 * k;
+      float v[8] = {lo[k][0], lo[k][1], lo[k][2], lo[k][3], hi[k][0], hi[k][1], hi[k][2], hi[k][3]};
+      finish(x / PPR, x % PPR, v);
+    }
   }
   if (tid == 0) __hip_atomic_store(cnt + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -514,16 +531,10 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
                                        {{1, 0.60, 2.7, 3}, {2, 1.0, 5.1, 5}, {4, 2.1, 7.0, 12}}};
   double least = 0;
   for (const Cost& c : kCost[mx ? 1 : 0]) {
-#ifdef XRMM_TUNE
-    if (const char* e = getenv("MXT")) if (atoi(e) != c.t) continue;
-#endif
     const int64_t mt = (M + 64 * c.t - 1) / (64 * c.t), nt = (N + 64 * c.t - 1) / (64 * c.t), n = mt * nt;
     if (n > 0x3FFFFFFF) continue;
     for (int64_t s = 1; s <= 8; ++s) {
       if (s > 1 && (!have_ws || n > MX_COUNTERS / 4 || n * s > 2 * cus || steps < 4 * s)) break;
-#ifdef XRMM_TUNE
-      if (const char* e = getenv("MXS")) if (atoi(e) != s) continue;
-#endif
       MxPlan p{};
       p.t = c.t;
       p.mt = static_cast<uint32_t>(mt);
