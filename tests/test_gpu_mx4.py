@@ -250,6 +250,21 @@ def test_product_few_rows(gpu, M, K, N, dt):
     check_product(A.double().numpy(), codes, scales, bias, y)
 
 
+@pytest.mark.parametrize("M", [20, 33])
+@pytest.mark.parametrize("act", ["f16", "mx4"])
+def test_rows_past_the_tiled_products_k(gpu, M, act):
+    K, N = (1 << 21) + 96, 3
+    codes, scales = weights(N, K, 3, spread=1, center=119)
+    if act == "mx4":
+        ac, as_ = weights(M, K, 4, spread=1, center=124)
+        y = ops().matmul_mx4(ac, codes, scales, A_scales=as_, out_dtype=torch.float32)
+        A = LB.mx4_decode(ac.cpu().numpy(), as_.cpu().numpy())
+    else:
+        A = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).half()
+        y, A = ops().matmul_mx4(A.cuda(), codes, scales), A.double().numpy()
+    check_product(A, codes, scales, None, y)
+
+
 def test_kernel_names(gpu):
     assert ops().matmul_mx4_kernel(1, 4096, 4096).startswith("mx4_")
     with pytest.raises(ValueError):

@@ -82,48 +82,63 @@ hipError_t quantize_for(const MxQuantArgs& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Product, few rows. The weights are the MFMA's first operand: lane (c, g) = (lane % 16,
-// lane / 16) loads block 4 it + g of column c, 16 consecutive bytes, straight
-// into the fragment (the order of k inside an MFMA is free as long as both operands agree),
-// and the second operand's lane (c, g) holds the same block of row c. float16 / bfloat16
-// activations: each byte of codes becomes two 16-bit values times its block's scale in one
-// conversion instruction, v_mfma_f32_16x16x32 four times a block. MX4 activations: one
-// v_mfma_scale_f32_16x16x128 for the four blocks, scales applied by the instruction.
+// Product, up to 16 rows (and any number past the tiled product's K): a workgroup takes 16 rows and columns, its waves every WV-th group of four blocks along K. Nothing goes through
+// LDS until the waves' sums meet, so no wave waits for another, and K is not split over workgroups, whose exchange costs
+// three trips past the caches (8 to 10 us). The loop is short on purpose: the kernel lives for a few
+// microseconds, and code that is run once or twice is fetched slower than it runs (unrolled by four with loads ahead: 21 us at
+// 1 x 4096 x 14336 for 15).
 //
-// A wave takes every WV-th group of four blocks, with nothing in LDS until the waves' sums meet, so no wave waits
-// for another; sixteen waves a CU keep the loads in flight. The loop is short on purpose: the kernel
-// lives for a few microseconds, and code that is run once or twice is fetched slower than it runs (unrolled by four, loads
-// of the next four groups ahead: 21 us at 1 x 4096 x 14336 for 15 here; 8 x 4096 x 4096 8.6 for 7.6).
+// The weights are the MFMA's first operand. Lane (c, g) = (lane % 16, lane / 16) loads block g of column c, 16
+// consecutive bytes. MX4 activations are loaded alike, and one v_mfma_scale_f32_16x16x128 takes both with
+// their scales. 16-bit activations: eight values of a lane in the order of the weights' loads would lie 64 bytes from the
+// next lane's (28.5 us at 16 x 4096 x 14336 for 25.4, 23.2 at 16 x 14336 x 4096 for 22.2). So the
+// weights are transposed among the four lane groups (v_permlane swaps): lane (c, g) then
+// holds dword g of each block, and the activations' loads are runs of 64 bytes. Each byte of codes becomes two 16-bit values
+// times its block's scale in one conversion; v_mfma_f32_16x16x32 takes a block. What bounds it past four rows is the
+// activations' way from L2 to every CU (about 40 GB/s a CU).
 //
 // A bfloat16 holds every E2M1 value times 2^(byte - 127) exactly. A binary16 does for scales in
-// [2^-23, 2^13]; a workgroup that met another scale sums its share again, with weights in bfloat16 and the
+// [2^-23, 2^13]; a workgroup that met another scale sums everything again, with weights in bfloat16 and the
 // activations as the sum of two bfloat16 terms (8 and 3 bits: exact), so every scale is right.
 
+// (a, b) -> a's lower half and b's lower half, a's upper half and b's upper half; and the same of odd and even rows of 16 lanes
+__device__ __forceinline__ void mx_swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void mx_swap16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+
 template <int AT, int WV, bool AL>
-__global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a) {
+__global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a, uint32_t col_tiles) {
   constexpr bool MX = AT < 0;
+  typedef typename MxFrag<AT>::t frag;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x % col_tiles) * 16, m0 = static_cast<int64_t>(blockIdx.x / col_tiles) * 16;
   const uint32_t kb = static_cast<uint32_t>(a.kb), K = static_cast<uint32_t>(a.K);
-  const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < 16 ? a.N - n0 : 16), rowsA = static_cast<uint32_t>(a.M);  // at most 16
+  const uint32_t rowsB = static_cast<uint32_t>(a.N - n0 < 16 ? a.N - n0 : 16), rowsA = static_cast<uint32_t>(a.M - m0 < 16 ? a.M - m0 : 16);
   const uint32_t rowA = MX ? kb * MX_BLOB : K * 2u;
-  const uint32_t mis = AL ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.A)) & 3u;
-  const rsrc_t rA = mk_rsrc(static_cast<const uint8_t*>(a.A) - mis, (rowsA * rowA + mis + 3u) & ~3u);
+  const uint8_t* pA = static_cast<const uint8_t*>(a.A) + m0 * rowA;
+  const uint32_t mis = AL ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(pA)) & 3u;
+  const rsrc_t rA = mk_rsrc(pA - mis, (rowsA * rowA + mis + 3u) & ~3u);
   const rsrc_t rB = mk_rsrc(a.B + n0 * a.kb * MX_BLOB, rowsB * kb * MX_BLOB);
   const rsrc_t rS = mk_rsrc(a.S + n0 * a.kb, rowsB * kb);
-  const rsrc_t rT = mk_rsrc(MX ? a.As : a.S, MX ? rowsA * kb : 0u);
-  const uint32_t cb = static_cast<uint32_t>(c) < rowsB ? c * kb : MX_OOB / 16, ca = static_cast<uint32_t>(c);
-  const bool oka = ca < rowsA, okb = static_cast<uint32_t>(c) < rowsB;
-  typedef typename MxFrag<AT>::t frag;
+  const rsrc_t rT = mk_rsrc(MX ? a.As + m0 * a.kb : a.S, MX ? rowsA * kb : 0u);
+  const bool okb = static_cast<uint32_t>(c) < rowsB;
+  const uint32_t cb = c * kb;
 
-  // Piece d (eight values of K) of block b of the lane's row
-  auto piece = [&](uint32_t b, uint32_t d) {
-    const uint32_t k = b * MX_BLOCK + 8 * d, at = ca * rowA + k * 2u + mis;
+  // Eight values of K from k on of the lane's row
+  auto piece = [&](uint32_t k) {
+    const uint32_t at = c * rowA + k * 2u + mis;
+    const bool ok = static_cast<uint32_t>(c) < rowsA && k < K;
     if constexpr (AL) {  // K a multiple of 8: a piece is whole or absent
-      return bld16(rA, oka && b < kb && k < K ? at : MX_OOB, 0);
+      return bld16(rA, ok ? at : MX_OOB, 0);
     } else {
-      const bool ok = oka && b < kb && k < K;
       u32x4 v = bld16(rA, ok ? at & ~3u : MX_OOB, 0);
       const uint32_t x = bld_u32(rA, ok ? (at & ~3u) + 16u : MX_OOB, 0);
 #pragma unroll
@@ -137,25 +152,43 @@ __global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a) {
 
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   bool misfit = false;
-#pragma unroll 1
-  for (uint32_t b = wave * 4 + g; b - g < kb; b += WV * 4) {
+  u32x4 w;
+  uint32_t s;
+  auto load = [&](uint32_t b) {
     const bool ok = okb && b < kb;
-    const u32x4 w = bld16_nt(rB, ok ? (cb + b) * MX_BLOB : MX_OOB, 0);
-    const uint32_t s = bld_u8(rS, ok ? cb + b : MX_OOB, 0);
+    w = bld16_nt(rB, ok ? (cb + b) * MX_BLOB : MX_OOB, 0);
+    s = bld_u8(rS, ok ? cb + b : MX_OOB, 0);
+  };
+  load(wave * 4 + g);
+#pragma unroll 1
+  for (uint32_t b0 = wave * 4; b0 < kb; b0 += WV * 4) {
+    const uint32_t nb = b0 + WV * 4 + g;
     if constexpr (MX) {
-      const bool have = oka && b < kb;
-      const u32x4 x = bld16(rA, have ? (ca * kb + b) * MX_BLOB : MX_OOB, 0);
-      const uint32_t t = bld_u8(rT, have ? ca * kb + b : MX_OOB, 0);
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_fp4(w), mx_fp4(x), acc, 4, 4, 0, static_cast<int>(s), 0, static_cast<int>(t));
+      const bool have = static_cast<uint32_t>(c) < rowsA && b0 + g < kb;
+      const u32x4 x = bld16(rA, have ? (cb + b0 + g) * MX_BLOB : MX_OOB, 0), wc = w;
+      const uint32_t t = bld_u8(rT, have ? cb + b0 + g : MX_OOB, 0), sc = s;
+      load(nb);
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_fp4(wc), mx_fp4(x), acc, 4, 4, 0, static_cast<int>(sc), 0, static_cast<int>(t));
     } else {
       u32x4 x[4];
 #pragma unroll
-      for (uint32_t d = 0; d < 4; ++d) x[d] = piece(b, d);
+      for (uint32_t d = 0; d < 4; ++d) x[d] = piece((b0 + d) * MX_BLOCK + 8 * g);
+      uint32_t y[4] = {w[0], w[1], w[2], w[3]}, s1 = s << (8 * g);
       if (AT == LT_F16) misfit |= !mx_f16_fits(s, w);
-      const float sf = e8m0(s);
+      load(nb);
+      mx_swap32(y[0], y[2]);
+      mx_swap32(y[1], y[3]);
+      mx_swap16(y[0], y[1]);
+      mx_swap16(y[2], y[3]);
+      uint32_t s2 = s1;
+      mx_swap32(s1, s2);
+      s1 |= s2;
+      s2 = s1;
+      mx_swap16(s1, s2);
+      s1 |= s2;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        const frag wf = mx_dq8<AT>(w[d], sf);
+        const frag wf = mx_dq8<AT>(y[d], e8m0((s1 >> (8 * d)) & 255u));
         if constexpr (AT == LT_F16) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(f16x8, x[d]), acc, 0, 0, 0);
         else acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, __builtin_bit_cast(bf16x8, x[d]), acc, 0, 0, 0);
       }
@@ -165,13 +198,11 @@ __global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a) {
     if (__syncthreads_or(misfit)) {
       acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-      for (uint32_t q = (wave * 4 + g) * 4; (q >> 2) - g < kb; q += (q & 3u) == 3u ? WV * 16 - 3 : 1) {
-        const uint32_t b = q >> 2, d = q & 3u;
-        const bool ok = okb && b < kb;
-        const float sf = e8m0(bld_u8(rS, ok ? cb + b : MX_OOB, 0));
-        const bf16x8 wf = mx_dq8<LT_BF16>(bld_u32(rB, ok ? (cb + b) * MX_BLOB + 4 * d : MX_OOB, 0), sf);
+      for (uint32_t q = wave; q < kb; q += WV) {  // one block at a time
+        const float sf = e8m0(bld_u8(rS, okb ? cb + q : MX_OOB, 0));
+        const bf16x8 wf = mx_dq8<LT_BF16>(bld_u32(rB, okb ? (cb + q) * MX_BLOB + 4 * g : MX_OOB, 0), sf);
         bf16x8 hi, lo;
-        split_f16(__builtin_bit_cast(f16x8, piece(b, d)), hi, lo);
+        split_f16(__builtin_bit_cast(f16x8, piece(q * MX_BLOCK + 8 * g)), hi, lo);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, hi, acc, 0, 0, 0);
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, lo, acc, 0, 0, 0);
       }
@@ -182,14 +213,14 @@ __global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a) {
   __shared__ f32x4 red[WV][64];
   red[wave][lane] = acc;
   __syncthreads();
-  if (wave != 0 || c >= a.M) return;
+  const int64_t m = m0 + c, n = n0 + g * 4;
+  if (wave != 0 || m >= a.M) return;
   f32x4 v = red[0][lane];
 #pragma unroll
-  for (int w = 1; w < WV; ++w) v += red[w][lane];
-  const int64_t n = n0 + g * 4;
+  for (int w2 = 1; w2 < WV; ++w2) v += red[w2][lane];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (n + e < a.N) st_lt(a.Y, c * a.N + n + e, v[e] + (a.bias ? ld_lt(a.bias, n + e, a.out) : 0.f), a.out);
+    if (n + e < a.N) st_lt(a.Y, m * a.N + n + e, v[e] + (a.bias ? ld_lt(a.bias, n + e, a.out) : 0.f), a.out);
 }
 
 // ---------------------------------------------------------------------------
@@ -328,14 +359,16 @@ hipError_t dot_for(const MxArgs& a, hipStream_t st) {
   }
 }
 
-constexpr int MXR_WAVES = 8;
+constexpr int MXR_WAVES = 8;  // sixteen: 26.2 for 25.4 us at 16 x 4096 x 14336
 
 template <int AT>
 hipError_t rows_for(const MxArgs& a, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>((a.N + 15) / 16)), block(64 * MXR_WAVES);
+  const int64_t ct = (a.N + 15) / 16, n = ct * ((a.M + 15) / 16);
+  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<uint32_t>(n)), block(64 * MXR_WAVES);
   const bool al = a.K % 8 == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15u) == 0;
-  if (AT < 0 || al) k_mx4_rows<AT, MXR_WAVES, true><<<grid, block, 0, st>>>(a);
-  else if constexpr (AT >= 0) k_mx4_rows<AT, MXR_WAVES, false><<<grid, block, 0, st>>>(a);
+  if (AT < 0 || al) k_mx4_rows<AT, MXR_WAVES, true><<<grid, block, 0, st>>>(a, static_cast<uint32_t>(ct));
+  else if constexpr (AT >= 0) k_mx4_rows<AT, MXR_WAVES, false><<<grid, block, 0, st>>>(a, static_cast<uint32_t>(ct));
   return hipGetLastError();
 }
 
