@@ -585,6 +585,10 @@ struct KvTile {
   static constexpr int64_t PART = KVM_ROWS * (D + 2) * 4;
 };
 
+// The slot of a token's K piece: a fragment reads one piece of eight consecutive tokens, a thread stores pieces 2 p and 2 p + 1
+// of one, eight p after each other; both meet eight different columns of the banks.
+__device__ __forceinline__ int kv_kslot(int t, int piece) { return piece ^ ((t ^ (piece >> 3)) & 7); }
+
 template <int D>
 __device__ __forceinline__ int kv_vslot(int d, int piece) {
   return KvTile<D>::TT == 64 ? piece ^ ((d ^ (d >> 3)) & 7) : piece ^ (((d >> 1) ^ (d >> 3)) & 3);
@@ -625,51 +629,56 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   const int wlo = row_lo(query(w0)), whi = live ? row_hi(query(w0 + 31)) : 0, full_lo = row_lo(query(w0 + 31)), full_hi = row_hi(query(w0));
 
   // ---- moving a tile: K pieces of 16 codes of a token, V pieces of four tokens by eight d
-  // Everything of a tile is loaded together, from pages looked up a tile before: one for each 16 tokens.
+  // Everything of a tile is loaded together, from pages looked up a tile before. Lane l looks up the page of the 16 tokens
+  // l % GR and loads one scale of theirs, K's or (l & GR) V's; what a wave needs of them it reads from the lanes.
   uint32_t kc[KN][4], vc[VN][8];
-  float ksn[GR], vsn[GR];     // the loaded tile's scales
-  uint32_t none_n = 0;        // and its 16-token groups in no page, a bit each
-  int32_t pg[GR];             // pages of the tile to be loaded next
+  int32_t pgl;                 // this lane's page of the tile to be loaded next
+  float scn;                   // this lane's scale of the loaded tile
+  uint32_t none_n = 0;         // the loaded tile's 16-token groups in no page, a bit each
   bool bad = false;
+  const int lg = lane & (GR - 1);
   auto find = [&](int t0) {
-#pragma unroll
-    for (int u = 0; u < GR; ++u) {
-      const int32_t p = kv_page(c, b, t0 + 16 * u);
-      pg[u] = t0 + 16 * u < thi ? p : -2;
-    }
-  };
-  auto page_of = [&](int t) {  // of token t of the tile, page 0 where there is none
-    const int32_t p0 = pg[0], p1 = pg[1], p2 = pg[GR - 2], p3 = pg[GR - 1];
-    int32_t p = (t & 16) != 0 ? p1 : p0;
-    if (GR == 4 && (t & 32) != 0) p = (t & 16) != 0 ? p3 : p2;
-    return static_cast<uint32_t>(p < 0 ? 0 : p);
+    const int32_t p = kv_page(c, b, t0 + 16 * lg);
+    pgl = t0 + 16 * lg < thi ? p : -2;
   };
   const uint32_t page_bytes = static_cast<uint32_t>(c.page) * D;  // of one head
-  auto code = [&](const uint8_t* base, int t0, int t, int d) {    // where d of token t0 + t lies
-    const uint64_t at = static_cast<uint64_t>(page_of(t)) * static_cast<uint32_t>(c.Hkv) + static_cast<uint32_t>(h);
-    return base + at * page_bytes + (static_cast<uint32_t>((t0 + t) & (c.page - 1)) * D + static_cast<uint32_t>(d));
+  auto page_of = [&](int u) {  // of a group, page 0 where there is none
+    const int32_t p = __builtin_amdgcn_readlane(pgl, u);
+    return static_cast<uint32_t>(p < 0 ? 0 : p);
+  };
+  // where the first code of a group of 16 tokens lies
+  auto group = [&](const uint8_t* base, int t0, int u) {
+    const uint64_t at = static_cast<uint64_t>(page_of(u)) * static_cast<uint32_t>(c.Hkv) + static_cast<uint32_t>(h);
+    return base + at * page_bytes + static_cast<uint32_t>((t0 + 16 * u) & (c.page - 1)) * D;
+  };
+  // The group of a thread's piece: one for the wave where its 64 pieces lie in 16 tokens, else chosen by lane.
+  constexpr int KPT = D / 16, VPT = D / 32;  // K pieces of a token, V pieces (of four tokens) a token
+  auto src_of = [&](const uint8_t* base, int t0, int x0, int per, int t, uint32_t off) {  // x0: the wave's first piece
+    if (16 * per % 64 == 0) return group(base, t0, x0 / (16 * per)) + off;
+    const uint8_t* g0 = group(base, t0, 0);
+    const uint8_t* g1 = group(base, t0, 1);
+    const uint8_t* g2 = group(base, t0, GR - 2);
+    const uint8_t* g3 = group(base, t0, GR - 1);
+    const uint8_t* r = (t & 16) != 0 ? g1 : g0;
+    if (GR == 4 && (t & 32) != 0) r = (t & 16) != 0 ? g3 : g2;
+    return r + off;
   };
   auto load = [&](int t0) {
-    none_n = 0;
-#pragma unroll
-    for (int u = 0; u < GR; ++u) {
-      const int64_t at = static_cast<int64_t>(pg[u] < 0 ? 0 : pg[u]) * c.Hkv + h;
-      ksn[u] = c.ks[at];
-      vsn[u] = c.vs[at];
-      none_n |= pg[u] < 0 ? 1u << u : 0u;
-      bad |= pg[u] == -1;
-    }
+    const int64_t at = static_cast<int64_t>(pgl < 0 ? 0 : pgl) * c.Hkv + h;
+    scn = (lane & GR) != 0 ? c.vs[at] : c.ks[at];
+    none_n = static_cast<uint32_t>(__ballot(pgl < 0)) & ((1u << GR) - 1u);
+    bad |= pgl == -1;
 #pragma unroll
     for (int i = 0; i < KN; ++i) {
-      const int x = tid + KVM_T * i;
-      const u32x4 v = ld16(code(c.k, t0, x / (D / 16), x % (D / 16) * 16));
+      const int x = tid + KVM_T * i, t = x / KPT;
+      const u32x4 v = ld16(src_of(c.k, t0, 64 * wave + KVM_T * i, KPT, t, static_cast<uint32_t>(t % 16 * D + x % KPT * 16)));
 #pragma unroll
       for (int e = 0; e < 4; ++e) kc[i][e] = v[e];
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
-      const int x = tid + KVM_T * i;
-      const uint8_t* src = code(c.v, t0, x / (D / 8) * 4, x % (D / 8) * 8);
+      const int x = tid + KVM_T * i, t = x / (4 * VPT) * 4;
+      const uint8_t* src = src_of(c.v, t0, 64 * wave + KVM_T * i, VPT, t, static_cast<uint32_t>(t % 16 * D + x % (4 * VPT) * 8));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const u32x2 v = *reinterpret_cast<const u32x2*>(src + e * D);
@@ -685,8 +694,8 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     for (int i = 0; i < KN; ++i) {
       const int x = tid + KVM_T * i, t = x / (D / 16), p = x % (D / 16);
       if (KN * KVM_T > TT * (D / 16) && t >= TT) break;
-      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + ((2 * p) ^ (t & 7)) * 16) = cat8(kv_half4<FP8>(kc[i][0]), kv_half4<FP8>(kc[i][1]));
-      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + ((2 * p + 1) ^ (t & 7)) * 16) = cat8(kv_half4<FP8>(kc[i][2]), kv_half4<FP8>(kc[i][3]));
+      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + kv_kslot(t, 2 * p) * 16) = cat8(kv_half4<FP8>(kc[i][0]), kv_half4<FP8>(kc[i][1]));
+      *reinterpret_cast<f16x8*>(ks + t * Ti::KP + kv_kslot(t, 2 * p + 1) * 16) = cat8(kv_half4<FP8>(kc[i][2]), kv_half4<FP8>(kc[i][3]));
     }
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
@@ -774,16 +783,12 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;
-  float vref = 0.f;  // the value scale that the sums are in units of
-  // scales and missing groups of the tile in LDS
-  float ksc[GR], vsc[GR];
+  float vref = 0.f, vinv = 0.f;  // the value scale that the sums are in units of, and KV_P times its inverse
+  // scale (as scn) and missing groups of the tile in LDS
+  float scl;
   uint32_t none;
   auto take = [&] {
-#pragma unroll
-    for (int u = 0; u < GR; ++u) {
-      ksc[u] = ksn[u];
-      vsc[u] = vsn[u];
-    }
+    scl = scn;
     none = none_n;
   };
   store(tlo, 0);
@@ -816,28 +821,32 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     for (int x = 0; x < D / 16; ++x)
 #pragma unroll
       for (int u = 0; u < TT / 32; ++u) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + (((2 * x + hf) ^ (col & 7)) * 16));
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + kv_kslot(col, 2 * x + hf) * 16);
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], x == 0 ? f32x16{} : s[u], 0, 0, 0);
       }
     const uint32_t no = none;
-    float kq[GR], vw[GR];
-    const float ref = vref;
-    bool plain = true;  // factors of the usual kind: see below
+    const float ref = vref, sc = scl;
+    // a value scale above all before it: the sums go into its units (a wave's own: its sums alone are in these)
+    {
+      float vtop = 0.f;
 #pragma unroll
-    for (int u = 0; u < GR; ++u) {
-      kq[u] = qs * ksc[u];
-      vw[u] = vsc[u];
-      if ((no >> u & 1u) == 0 && vsc[u] > vref && vsc[u] <= 3.4028235e38f) vref = vsc[u];  // a wave's own: its sums alone are in these units
+      for (int u = 0; u < GR; ++u) {
+        const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sc), GR + u));
+        vtop = (no >> u & 1u) == 0 && v <= 3.4028235e38f ? fmaxf(vtop, v) : vtop;
+      }
+      if (vtop > vref) {
+        vref = vtop;
+        vinv = KV_P / vref;
+      }
     }
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-    for (int u = 0; u < GR; ++u) {
-      vw[u] *= inv * KV_P;
-      plain &= kq[u] >= 0.f && vw[u] >= 0x1p-8f && vw[u] <= KV_P;
-    }
+    // lane-wise: K's factor of the rows' scores, or V's of their weights; its logarithm and inverse
+    const float wl = sc * vinv, lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
+    // factors of the usual kind, no masks: see below
+    const bool usual = (lane & GR) != 0 ? wl >= 0x1p-8f && wl <= 1.001f * KV_P : sc >= 0.f && a.scale >= 0.f;
+    const bool plain = (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && no == 0 && t0 >= full_lo && t0 + TT <= full_hi;
+    auto of = [&](float x, int u) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), u)); };
     move();
     {
-      plain = __all(plain && !(t0 < full_lo || t0 + TT > full_hi || no != 0));
       float top = -__builtin_inff();
       if (plain) {
         // no masks, key factors not negative: a group's largest score is its largest sum's
@@ -846,7 +855,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
           float x = s[u / 2][8 * (u & 1)];
 #pragma unroll
           for (int e = 1; e < 8; ++e) x = fmaxf(x, s[u / 2][8 * (u & 1) + e]);
-          top = fmaxf(top, x * kq[u]);
+          top = fmaxf(top, x * (qs * of(sc, u)));
         }
       } else {
 #pragma unroll
@@ -855,7 +864,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
           for (int e = 0; e < 16; ++e) {
             const int tok = 32 * u + 8 * (e >> 2) + 4 * hf + (e & 3);
             const bool out = (no >> (2 * u + (e >> 3)) & 1u) != 0 || t0 + tok < lo || t0 + tok >= hi;
-            s[u][e] = out ? -__builtin_inff() : s[u][e] * kq[2 * u + (e >> 3)];
+            s[u][e] = out ? -__builtin_inff() : s[u][e] * (qs * of(sc, 2 * u + (e >> 3)));
             top = fmaxf(top, s[u][e]);
           }
       }
@@ -876,11 +885,11 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
       for (int u = 0; u < TT / 32; ++u)
 #pragma unroll
         for (int sl = 0; sl < 2; ++sl) {
-          const float w = vw[2 * u + sl];
+          const int gu = 2 * u + sl;
           f16x8 pf;
           if (plain) {
             // the exponential with the value's factor in its exponent: one multiply-add and one exponential a weight
-            const float kf = kq[2 * u + sl], lw = __builtin_amdgcn_logf(w) - base;  // log2
+            const float kf = qs * of(sc, gu), lw = of(lwl, GR + gu) - base;
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -891,8 +900,9 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
               pf[e] = h2[0];
               pf[e + 1] = h2[1];
             }
-            l += sum * __builtin_amdgcn_rcpf(w);
+            l += sum * of(rwl, GR + gu);
           } else {
+            const float w = of(wl, GR + gu);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float v = s[u][8 * sl + e], p = __builtin_amdgcn_exp2f(v - base);
