@@ -186,6 +186,19 @@ def test_attention(gpu, kind, dt, lens, counts, Hq, Hkv, D, page, window):
         check_attention(c, q, counts, True, window=window)
 
 
+@pytest.mark.parametrize("kind,dt,D,L,window", [("int8", "f16", 64, 2000, 0), ("e4m3", "bf16", 128, 2500, 0), ("int8", "bf16", 96, 3000, 1800),
+                                                ("e4m3", "f16", 256, 1500, 0)])
+def test_attention_many_rows_with_tokens_split(gpu, kind, dt, D, L, window):
+    """Rows enough for tiles of 128 and too few of them to fill the card: their tokens are split and joined."""
+    n, Hq = 520, 8
+    c = Cache(kind, [L], 1, D, 64, seed=D, scales="any")
+    c.vs[c.table[0, 3]] *= np.float32(64.0)  # the parts' sums are in units of different value scales
+    need = ops().kv8_attention_workspace_bytes(n, Hq, 1, D, batch=1, table_width=c.table.shape[1], page_size=64, window=window)
+    assert need > 4096 and (need - 4096) % (128 * (D + 2) * 4) == 0
+    q = torch.randn(n, Hq, D, generator=torch.Generator().manual_seed(D)).to(DT[dt]).cuda()
+    check_attention(c, q, [n], False, window=window)
+
+
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("counts", [[1, 1], [40, 25]])
 def test_attention_not_causal_and_other_scale(gpu, kind, counts):

@@ -1008,41 +1008,60 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   }
 }
 
+// Tokens are split only as far as the card has room for more workgroups at once: a start, a join and the code's own fetch
+// cost more than even shares gain (one sequence of 65000: 129 us in shares of 256 tokens, 83 of 512, 57 of 1024, 39 of 2048,
+// one a CU; 48 of up to 8000: 227 us in shares of 1024, 170 of 2048, 108 unsplit; 8 of 4000: 35 of 512, 25 of 1024, 32 of 2048).
+// Up to 16 rows of a key head take k_kv8_rows, more whichever is estimated faster (us; measured at head size 128):
+//   rows: for each round of the CUs 7, and the share's tokens at 75 a us; a join 5
+//   tile: for each round of two workgroups a CU (heads of 256: one) 10, and the tokens at 36, 28, 24 or 18 a us with one to four
+//         waves in use; a join 3 and 2 a part (its parts of 128 rows are read one after the other)
+// 8 to 32 new tokens on 30000 with four heads a group: 41 to 79 us by rows, 89 to 184 by tiles; 32 sequences with 16 and 32 on 1000:
+// 89 and 172 by rows, 43 and 56 by tiles.
 struct KvPlan {
   bool tile;  // k_kv8_tile, else k_kv8_rows
   int64_t row_tiles, splits, chunk, ws_bytes;
+  double time;
 };
 
-// Up to 16 rows of a key head take k_kv8_rows. Tokens are split only as far as the card has room for more
-// workgroups at once (a start, a join and the code's own fetch cost more than even shares gain): one of k_kv8_rows a CU, two of k_kv8_tile
-// (heads of 256: one). One sequence of 65000: 129 us in shares of 256 tokens, 83 of 512, 57 of 1024, 39 of 2048 (one a
-// CU); 48 of up to 8000: 227 us in shares of 1024, 170 of 2048, 108 unsplit; 8 of 4000: 35 of 512, 25 of 1024, 32 of 2048.
-KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
-  const int64_t G = a.Hq / a.c.Hkv, cus = device_cus() > 0 ? device_cus() : 256;
+KvPlan kind_plan(const KvAttnArgs& a, bool have_ws, bool tile) {
+  const int64_t nrows = static_cast<int64_t>(a.max_new) * (a.Hq / a.c.Hkv), cus = device_cus() > 0 ? device_cus() : 256;
+  const int64_t rows = tile ? KVM_ROWS : 16;
   KvPlan p{};
-  p.tile = a.max_new * G > 16;
-  const int64_t rows = p.tile ? KVM_ROWS : 16;
-  p.row_tiles = (a.max_new * G + rows - 1) / rows;
+  p.tile = tile;
+  p.row_tiles = (nrows + rows - 1) / rows;
   const int64_t units = p.row_tiles * a.c.Hkv * a.c.B;
   int64_t span = static_cast<int64_t>(a.c.width) << a.c.page_log2;
   if (a.window > 0) {  // what the rows' windows cover, from a multiple of a tile's tokens on
     const int64_t seen = static_cast<int64_t>(a.window) + (a.causal ? rows : a.max_new) + 64;
     span = span < seen ? span : seen;
   }
-  p.splits = 1;
-  p.chunk = span > 0 ? span : 1;
-  if (have_ws && units * 4 <= KV_COUNTERS && span > KVR_PASS) {
-    const int64_t room = p.tile && a.c.D <= 128 ? 2 * cus : cus, want = room / units > 1 ? room / units : 1;
-    int64_t chunk = ((span + want - 1) / want + KVR_PASS - 1) / KVR_PASS * KVR_PASS;
-    if (p.tile && chunk < 2 * KVR_PASS) chunk = 2 * KVR_PASS;
-    const int64_t s = (span + chunk - 1) / chunk;
-    if (s > 1) {
-      p.splits = s;
+  span = span > 0 ? span : 1;
+  const int64_t room = tile && a.c.D <= 128 ? 2 * cus : cus;
+  const int live = nrows < KVM_ROWS ? static_cast<int>((nrows + 31) / 32) : 4;
+  static constexpr double kTile[5] = {0, 36, 28, 24, 18};
+  const double rate = tile ? kTile[live] : 75.0, start = tile ? 10.0 : 7.0, wide = a.c.D > 128 ? 2.0 : 1.0;
+  const bool can = have_ws && units * 4 <= KV_COUNTERS && span > KVR_PASS && units < room;
+  const int64_t most = can ? room / units : 1;
+  for (int64_t want = tile ? 1 : most; want <= most; want = tile ? want + (want + 3) / 4 : want + 1) {
+    int64_t chunk = want > 1 ? ((span + want - 1) / want + KVR_PASS - 1) / KVR_PASS * KVR_PASS : span;
+    const int64_t parts = (span + chunk - 1) / chunk;
+    const double time = static_cast<double>((units * parts + room - 1) / room) * (start + wide * static_cast<double>(chunk) / rate) +
+                        (parts == 1 ? 0.0 : tile ? 3.0 + 2.0 * static_cast<double>(parts) : 5.0);
+    if (p.splits == 0 || time < p.time) {
+      p.splits = parts;
       p.chunk = chunk;
-      p.ws_bytes = KV_COUNTERS + units * s * rows * (a.c.D + 2) * 4;
+      p.time = time;
+      p.ws_bytes = parts > 1 ? KV_COUNTERS + units * parts * rows * (a.c.D + 2) * 4 : 0;
     }
   }
   return p;
+}
+
+KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
+  const KvPlan rows = kind_plan(a, have_ws, false);
+  if (static_cast<int64_t>(a.max_new) * (a.Hq / a.c.Hkv) <= 16) return rows;
+  const KvPlan tile = kind_plan(a, have_ws, true);
+  return tile.time < rows.time ? tile : rows;
 }
 
 template <int D, bool FP8>
