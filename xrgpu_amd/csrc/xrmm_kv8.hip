@@ -229,8 +229,7 @@ __device__ __forceinline__ KvBytes<N> kv_bytes(const uint8_t* p) {
 // page after that looked up. Workgroups of one (sequence, head, rows) leave their
 // unnormalised outputs, maxima and sums in the workspace, and the last to arrive joins them in
 // token order.
-constexpr int KVR_WAVES = 8;
-constexpr int KVR_PASS = KVR_WAVES * KVT;  // tokens of a step of all waves
+constexpr int KVR_PASS = 8 * KVT;  // shares of tokens are multiples of it: a step of all waves, eight at most
 constexpr int64_t KV_COUNTERS = 4096;      // bytes of arrival counters at the head of the workspace
 
 template <int D>
@@ -244,8 +243,8 @@ struct KvStep {
   KvBytes<D / 16> v[8];
 };
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+template <int D, bool FP8, int W>
+__global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
   constexpr int KD = D / 4, VD = D / 16;  // codes of a token that a lane holds
   const KvCache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
@@ -299,7 +298,7 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   KvStep<D> cur;
   find(tlo + wave * KVT, pg);
   load(cur, pg, tlo + wave * KVT);
-  find(tlo + wave * KVT + KVR_PASS, pg);
+  find(tlo + wave * KVT + (W * KVT), pg);
 
   // this lane's row: its query as binary16 (scaled by a power of two for bfloat16), what it sees
   f16x8 q[KD / 8];
@@ -348,10 +347,10 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   bool bad = false;
 
 #pragma unroll 1
-  for (int t0 = tlo + wave * KVT; t0 < thi; t0 += KVR_PASS) {
+  for (int t0 = tlo + wave * KVT; t0 < thi; t0 += (W * KVT)) {
     KvStep<D> nxt;
-    load(nxt, pg, t0 + KVR_PASS);
-    find(t0 + 2 * KVR_PASS, pg);
+    load(nxt, pg, t0 + (W * KVT));
+    find(t0 + 2 * (W * KVT), pg);
     bad |= cur.pg[0] == -1 || cur.pg[1] == -1;
     // scores
     f32x4 s[2];
@@ -433,8 +432,8 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
 
   // The waves' parts meet in LDS. Sums of rows: over the four lanes of a column, then the waves.
   constexpr int JT = VD < 8 ? VD : 8;  // output tiles of a round
-  __shared__ float wm[KVR_WAVES][16], wl[KVR_WAVES][16];
-  __shared__ f32x4 red[KVR_WAVES][JT][64];
+  __shared__ float wm[W][16], wl[W][16];
+  __shared__ f32x4 red[W][JT][64];
   __shared__ float row[16][D];
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
@@ -445,11 +444,11 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   __syncthreads();
   float top = wm[0][col];
 #pragma unroll
-  for (int w = 1; w < KVR_WAVES; ++w) top = fmaxf(top, wm[w][col]);
+  for (int w = 1; w < W; ++w) top = fmaxf(top, wm[w][col]);
   const float base = top == -__builtin_inff() ? 0.f : top;
   float sum = 0.f;
 #pragma unroll
-  for (int w = 0; w < KVR_WAVES; ++w) sum += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - base);
+  for (int w = 0; w < W; ++w) sum += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - base);
   const float mine = __builtin_amdgcn_exp2f(m - base) * vref * (1.f / KV_P);
 #pragma unroll
   for (int j0 = 0; j0 < VD; j0 += JT) {
@@ -457,12 +456,13 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
 #pragma unroll
     for (int j = 0; j < JT; ++j) red[wave][j][lane] = o[j0 + j] * mine;
     __syncthreads();
-    if (wave < JT) {  // wave w finishes tile j0 + w
-      f32x4 v = red[0][wave][lane];
+#pragma unroll 1
+    for (int j = wave; j < JT; j += W) {  // the waves finish a tile each
+      f32x4 v = red[0][j][lane];
 #pragma unroll
-      for (int w = 1; w < KVR_WAVES; ++w) v += red[w][wave][lane];
+      for (int w = 1; w < W; ++w) v += red[w][j][lane];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) row[col][VD * (4 * g + e) + j0 + wave] = v[e];
+      for (int e = 0; e < 4; ++e) row[col][VD * (4 * g + e) + j0 + j] = v[e];
     }
   }
   // sums of this workgroup's tokens: the rows' outputs in `row`, maxima and sums where wave is 0 and g is 0
@@ -482,7 +482,7 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   };
   if (parts == 1) {
 #pragma unroll 1
-    for (int p = tid; p < pieces; p += 64 * KVR_WAVES) put(p, *reinterpret_cast<const f32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]), rl[p / (D / 4)]);
+    for (int p = tid; p < pieces; p += 64 * W) put(p, *reinterpret_cast<const f32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]), rl[p / (D / 4)]);
     return;
   }
   constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   uint32_t* cnt = static_cast<uint32_t*>(a.ws);
   const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + KV_COUNTERS + static_cast<int64_t>(unit) * splits * PART, splits * PART);
 #pragma unroll 1
-  for (int p = tid; p < pieces; p += 64 * KVR_WAVES)
+  for (int p = tid; p < pieces; p += 64 * W)
     __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]), rW, split * PART + p * 16, 0, COHERENT);
   if (tid < rows) {
     const u32x2 ml = {__builtin_bit_cast(uint32_t, rm[tid]), __builtin_bit_cast(uint32_t, rl[tid])};
@@ -504,12 +504,12 @@ __global__ __launch_bounds__(64 * KVR_WAVES, 2) void k_kv8_rows(KvAttnArgs a, ui
   if (!s_last) return;
   if (tid == 0) __hip_atomic_store(cnt + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // The join: `groups` groups of threads take every groups-th part each, four parts' loads in flight, then meet in LDS.
-  const int groups = pieces < 64 * KVR_WAVES ? 64 * KVR_WAVES / pieces : 1;
+  const int groups = pieces < 64 * W ? 64 * W / pieces : 1;
   f32x4* jo = &red[0][0][0];                                                 // [512]
-  float *jm = reinterpret_cast<float*>(jo + 64 * KVR_WAVES), *jl = jm + 64 * KVR_WAVES;  // [512] each
-  static_assert(sizeof(red) >= 64 * KVR_WAVES * 24, "the join fits the waves' sums");
+  float *jm = reinterpret_cast<float*>(jo + 64 * W), *jl = jm + 64 * W;  // [512] each
+  static_assert(sizeof(red) >= 64 * W * 24, "the join fits the waves' sums");
 #pragma unroll 1
-  for (int p0 = 0; p0 < pieces; p0 += 64 * KVR_WAVES) {
+  for (int p0 = 0; p0 < pieces; p0 += 64 * W) {
     const int p = p0 + (groups > 1 ? tid % pieces : tid), grp = groups > 1 ? tid / pieces : 0;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     float vm = -__builtin_inff(), vl = 0.f;
@@ -1019,6 +1019,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 // 89 and 172 by rows, 43 and 56 by tiles.
 struct KvPlan {
   bool tile;  // k_kv8_tile, else k_kv8_rows
+  int waves;  // of k_kv8_rows
   int64_t row_tiles, splits, chunk, ws_bytes;
   double time;
 };
@@ -1054,6 +1055,10 @@ KvPlan kind_plan(const KvAttnArgs& a, bool have_ws, bool tile) {
       p.ws_bytes = parts > 1 ? KV_COUNTERS + units * parts * rows * (a.c.D + 2) * 4 : 0;
     }
   }
+  // Waves: two for a share of 64 tokens, four up to 256, and to 2048 where that keeps more than one workgroup a CU resident (us with
+  // 8, 4 and 2 at 47 sequences of 12 tokens: 15.5, 10.1, 9.1; 100: 19.4, 12.8, 12.8; 400: 28, 21, 23; 1500: 51, 41, 60; 48
+  // of up to 8000: 109, 131, 214; one of 65000: 40, 47, 72).
+  p.waves = p.chunk <= 2 * KVT ? 2 : p.chunk <= 8 * KVT || (p.chunk <= 2048 && units * p.splits > cus) ? 4 : 8;
   return p;
 }
 
@@ -1071,7 +1076,11 @@ hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(n));
   const uint32_t rt = static_cast<uint32_t>(p.row_tiles), sp = static_cast<uint32_t>(p.splits), ch = static_cast<uint32_t>(p.chunk);
   if (!p.tile) {
-    k_kv8_rows<D, FP8><<<grid, 64 * KVR_WAVES, 0, st>>>(a, rt, sp, ch);
+    switch (p.waves) {
+      case 2: k_kv8_rows<D, FP8, 2><<<grid, 128, 0, st>>>(a, rt, sp, ch); break;
+      case 4: k_kv8_rows<D, FP8, 4><<<grid, 256, 0, st>>>(a, rt, sp, ch); break;
+      default: k_kv8_rows<D, FP8, 8><<<grid, 512, 0, st>>>(a, rt, sp, ch);
+    }
     return hipGetLastError();
   }
   constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16), lds = 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
