@@ -6,8 +6,7 @@
 // in slot p ^ (r % 8), which spreads a fragment's rows over all banks without padding.
 //
 // Two stages. While step s computes, the pieces of step s + 1 go from registers to the other
-// stage, a quarter beside each K slice, and each is loaded anew for step s + 2 at once, so a load has a whole step to
-// arrive. The barrier stands before the last slice's MFMAs: the next stage's first fragments are
+// stage, a quarter beside each K slice. Their loads left two or four steps before (mxg_ahead). The barrier stands before the last slice's MFMAs: the next stage's first fragments are
 // read behind them.
 //
 // The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
@@ -21,7 +20,11 @@ int device_cus();
 
 namespace {
 
-constexpr int MXG_AHEAD = 2;  // K steps that loads run ahead (four: 26.6 for 26.7 us at 37 x 14336 x 4096)
+// K steps that loads run ahead. Tiles of 64 and 128 with 16-bit activations take four: one of the few workgroups that K's
+// split leaves a CU waits on its loads (512 x 4096 x 4096 on 128-tiles 57 -> 48 us, split in two 43 -> 39; 128 rows on 64-tiles
+// 34 -> 30). An MX4 step computes four times as long for the same bytes, and the registers of 256-tiles hold no more: two
+// (MX4 512 x 4096 x 4096 on 128-tiles 22.9 us, with four 25.7).
+constexpr int mxg_ahead(bool mx, int t) { return mx || t > 2 ? 2 : 4; }
 
 template <int AT, int WM, int TM, int TN>
 struct MxTile {
@@ -43,7 +46,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   typedef MxTile<AT, WM, TM, TN> Ti;
   constexpr bool MX = Ti::MX;
   constexpr int T = Ti::T, RA = Ti::RA, RB = Ti::RB, NA = RA * 8 / T, NB = MX ? RB * 8 / T : (2 * RB + T - 1) / T;
-  constexpr int D = MXG_AHEAD;
+  constexpr int D = mxg_ahead(MX, TN);
   constexpr bool ONE = TN > 2;  // one set of pieces: see part
   constexpr int NS = MX ? (RA + RB + T - 1) / T : NB, TR = T / 8;  // TR: rows that the threads cover with one piece each
   typedef typename MxFrag<AT>::t half8;
@@ -512,10 +515,10 @@ hipError_t gemm_at(const MxArgs& a, const MxPlan& p, hipStream_t st) {
 
 // The plan with the least estimated time. A tile size costs a CU so much for a K step: what one workgroup alone takes,
 // or the work of all its workgroups at the rate of a full CU (units of 64 x 64; us measured at 2.4 GHz):
-//   16-bit activations, steps of 64:  64-tiles 0.45, 3.3 units a us; 128-tiles 0.75, 6; 256-tiles 1.8, 8.9
+//   16-bit activations, steps of 64:  64-tiles 0.43, 3.3 units a us; 128-tiles 0.66, 6; 256-tiles 1.8, 8.9
 //   both MX4, steps of 256:           64-tiles 0.60, 2.7 units a us; 128-tiles 1.0, 5.1; 256-tiles 2.1, 7
 // and a start of 3, 5 or 12 us; a split exchange costs 5 us and what its parts weigh. It places 512 x 4096 x 4096 on 64- or 128-tiles
-// (35 to 42 us; 256-tiles 55), 128 rows on 64-tiles with K split (17; 128-tiles 24), the prefills on 256-tiles (237; 128-tiles 281).
+// (39 to 44 us; 256-tiles 55), 128 rows on 64-tiles with K split (21; 128-tiles 25), the prefills on 256-tiles (233; 128-tiles 281).
 MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) {
   MxPlan best{};
   const bool mx = a_type < 0;
@@ -527,19 +530,20 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
     int t;
     double alone, rate, start;
   };
-  static constexpr Cost kCost[2][3] = {{{1, 0.45, 3.3, 3}, {2, 0.75, 6.0, 5}, {4, 1.8, 8.9, 12}},
+  static constexpr Cost kCost[2][3] = {{{1, 0.43, 3.3, 3}, {2, 0.66, 6.0, 5}, {4, 1.8, 8.9, 12}},
                                        {{1, 0.60, 2.7, 3}, {2, 1.0, 5.1, 5}, {4, 2.1, 7.0, 12}}};
   double least = 0;
   for (const Cost& c : kCost[mx ? 1 : 0]) {
     const int64_t mt = (M + 64 * c.t - 1) / (64 * c.t), nt = (N + 64 * c.t - 1) / (64 * c.t), n = mt * nt;
     if (n > 0x3FFFFFFF) continue;
+    const int64_t ahead = mxg_ahead(mx, c.t);  // a split's steps are a multiple
     for (int64_t s = 1; s <= 8; ++s) {
       if (s > 1 && (!have_ws || n > MX_COUNTERS / 4 || n * s > 2 * cus || steps < 4 * s)) break;
       MxPlan p{};
       p.t = c.t;
       p.mt = static_cast<uint32_t>(mt);
       p.nb = static_cast<uint32_t>(nt);
-      p.per = static_cast<uint32_t>((steps + MXG_AHEAD * s - 1) / (MXG_AHEAD * s) * MXG_AHEAD);
+      p.per = static_cast<uint32_t>((steps + ahead * s - 1) / (ahead * s) * ahead);
       p.splits = static_cast<uint32_t>((steps + p.per - 1) / p.per);
       if (p.splits != s) continue;
       double rounds = static_cast<double>((n * s + cus - 1) / cus);  // tiles of the fullest CU
