@@ -269,3 +269,20 @@ def test_kernel_names(gpu):
     assert ops().matmul_mx4_kernel(1, 4096, 4096).startswith("mx4_")
     with pytest.raises(ValueError):
         ops().matmul_mx4_kernel(1, 0, 4096)
+
+
+@pytest.mark.parametrize("act", ["mx4", "f16"])
+@pytest.mark.parametrize("K", [1056, 256, 2080])
+def test_wide_tiles_with_ragged_edges(gpu, act, K):
+    """256-tiles: rows, columns and blocks that end inside them, and scales that start at any byte."""
+    M, N = 4101, 4166
+    codes, scales = weights(N, K, K)
+    assert ops().matmul_mx4_kernel(M, K, N, torch.uint8 if act == "mx4" else DT[act]) == "mx4_gemm_256"
+    g = torch.Generator().manual_seed(K)
+    if act == "mx4":
+        ac, as_ = weights(M, K, K + 1, spread=4, center=126)
+        y = ops().matmul_mx4(ac, codes, scales, A_scales=as_, out_dtype=torch.float32)
+        check_product(LB.mx4_decode(ac.cpu().numpy(), as_.cpu().numpy()), codes, scales, None, y)
+    else:
+        A = torch.randn(M, K, generator=g).to(DT[act])
+        check_product(A.double().numpy(), codes, scales, None, ops().matmul_mx4(A.cuda(), codes, scales))

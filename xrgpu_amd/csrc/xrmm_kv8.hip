@@ -58,7 +58,7 @@ constexpr int KVA_T = 256;
 constexpr int KVA_H = 4;  // pieces of eight values that a thread keeps between the magnitudes and the codes (64 slots of 128 values)
 
 // The tokens' addresses need neither page nor scale, so their loads leave before those are looked up, and a page of
-// up to 8192 values is read once: 4100 tokens of 8 heads of 128 (bfloat16, int8) in 8.0 us, 14.0 with loads of
+// up to 8192 values is read once: 4100 tokens of 8 heads of 128 (bfloat16, e4m3) in 8.0 us, 14.0 with loads of
 // four values, read twice, and a division for each. What is left is the chain lengths -> page -> scale -> codes of a
 // workgroup that runs once.
 template <typename T, bool FP8>

@@ -9,6 +9,11 @@
 // stage, a quarter beside each K slice. Their loads left two or four steps before (mxg_ahead). The barrier stands before the last slice's MFMAs: the next stage's first fragments are
 // read behind them.
 //
+// 256-tiles of two MX4 operands need no conversion, and their pieces go from memory to LDS without registers: once all
+// waves have read the last fragments of a stage, step s + 2 is fetched into it. With pieces in registers the tile
+// spilled (4096 x 4096 x 14336 182 us, 174 now; 4096 x 14336 x 4096 153 -> 142). Four waves of 128 x 128 read a third less LDS, but one wave a SIMD
+// covers less: 190 us.
+//
 // The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
 #include <atomic>
 
@@ -41,13 +46,19 @@ struct MxGrid {
   uint32_t mt, nb, ns, nbig, splits, per;
 };
 
+// 16 bytes a lane from memory to LDS, at `to` (the same for the wave) + 16 times the lane.
+__device__ __forceinline__ void lds16(rsrc_t r, unsigned char* to, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)to, 16, static_cast<int>(voff), static_cast<int>(soff), 0, 0);
+}
+
 template <int AT, int WM, int TM, int TN, bool AL>
 __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n0, const MxGrid& g, uint32_t tile, uint32_t split) {
   typedef MxTile<AT, WM, TM, TN> Ti;
   constexpr bool MX = Ti::MX;
   constexpr int T = Ti::T, RA = Ti::RA, RB = Ti::RB, NA = RA * 8 / T, NB = MX ? RB * 8 / T : (2 * RB + T - 1) / T;
   constexpr int D = mxg_ahead(MX, TN);
-  constexpr bool ONE = TN > 2;  // one set of pieces: see part
+  constexpr bool DMA = MX && TN > 2;   // pieces go from memory to LDS by themselves
+  constexpr bool ONE = !MX && TN > 2;  // one set of pieces: see part
   constexpr int NS = MX ? (RA + RB + T - 1) / T : NB, TR = T / 8;  // TR: rows that the threads cover with one piece each
   typedef typename MxFrag<AT>::t half8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -89,12 +100,12 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
 
   // ---- staging registers
   struct Set {
-    u32x4 b[NB];  // 16-bit activations: blocks of weights; MX4: pieces
+    u32x4 b[DMA ? 1 : NB];  // 16-bit activations: blocks of weights; MX4: pieces
     uint32_t s[NS][MX ? 3 : 1];
-    u32x4 a[ONE ? 1 : NA];
+    u32x4 a[ONE || DMA ? 1 : NA];
     uint32_t x[ONE || AL ? 1 : NA];
   };
-  u32x4 oa[NA], ob[NB];
+  u32x4 oa[NA];
   uint32_t ox[AL ? 1 : NA];
   bool misfit = false;
 
@@ -125,7 +136,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   };
   auto load_b = [&](int i, uint32_t s, bool in, u32x4* rb) { rb[i] = bld16(rB, in ? vb[i] : MX_OOB, s * 128u); };  // MX4 operands
   auto load_set = [&](Set& w, uint32_t s) {
-    if constexpr (!ONE) {
+    if constexpr (!ONE && !DMA) {
       const bool in = inside(s);
 #pragma unroll
       for (int i = 0; i < NA; ++i) load_a(i, s, in, w.a, w.x);
@@ -135,19 +146,30 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     }
     if constexpr (MX) {
       // eight scale bytes a row: three dwords
-      const bool in = s * 8u < kbe;
+      const uint32_t b = s * 8u < kbe ? s * 8u : (kbe - 1u) & ~7u;  // past the end the last step's, which part() drops
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int d = 0; d < 3; ++d) w.s[i][MX ? d : 0] = bld_u32(rS[i], (in ? sbase[i] & ~3u : MX_OOB) + 4u * d, s * 8u);
+        for (int d = 0; d < 3; ++d) w.s[i][MX ? d : 0] = bld_u32(rS[i], (sbase[i] & ~3u) + 4u * d, b);
     } else {
       const bool in = s * 2u + static_cast<uint32_t>(tid & 1) < kbe;
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        w.b[i] = bld16(rB, in ? vb[i] : MX_OOB, s * 32u);
+        w.b[DMA ? 0 : i] = bld16(rB, in ? vb[i] : MX_OOB, s * 32u);
         w.s[i][0] = bld_u8(rS[i], in ? sbase[i] : MX_OOB, s * 2u);
       }
     }
+  };
+  // DMA: step s to LDS stage `st`. What lies past a row's or the split's end may stay as it was there: codes are finite whatever their
+  // bits, rows past the end leave no output, and blocks past it have the scale 2^-127 on both sides.
+  auto fetch = [&](uint32_t s, int st) {
+    const bool in = inside(s);
+    unsigned char* base = smem + st * Ti::STAGE + wave * 1024;  // lane l writes 16 bytes at 16 l
+#pragma unroll
+    for (int i = 0; i < NA; ++i) lds16(rA, base + TR * i * 128, in ? va[i] : MX_OOB, s * 128u);
+    if constexpr (MX)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) lds16(rB, base + (RA + TR * i) * 128, in ? vb[i] : MX_OOB, s * 128u);
   };
   // Quarter d of the pieces of step s to LDS stage `st`; with one set of pieces, each piece's load for step s + 1
   auto part = [&](int d, uint32_t s, int st, const Set& w) {
@@ -155,8 +177,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     const bool in = inside(s + 1);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      if (i * 4 / NA != d) continue;
-      u32x4 v = ONE ? oa[i] : w.a[ONE ? 0 : i];
+      if (DMA || i * 4 / NA != d) continue;
+      u32x4 v = ONE ? oa[i] : w.a[ONE || DMA ? 0 : i];
       if constexpr (!MX && !AL) {
         const uint32_t k = s * 64u + spiece * 8u, r = srow + TR * i;
         const uint32_t sh = (r * rowA + misA) & 3u;  // a step's pieces start at multiples of 16 bytes of a row
@@ -177,11 +199,10 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     if constexpr (MX) {
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        if (i * 4 / NB != d) continue;
-        *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = ONE ? ob[i] : w.b[i];
-        if (ONE) load_b(i, s + 1, in, ob);
+        if (DMA || i * 4 / NB != d) continue;
+        *reinterpret_cast<u32x4*>(base + (RA + srow + TR * i) * 128 + (tid & 7) * 16) = w.b[DMA ? 0 : i];
       }
-      if (d == 0) {
+      if (d == (DMA ? 3 : 0)) {
         const uint32_t b0 = s * 8u, n = b0 < kbe ? kbe - b0 : 0u;  // scales of blocks past K are 2^-127 on both sides: products of 0
         const uint32_t k0 = n >= 4u ? ~0u : (1u << (8u * n)) - 1u, k1 = n >= 8u ? ~0u : n <= 4u ? 0u : (1u << (8u * (n - 4u))) - 1u;
 #pragma unroll
@@ -198,7 +219,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
         const int c = tid + T * i, r = c >> 1;
-        const u32x4 wb = w.b[i];
+        const u32x4 wb = w.b[DMA ? 0 : i];
         if (AT == LT_F16 && d == 0) misfit |= !mx_f16_fits(w.s[i][0], wb);
         if (NB * T == 2 * RB || c < 2 * RB)
           *reinterpret_cast<half8*>(base + (RA + r) * 128 + ((((c & 1) * 4 + d) ^ (r & 7)) * 16)) = mx_dq8<AT>(wb[d], e8m0(w.s[i][0]));
@@ -279,10 +300,49 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   if constexpr (ONE) {
 #pragma unroll
     for (int i = 0; i < NA; ++i) load_a(i, s0, inside(s0), oa, ox);
-    if constexpr (MX)
-#pragma unroll
-      for (int i = 0; i < NB; ++i) load_b(i, s0, inside(s0), ob);
   }
+  if constexpr (DMA) {
+    auto joined = [&]() {  // what this wave fetched has arrived, and then every wave's
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt 0
+      __syncthreads();
+    };
+    fetch(s0, 0);
+    load_set(w[0], s0);
+    part(3, s0, 0, w[0]);
+    joined();
+    load_set(w[0], s0 + 1);
+    fetch(s0 + 1, 1);
+    read(0, 0);
+    read_scales(0);
+    auto round = [&](uint32_t s, int st) {
+      read(st, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      mfmas(std::integral_constant<int, 0>{});
+      __builtin_amdgcn_sched_barrier(0);
+      read(st, 2);
+      __builtin_amdgcn_sched_barrier(0);
+      mfmas(std::integral_constant<int, 1>{});
+      __builtin_amdgcn_sched_barrier(0);
+      read(st, 3);
+      __builtin_amdgcn_sched_barrier(0);
+      mfmas(std::integral_constant<int, 2>{});
+      part(3, s + 1, st ^ 1, w[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      joined();
+      read(st ^ 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      load_set(w[0], s + 2);
+      fetch(s + 2, st);
+      mfmas(std::integral_constant<int, 3>{});
+      read_scales(st ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    for (uint32_t s = s0; s < s1; s += 2) {
+      round(s, 0);
+      round(s + 1, 1);
+    }
+    joined();
+  } else {
 #pragma unroll
   for (int i = 0; i < D; ++i) load_set(w[i], s0 + i);
 #pragma unroll
@@ -293,6 +353,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   for (uint32_t s = s0; s < s1; s += D) {
 #pragma unroll
     for (int i = 0; i < D; ++i) step(s + i, i & 1, w[(i + 1) % D], w[i]);
+  }
   }
 
   if constexpr (AT == LT_F16) {
