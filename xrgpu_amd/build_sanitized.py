@@ -1,7 +1,7 @@
 """Host-sanitizer build of libxrmm and the job-JSON runner (CPU checks only).
 
 ``python -m xrgpu_amd.build_sanitized`` compiles the host code of the C ABI
-(``xrmm_api.cpp``, ``xrmm_operator.cpp``: argument checks, planning, the
+(``xrmm_api.cpp``, ``xrmm_lowbit_api.cpp``, ``xrmm_operator.cpp``: argument checks, planning, the
 request lifecycle) and the runner (``xrmm_execute.cpp``: the hand-written JSON
 parser of job files) with AddressSanitizer and UndefinedBehaviorSanitizer, and
 links them with the kernel objects of the regular build (device code is not
@@ -30,7 +30,7 @@ from xrgpu_amd import build as B
 
 SAN_DIR = os.path.join(B.LIB_DIR, "sanitize")
 SAN_OBJ = os.path.join(B.OBJ_DIR, "sanitize")
-HOST_UNITS = ("xrmm_api.cpp", "xrmm_operator.cpp")
+HOST_UNITS = ("xrmm_api.cpp", "xrmm_operator.cpp", "xrmm_lowbit_api.cpp")
 # hipcc: the sanitizers apply to the host compilation only
 HOST_SAN = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
             "-Xarch_host", "-fno-sanitize-recover=undefined", "-Xarch_host", "-fno-omit-frame-pointer",

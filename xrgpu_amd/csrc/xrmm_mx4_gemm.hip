@@ -12,7 +12,7 @@
 // 256-tiles of two MX4 operands need no conversion, and their pieces go from memory to LDS without registers: once all
 // waves have read the last fragments of a stage, step s + 2 is fetched into it. With pieces in registers the tile
 // spilled (4096 x 4096 x 14336 182 us, 174 now; 4096 x 14336 x 4096 153 -> 142). Four waves of 128 x 128 read a third less LDS, but one wave a SIMD
-// covers less: 190 us. What bounds it is the pieces' way from L2: a step's 64 KB take 2.2 us of a CU (7.6 TB/s of all), the step 1.5 without
+// covers less: 190 us. What bounds it is the pieces' way from L2: a step's 64 KB take 2.2 us of a CU (7.6 TB/s of all), the step 1.8 without
 // them; half steps fetched three ahead arrive no sooner (182 us: twice the requests).
 //
 // The weights are the MFMAs' first operand: a lane then holds four consecutive columns of one row.
