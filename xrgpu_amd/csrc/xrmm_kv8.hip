@@ -268,7 +268,8 @@ __device__ __forceinline__ KvBytes<N> kv_bytes(const uint8_t* p) {
 // tokens; its waves take turns at steps of 32 tokens, with the next step's codes in flight and the
 // page after that looked up. Workgroups of one (sequence, head, rows) leave their
 // unnormalised outputs, maxima and sums in the workspace, and the last to arrive joins them in
-// token order.
+// token order. 48 sequences of up to 8000 tokens, 8 heads of 128, e4m3: 102 us (5.0 TB/s), unsplit; one of 65000, int8: 37 us, of
+// which the join is about 8.
 constexpr int KVR_PASS = 8 * KVT;  // shares of tokens are multiples of it: a step of all waves, eight at most
 constexpr int64_t KV_COUNTERS = 4096;      // bytes of arrival counters at the head of the workspace
 
@@ -604,6 +605,9 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 // above with v_mfma_f32_32x32x16: a row's maximum, sum and factor belong to a lane, and P goes from one product
 // into the next without leaving its lane. Pieces of 16 bytes are swizzled by their row, so that neither the
 // fragments' rows nor the transposing stores meet in a bank.
+//
+// VALU instructions bound it, about 500 a wave and 64 tokens (codes to binary16, softmax); MFMAs run a fifth of the time. Two chunks
+// of 2000 on 4000 tokens, 32 heads of 128 on 8: 268 us; 32 tokens a tile with three workgroups a CU 476, eight waves 276.
 //
 // Two stages: while tile i computes, tile i + 1 goes from registers to LDS, tile i + 2 is loaded and the
 // pages of tile i + 3 are looked up. One barrier a tile.
