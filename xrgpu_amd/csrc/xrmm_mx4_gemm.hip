@@ -407,7 +407,9 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
   const uint32_t at = static_cast<uint32_t>(wave) * (TM * TN * 4096u);
   const int64_t nw = n0 + wn * 32 * TN, mw = m0 + wm * 32 * TM;
   const int osz = a.out == LT_F32 ? 4 : 2;
-  const bool vec = (a.N * osz & 15) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 15u) == 0;
+  typedef f32x4 f32x4_4 __attribute__((aligned(4)));  // wide stores start at any dword
+  typedef u32x4 u32x4_4 __attribute__((aligned(4)));
+  const bool vec = (a.N * osz & 3) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 3u) == 0;
   auto finish = [&](int r, int p, float (&v)[8]) {  // eight values of row r of the wave's rows, from column 8 p on
     const int64_t m = mw + r, n = nw + 8 * p;
     if (m >= a.M || n >= a.N) return;
@@ -428,9 +430,9 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
     const int64_t o = m * a.N + n;
     if (a.out == LT_F32) {
       float* y = static_cast<float*>(a.Y) + o;
-      if (vec) {
-        *reinterpret_cast<f32x4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
-        if (left > 4) *reinterpret_cast<f32x4*>(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      if (vec && left == 8) {
+        *reinterpret_cast<f32x4_4*>(y) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_4*>(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
         return;
       }
     } else if (vec && left == 8) {
@@ -439,7 +441,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, uint32_t row, int64_t n
       for (int e = 0; e < 4; ++e)
         x[e] = a.out == LT_F16 ? __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(v[2 * e]), static_cast<f16>(v[2 * e + 1])})
                                : __builtin_bit_cast(uint32_t, bf16x2{static_cast<bf16>(v[2 * e]), static_cast<bf16>(v[2 * e + 1])});
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.Y) + o) = x;
+      *reinterpret_cast<u32x4_4*>(static_cast<uint16_t*>(a.Y) + o) = x;
       return;
     }
 #pragma unroll
@@ -576,11 +578,16 @@ hipError_t gemm_at(const MxArgs& a, const MxPlan& p, hipStream_t st) {
 }  // namespace
 
 // The plan with the least estimated time. A tile size costs a CU so much for a K step: what one workgroup alone takes,
-// or the work of all its workgroups at the rate of a full CU (units of 64 x 64; us measured at 2.4 GHz):
-//   16-bit activations, steps of 64:  64-tiles 0.43, 3.3 units a us; 128-tiles 0.66, 6; 256-tiles 1.8, 8.9
-//   both MX4, steps of 256:           64-tiles 0.60, 2.7 units a us; 128-tiles 1.0, 5.1; 256-tiles 2.1, 7
-// and a start of 3, 5 or 12 us; a split exchange costs 5 us and what its parts weigh. It places 512 x 4096 x 4096 on 64- or 128-tiles
-// (39 to 44 us; 256-tiles 55), 128 rows on 64-tiles with K split (21; 128-tiles 25), the prefills on 256-tiles (233; 128-tiles 281).
+// or the work of all its workgroups at the rate of a full CU (units of 64 x 64; us measured at 2.4 GHz); and a start, and
+// so much more for each further round of the CUs:
+//   16-bit activations, steps of 64:  64-tiles 0.43, 3.3 units a us; 128-tiles 0.66, 6; 256-tiles 1.8, 8.9; starts 3, 5, 12 (a round)
+//   both MX4, steps of 256:           64-tiles 0.60, 2.35 units a us; 128-tiles 1.0, 4.3; 256-tiles 1.0, 6.67; starts 3, 5 (1.7 a round),
+//                                     8.2 (a round)
+// MX4 256-tiles wait on memory that all CUs share: a round that leaves CUs out is faster, 0.4 of a full one with a few
+// tiles, 0.9 with half the CUs. A split exchange costs 5 us and what its parts weigh.
+// It places 512 x 4096 x 4096 of 16 bits on 64- or 128-tiles (39 to 44 us; 256-tiles 55), 128 rows on 64-tiles with K split (21; 128-tiles 25),
+// 2048 x 4096 x 14336 on 256-tiles (233; 128-tiles 281); MX4 700 x 4096 x 14336 on 256-tiles (44 us; 128-tiles 53), 512 rows on 128-tiles
+// (38.5; 256-tiles 45, 64-tiles 53).
 MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) {
   MxPlan best{};
   const bool mx = a_type < 0;
@@ -590,10 +597,10 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
   const int64_t steps = (kb + (mx ? 7 : 1)) / (mx ? 8 : 2);
   struct Cost {
     int t;
-    double alone, rate, start;
+    double alone, rate, start, more;
   };
-  static constexpr Cost kCost[2][3] = {{{1, 0.43, 3.3, 3}, {2, 0.66, 6.0, 5}, {4, 1.8, 8.9, 12}},
-                                       {{1, 0.60, 2.7, 3}, {2, 1.0, 5.1, 5}, {4, 2.1, 7.0, 12}}};
+  static constexpr Cost kCost[2][3] = {{{1, 0.43, 3.3, 3, 0}, {2, 0.66, 6.0, 5, 0}, {4, 1.8, 8.9, 12, 12}},
+                                       {{1, 0.60, 2.35, 3, 0}, {2, 1.0, 4.3, 5, 1.7}, {4, 1.0, 6.67, 8.2, 8.2}}};
   double least = 0;
   for (const Cost& c : kCost[mx ? 1 : 0]) {
     const int64_t mt = (M + 64 * c.t - 1) / (64 * c.t), nt = (N + 64 * c.t - 1) / (64 * c.t), n = mt * nt;
@@ -609,6 +616,10 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
       p.splits = static_cast<uint32_t>((steps + p.per - 1) / p.per);
       if (p.splits != s) continue;
       double rounds = static_cast<double>((n * s + cus - 1) / cus);  // tiles of the fullest CU
+      if (mx && c.t == 4 && n * s % cus != 0) {
+        const double part = static_cast<double>(n * s % cus) / static_cast<double>(cus);
+        rounds = static_cast<double>(n * s / cus) + 0.4 + (part < 0.6 ? part : 0.6);
+      }
       if (c.t == 4 && s == 1 && rounds > 1 && cus % mt == 0) {
         // columns of wide tiles and narrow ones (192) mixed, where that makes fewer rounds of the CUs
         const int64_t per = cus / mt;
@@ -623,7 +634,7 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
         }
       }
       const double units = static_cast<double>(c.t * c.t), step = units * rounds / c.rate;
-      double time = c.start * (c.t == 4 ? rounds : 1.0) + static_cast<double>(p.per) * (step > c.alone ? step : c.alone);
+      double time = c.start + c.more * (rounds > 1 ? rounds - 1 : 0) + static_cast<double>(p.per) * (step > c.alone ? step : c.alone);
       if (s > 1) {
         p.ws_bytes = MX_COUNTERS + n * s * c.t * c.t * 16384;
         time += 5.0 + static_cast<double>(p.ws_bytes) * 0.5e-6;  // written and read back at about 4 TB/s
