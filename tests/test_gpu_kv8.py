@@ -338,3 +338,17 @@ def test_append_then_attention_is_a_decode_step(gpu):
         k, v = (torch.randn(2 * n, 2, 64, generator=g).half().cuda() for _ in range(2))
         d = check_append(c, k, v, [n, n], False)
         check_attention(c, q, [n, n], False, d=d)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv,D,n", [(6, 2, 64, 1), (5, 1, 96, 3), (4, 4, 128, 1), (3, 1, 256, 2), (4, 2, 128, 70)])
+def test_attention_queries_and_outputs_at_any_element(gpu, dt, Hq, Hkv, D, n):
+    """Tokens an odd number of elements apart, from an odd element on; outputs from an odd element on."""
+    c = Cache("int8", [150, 90], Hkv, D, 32, seed=D)
+    wide = torch.randn(2 * n, Hq * D + 3, device="cuda").to(DT[dt])
+    q = wide[:, 1:1 + Hq * D].unflatten(1, (Hq, D))
+    store = torch.full((2 * n * Hq * D + 3,), 7.0, device="cuda").to(DT[dt])
+    out = store[1:-2].view(2 * n, Hq, D)
+    check_attention(c, q, [n, n], False, out=out)
+    assert (store[0] == 7) and (store[-2:] == 7).all()
+    check_attention(c, q, [n, n], False, got=out, d=c.dev())

@@ -268,8 +268,9 @@ __device__ __forceinline__ KvBytes<N> kv_bytes(const uint8_t* p) {
 // tokens; its waves take turns at steps of 32 tokens, with the next step's codes in flight and the
 // page after that looked up. Workgroups of one (sequence, head, rows) leave their
 // unnormalised outputs, maxima and sums in the workspace, and the last to arrive joins them in
-// token order. 48 sequences of up to 8000 tokens, 8 heads of 128, e4m3: 102 us (5.0 TB/s), unsplit; one of 65000, int8: 37 us, of
-// which the join is about 8.
+// token order. 48 sequences of up to 8000 tokens, 8 heads of 128, e4m3: 97 us (5.2 TB/s), unsplit; one of 65000, int8: 34.5 us, of
+// which the join is about 8. The kernel's start shows in short calls: with queries loaded value by value a token on 4 took 9.5 us
+// at head size 256 and 5.4 at 64, in pieces of 16 bytes (outputs of 8) 8.3 and 4.8.
 constexpr int KVR_PASS = 8 * KVT;  // shares of tokens are multiples of it: a step of all waves, eight at most
 constexpr int64_t KV_COUNTERS = 4096;      // bytes of arrival counters at the head of the workspace
 
@@ -348,22 +349,26 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   {
     const int r = r0 + col;
     const bool ok = r < nrows;
-    const int i = ok ? r / G : 0, hq = h * G + (ok ? r % G : 0);
+    const int rr = ok ? r : nrows - 1, i = rr / G, hq = h * G + rr % G;
     const int64_t at = (first + i) * a.q_stride + static_cast<int64_t>(hq) * D + g * KD;
     hi = ok ? row_hi(i) : 0;
     lo = row_lo(i);
-    if (a.dtype == LT_F16) {
+    // at any element's address; rows past the last read its row and see nothing
+    typedef f16x8 f16x8_2 __attribute__((aligned(2)));
+    const f16* src = static_cast<const f16*>(a.q) + at;
 #pragma unroll
-      for (int e = 0; e < KD; ++e) q[e / 8][e % 8] = ok ? static_cast<const f16*>(a.q)[at + e] : static_cast<f16>(0.f);
-    } else {
-      float v[KD];
-#pragma unroll
-      for (int e = 0; e < KD; ++e) v[e] = ok ? static_cast<float>(static_cast<const bf16*>(a.q)[at + e]) : 0.f;
+    for (int x = 0; x < KD / 8; ++x) q[x] = *reinterpret_cast<const f16x8_2*>(src + 8 * x);
+    if (a.dtype != LT_F16) {
       uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < KD; ++e) {
-        const uint32_t m = __builtin_bit_cast(uint32_t, v[e]) & 0x7FFFFFFFu;
-        top = top > m ? top : m;
+      for (int x = 0; x < KD / 8; ++x) {
+        const u32x4 v = __builtin_bit_cast(u32x4, q[x]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t m0 = (v[e] << 16) & 0x7FFFFFFFu, m1 = v[e] & 0x7FFF0000u;
+          top = top > m0 ? top : m0;
+          top = top > m1 ? top : m1;
+        }
       }
 #pragma unroll
       for (int o = 16; o <= 32; o <<= 1) {
@@ -375,7 +380,11 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
       if (top >= 0x7F800000u || top < 0x00800000u) e2 = 0;
       const float s1 = two(-(e2 / 2)), s2 = two(-(e2 - e2 / 2));
 #pragma unroll
-      for (int e = 0; e < KD; ++e) q[e / 8][e % 8] = static_cast<f16>(v[e] * s1 * s2);
+      for (int x = 0; x < KD / 8; ++x) {
+        const bf16x8 v = __builtin_bit_cast(bf16x8, q[x]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[x][e] = static_cast<f16>(static_cast<float>(v[e]) * s1 * s2);
+      }
       qs = qs * two(e2 / 2) * two(e2 - e2 / 2);
     }
   }
@@ -518,8 +527,10 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
     const int r = r0 + p / (D / 4);
     const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
     const int64_t at = (static_cast<int64_t>(first + r / G) * a.Hq + h * G + r % G) * D + p % (D / 4) * 4;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) st_lt(a.o, at + e, v[e] * inv, a.dtype);
+    typedef u32x2 u32x2_2 __attribute__((aligned(2)));
+    v *= inv;
+    *reinterpret_cast<u32x2_2*>(static_cast<uint16_t*>(a.o) + at) =
+        a.dtype == LT_F16 ? __builtin_bit_cast(u32x2, __builtin_convertvector(v, f16x4)) : __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
   };
   if (parts == 1) {
 #pragma unroll 1
