@@ -450,6 +450,11 @@ int xrmm_matmul_mx4(const void* A, const void* A_scales, int32_t a_dtype, const 
  * NULL for an invalid geometry. No device work. */
 const char* xrmm_matmul_mx4_kernel(int64_t M, int64_t K, int64_t N, int32_t a_dtype);
 
+/* The tiles of that geometry, for 256 CUs where there is no device: plan[0] rows and columns of a tile (0: the
+ * geometry runs untiled), [1] row tiles, [2] column tiles of that width, [3] column tiles of 192 behind them,
+ * [4] splits of K, [5] bytes of workspace. No device work. */
+int xrmm_matmul_mx4_plan(int64_t M, int64_t K, int64_t N, int32_t a_dtype, int32_t have_workspace, int64_t* plan);
+
 /* ---------------------------------------------------------------------------
  * Attention over a paged 8-bit cache (no counterpart in the reference). k_cache and
  * v_cache: [pages, kv_heads, page_size, head_dim] of XRMM_I8 or XRMM_E4M3 codes

@@ -81,6 +81,7 @@ def _sig(lib):
     s("xrmm_matmul_mx4_workspace_bytes", _i64, _i64, _i64, _i64, _i32)
     s("xrmm_matmul_mx4", ctypes.c_int, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp)
     s("xrmm_matmul_mx4_kernel", ctypes.c_char_p, _i64, _i64, _i64, _i32)
+    s("xrmm_matmul_mx4_plan", ctypes.c_int, _i64, _i64, _i64, _i32, _i32, ctypes.POINTER(_i64))
     s("xrmm_kv8_append", ctypes.c_int, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
       _i32, _i32, _i32, _i64, _i32, _i32, _i32, _vp)
     s("xrmm_kv8_attention_workspace_bytes", _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32)

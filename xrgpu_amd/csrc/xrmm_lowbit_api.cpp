@@ -5,7 +5,7 @@
 #include <string>
 
 #include "../../include/xrmm.h"
-#include "xrmm_lowbit.h"
+#include "xrmm_mx4.h"
 
 namespace {
 
@@ -143,6 +143,16 @@ const char* xrmm_matmul_mx4_kernel(int64_t M, int64_t K, int64_t N, int32_t a_dt
   a.A = probe;
   set_status(XRMM_OK, "");
   return xrmm::mx4_kernel_name(a);
+}
+
+int xrmm_matmul_mx4_plan(int64_t M, int64_t K, int64_t N, int32_t a_dtype, int32_t have_workspace, int64_t* plan) {
+  xrmm::MxArgs a;
+  if (plan == nullptr) return fail("matmul_mx4_plan: null plan");
+  if (int rc = mx4_geometry(a, M, K, N, a_dtype, XRMM_F32)) return rc;
+  const xrmm::MxPlan p = xrmm::mx4_gemm_plan(M, K, N, a.a_type, have_workspace != 0);
+  const int64_t v[6] = {64 * p.t, p.mt, p.nb, p.ns, p.splits, p.ws_bytes};
+  for (int i = 0; i < 6; ++i) plan[i] = v[i];
+  return set_status(XRMM_OK, "");
 }
 
 int xrmm_kv8_append(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int32_t dtype, void* k_cache,

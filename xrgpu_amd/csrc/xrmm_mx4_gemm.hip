@@ -621,7 +621,8 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
         rounds = static_cast<double>(n * s / cus) + 0.4 + (part < 0.6 ? part : 0.6);
       }
       if (c.t == 4 && s == 1 && rounds > 1 && cus % mt == 0) {
-        // columns of wide tiles and narrow ones (192) mixed, where that makes fewer rounds of the CUs
+        // columns of wide tiles and narrow ones (192) mixed, where that makes fewer rounds of the CUs: k whole rounds of wide
+        // ones, and at most j of narrow ones, as many as the columns behind them need
         const int64_t per = cus / mt;
         for (int64_t j = 1; j <= 16; ++j) {
           const int64_t rest = N - 192 * j * per, k = rest > 0 ? (rest + 256 * per - 1) / (256 * per) : 0;
@@ -629,7 +630,7 @@ MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) 
           if (r < rounds - 0.05) {
             rounds = r;
             p.nb = static_cast<uint32_t>(k * per);
-            p.ns = static_cast<uint32_t>(j * per);
+            p.ns = static_cast<uint32_t>((N - 256 * k * per + 191) / 192);
           }
         }
       }
