@@ -211,7 +211,20 @@ __global__ __launch_bounds__(KVA_T) void k_kv8_append(KvAppendArgs a, uint32_t t
 // read one key head: row r is query r / G, head r % G of the group.
 
 constexpr int KVT = 32;      // tokens of a step
-constexpr float KV_P = 1024.f;  // weights enter binary16 times this: small ones stay normal
+
+// A token's softmax weight times its page's value scale enters binary16 as p vs 2^(KV_PE - e), where 2^e is a power of two
+// above every value scale so far in magnitude: 2^KV_PE at most, so that small weights stay normal. Only
+// exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is.
+constexpr int KV_PE = 11;
+constexpr int KV_NONE = -1000;  // e before any scale
+
+// The smallest e with |scale| < 2^e; KV_NONE for 0 and for what is not finite.
+__device__ __forceinline__ int kv_scale_exp(float scale) {
+  const uint32_t m = __builtin_bit_cast(uint32_t, scale) & 0x7FFFFFFFu;
+  return m - 1u < 0x7F7FFFFFu ? __builtin_amdgcn_frexp_expf(scale) : KV_NONE;
+}
+
+__device__ __forceinline__ float kv_shift(float x, int e) { return __builtin_ldexpf(x, e); }
 
 // Four codes -> four binary16 values, exact.
 template <bool FP8>
@@ -393,7 +406,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
   for (int j = 0; j < VD; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float vref = 0.f;  // the value scale that the sums are in units of
+  int ve = KV_NONE;  // the sums are in units of 2^(ve - KV_PE)
   bool bad = false;
 
 #pragma unroll 1
@@ -414,11 +427,12 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
       }
     }
     // a page's value scale above all before it: the sums go into its units
-    const float ref = vref;
+    const int was = ve;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (cur.pg[u] >= 0 && cur.vs[u] > vref && cur.vs[u] <= 3.4028235e38f) vref = cur.vs[u];
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+    for (int u = 0; u < 2; ++u) {
+      const int e = kv_scale_exp(cur.vs[u]);
+      ve = cur.pg[u] >= 0 && e > ve ? e : ve;
+    }
     const bool masked = t0 < full_lo || t0 + KVT > full_hi || cur.pg[0] < 0 || cur.pg[1] < 0;
     float top = -__builtin_inff();
 #pragma unroll
@@ -439,13 +453,13 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
     const float f = __builtin_amdgcn_exp2f(m - base);
     m = mn;
     l *= f;
-    const float fo = ref < vref ? f * (ref / vref) : f;
+    const float fo = kv_shift(f, was - ve);
 #pragma unroll
     for (int j = 0; j < VD; ++j) o[j] *= fo;
     f16x8 pf;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float w = cur.vs[u] * inv * KV_P;
+      const float w = kv_shift(cur.vs[u], KV_PE - ve);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float v = s[u][e], p = __builtin_amdgcn_exp2f(v - base);
@@ -499,12 +513,15 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   float sum = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) sum += wl[w][col] * __builtin_amdgcn_exp2f(wm[w][col] - base);
-  const float mine = __builtin_amdgcn_exp2f(m - base) * vref * (1.f / KV_P);
+  const float mine = __builtin_amdgcn_exp2f(m - base);
 #pragma unroll
   for (int j0 = 0; j0 < VD; j0 += JT) {
     if (j0 > 0) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < JT; ++j) red[wave][j][lane] = o[j0 + j] * mine;
+    for (int j = 0; j < JT; ++j) {
+      const f32x4 v = o[j0 + j] * mine;
+      red[wave][j][lane] = f32x4{kv_shift(v[0], ve - KV_PE), kv_shift(v[1], ve - KV_PE), kv_shift(v[2], ve - KV_PE), kv_shift(v[3], ve - KV_PE)};
+    }
     __syncthreads();
 #pragma unroll 1
     for (int j = wave; j < JT; j += W) {  // the waves finish a tile each
@@ -624,11 +641,11 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 // pages of tile i + 3 are looked up. One barrier a tile.
 //
 // A row's maximum may lag by up to 2^KV_LAG: the outputs are rescaled only when some row of the wave outgrows that
-// (KV_P 2^KV_LAG stays inside binary16). Workgroups of one key head follow each other on one XCD's L2 where heads and
+// (2^(KV_PE + KV_LAG) stays inside binary16). Workgroups of one key head follow each other on one XCD's L2 where heads and
 // sequences make a multiple of eight; the rows that see the most tokens come first. Few workgroups
 // and long contexts: tokens are split and joined as above.
 constexpr int KVM_WAVES = 4, KVM_ROWS = 32 * KVM_WAVES, KVM_T = 64 * KVM_WAVES;
-constexpr float KV_LAG = 5.f;
+constexpr float KV_LAG = 4.f;
 
 template <int D>
 struct KvTile {
@@ -838,7 +855,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;
-  float vref = 0.f, vinv = 0.f;  // the value scale that the sums are in units of, and KV_P times its inverse
+  int ve = KV_NONE;  // the sums are in units of 2^(ve - KV_PE)
   // scale (as scn) and missing groups of the tile in LDS
   float scl;
   uint32_t none;
@@ -883,24 +900,21 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     // products are short (2048 tokens on themselves 51 -> 46.5 us); with 96, 128 and 256 it costs 0 to 3 %.
     if constexpr (D <= 64) __builtin_amdgcn_s_setprio(1);
     const uint32_t no = none;
-    const float ref = vref, sc = scl;
+    const float sc = scl;
+    const int was = ve;
     // a value scale above all before it: the sums go into its units (a wave's own: its sums alone are in these)
     {
-      float vtop = 0.f;
+      const int el = kv_scale_exp(sc);
 #pragma unroll
       for (int u = 0; u < GR; ++u) {
-        const float v = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, sc), GR + u));
-        vtop = (no >> u & 1u) == 0 && v <= 3.4028235e38f ? fmaxf(vtop, v) : vtop;
-      }
-      if (vtop > vref) {
-        vref = vtop;
-        vinv = KV_P / vref;
+        const int e = __builtin_amdgcn_readlane(el, GR + u);
+        ve = (no >> u & 1u) == 0 && e > ve ? e : ve;
       }
     }
-    // lane-wise: K's factor of the rows' scores, or V's of their weights; its logarithm and inverse
-    const float wl = sc * vinv, lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
+    // lane-wise: V's factor of the weights, its logarithm and inverse; or K's of the scores
+    const float wl = kv_shift(sc, KV_PE - ve), lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
     // factors of the usual kind, no masks: see below
-    const bool usual = (lane & GR) != 0 ? wl >= 0x1p-8f && wl <= 1.001f * KV_P : sc >= 0.f && a.scale >= 0.f;
+    const bool usual = (lane & GR) != 0 ? wl >= 0x1p-8f && wl < 0x1p11f : sc >= 0.f && a.scale >= 0.f;
     const bool plain = (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && no == 0 && t0 >= full_lo && t0 + TT <= full_hi;
     auto of = [&](float x, int u) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), u)); };
     move();
@@ -927,12 +941,12 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
           }
       }
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > m + KV_LAG || ref < vref)) {
+      if (__any(top > m + KV_LAG || was < ve)) {
         const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
         const float f = __builtin_amdgcn_exp2f(m - base);
         m = mn;
         l *= f;
-        const float fo = ref < vref ? f * (ref / vref) : f;
+        const float fo = kv_shift(f, was - ve);
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
@@ -983,7 +997,6 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   if (__any(bad) && lane == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   l += __shfl_xor(l, 32, 64);
-  const float unit_v = vref * (1.f / KV_P);
   if (parts > 1) {
     constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
     constexpr uint32_t PART = static_cast<uint32_t>(Ti::PART), ML = KVM_ROWS * D * 4;
@@ -996,7 +1009,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
       for (int j = 0; j < JT; ++j)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          const f32x4 v = {o[j][4 * y] * unit_v, o[j][4 * y + 1] * unit_v, o[j][4 * y + 2] * unit_v, o[j][4 * y + 3] * unit_v};
+          const f32x4 v = {kv_shift(o[j][4 * y], ve - KV_PE), kv_shift(o[j][4 * y + 1], ve - KV_PE), kv_shift(o[j][4 * y + 2], ve - KV_PE), kv_shift(o[j][4 * y + 3], ve - KV_PE)};
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), rW, split * PART + at + j * 128 + y * 32, 0, COHERENT);
         }
       if (hf == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__builtin_bit_cast(uint32_t, m), __builtin_bit_cast(uint32_t, l)}, rW, split * PART + ml, 0, COHERENT);
@@ -1036,7 +1049,8 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     }
   }
   // 32 rows through the wave's part of LDS in the output's type, then whole pieces of 16 bytes
-  const float inv = (l != 0.f ? 1.f / l : 0.f) * (parts > 1 ? 1.f : unit_v);
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  const int unit_e = parts > 1 ? 0 : ve - KV_PE;
   constexpr int PITCH = D * 2 + 16;
   unsigned char* strip = smem + wave * (32 * PITCH);
 #pragma unroll
@@ -1046,7 +1060,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
       u32x2 v;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float x0 = o[j][4 * y + 2 * e] * inv, x1 = o[j][4 * y + 2 * e + 1] * inv;
+        const float x0 = kv_shift(o[j][4 * y + 2 * e] * inv, unit_e), x1 = kv_shift(o[j][4 * y + 2 * e + 1] * inv, unit_e);
         v[e] = a.dtype == LT_F16 ? __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(x0), static_cast<f16>(x1)})
                                  : __builtin_bit_cast(uint32_t, bf16x2{static_cast<bf16>(x0), static_cast<bf16>(x1)});
       }
