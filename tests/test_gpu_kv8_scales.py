@@ -109,3 +109,37 @@ def test_appended_tiny_values(gpu, counts):
     assert 0 < c.vs[c.table[0]].max() < 2.0 ** -119
     out = check(c, queries(sum(counts), 4, 64, "bf16"), counts)
     assert np.abs(out).max() > 2.0 ** -124
+
+
+@KIND
+@HEADS
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("counts,Hq", [([1, 1], 4), ([5, 3], 4), ([70, 40], 1), ([200, 120], 4)])
+def test_hidden_pages_change_nothing(gpu, kind, D, page, counts, Hq, window):
+    """A value scale 2^60 times the others, where the causal mask or the window hides it from some rows or from all."""
+    lens = [max(300, counts[0]), max(200, counts[1])]
+    c = Cache(kind, lens, 1, D, page, seed=D)
+    far = max(0, min(lens) - min(counts) - 100) // page  # behind the windows; with none, every row sees it
+    c.vs[c.table[:, far]] *= np.float32(2.0 ** 60 if window else 1.0)
+    last = [(x - 1) // page for x in lens]  # hidden from the rows before it
+    for b in (0, 1):
+        c.vs[c.table[b, last[b]]] *= np.float32(2.0 ** 60)
+    check(c, queries(sum(counts), Hq, D, "bf16"), counts, window=window)
+
+
+@KIND
+@ROWS
+def test_a_large_scale_after_a_row_changes_no_bit_of_it(gpu, kind, counts):
+    c = Cache(kind, [150, 90], 2, 64, 16, seed=3)
+    q = queries(sum(counts), 4, 64, "f16")
+    a = ops().kv8_attention(q, **c.dev(), starts=starts_of(counts), max_new=max(counts))
+    first = 0
+    for n, L in zip(counts, (150, 90)):
+        page = (L - 1) // 16
+        hidden = min(max(0, page * 16 - (L - n)), n)  # rows at positions before the last page
+        c2 = Cache(kind, [150, 90], 2, 64, 16, seed=3)
+        for b, x in enumerate((150, 90)):
+            c2.vs[c2.table[b, (x - 1) // 16]] *= np.float32(2.0 ** 30)
+        b = ops().kv8_attention(q, **c2.dev(), starts=starts_of(counts), max_new=max(counts))
+        assert torch.equal(a[first:first + hidden], b[first:first + hidden])
+        first += n

@@ -213,7 +213,8 @@ __global__ __launch_bounds__(KVA_T) void k_kv8_append(KvAppendArgs a, uint32_t t
 constexpr int KVT = 32;      // tokens of a step
 
 // A token's softmax weight times its page's value scale enters binary16 as p vs 2^(KV_PE - e), where 2^e is a power of two
-// above every value scale so far in magnitude: 2^KV_PE at most, so that small weights stay normal. Only
+// above every value scale that the row has seen so far in magnitude: 2^KV_PE at most, so that small weights stay normal. A page
+// that a row's mask hides does not count for it, so what the row cannot see does not change it. Only
 // exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is.
 constexpr int KV_PE = 11;
 constexpr int KV_NONE = -1000;  // e before any scale
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   float m = -__builtin_inff(), l = 0.f;
 #pragma unroll
   for (int j = 0; j < VD; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  int ve = KV_NONE;  // the sums are in units of 2^(ve - KV_PE)
+  int ve = KV_NONE;  // this lane's row's sums are in units of 2^(ve - KV_PE)
   bool bad = false;
 
 #pragma unroll 1
@@ -426,14 +427,21 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
         s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[x], s[u], 0, 0, 0);
       }
     }
-    // a page's value scale above all before it: the sums go into its units
-    const int was = ve;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int e = kv_scale_exp(cur.vs[u]);
-      ve = cur.pg[u] >= 0 && e > ve ? e : ve;
-    }
     const bool masked = t0 < full_lo || t0 + KVT > full_hi || cur.pg[0] < 0 || cur.pg[1] < 0;
+    // a page's value scale above all that the row has seen: its sums go into that one's units
+    const int was = ve;
+    {
+      int e[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) e[u] = kv_scale_exp(cur.vs[u]);
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (cur.pg[u] < 0 || t0 + 16 * u >= hi || t0 + 16 * u + 16 <= lo) e[u] = KV_NONE;
+      }
+      const int top = e[0] > e[1] ? e[0] : e[1];
+      ve = top > ve ? top : ve;
+    }
     float top = -__builtin_inff();
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -855,7 +863,9 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
   float m = -__builtin_inff(), l = 0.f;
-  int ve = KV_NONE;  // the sums are in units of 2^(ve - KV_PE)
+  int ve = KV_NONE;                  // this lane's row's sums are in units of 2^(ve - KV_PE)
+  int most = KV_NONE, least = KV_NONE;  // at least, and at most, what ve is in every row of the wave
+  float up = 0.f, down = 1.f;        // most - ve, and 2^-up
   // scale (as scn) and missing groups of the tile in LDS
   float scl;
   uint32_t none;
@@ -888,6 +898,38 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
       __syncthreads();
       continue;
     }
+    const uint32_t no = none;
+    const float sc = scl;
+    const int was = ve;
+    const bool open = no == 0 && t0 >= full_lo && t0 + TT <= full_hi;  // every row sees all of it
+    // a value scale above all that a row has seen: its sums go into that one's units
+    {
+      const int el = kv_scale_exp(sc);
+      int e[GR], top = KV_NONE;
+#pragma unroll
+      for (int u = 0; u < GR; ++u) {
+        e[u] = __builtin_amdgcn_readlane(el, GR + u);
+        top = e[u] > top ? e[u] : top;
+      }
+      if (!open || top > least) {
+        if (open) {
+          ve = top > ve ? top : ve;
+          least = top;
+        } else {
+          top = KV_NONE;
+#pragma unroll
+          for (int u = 0; u < GR; ++u) {
+            const int t = t0 + 16 * u;
+            const bool have = (no >> u & 1u) == 0;
+            top = have && t < whi && t + 16 > wlo && e[u] > top ? e[u] : top;
+            ve = have && t < hi && t + 16 > lo && e[u] > ve ? e[u] : ve;
+          }
+        }
+        most = top > most ? top : most;
+        up = static_cast<float>(most - ve);
+        down = kv_shift(1.f, ve - most);
+      }
+    }
     f32x16 s[TT / 32];
 #pragma unroll
     for (int x = 0; x < D / 16; ++x)
@@ -899,23 +941,11 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     // A wave in between its products goes first, so that the SIMD's other one has the matrix cores meanwhile. It pays for heads of 64, whose
     // products are short (2048 tokens on themselves 51 -> 46.5 us); with 96, 128 and 256 it costs 0 to 3 %.
     if constexpr (D <= 64) __builtin_amdgcn_s_setprio(1);
-    const uint32_t no = none;
-    const float sc = scl;
-    const int was = ve;
-    // a value scale above all before it: the sums go into its units (a wave's own: its sums alone are in these)
-    {
-      const int el = kv_scale_exp(sc);
-#pragma unroll
-      for (int u = 0; u < GR; ++u) {
-        const int e = __builtin_amdgcn_readlane(el, GR + u);
-        ve = (no >> u & 1u) == 0 && e > ve ? e : ve;
-      }
-    }
-    // lane-wise: V's factor of the weights, its logarithm and inverse; or K's of the scores
-    const float wl = kv_shift(sc, KV_PE - ve), lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
+    // lane-wise: V's factor of the weights, its logarithm and inverse, in units of 2^(most - KV_PE); or K's of the scores
+    const float wl = kv_shift(sc, KV_PE - most), lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
     // factors of the usual kind, no masks: see below
     const bool usual = (lane & GR) != 0 ? wl >= 0x1p-8f && wl < 0x1p11f : sc >= 0.f && a.scale >= 0.f;
-    const bool plain = (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && no == 0 && t0 >= full_lo && t0 + TT <= full_hi;
+    const bool plain = (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && open;
     auto of = [&](float x, int u) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), u)); };
     move();
     {
@@ -952,7 +982,8 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[j][e] *= fo;
       }
-      const float base = m == -__builtin_inff() ? 0.f : m;
+      const float base = m == -__builtin_inff() ? 0.f : m, rise = up - base;
+      float sums = 0.f;
       if constexpr (D <= 64) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int u = 0; u < TT / 32; ++u)
@@ -962,7 +993,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
           f16x8 pf;
           if (plain) {
             // the exponential with the value's factor in its exponent: one multiply-add and one exponential a weight
-            const float kf = qs * of(sc, gu), lw = of(lwl, GR + gu) - base;
+            const float kf = qs * of(sc, gu), lw = of(lwl, GR + gu) + rise;
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -973,9 +1004,9 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
               pf[e] = h2[0];
               pf[e + 1] = h2[1];
             }
-            l += sum * of(rwl, GR + gu);
+            sums += sum * of(rwl, GR + gu);
           } else {
-            const float w = of(wl, GR + gu);
+            const float w = kv_shift(of(sc, GR + gu), KV_PE - ve);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float v = s[u][8 * sl + e], p = __builtin_amdgcn_exp2f(v - base);
@@ -991,6 +1022,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
             o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
           }
         }
+      l += sums * down;
     }
     __syncthreads();
   }
