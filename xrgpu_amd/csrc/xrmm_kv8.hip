@@ -329,11 +329,14 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   const int tlo = lo_all + static_cast<int>(split * chunk);
   const int thi = splits > 1 && split + 1 < parts ? tlo + static_cast<int>(chunk) : hi_all;
 
+  // the first token that a row sees: pages wholly before it may be gone (no branch around the lookup: it would be waited for)
+  const int seen = row_lo(i0);
   auto find = [&](int t0, int32_t (&pg)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int32_t p = kv_page(c, b, t0 + 16 * u);
-      pg[u] = t0 + 16 * u < thi ? p : -2;
+      const int t = t0 + 16 * u;
+      const int32_t p = kv_page(c, b, t);
+      pg[u] = ((t < thi) & (t + 16 > seen)) ? p : -2;
     }
   };
   auto load = [&](KvStep<D>& s, const int32_t (&pg)[2], int t0) {
@@ -716,10 +719,11 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   float scn;                   // this lane's scale of the loaded tile
   uint32_t none_n = 0;         // the loaded tile's 16-token groups in no page, a bit each
   bool bad = false;
-  const int lg = lane & (GR - 1);
+  const int lg = lane & (GR - 1), seen = row_lo(query(r0));  // the first token that a row sees: pages wholly before it may be gone
   auto find = [&](int t0) {
-    const int32_t p = kv_page(c, b, t0 + 16 * lg);
-    pgl = t0 + 16 * lg < thi ? p : -2;
+    const int t = t0 + 16 * lg;
+    const int32_t p = kv_page(c, b, t);
+    pgl = ((t < thi) & (t + 16 > seen)) ? p : -2;
   };
   const uint32_t page_bytes = static_cast<uint32_t>(c.page) * D;  // of one head
   auto page_of = [&](int u) {  // of a group, page 0 where there is none
