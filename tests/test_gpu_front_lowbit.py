@@ -114,3 +114,47 @@ def test_append_and_attention(gpu, dt, n):
     assert f.kv8_append(k[:0], v[:0], *c, None, None, None) is None
     with pytest.raises(ValueError):
         ops.kv8_attention(q, *c, window=-1)
+
+
+@pytest.mark.parametrize("call", ["product", "attention"])
+def test_a_workspace_lives_until_the_launch_that_uses_it(gpu, call):
+    """Another thread may replace the table's workspace while a call is without the interpreter's lock: here the
+    entry point itself does, in place of a launch. The call's workspace must not come back as another tensor's memory."""
+    import ctypes
+
+    from xrgpu_amd import _native as nat
+    ops = _ops()
+    names = ["xrmm_mx4_quantize", "xrmm_matmul_mx4_workspace_bytes", "xrmm_matmul_mx4", "xrmm_kv8_append",
+             "xrmm_kv8_attention_workspace_bytes", "xrmm_kv8_attention"]
+    address = [ctypes.cast(getattr(nat.lib(), n), ctypes.c_void_p).value for n in names]
+    if call == "product":
+        B, S = weights(64, 8192)
+        A = torch.randn(40, 8192, device="cuda").half()
+        run, which, at = (lambda: ops._FRONT.matmul_mx4(A, B, S, None, None, None)), 2, -3
+        ops.matmul_mx4(A, B, S)
+    else:
+        c = cache([5000], H=1, D=128, page=64)
+        q = torch.randn(1, 4, 128, device="cuda").half()
+        run, which, at = (lambda: ops._FRONT.kv8_attention(q, *c, None, None, None, True, 0, None)), 5, -3
+        ops.kv8_attention(q, *c)
+    fn = getattr(nat.lib(), names[which])
+    seen = []
+
+    def entry(*args):
+        ws, size = args[at], args[at + 1]
+        key = next(k for k, t in ops._WORKSPACES.items() if t.data_ptr() == ws)
+        ops._WORKSPACES[key] = torch.zeros(2 * size, dtype=torch.uint8, device="cuda")
+        seen.append((ws, [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(4)]))
+        return 0
+
+    fake = ctypes.CFUNCTYPE(fn.restype, *fn.argtypes)(entry)
+    there = list(address)
+    there[which] = ctypes.cast(fake, ctypes.c_void_p).value
+    bind = ops._FRONT.bind_lowbit
+    try:
+        bind(ops._WORKSPACES, torch._C._cuda_isCurrentStreamCapturing, *there)
+        assert torch.is_tensor(run())
+    finally:
+        bind(ops._WORKSPACES, torch._C._cuda_isCurrentStreamCapturing, *address)
+    (ws, others), = seen
+    assert ws and all(t.data_ptr() != ws for t in others)

@@ -12,8 +12,8 @@
 // return values and no exceptions: a throw costs 4 us, more than the checks (a float32
 // call on a workspace 17 x 1024 x 1024 took 18.7 us on the host with throws and every
 // check made twice, 15.8 without a front end).
-// Nothing is kept between calls; the MX4 and kv8 calls look their workspace up in ops.py's own table (its
-// bytes come back as above where it is not there yet, too small, or a graph is being captured). Measured, among other passes: Qkv 4 x 4096 x (4096 + 2 x
+// Nothing is kept between calls; the MX4 and kv8 calls look their workspace up in ops.py's own table and hold it until
+// they return (its bytes come back as above where it is not there yet, too small, or a graph is being captured). Measured, among other passes: Qkv 4 x 4096 x (4096 + 2 x
 // 1024) 17.8 -> 7.6 us a call, MatMulNBits 1 x 4096 x 14336 8.4 -> 6.9.
 #include <Python.h>
 #include <torch/csrc/Dtype.h>
@@ -427,7 +427,8 @@ PyObject *g_workspaces, *g_capturing;  // {(device, stream): uint8 tensor} of op
 int lt(at::ScalarType t) { return t == at::kHalf ? F16 : t == at::kFloat ? F32 : t == at::kBFloat16 ? BF16 : -1; }
 
 // ops.py's workspace of the stream where it is large enough and no graph is captured; else none, and `need` is ops.py's to meet.
-bool kept_workspace(int dev, void* st, int64_t need, void*& ws, int64_t& bytes) {
+// The caller holds the tensor until its launch is enqueued: meanwhile another thread may put a larger one in its place.
+bool kept_workspace(int dev, void* st, int64_t need, at::Tensor& ws) {
   PyObject* c = PyObject_CallNoArgs(g_capturing);
   const bool eager = c == Py_False;
   Py_XDECREF(c);
@@ -439,11 +440,12 @@ bool kept_workspace(int dev, void* st, int64_t need, void*& ws, int64_t& bytes) 
   PyObject* o = key ? PyDict_GetItem(g_workspaces, key) : nullptr;  // borrowed
   Py_XDECREF(key);
   if (o == nullptr || !THPVariable_CheckExact(o)) return false;
-  const at::Tensor& t = THPVariable_Unpack(o);
-  ws = t.data_ptr();
-  bytes = t.numel();
-  return bytes >= need;
+  ws = THPVariable_Unpack(o);
+  return ws.numel() >= need;
 }
+
+void* data_of(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int64_t bytes_of(const at::Tensor& t) { return t.defined() ? t.numel() : 0; }
 
 // A tensor [tokens, heads, dim] whose tokens may lie apart.
 bool token_rows(PyObject* o, int& dev, int64_t heads, int64_t dim, const at::Tensor*& out, int64_t& stride) {
@@ -559,12 +561,11 @@ PyObject* matmul_mx4(PyObject*, PyObject* const* v, Py_ssize_t n) {
     }
     const int64_t M = A->numel() / (mx ? kb * 16 : K);
     const int at_ = mx ? U8 : lt(A->scalar_type());
-    void *st, *ws = nullptr;
+    void* st;
     if (!stream_of(dev, st)) Py_RETURN_NONE;
     const int64_t need = g_mx4_ws(M, K, N, at_);
-    int64_t bytes = 0;
-    if (need > 0 && !kept_workspace(dev, st, need, ws, bytes)) return PyLong_FromLongLong(need);
-    at::Tensor y;
+    at::Tensor y, ws;
+    if (need > 0 && !kept_workspace(dev, st, need, ws)) return PyLong_FromLongLong(need);
     int rc;
     {
       NoGil ng;
@@ -572,7 +573,7 @@ PyObject* matmul_mx4(PyObject*, PyObject* const* v, Py_ssize_t n) {
       s.push_back(N);
       y = at::empty(s, A->options().dtype(out));
       rc = g_mx4(A->data_ptr(), T ? T->data_ptr() : nullptr, at_, B->data_ptr(), S->data_ptr(), bias, y.data_ptr(), lt(out), M, K,
-                 N, ws, bytes, st);
+                 N, data_of(ws), bytes_of(ws), st);
     }
     if (!checked(rc)) return nullptr;
     return THPVariable_Wrap(y);
@@ -615,7 +616,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     int64_t qs = 0;
     int32_t most = 0, window = 0;
     float scale;
-    void *st, *ws = nullptr;
+    void* st;
     if (!c.set(v + 1, v[7], v[12], dev) || !small(v[8], most) || !PyBool_Check(v[10]) || none(v[11]) || !small(v[11], window) ||
         !THPVariable_CheckExact(v[0]) || THPVariable_Unpack(v[0]).dim() != 3)
       Py_RETURN_NONE;
@@ -629,16 +630,16 @@ PyObject* kv8_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const int32_t B = static_cast<int32_t>(c.B), W = static_cast<int32_t>(c.W), page = static_cast<int32_t>(c.page),
                   H = static_cast<int32_t>(c.H), D = static_cast<int32_t>(c.D), causal = v[10] == Py_True;
     const int64_t need = g_attend_ws(q->size(0), most, c.starts != nullptr, B, W, page, static_cast<int32_t>(Hq), H, D, causal, window);
-    int64_t bytes = 0;
-    if (need > 0 && !kept_workspace(dev, st, need, ws, bytes)) return PyLong_FromLongLong(need);
-    at::Tensor o;
+    at::Tensor o, ws;
+    if (need > 0 && !kept_workspace(dev, st, need, ws)) return PyLong_FromLongLong(need);
     int rc;
     {
       NoGil ng;
       o = at::empty(q->sizes(), q->options());
       rc = g_attend(q->data_ptr(), qs, o.data_ptr(), lt(q->scalar_type()), c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(),
                     c.vs->data_ptr(), c.dt, c.table->data_ptr(), c.lengths->data_ptr(), c.starts, c.status, q->size(0), most, B, W,
-                    c.P, page, static_cast<int32_t>(Hq), H, D, scale, causal, window, ws, bytes, st);
+                    c.P, page, static_cast<int32_t>(Hq), H, D, scale, causal, window, data_of(ws),
+                    bytes_of(ws), st);
     }
     if (!checked(rc)) return nullptr;
     return THPVariable_Wrap(o);
