@@ -1,8 +1,7 @@
 """GPU: attention at the edges of windows, tables and lengths; tolerances as in test_gpu_kv8_scales.py."""
-import numpy as np
 import pytest
 
-from tests.test_gpu_kv8 import Cache
+from tests.test_gpu_kv8 import Cache, ops, starts_of
 from tests.test_gpu_kv8_scales import check, queries
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +18,28 @@ def test_pages_behind_the_window_may_be_gone(gpu, page, D, counts, window):
         c.table[b, : max(0, x - n - window + 1) // page] = -1
     assert (c.table[:, 0] == -1).all() or counts[0] == 200
     check(c, queries(sum(counts), 2, D, "f16"), counts, window=window)
+
+
+@pytest.mark.parametrize("counts", [[10, 3], [70, 200]])  # the first rows stand before position 0
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 62])
+def test_windows_without_end(gpu, counts, causal, window):
+    lens = [3, 150]
+    c = Cache("int8", lens, 1, 64, 16, seed=1)
+    q = queries(sum(counts), 2, 64, "f16")
+    check(c, q, counts, causal=causal, window=window)
+    a = ops().kv8_attention(q, **c.dev(), starts=starts_of(counts), max_new=1 << 40, causal=causal, window=window)
+    assert torch.equal(a, ops().kv8_attention(q, **c.dev(), starts=starts_of(counts), causal=causal))
+
+
+def test_negative_lengths_see_nothing(gpu):
+    c = Cache("int8", [20, 40], 1, 64, 16, seed=2)
+    q = queries(4, 2, 64, "f16")
+    good = ops().kv8_attention(q, **c.dev())
+    for bad in (-1, -(1 << 31)):
+        d = c.dev()
+        d["lengths"][0] = bad
+        for kw in ({}, {"window": (1 << 31) - 1}, {"causal": False}):
+            o = ops().kv8_attention(q, **d, **kw)
+            assert (o[:2] == 0).all()
+        assert torch.equal(ops().kv8_attention(q, **d)[2:], good[2:])

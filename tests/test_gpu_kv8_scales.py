@@ -29,7 +29,7 @@ def seen_top(c, counts, Hq, causal, window):
     return top * LB.QMAX[c.kind]
 
 
-def check(c, q, counts, *, causal=True, window=0, scale=None, workspace=True):
+def check(c, q, counts, *, causal=True, window=0, scale=None):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     o = ops().kv8_attention(q, **c.dev(), starts=starts_of(counts), max_new=max(counts), causal=causal, window=window, scale=scale,
                             status=status)

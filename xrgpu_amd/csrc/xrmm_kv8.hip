@@ -315,14 +315,14 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   const int nrows = count * G, r0 = tile * 16;
   if (r0 >= nrows) return;
   // positions past the table are left out: the walk over tokens ends with the table
-  const int span = c.width << c.page_log2, all = c.lengths[b], past = all - count;
-  const int len = all < 0 ? 0 : all < span ? all : span;
+  const int span = c.width << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0, past = all - count;
+  const int len = all < span ? all : span;
   if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   // the tokens that any of the rows sees, and those that all of them see
   const int last = r0 + 16 < nrows ? r0 + 15 : nrows - 1, i0 = r0 / G, i1 = last / G;
   auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
-  auto row_lo = [&](int i) { return a.window > 0 && past + i - a.window + 1 > 0 ? past + i - a.window + 1 : 0; };
+  auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
   const int lo_all = row_lo(i0) / KVT * KVT, hi_all = row_hi(i1), full_lo = row_lo(i1), full_hi = row_hi(i0);
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;  // at most `splits`
   if (split >= parts) return;
@@ -695,11 +695,11 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
   const int nrows = count * G, r0 = tile * KVM_ROWS;
   if (r0 >= nrows) return;
-  const int span = c.width << c.page_log2, all = c.lengths[b], past = all - count;
-  const int len = all < 0 ? 0 : all < span ? all : span;
+  const int span = c.width << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0, past = all - count;
+  const int len = all < span ? all : span;
   if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
   auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
-  auto row_lo = [&](int i) { return a.window > 0 && past + i - a.window + 1 > 0 ? past + i - a.window + 1 : 0; };
+  auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
   auto query = [&](int r) { return (r < nrows ? r : nrows - 1) / G; };  // of a row, the last one's past the end
   const int lo_all = row_lo(query(r0)) / TT * TT, hi_all = row_hi(query(r0 + KVM_ROWS - 1));
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;

@@ -795,6 +795,11 @@ def matmul_mx4_kernel(M, K, N, dtype=torch.float16) -> str:
     return r.decode()
 
 
+def _i32(v):
+    """A bound for the C entry points, whose integers have 32 bits: a larger one bounds nothing more."""
+    return max(-1 << 31, min(int(v), (1 << 31) - 1))
+
+
 def _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status):
     if k_cache.dtype not in _CACHE or v_cache.dtype != k_cache.dtype:
         raise nat.XrmmInvalid("k_cache and v_cache must both be int8 or float8_e4m3fn")
@@ -813,6 +818,8 @@ def _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, sta
         raise nat.XrmmInvalid(f"starts must be int32 [{B + 1}]")
     if status is not None and (status.dtype not in (torch.int32, torch.uint32) or status.numel() < 1):
         raise nat.XrmmInvalid("status must be an int32 or uint32 tensor of at least one element")
+    if max(B, *block_table.shape, *k_cache.shape) >= 1 << 31:
+        raise nat.XrmmInvalid("the cache's and the table's dimensions must be below 2^31")
     return B, P, H, int(k_cache.shape[2]), int(k_cache.shape[3])
 
 
@@ -858,7 +865,7 @@ def kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     nat.check(nat.lib().xrmm_kv8_append(
         _ptr(k), _ptr(v), ks, vs, _LT[k.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
         _CACHE[k_cache.dtype], _ptr(block_table), _ptr(lengths), _ptr(starts), _ptr(status), int(k.shape[0]),
-        int(max_new or 0), B, int(block_table.shape[1]), P, page, H, D, _stream(stream, dev)))
+        _i32(max_new or 0), B, int(block_table.shape[1]), P, page, H, D, _stream(stream, dev)))
 
 
 def kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths, *, starts=None, max_new=None, scale=None,
@@ -886,24 +893,24 @@ def kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     _check_out(out, (T, Hq, D), q.dtype)
     dev = _check_dev(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status, out)
     _same_device(dev, q)
-    W, most = int(block_table.shape[1]), int(max_new or 0)
+    W, most, window = int(block_table.shape[1]), _i32(max_new or 0), _i32(window)
     lib = nat.lib()
     s = _stream(stream, dev)
     need = int(lib.xrmm_kv8_attention_workspace_bytes(T, most, int(starts is not None), B, W, page, Hq, H, D, int(causal),
-                                                      int(window)))
+                                                      window))
     ws, nws = _take_workspace(need, workspace, q, dev, s, stream)
     if out is None:
         out = _empty((T, Hq, D), q.dtype, q.device, stream)
     nat.check(lib.xrmm_kv8_attention(
         _ptr(q), qs, _ptr(out), _LT[q.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
         _CACHE[k_cache.dtype], _ptr(block_table), _ptr(lengths), _ptr(starts), _ptr(status), T, most, B, W, P, page, Hq, H,
-        D, float(D ** -0.5 if scale is None else scale), int(causal), int(window), _ptr(ws), nws, s))
+        D, float(D ** -0.5 if scale is None else scale), int(causal), window, _ptr(ws), nws, s))
     return out
 
 
 def kv8_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batch, table_width, page_size, max_new=0, ragged=False,
                                   causal=True, window=0):
     """Bytes of the split workspace of a kv8_attention call (0: none); ``ragged``: the call has ``starts``."""
-    return int(nat.lib().xrmm_kv8_attention_workspace_bytes(int(T), int(max_new), int(ragged), int(batch), int(table_width),
+    return int(nat.lib().xrmm_kv8_attention_workspace_bytes(int(T), _i32(max_new), int(ragged), int(batch), int(table_width),
                                                             int(page_size), int(q_heads), int(kv_heads), int(head_dim),
-                                                            int(causal), int(window)))
+                                                            int(causal), _i32(window)))
