@@ -43,3 +43,36 @@ def test_negative_lengths_see_nothing(gpu):
             o = ops().kv8_attention(q, **d, **kw)
             assert (o[:2] == 0).all()
         assert torch.equal(ops().kv8_attention(q, **d)[2:], good[2:])
+
+
+@pytest.mark.parametrize("n,D,page", [(1, 64, 256), (6, 128, 256), (150, 64, 256), (150, 256, 128)])
+def test_positions_up_to_2_to_the_31(gpu, n, D, page):
+    """A window at the end of the longest table gives what it gives at a short one's end, where all pages before it are gone."""
+    far, pages = (0x7FFFFF00 // page) * page, 1024 // page
+    c = Cache("int8", [1024], 1, D, page, seed=5, extra=0)
+    q, kv = queries(n, 2, D, "f16"), queries(n, 1, D, "bf16", seed=1)
+    near, there = c.dev(), c.dev()
+    table = torch.full((1, far // page), -1, dtype=torch.int32, device="cuda")
+    table[:, -pages:] = near["block_table"]
+    there["block_table"], there["lengths"] = table, torch.tensor([far], dtype=torch.int32, device="cuda")
+    out = []
+    for d in (near, there):
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        ops().kv8_append(kv, kv, **d, status=status)
+        out.append(ops().kv8_attention(q, **d, window=300, status=status))
+        assert int(status.item()) == 0
+    assert torch.equal(*out)
+    for name in ("k_cache", "v_cache", "k_scales", "v_scales"):
+        assert torch.equal(near[name].view(torch.uint8), there[name].view(torch.uint8))
+
+
+@pytest.mark.parametrize("n", [1, 20, 150])
+@pytest.mark.parametrize("length", [0x7FFFFFFF, 0x7FFFFF00, 5000])
+def test_lengths_past_the_table_behind_a_window(gpu, n, length):
+    """Windows that begin past the table's end: nothing is left to see, and the walk ends at once."""
+    c = Cache("int8", [100], 1, 64, 16, seed=6)
+    d = c.dev()
+    d["lengths"][0] = length
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert (ops().kv8_attention(queries(n, 2, 64, "f16"), **d, window=20, status=status) == 0).all()
+    assert int(status.item()) == 55

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(KVA_T) void k_kv8_append(KvAppendArgs a, uint32_t t
   };
   each_held([&](int j) { held[j] = *reinterpret_cast<const vec*>(piece(tid + j * KVA_T)); });
 
-  const int32_t page = base < 0 || base > 0x7FFFFFFF ? -1 : kv_page(c, b, static_cast<int>(base));
+  const int32_t page = base < 0 || base > 0x7FFFFFFF ? -1 : kv_page(c, b, static_cast<uint32_t>(base));
   if (page < 0) {
     if (tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
     return;
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   const int last = r0 + 16 < nrows ? r0 + 15 : nrows - 1, i0 = r0 / G, i1 = last / G;
   auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
   auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
-  const int lo_all = row_lo(i0) / KVT * KVT, hi_all = row_hi(i1), full_lo = row_lo(i1), full_hi = row_hi(i0);
+  const int hi_all = row_hi(i1), lo_all = (row_lo(i0) < hi_all ? row_lo(i0) : hi_all) / KVT * KVT, full_lo = row_lo(i1), full_hi = row_hi(i0);
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;  // at most `splits`
   if (split >= parts) return;
   const int tlo = lo_all + static_cast<int>(split * chunk);
@@ -331,23 +331,23 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 
   // the first token that a row sees: pages wholly before it may be gone (no branch around the lookup: it would be waited for)
   const int seen = row_lo(i0);
-  auto find = [&](int t0, int32_t (&pg)[2]) {
+  auto find = [&](uint32_t t0, int32_t (&pg)[2]) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = t0 + 16 * u;
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t t = t0 + 16 * u;
       const int32_t p = kv_page(c, b, t);
-      pg[u] = ((t < thi) & (t + 16 > seen)) ? p : -2;
+      pg[u] = ((t < static_cast<uint32_t>(thi)) & (t + 16 > static_cast<uint32_t>(seen))) ? p : -2;
     }
   };
-  auto load = [&](KvStep<D>& s, const int32_t (&pg)[2], int t0) {
+  auto load = [&](KvStep<D>& s, const int32_t (&pg)[2], uint32_t t0) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = t0 + 16 * u;
+    for (uint32_t u = 0; u < 2; ++u) {
+      const uint32_t t = t0 + 16 * u;
       s.pg[u] = pg[u];
       const int64_t at = static_cast<int64_t>(pg[u] < 0 ? 0 : pg[u]) * c.Hkv + h;
       s.ks[u] = c.ks[at];
       s.vs[u] = c.vs[at];
-      const int64_t slot = (at * c.page + (t & (c.page - 1))) * D;
+      const int64_t slot = (at * c.page + (t & static_cast<uint32_t>(c.page - 1))) * D;
       s.k[u] = kv_bytes<KD>(c.k + slot + col * D + g * KD);
 #pragma unroll
       for (int x = 0; x < 4; ++x) s.v[4 * u + x] = kv_bytes<VD>(c.v + slot + (4 * g + x) * D + col * VD);
@@ -355,9 +355,10 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   };
   int32_t pg[2];
   KvStep<D> cur;
-  find(tlo + wave * KVT, pg);
-  load(cur, pg, tlo + wave * KVT);
-  find(tlo + wave * KVT + (W * KVT), pg);
+  const uint32_t tw = static_cast<uint32_t>(tlo + wave * KVT);
+  find(tw, pg);
+  load(cur, pg, tw);
+  find(tw + W * KVT, pg);
 
   // this lane's row: its query as binary16 (scaled by a power of two for bfloat16), what it sees
   f16x8 q[KD / 8];
@@ -416,8 +417,8 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 #pragma unroll 1
   for (int t0 = tlo + wave * KVT; t0 < thi; t0 += (W * KVT)) {
     KvStep<D> nxt;
-    load(nxt, pg, t0 + (W * KVT));
-    find(t0 + 2 * (W * KVT), pg);
+    load(nxt, pg, static_cast<uint32_t>(t0) + W * KVT);
+    find(static_cast<uint32_t>(t0) + 2 * (W * KVT), pg);
     bad |= cur.pg[0] == -1 || cur.pg[1] == -1;
     // scores
     f32x4 s[2];
@@ -701,7 +702,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
   auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
   auto query = [&](int r) { return (r < nrows ? r : nrows - 1) / G; };  // of a row, the last one's past the end
-  const int lo_all = row_lo(query(r0)) / TT * TT, hi_all = row_hi(query(r0 + KVM_ROWS - 1));
+  const int hi_all = row_hi(query(r0 + KVM_ROWS - 1)), lo_all = (row_lo(query(r0)) < hi_all ? row_lo(query(r0)) : hi_all) / TT * TT;
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;
   if (split >= parts) return;
   const int tlo = lo_all + static_cast<int>(split * chunk);

@@ -119,11 +119,11 @@ __device__ __forceinline__ bool kv_rows(const KvCache& c, int b, int most, int& 
   return ok;
 }
 
-// The page that holds token t of sequence b, or -1 where there is none. Reads the table in any case (the
-// host gives an empty one the address of the lengths), so that lookups need no branches.
-__device__ __forceinline__ int32_t kv_page(const KvCache& c, int b, int t) {
-  const int i = t >> c.page_log2;
-  const bool in = t >= 0 && i < c.width;
+// The page that holds token t of sequence b, or -1 where there is none: also past 2^31, where walks look ahead, as tables
+// span less. Reads the table in any case (the host gives an empty one the address of the lengths), so that lookups need no branches.
+__device__ __forceinline__ int32_t kv_page(const KvCache& c, int b, uint32_t t) {
+  const uint32_t i = t >> c.page_log2;
+  const bool in = i < static_cast<uint32_t>(c.width);
   const int32_t p = c.table[static_cast<int64_t>(b) * c.width + (in ? i : 0)];
   return in && p >= 0 && p < c.pages ? p : -1;
 }
