@@ -437,7 +437,7 @@ int xrmm_mx4_quantize(const void* x, void* codes, void* scales, int64_t rows, in
  * XRMM_BF16; bias has that type). a_dtype: XRMM_F16 or XRMM_BF16 (A_scales NULL), or
  * XRMM_U8: A holds MX4 codes [M, kb, 16] with A_scales [M, kb]. Codes are 16-byte
  * aligned; K at most 2^23. Weights past float32's range (scale bytes 253 and 254)
- * are infinite. The workspace, at least xrmm_matmul_mx4_workspace_bytes (0: none
+ * may count as infinite. The workspace, at least xrmm_matmul_mx4_workspace_bytes (0: none
  * used), is optional and has the form of xrmm_matmul_nbits_ws's: 256-byte
  * aligned, its first 4096 bytes zero before its first use and after every call. With it,
  * geometries with few output tiles split K across workgroups (added in a fixed order). */

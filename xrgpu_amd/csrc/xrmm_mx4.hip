@@ -228,7 +228,8 @@ __global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a, uint32_t col_
 // Product, one or two rows of 16-bit activations. A wave holds 64 blocks of K, one a lane, of every row in
 // registers and walks over columns: a column's 64 blocks are one load of 1 KB. A lane sums its block
 // from the codes as they are (exact in 16 bits whatever the scale; two products and a float32 sum in one v_dot2) and
-// then applies the scale, so no scale is out of range. The lanes' sums meet by DPP, the chunks of K in LDS,
+// then applies the scale to the sum's exponent, so no scale is out of range. For bfloat16 activations the codes count 2^-8 of their
+// value meanwhile: 32 products of 6 and the largest bfloat16 would pass float32. The lanes' sums meet by DPP, the chunks of K in LDS,
 // in order. Nothing but the loop over columns repeats, and it is short: the kernel lives for a few microseconds, and
 // unrolled code is fetched slower than it runs. 1 x 4096 x 14336: 9.0 us, 31 MB.
 
@@ -255,6 +256,7 @@ constexpr int MXD_MAX_WAVES = 16, MXD_MAX_COLS = 64;
 template <int AT, int R, bool AL>
 __global__ __launch_bounds__(64 * MXD_MAX_WAVES) void k_mx4_dot(MxArgs a, uint32_t ncols, uint32_t chunk_waves, uint32_t col_waves) {
   constexpr int P = 2;  // columns whose loads are in flight together
+  constexpr int UP = AT == LT_F16 ? 0 : 8;
   __shared__ float part[MXD_MAX_WAVES][MXD_MAX_COLS][R];
   const int tid = threadIdx.x, lane = tid & 63;
   const uint32_t wave = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(tid >> 6));
@@ -310,16 +312,16 @@ __global__ __launch_bounds__(64 * MXD_MAX_WAVES) void k_mx4_dot(MxArgs a, uint32
         for (int r = 0; r < R; ++r) sum[r] = 0.f;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const u32x4 wv = __builtin_bit_cast(u32x4, mx_dq8<AT>(w[p][d], 1.f));
+          const u32x4 wv = __builtin_bit_cast(u32x4, mx_dq8<AT>(w[p][d], 1.f / (1 << UP)));
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int r = 0; r < R; ++r) sum[r] = mx_dot2<AT>(wv[e], x[r][d][e], sum[r]);
         }
-        const float sc = e8m0(s[p]);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float t = mx_wave_total(in ? sum[r] * sc : 0.f);
+          const float scaled = s[p] == 255u ? __builtin_nanf("") : __builtin_ldexpf(sum[r], static_cast<int>(s[p]) - 127 + UP);
+          const float t = mx_wave_total(in ? scaled : 0.f);
           if (lane == r && cp < cols) part[wave][cp][r] += t;
         }
       }
