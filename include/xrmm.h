@@ -467,8 +467,9 @@ int xrmm_matmul_mx4_plan(int64_t M, int64_t K, int64_t N, int32_t a_dtype, int32
  * rows / batch each when starts is NULL; they are the sequence's last ones. max_new:
  * at least the most tokens a sequence has in the call (0: not known). head_dim 64,
  * 96, 128 or 256; page_size a power of two from 16 to 256. A page outside [0, pages), a
- * position below 0 or past the table, or `starts` outside the rows is left out and
- * raises `status` (a device uint32, or NULL) to 55.
+ * position past the table, or `starts` outside the rows is left out and raises
+ * `status` (a device uint32, or NULL) to 55. Positions below 0 (more new tokens than
+ * `lengths` counts) raise it where tokens are written, not where they query.
  *
  * xrmm_kv8_append writes the call's tokens (k, v [rows, kv_heads, head_dim] of dtype,
  * token strides in elements). Let e(r) be the smallest integer >= -126 with
@@ -487,9 +488,14 @@ int xrmm_kv8_append(const void* k, const void* v, int64_t k_stride, int64_t v_st
  * rounded once; q [rows, q_heads, head_dim] of dtype XRMM_F16 or XRMM_BF16, token
  * stride in elements; query head h reads key head h / (q_heads / kv_heads). Query i of a
  * sequence's n stands at p = length - n + i and sees tokens 0 <= t < length, t <= p if
- * causal, t > p - window if window > 0; a row that sees none is 0. Cache scales are any
- * float32. e4m3 NaN codes must not occur (xrmm_kv8_append writes none): rows that do not
- * see such a token may be NaN too. The workspace, at least
+ * causal, t > p - window if window > 0; a row that sees none, as a causal one before
+ * position 0, is 0. Rows that `starts` leaves out are not written. Pages that no row's
+ * window reaches may be missing from the table. Cache scales are any float32. A weight
+ * times its value scale enters the second product with binary16's eleven bits; below
+ * 2^-25 of the largest value scale that the row sees it has fewer, and below 2^-35 none.
+ * The sums over tokens are divided last: they may pass float32 where values come within
+ * a factor of the length of its largest. e4m3 NaN codes must not occur (xrmm_kv8_append
+ * writes none): rows that do not see such a token may be NaN too. The workspace, at least
  * xrmm_kv8_attention_workspace_bytes (0: none used), is optional, of the same form as
  * xrmm_matmul_mx4's; with it, long contexts of few rows are split across
  * workgroups and joined in a fixed order. */

@@ -76,3 +76,15 @@ def test_lengths_past_the_table_behind_a_window(gpu, n, length):
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
     assert (ops().kv8_attention(queries(n, 2, 64, "f16"), **d, window=20, status=status) == 0).all()
     assert int(status.item()) == 55
+
+
+@pytest.mark.parametrize("n", [5, 40])
+def test_positions_below_0_raise_the_status_where_tokens_are_written(gpu, n):
+    c = Cache("int8", [3], 1, 64, 16, seed=7)
+    d = c.dev()
+    q, kv = queries(n, 2, 64, "f16"), queries(n, 1, 64, "f16")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    o = ops().kv8_attention(q, **d, status=status)
+    assert int(status.item()) == 0 and (o[: n - 3] == 0).all() and (o[n - 3:] != 0).any()
+    ops().kv8_append(kv, kv, **d, status=status)
+    assert int(status.item()) == 55

@@ -849,7 +849,7 @@ def kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     ``[batch]``. A page and head has one scale: a power of two that covers what entered, from the first slot on; a larger
     value multiplies it by a power of two and the codes already there are rounded to it. A NaN or an infinity makes the
     scale NaN. ``max_new``: at least the most tokens of one sequence (a bound on the work; T when not given). Pages
-    outside the cache, positions past the table and rows outside T are left out and raise the device word
+    outside the cache, positions below 0 or past the table and rows outside T are left out and raise the device word
     ``status`` (int32) to 55."""
     if stream is None and _front() and _FRONT.kv8_append(k, v, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
                                                          starts, max_new, status):
@@ -875,7 +875,7 @@ def kv8_attention(q, k_cache, v_cache, k_scales, v_scales, block_table, lengths,
     q ``[T, q_heads, head_dim]`` float16 or bfloat16 (token stride free), q_heads a multiple of the cache's heads; the
     queries are each sequence's last tokens, as in kv8_append, whose keys and values are already in the cache.
     Query at position p sees tokens t < lengths[b], t <= p if ``causal``, t > p - window if ``window``. A row that sees none
-    is 0. ``scale``: head_dim^-0.5 when not given. Returns ``[T, q_heads, head_dim]`` of q's dtype. Long contexts of few rows
+    is 0, as a causal one before position 0; rows that ``starts`` leaves out are not written. ``scale``: head_dim^-0.5 when not given. Returns ``[T, q_heads, head_dim]`` of q's dtype. Long contexts of few rows
     are split across workgroups on a workspace (``kv8_attention_workspace_bytes``; see ``matmul_nbits`` for whose it is and
     for graph capture)."""
     if out is None and workspace is None and stream is None and _front():
