@@ -502,6 +502,10 @@ int xrmm_kv8_append(const void* k, const void* v, int64_t k_stride, int64_t v_st
 int64_t xrmm_kv8_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
                                            int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t causal, int32_t window);
+/* Kernel family that xrmm_kv8_attention picks with a workspace, NULL for an invalid geometry. No device work. */
+const char* xrmm_kv8_attention_kernel(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
+                                      int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t causal,
+                                      int32_t window);
 int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
                        const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
                        const void* block_table, const void* lengths, const void* starts, void* status, int64_t rows,

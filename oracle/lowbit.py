@@ -155,3 +155,39 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, table, lengths, counts, k
                     aqk[first + i, h] = (np.abs(kk) @ np.abs(q[first + i, h])).max() * abs(scale)
         first += n
     return o, av, aqk
+
+
+def attention_of_all(q, k_codes, v_codes, k_scales, v_scales, table, lengths, counts, kind, *, scale, causal=True, window=0):
+    """What attention gives, with all rows of a key head at once, for caches whose values are finite."""
+    q = np.asarray(q, np.float64)
+    T, Hq, D = q.shape
+    P, H, page, _ = k_codes.shape
+    G = Hq // H
+    o, av, aqk = np.zeros((T, Hq, D)), np.zeros((T, Hq, D)), np.zeros((T, Hq))
+    first = 0
+    for b, n in enumerate(counts):
+        L = int(lengths[b])
+        if L > 0 and n:
+            t, p = np.arange(L), np.arange(L - n, L)[:, None]
+            pages = np.where(t // page < table.shape[1], table[b, np.minimum(t // page, table.shape[1] - 1)], -1)
+            have = (pages >= 0) & (pages < P)
+            pages = np.where(have, pages, 0)
+            see = np.broadcast_to(have, (n, L))
+            if causal:
+                see = see & (t <= p)
+            if window:
+                see = see & (t > p - window)
+            see = np.repeat(see, G, 0)  # [n G, L]
+            any_ = see.any(1, keepdims=True)
+            for h in range(H):
+                kk, vv = (decode8(c[pages, h, t % page], kind) * s[pages, h].astype(np.float64)[:, None]
+                          for c, s in ((k_codes, k_scales), (v_codes, v_scales)))
+                qq = q[first:first + n, h * G:(h + 1) * G].reshape(n * G, D)
+                z = np.where(see, qq @ kk.T * scale, -np.inf)
+                w = np.exp(z - np.where(any_, z.max(1, keepdims=True), 0.0))
+                w /= np.where(any_, w.sum(1, keepdims=True), 1.0)
+                to = np.s_[first:first + n, h * G:(h + 1) * G]
+                o[to], av[to] = (w @ vv).reshape(n, G, D), (w @ np.abs(vv)).reshape(n, G, D)
+                aqk[to] = np.where(see, np.abs(qq) @ np.abs(kk).T, 0.0).max(1).reshape(n, G) * abs(scale)
+        first += n
+    return o, av, aqk

@@ -66,3 +66,17 @@ def test_attention_uniform_and_empty_rows():
     v = LB.decode8(c, "int8")[1, 0]
     assert (o[0] == 0).all()  # position -1 sees nothing
     assert np.allclose(o[1], v[0]) and np.allclose(o[2], v[:2].mean(0))
+
+
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 9), (False, 0), (False, 12)])
+def test_attention_of_all_rows_is_attention_row_by_row(causal, window):
+    rng = np.random.default_rng(window)
+    k, v = (rng.integers(-127, 128, (9, 2, 16, 8)).astype(np.int8).view(np.uint8) for _ in range(2))
+    ks, vs = (rng.uniform(-0.02, 0.03, (9, 2)).astype(np.float32) for _ in range(2))
+    table, lengths, counts = rng.permutation(9)[:8].reshape(2, 4).astype(np.int32), [50, 3], [7, 5]
+    table[0, 1], table[1, 1:] = -1, -1
+    args = (rng.standard_normal((12, 6, 8)), k, v, ks, vs, table, lengths, counts, "int8")
+    a = LB.attention(*args, scale=0.3, causal=causal, window=window)
+    b = LB.attention_of_all(*args, scale=0.3, causal=causal, window=window)
+    for x, y in zip(a, b):
+        assert np.allclose(x, y, rtol=1e-12, atol=1e-14)

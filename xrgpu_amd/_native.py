@@ -85,6 +85,7 @@ def _sig(lib):
     s("xrmm_kv8_append", ctypes.c_int, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64,
       _i32, _i32, _i32, _i64, _i32, _i32, _i32, _vp)
     s("xrmm_kv8_attention_workspace_bytes", _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32)
+    s("xrmm_kv8_attention_kernel", ctypes.c_char_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32)
     s("xrmm_kv8_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32,
       _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
     s("xrmm_stream_read", ctypes.c_int, _vp, ctypes.c_uint64, _vp, _i32, _vp)

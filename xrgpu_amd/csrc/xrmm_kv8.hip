@@ -1209,6 +1209,10 @@ int64_t kv8_workspace_bytes(const KvAttnArgs& a) {
   return a.c.B == 0 || a.max_new == 0 ? 0 : attention_plan(a, true).ws_bytes;
 }
 
+const char* kv8_kernel_name(const KvAttnArgs& a) {
+  return a.c.B > 0 && a.max_new > 0 && attention_plan(a, true).tile ? "kv8_tile" : "kv8_rows";
+}
+
 hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st) {
   if (a.c.B == 0 || a.max_new == 0) return hipSuccess;
   KvPlan p = attention_plan(a, a.ws != nullptr);

@@ -79,6 +79,7 @@ struct KvAttnArgs {
 hipError_t launch_kv8_append(const KvAppendArgs& a, hipStream_t st);
 hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st);
 int64_t kv8_workspace_bytes(const KvAttnArgs& a);
+const char* kv8_kernel_name(const KvAttnArgs& a);
 
 hipError_t launch_mx4_quantize(const MxQuantArgs& a, hipStream_t st);
 hipError_t launch_matmul_mx4(const MxArgs& a, hipStream_t st);

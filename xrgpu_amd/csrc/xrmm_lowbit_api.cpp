@@ -211,16 +211,36 @@ int attention_of(xrmm::KvAttnArgs& a, const void* q, int64_t q_stride, void* o, 
 
 }  // namespace
 
+namespace {
+
+// The arguments that decide a call's plan, with pointers that are never read.
+int attention_geometry(xrmm::KvAttnArgs& a, int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
+                       int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t causal, int32_t window) {
+  static const int32_t probe[4] __attribute__((aligned(16))) = {};
+  return attention_of(a, probe, INT64_MAX, nullptr, XRMM_F16, probe, probe, probe, probe, XRMM_I8, probe, probe,
+                      ragged ? probe : nullptr, nullptr, rows, max_new, batch, table_width, 1, page_size, q_heads, kv_heads,
+                      head_dim, 1.f, causal, window);
+}
+
+}  // namespace
+
 int64_t xrmm_kv8_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
                                            int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
                                            int32_t causal, int32_t window) {
   xrmm::KvAttnArgs a;
-  static const int32_t probe[4] __attribute__((aligned(16))) = {};
-  const int rc = attention_of(a, probe, INT64_MAX, nullptr, XRMM_F16, probe, probe, probe, probe, XRMM_I8, probe, probe,
-                              ragged ? probe : nullptr, nullptr, rows, max_new, batch, table_width, 1, page_size, q_heads,
-                              kv_heads, head_dim, 1.f, causal, window);
+  const int rc = attention_geometry(a, rows, max_new, ragged, batch, table_width, page_size, q_heads, kv_heads, head_dim, causal, window);
   set_status(XRMM_OK, "");
   return rc ? 0 : xrmm::kv8_workspace_bytes(a);
+}
+
+const char* xrmm_kv8_attention_kernel(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t table_width,
+                                      int32_t page_size, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t causal,
+                                      int32_t window) {
+  xrmm::KvAttnArgs a;
+  if (attention_geometry(a, rows, max_new, ragged, batch, table_width, page_size, q_heads, kv_heads, head_dim, causal, window))
+    return nullptr;
+  set_status(XRMM_OK, "");
+  return xrmm::kv8_kernel_name(a);
 }
 
 int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,

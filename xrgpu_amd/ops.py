@@ -914,3 +914,12 @@ def kv8_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batch, tabl
     return int(nat.lib().xrmm_kv8_attention_workspace_bytes(int(T), _i32(max_new), int(ragged), int(batch), int(table_width),
                                                             int(page_size), int(q_heads), int(kv_heads), int(head_dim),
                                                             int(causal), _i32(window)))
+
+
+def kv8_attention_kernel(T, q_heads, kv_heads, head_dim, *, batch, table_width, page_size, max_new=0, ragged=False, causal=True,
+                         window=0) -> str:
+    r = nat.lib().xrmm_kv8_attention_kernel(int(T), _i32(max_new), int(ragged), int(batch), int(table_width), int(page_size),
+                                            int(q_heads), int(kv_heads), int(head_dim), int(causal), _i32(window))
+    if r is None:
+        raise nat.XrmmInvalid(nat.last_error())
+    return r.decode()
