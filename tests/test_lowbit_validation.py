@@ -123,3 +123,18 @@ def test_kv8_front_refuses_tokens():
                    (torch.zeros(2, 2, 96, dtype=H16), r"\[tokens, 2, 64\]"), (x, "on the GPU")):
         with pytest.raises(nat.XrmmInvalid, match=msg):
             ops.kv8_attention(q, **cache())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.int8])
+def test_mx4_geometry_calls_refuse_other_types(dtype):
+    for f in (ops.matmul_mx4_workspace_bytes, ops.matmul_mx4_kernel):
+        with pytest.raises(nat.XrmmInvalid, match="dtype must be"):
+            f(40, 4096, 64, dtype)
+
+
+def test_kv8_attention_kernel_names_and_refuses():
+    kw = dict(batch=1, table_width=4, page_size=64)
+    assert ops.kv8_attention_kernel(1, 8, 2, 128, **kw) == "kv8_rows"
+    assert ops.kv8_attention_kernel(200, 64, 8, 128, **kw) == "kv8_tile"
+    with pytest.raises(nat.XrmmInvalid, match="head size"):
+        ops.kv8_attention_kernel(1, 8, 2, 80, **kw)

@@ -782,14 +782,20 @@ def matmul_mx4(A, B, scales, bias=None, *, A_scales=None, out_dtype=None, out=No
     return out
 
 
+def _mx4_dtype(dtype):
+    if dtype not in (torch.uint8, torch.float16, torch.bfloat16):
+        raise nat.XrmmInvalid("dtype must be float16, bfloat16 or uint8 (MX4 codes)")
+    return nat.U8 if dtype == torch.uint8 else _LT[dtype]
+
+
 def matmul_mx4_workspace_bytes(M, K, N, dtype=torch.float16):
     """Bytes of the split-K workspace of a matmul_mx4 geometry (0: none); dtype is A's (uint8: MX4 codes)."""
     return int(nat.lib().xrmm_matmul_mx4_workspace_bytes(int(M), int(K), int(N),
-                                                          nat.U8 if dtype == torch.uint8 else _LT[dtype]))
+                                                          _mx4_dtype(dtype)))
 
 
 def matmul_mx4_kernel(M, K, N, dtype=torch.float16) -> str:
-    r = nat.lib().xrmm_matmul_mx4_kernel(int(M), int(K), int(N), nat.U8 if dtype == torch.uint8 else _LT[dtype])
+    r = nat.lib().xrmm_matmul_mx4_kernel(int(M), int(K), int(N), _mx4_dtype(dtype))
     if r is None:
         raise nat.XrmmInvalid(nat.last_error())
     return r.decode()
