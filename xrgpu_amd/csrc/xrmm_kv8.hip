@@ -935,14 +935,26 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
         down = kv_shift(1.f, ve - most);
       }
     }
+    // Fragments are read ahead of their products: heads of 256 have one wave a SIMD, which waits for what it reads (1108 us read by read,
+    // 978 four ahead of both products; two chunks of 2000 on 4000, 32 heads on 8). With 64 to 128 two ahead of K's: 280 for 286 at 96.
     f32x16 s[TT / 32];
+    constexpr int KA = D > 128 ? 4 : 2;
+    auto kfrag = [&](int x, int u) { return *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + kv_kslot(col, 2 * x + hf) * 16); };
+    f16x8 kf[KA][TT / 32];
 #pragma unroll
-    for (int x = 0; x < D / 16; ++x)
+    for (int x = 0; x < KA; ++x)
+#pragma unroll
+      for (int u = 0; u < TT / 32; ++u) kf[x][u] = kfrag(x, u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
 #pragma unroll
       for (int u = 0; u < TT / 32; ++u) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + kv_kslot(col, 2 * x + hf) * 16);
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, q[x], x == 0 ? f32x16{} : s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % KA][u], q[x], x == 0 ? f32x16{} : s[u], 0, 0, 0);
+        if (x + KA < D / 16) kf[x % KA][u] = kfrag(x + KA, u);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
     // A wave in between its products goes first, so that the SIMD's other one has the matrix cores meanwhile. It pays for heads of 64, whose
     // products are short (2048 tokens on themselves 51 -> 46.5 us); with 96, 128 and 256 it costs 0 to 3 %.
     if constexpr (D <= 64) __builtin_amdgcn_s_setprio(1);
@@ -1020,11 +1032,25 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
               pf[e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
             }
           }
-#pragma unroll
-          for (int j = 0; j < JT; ++j) {
+          auto vfrag = [&](int j) {
             const int d = 32 * j + col;
-            const f16x8 vf = *reinterpret_cast<const f16x8*>(vs + d * Ti::VP + kv_vslot<D>(d, u * 4 + sl * 2 + hf) * 16);
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
+            return *reinterpret_cast<const f16x8*>(vs + d * Ti::VP + kv_vslot<D>(d, u * 4 + sl * 2 + hf) * 16);
+          };
+          if constexpr (D > 128) {
+            constexpr int VA = 4;
+            f16x8 vf[VA];
+#pragma unroll
+            for (int j = 0; j < VA; ++j) vf[j] = vfrag(j);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+              o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j % VA], pf, o[j], 0, 0, 0);
+              if (j + VA < JT) vf[j % VA] = vfrag(j + VA);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < JT; ++j) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vfrag(j), pf, o[j], 0, 0, 0);
           }
         }
       l += sums * down;
