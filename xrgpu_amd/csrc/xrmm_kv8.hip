@@ -1107,7 +1107,13 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[j][e] = o[j][e] * f0 + v[j][e >> 2][e & 3] * f1;
+          for (int y = 0; y < 4; ++y) {
+            const f32x4 x4 = v[j][y];  // elements by name: this compiler may fold v[e >> 2][e & 3] over an array of vectors to element 0
+            o[j][4 * y] = o[j][4 * y] * f0 + x4.x * f1;
+            o[j][4 * y + 1] = o[j][4 * y + 1] * f0 + x4.y * f1;
+            o[j][4 * y + 2] = o[j][4 * y + 2] * f0 + x4.z * f1;
+            o[j][4 * y + 3] = o[j][4 * y + 3] * f0 + x4.w * f1;
+          }
       }
     }
   }
