@@ -215,7 +215,10 @@ constexpr int KVT = 32;      // tokens of a step
 // A token's softmax weight times its page's value scale enters binary16 as p vs 2^(KV_PE - e), where 2^e is a power of two
 // above every value scale that the row has seen so far in magnitude: 2^KV_PE at most, so that small weights stay normal. A page
 // that a row's mask hides does not count for it, so what the row cannot see does not change it. Only
-// exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is.
+// exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
+// the codes are exact in and the products run in at one pass; its eleven bits of a weight raise the error of float16 outputs against 64 bits
+// from 2.1e-4 with float32 weights to 2.6e-4 (two chunks of 2000 on 4000; single tokens 2.3e-4 to 2.5e-4), bfloat16 ones not at all. The
+// denominator sums the weights before they are rounded.
 constexpr int KV_PE = 11;
 constexpr int KV_NONE = -1000;  // e before any scale
 
@@ -282,7 +285,7 @@ __device__ __forceinline__ KvBytes<N> kv_bytes(const uint8_t* p) {
 // tokens; its waves take turns at steps of 32 tokens, with the next step's codes in flight and the
 // page after that looked up. Workgroups of one (sequence, head, rows) leave their
 // unnormalised outputs, maxima and sums in the workspace, and the last to arrive joins them in
-// token order. 48 sequences of up to 8000 tokens, 8 heads of 128, e4m3: 97 us (5.2 TB/s), unsplit; one of 65000, int8: 34.5 us, of
+// token order. 48 sequences of up to 8000 tokens, 8 heads of 128, e4m3: 96 us (5.2 TB/s), unsplit; one of 65000, int8: 35 us, of
 // which the join is about 8. The kernel's start shows in short calls: with queries loaded value by value a token on 4 took 9.5 us
 // at head size 256 and 5.4 at 64, in pieces of 16 bytes (outputs of 8) 8.3 and 4.8.
 constexpr int KVR_PASS = 8 * KVT;  // shares of tokens are multiples of it: a step of all waves, eight at most
@@ -647,7 +650,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 // fragments' rows nor the transposing stores meet in a bank.
 //
 // VALU instructions bound it, about 500 a wave and 64 tokens (codes to binary16, softmax); MFMAs run a fifth of the time. Two chunks
-// of 2000 on 4000 tokens, 32 heads of 128 on 8: 268 us; 32 tokens a tile with three workgroups a CU 476, eight waves 276.
+// of 2000 on 4000 tokens, 32 heads of 128 on 8: 264 to 272 us by the box; 32 tokens a tile with three workgroups a CU 476, eight waves 276.
 //
 // Two stages: while tile i computes, tile i + 1 goes from registers to LDS, tile i + 2 is loaded and the
 // pages of tile i + 3 are looked up. One barrier a tile.

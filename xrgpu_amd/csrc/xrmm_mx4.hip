@@ -95,8 +95,9 @@ hipError_t quantize_for(const MxQuantArgs& a, hipStream_t st) {
 // next lane's (28.5 us at 16 x 4096 x 14336 for 25.4, 23.2 at 16 x 14336 x 4096 for 22.2). So the
 // weights are transposed among the four lane groups (v_permlane swaps): lane (c, g) then
 // holds dword g of each block, and the activations' loads are runs of 64 bytes. Each byte of codes becomes two 16-bit values
-// times its block's scale in one conversion; v_mfma_f32_16x16x32 takes a block. What bounds it past four rows is the
-// activations' way from L2 to every CU (about 40 GB/s a CU).
+// times its block's scale in one conversion; v_mfma_f32_16x16x32 takes a block. What bounds it past four rows is that
+// every 16 columns load all activations anew: 128 KB from L2 beside 34 KB of weights at 16 x 4096, of which a CU gets about 40 GB/s. A wave
+// that keeps its share of the activations over several column tiles, as k_gemv_sk does, would load them once.
 //
 // A bfloat16 holds every E2M1 value times 2^(byte - 127) exactly. A binary16 does for scales in
 // [2^-23, 2^13]; a workgroup that met another scale sums everything again, with weights in bfloat16 and the
@@ -231,7 +232,8 @@ __global__ __launch_bounds__(64 * WV, 4) void k_mx4_rows(MxArgs a, uint32_t col_
 // then applies the scale to the sum's exponent, so no scale is out of range. For bfloat16 activations the codes count 2^-8 of their
 // value meanwhile: 32 products of 6 and the largest bfloat16 would pass float32. The lanes' sums meet by DPP, the chunks of K in LDS,
 // in order. Nothing but the loop over columns repeats, and it is short: the kernel lives for a few microseconds, and
-// unrolled code is fetched slower than it runs. 1 x 4096 x 14336: 9.0 us, 31 MB.
+// unrolled code is fetched slower than it runs. 1 x 4096 x 14336: 8.9 us, 31 MB (k_gemv_dot reads 6 % more bytes at
+// this size in 7 to 7.7: two or three workgroups a CU and two columns in flight a wave leave the rest).
 
 template <int AT>
 __device__ __forceinline__ float mx_dot2(uint32_t a, uint32_t b, float c) {

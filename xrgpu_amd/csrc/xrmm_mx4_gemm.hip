@@ -11,7 +11,8 @@
 //
 // 256-tiles of two MX4 operands need no conversion, and their pieces go from memory to LDS without registers: once all
 // waves have read the last fragments of a stage, step s + 2 is fetched into it. With pieces in registers the tile
-// spilled (4096 x 4096 x 14336 182 us, 174 now; 4096 x 14336 x 4096 153 -> 142). Four waves of 128 x 128 read a third less LDS, but one wave a SIMD
+// spilled (4096 x 4096 x 14336 with the activations' quantisation 182 us, 174 on the same box, 174 to 187 on others; 4096 x 14336 x 4096
+// alone 153 -> 142). Four waves of 128 x 128 read a third less LDS, but one wave a SIMD
 // covers less: 190 us. What bounds it is the pieces' way from L2: a step's 64 KB take 2.2 us of a CU (7.6 TB/s of all), the step 1.8 without
 // them; half steps fetched three ahead arrive no sooner (182 us: twice the requests).
 //
@@ -586,7 +587,7 @@ hipError_t gemm_at(const MxArgs& a, const MxPlan& p, hipStream_t st) {
 // MX4 256-tiles wait on memory that all CUs share: a round that leaves CUs out is faster, 0.4 of a full one with a few
 // tiles, 0.9 with half the CUs. A split exchange costs 5 us and what its parts weigh.
 // It places 512 x 4096 x 4096 of 16 bits on 64- or 128-tiles (39 to 44 us; 256-tiles 55), 128 rows on 64-tiles with K split (21; 128-tiles 25),
-// 2048 x 4096 x 14336 on 256-tiles (233; 128-tiles 281); MX4 700 x 4096 x 14336 on 256-tiles (44 us; 128-tiles 53), 512 rows on 128-tiles
+// 2048 x 4096 x 14336 on 256-tiles (231 to 244 by the box; 128-tiles 281); MX4 700 x 4096 x 14336 on 256-tiles (44 us; 128-tiles 53), 512 rows on 128-tiles
 // (38.5; 256-tiles 45, 64-tiles 53).
 MxPlan mx4_gemm_plan(int64_t M, int64_t K, int64_t N, int a_type, bool have_ws) {
   MxPlan best{};
