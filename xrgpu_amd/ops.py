@@ -790,11 +790,11 @@ def _mx4_dtype(dtype):
 
 def matmul_mx4_workspace_bytes(M, K, N, dtype=torch.float16):
     """Bytes of the split-K workspace of a matmul_mx4 geometry (0: none); dtype is A's (uint8: MX4 codes)."""
-    return int(nat.lib().xrmm_matmul_mx4_workspace_bytes(int(M), int(K), int(N),
-                                                          _mx4_dtype(dtype)))
+    return int(nat.lib().xrmm_matmul_mx4_workspace_bytes(int(M), int(K), int(N), _mx4_dtype(dtype)))
 
 
 def matmul_mx4_kernel(M, K, N, dtype=torch.float16) -> str:
+    """The kernel family of a matmul_mx4 geometry; dtype is A's (uint8: MX4 codes)."""
     r = nat.lib().xrmm_matmul_mx4_kernel(int(M), int(K), int(N), _mx4_dtype(dtype))
     if r is None:
         raise nat.XrmmInvalid(nat.last_error())
@@ -924,6 +924,7 @@ def kv8_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batch, tabl
 
 def kv8_attention_kernel(T, q_heads, kv_heads, head_dim, *, batch, table_width, page_size, max_new=0, ragged=False, causal=True,
                          window=0) -> str:
+    """The kernel that a kv8_attention call takes with a workspace: "kv8_rows" or "kv8_tile"."""
     r = nat.lib().xrmm_kv8_attention_kernel(int(T), _i32(max_new), int(ragged), int(batch), int(table_width), int(page_size),
                                             int(q_heads), int(kv_heads), int(head_dim), int(causal), _i32(window))
     if r is None:
