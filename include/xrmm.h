@@ -491,8 +491,9 @@ int xrmm_kv8_append(const void* k, const void* v, int64_t k_stride, int64_t v_st
  * causal, t > p - window if window > 0; a row that sees none, as a causal one before
  * position 0, is 0. Rows that `starts` leaves out are not written. Pages that no row's
  * window reaches may be missing from the table. Cache scales are any float32. A weight
- * times its value scale enters the second product with binary16's eleven bits; below
- * 2^-25 of the largest value scale that the row sees it has fewer, and below 2^-35 none.
+ * times its value scale enters the second product with binary16's eleven bits, or twice
+ * as many where a sequence has at most 16 rows of a key head; below 2^-25 of the largest
+ * value scale that the row sees it has fewer, and below 2^-35 none.
  * The sums over tokens are divided last: they may pass float32 where values come within
  * a factor of the length of its largest. e4m3 NaN codes must not occur (xrmm_kv8_append
  * writes none): rows that do not see such a token may be NaN too. The workspace, at least

@@ -37,7 +37,8 @@ def kernel_of(c, q, counts, *, causal=True, window=0, max_new=None, ragged=True)
                                       causal=causal, window=window)
 
 
-def check(c, q, counts, *, causal=True, window=0, scale=None, status=0, kernel=None, out=None, d=None, got=None, **kw):
+def check(c, q, counts, *, causal=True, window=0, scale=None, status=0, kernel=None, out=None, d=None, got=None,
+          weights=2.0 ** -10, **kw):
     if kernel is not None:
         assert kernel_of(c, q, counts, causal=causal, window=window) == kernel
     word = torch.zeros(1, dtype=torch.int32, device="cuda")
@@ -49,7 +50,7 @@ def check(c, q, counts, *, causal=True, window=0, scale=None, status=0, kernel=N
     ref, av, aqk = LB.attention_of_all(q.double().cpu().numpy(), c.k, c.v, c.ks, c.vs, c.table, c.lengths, counts, c.kind, scale=s,
                                        causal=causal, window=window)
     eps, n = torch.finfo(q.dtype).eps, float(max(int(c.lengths.max()), 1))
-    rel = 2.0 ** -10 + 2.0 ** -21 + n * 2.0 ** -23 + 2 * (D + 4) * 2.0 ** -24 * aqk[..., None]
+    rel = weights + 2.0 ** -21 + n * 2.0 ** -23 + 2 * (D + 4) * 2.0 ** -24 * aqk[..., None]
     top = seen_top(c, counts, Hq, causal, window)[..., None]
     tol = eps / 2 * np.abs(ref) + (1 + eps) * (rel * av + n * 2.0 ** -35 * top) + torch.finfo(q.dtype).tiny * eps
     out = o.double().cpu().numpy()
@@ -163,3 +164,15 @@ def test_a_large_scale_after_a_row_changes_no_bit_of_it(gpu, kind, counts):
         hidden = min(max(0, (L - 1) // page * page - (L - n)), n)  # rows at positions before the last page
         assert torch.equal(a[first:first + hidden], b[first:first + hidden])
         first += n
+
+
+@KIND
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,counts,Hq,Hkv,D,page,window", [
+    ([7, 1, 40], [1, 1, 1], 8, 2, 64, 16, 0), ([200], [1], 32, 8, 64, 16, 0), ([3000, 500], [1, 1], 8, 1, 128, 64, 0), ([64], [4], 4, 1, 96, 32, 0),
+    ([90, 300], [2, 8], 2, 2, 256, 128, 0), ([900], [3], 10, 2, 128, 64, 12)])
+def test_weights_of_single_tiles_keep_22_bits(gpu, kind, dt, lens, counts, Hq, Hkv, D, page, window):
+    """Two binary16 terms: 2^-22 of a weight, numerator and denominator together 2^-21; all else as above."""
+    assert max(counts) * Hq // Hkv <= 16
+    c = Cache(kind, lens, Hkv, D, page, seed=sum(lens), scales="any")
+    check(c, queries(sum(counts), Hq, D, dt), counts, window=window, kernel="kv8_rows", weights=2.0 ** -21)

@@ -216,9 +216,11 @@ constexpr int KVT = 32;      // tokens of a step
 // above every value scale that the row has seen so far in magnitude: 2^KV_PE at most, so that small weights stay normal. A page
 // that a row's mask hides does not count for it, so what the row cannot see does not change it. Only
 // exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
-// the codes are exact in and the products run in at one pass; its eleven bits of a weight raise the error of float16 outputs against 64 bits
-// from 2.1e-4 with float32 weights to 2.6e-4 (two chunks of 2000 on 4000; single tokens 2.3e-4 to 2.5e-4), bfloat16 ones not at all. The
-// denominator sums the weights before they are rounded.
+// the codes are exact in. Where a key head's rows of a sequence are one tile of 16, as in calls of single tokens, a weight is the sum of two
+// binary16 terms (22 bits): the cache's bytes bound these calls, and the second term costs them 0 to 2 % (48 sequences of up to 8000 95.2 -> 96.4 us).
+// Elsewhere instructions do, and a second term would cost 5 to 6 % by rows (32 tokens on 30000 71.6 -> 76.3) and 23 % by tiles (two chunks of
+// 2000 on 4000 272 -> 335): a weight keeps eleven bits, which raises the error of float16 outputs against 64 bits from 2.1e-4 with
+// float32 weights to 2.6e-4 (3.1e-4 in windows of few tokens), of bfloat16 ones not at all. The denominator sums the weights before they are rounded.
 constexpr int KV_PE = 11;
 constexpr int KV_NONE = -1000;  // e before any scale
 
@@ -302,7 +304,7 @@ struct KvStep {
   KvBytes<D / 16> v[8];
 };
 
-template <int D, bool FP8, int W>
+template <int D, bool FP8, int W, bool TWO>
 __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
   constexpr int KD = D / 4, VD = D / 16;  // codes of a token that a lane holds
   const KvCache& c = a.c;
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
     const float fo = kv_shift(f, was - ve);
 #pragma unroll
     for (int j = 0; j < VD; ++j) o[j] *= fo;
-    f16x8 pf;
+    f16x8 pf, pl;  // the weights; TWO: what binary16 leaves of them
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const float w = kv_shift(cur.vs[u], KV_PE - ve);
@@ -480,7 +482,9 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
         const float v = s[u][e], p = __builtin_amdgcn_exp2f(v - base);
         l += p;
         // a masked token's weight is 0 whatever its page's scale holds
-        pf[4 * u + e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
+        const float x = v == -__builtin_inff() ? 0.f : p * w;
+        pf[4 * u + e] = static_cast<f16>(x);
+        if constexpr (TWO) pl[4 * u + e] = static_cast<f16>(x - static_cast<float>(pf[4 * u + e]));
       }
     }
     // values
@@ -502,6 +506,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
       for (int z = 0; z < 4; ++z) {
         if (4 * y + z >= VD) break;
         const f16x8 vf = {t4[0][z], t4[1][z], t4[2][z], t4[3][z], t4[4][z], t4[5][z], t4[6][z], t4[7][z]};
+        if constexpr (TWO) o[4 * y + z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[4 * y + z], 0, 0, 0);
         o[4 * y + z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf, o[4 * y + z], 0, 0, 0);
       }
     }
@@ -1221,11 +1226,15 @@ hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
   const dim3 grid(static_cast<uint32_t>(n));
   const uint32_t rt = static_cast<uint32_t>(p.row_tiles), sp = static_cast<uint32_t>(p.splits), ch = static_cast<uint32_t>(p.chunk);
   if (!p.tile) {
-    switch (p.waves) {
-      case 2: k_kv8_rows<D, FP8, 2><<<grid, 128, 0, st>>>(a, rt, sp, ch); break;
-      case 4: k_kv8_rows<D, FP8, 4><<<grid, 256, 0, st>>>(a, rt, sp, ch); break;
-      default: k_kv8_rows<D, FP8, 8><<<grid, 512, 0, st>>>(a, rt, sp, ch);
-    }
+    auto rows = [&](auto two) {
+      switch (p.waves) {
+        case 2: k_kv8_rows<D, FP8, 2, decltype(two)::value><<<grid, 128, 0, st>>>(a, rt, sp, ch); break;
+        case 4: k_kv8_rows<D, FP8, 4, decltype(two)::value><<<grid, 256, 0, st>>>(a, rt, sp, ch); break;
+        default: k_kv8_rows<D, FP8, 8, decltype(two)::value><<<grid, 512, 0, st>>>(a, rt, sp, ch);
+      }
+    };
+    if (p.row_tiles == 1) rows(std::true_type{});
+    else rows(std::false_type{});
     return hipGetLastError();
   }
   constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16), lds = 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
