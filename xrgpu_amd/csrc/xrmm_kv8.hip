@@ -655,7 +655,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
 // fragments' rows nor the transposing stores meet in a bank.
 //
 // VALU instructions bound it, about 500 a wave and 64 tokens (codes to binary16, softmax); MFMAs run a fifth of the time. Two chunks
-// of 2000 on 4000 tokens, 32 heads of 128 on 8: 264 to 272 us by the box; 32 tokens a tile with three workgroups a CU 476, eight waves 276.
+// of 2000 on 4000 tokens, 32 heads of 128 on 8: 262 to 272 us by the box; 32 tokens a tile with three workgroups a CU 476, eight waves 276.
 //
 // Two stages: while tile i computes, tile i + 1 goes from registers to LDS, tile i + 2 is loaded and the
 // pages of tile i + 3 are looked up. One barrier a tile.
