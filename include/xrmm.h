@@ -514,6 +514,57 @@ int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dt
                        int32_t q_heads, int32_t kv_heads, int32_t head_dim, float scale, int32_t causal, int32_t window,
                        void* workspace, int64_t workspace_bytes, void* stream);
 
+/* xrmm_kv8_attention for a batch whose sequences share their first tokens: positions below shared_count * page_size of
+ * every sequence lie in the pages shared_pages (int32 [shared_count]), whatever the table's entries for them say (they
+ * are not read); the others in the table's, as before. All else is as in xrmm_kv8_attention. With a workspace, the
+ * shared tokens are read once for the rows of all sequences and joined with each sequence's own. */
+int64_t xrmm_kv8_shared_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t shared_count,
+                                                  int32_t table_width, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                                                  int32_t head_dim, int32_t causal, int32_t window);
+int xrmm_kv8_shared_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
+                              const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
+                              const void* shared_pages, int32_t shared_count, const void* block_table, const void* lengths,
+                              const void* starts, void* status, int64_t rows, int32_t max_new, int32_t batch,
+                              int32_t table_width, int64_t pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                              int32_t head_dim, float scale, int32_t causal, int32_t window, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Rotary positions (no counterpart in the reference). q [rows, q_heads, head_dim] and
+ * k [rows, k_heads, head_dim] (k_heads 0: none) of dtype XRMM_F32, XRMM_F16 or
+ * XRMM_BF16, token strides in elements. Pair i < rotary_dim / 2 of a head, its values
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved, becomes magnitude (a cos t - b sin t,
+ * b cos t + a sin t) with t = position * frequencies[i] (float64, radians) in 64 bits,
+ * the turn in float32, rounded once; inverse turns by -t, which is the gradient's map. Values behind
+ * rotary_dim pass. A row's position is positions[row] (XRMM_I32 or XRMM_I64), or, with lengths
+ * (int32 [batch]), that of kv8's calls: the rows are each sequence's last tokens, starts as there; rows
+ * that starts leave out are not written. An output may be its input's own memory. */
+int xrmm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_stride, int64_t k_stride, int64_t q_out_stride,
+              int64_t k_out_stride, int32_t dtype, const void* frequencies, int32_t rotary_dim, double magnitude,
+              const void* positions, int32_t positions_dtype, const void* lengths, const void* starts, int64_t rows, int32_t batch,
+              int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t interleaved, int32_t inverse, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * A token for each row of logits [rows, vocab] (XRMM_F32, XRMM_F16 or XRMM_BF16, row stride in
+ * elements; no counterpart in the reference). In descending order of the logits (of equal
+ * ones the lower index first) with weights w = exp((x - max) / temperature), kept are: the first top_k
+ * (0: all); of those the shortest prefix whose weight is at least top_p of theirs (one token at least;
+ * top_p >= 1: all); of those the ones with w >= min_p. The token is the first, by index, at
+ * which the running sum of the kept weights exceeds uniforms[row] (float32, [0, 1)) of their sum: tokens int32, shares
+ * float32: the logarithm of its part of that sum. Temperature 0 takes the largest. NaN and
+ * -infinity are never drawn; a row of nothing else gives token -1 and share -infinity. An infinity
+ * leaves only infinities. Weights are whole multiples of 2^-F of the largest, F = min(51, 62 -
+ * ceil(log2 vocab)): sums are exact, and a token of less than half a unit is not drawn. Arrays by row take the place
+ * of the one setting where not NULL (float32; top_k int32); in them a temperature not above 0 or NaN
+ * is 0, top_k below 1 is all, a NaN top_p or min_p is off, and others are clamped to [0, 1]. The
+ * workspace, at least xrmm_sample_workspace_bytes (0: none used), is optional and has the form of
+ * xrmm_matmul_mx4's; with it few rows are spread over the device. */
+int64_t xrmm_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int xrmm_sample(const void* logits, int64_t stride, int32_t dtype, const void* uniforms, const void* temperatures,
+                const void* top_ks, const void* top_ps, const void* min_ps, double temperature, int32_t top_k, double top_p,
+                double min_p, void* tokens, void* shares, int64_t rows, int64_t vocab, void* workspace, int64_t workspace_bytes,
+                void* stream);
+
 /* ---------------------------------------------------------------------------
  * Measurement (no counterpart in the reference, which publishes no throughput
  * for this path): read `bytes` (a multiple of 16) at 16-byte aligned `src`

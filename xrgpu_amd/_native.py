@@ -25,6 +25,7 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 _lib = None
 
@@ -88,6 +89,14 @@ def _sig(lib):
     s("xrmm_kv8_attention_kernel", ctypes.c_char_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32)
     s("xrmm_kv8_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32,
       _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
+    s("xrmm_kv8_shared_attention_workspace_bytes", _i64, _i64, *[_i32] * 11)
+    s("xrmm_kv8_shared_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
+      _i64, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
+    s("xrmm_rope", ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i32, _f64, _vp, _i32, _vp, _vp, _i64,
+      _i32, _i32, _i32, _i32, _i32, _i32, _vp)
+    s("xrmm_sample_workspace_bytes", _i64, _i64, _i64)
+    s("xrmm_sample", ctypes.c_int, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _f64, _i32, _f64, _f64, _vp, _vp, _i64, _i64, _vp,
+      _i64, _vp)
     s("xrmm_stream_read", ctypes.c_int, _vp, ctypes.c_uint64, _vp, _i32, _vp)
     s("xrmm_stream_read_ex", ctypes.c_int, _vp, ctypes.c_uint64, _vp, _i32, _i32, _i32, _vp)
     s("xrmm_mfma_peak_operand_bytes", _i64)

@@ -58,7 +58,11 @@ UNITS = [
     ("xrmm_mx4.hip", [], "mx4.o"),
     ("xrmm_mx4_gemm.hip", [], "mx4_gemm.o"),
     ("xrmm_kv8.hip", [], "kv8.o"),
+    ("xrmm_kv8_shared.hip", [], "kv8_shared.o"),
+    ("xrmm_rope.hip", [], "rope.o"),
+    ("xrmm_sample.hip", [], "sample.o"),
     ("xrmm_lowbit_api.cpp", [], "lowbit_api.o"),
+    ("xrmm_decode_api.cpp", [], "decode_api.o"),
     ("xrmm_probe.hip", [], "probe.o"),
     ("xrmm_api.cpp", [], "api.o"),
     ("xrmm_operator.cpp", [], "operator.o"),

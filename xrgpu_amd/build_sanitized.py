@@ -30,7 +30,7 @@ from xrgpu_amd import build as B
 
 SAN_DIR = os.path.join(B.LIB_DIR, "sanitize")
 SAN_OBJ = os.path.join(B.OBJ_DIR, "sanitize")
-HOST_UNITS = ("xrmm_api.cpp", "xrmm_operator.cpp", "xrmm_lowbit_api.cpp")
+HOST_UNITS = ("xrmm_api.cpp", "xrmm_operator.cpp", "xrmm_lowbit_api.cpp", "xrmm_decode_api.cpp")
 # hipcc: the sanitizers apply to the host compilation only
 HOST_SAN = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
             "-Xarch_host", "-fno-sanitize-recover=undefined", "-Xarch_host", "-fno-omit-frame-pointer",

@@ -262,4 +262,51 @@ int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dt
   return done(xrmm::launch_kv8_attention(a, static_cast<hipStream_t>(stream)), "kv8_attention launch");
 }
 
+namespace {
+
+int shared_of(xrmm::KvAttnArgs& a, const void* shared_pages, int32_t shared_count) {
+  if (shared_count < 0) return fail("kv8_shared_attention: negative count of shared pages");
+  if (static_cast<int64_t>(shared_count) * a.c.page > 0x7FFFFF00) return fail("kv8_shared_attention: the shared pages span 2^31 tokens or more");
+  if (shared_count > 0 && a.c.rows > 0 && !shared_pages) return fail("null tensor pointer");
+  if (!aligned(shared_pages, 4)) return fail("kv8_shared_attention: the shared pages must be 4-byte aligned");
+  a.shared = static_cast<const int32_t*>(shared_pages);
+  a.shared_pages = shared_count;
+  return XRMM_OK;
+}
+
+}  // namespace
+
+int64_t xrmm_kv8_shared_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t shared_count,
+                                                  int32_t table_width, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                                                  int32_t head_dim, int32_t causal, int32_t window) {
+  static const int32_t probe[1] = {};
+  xrmm::KvAttnArgs a;
+  int rc = attention_geometry(a, rows, max_new, ragged, batch, table_width, page_size, q_heads, kv_heads, head_dim, causal, window);
+  if (!rc) rc = shared_of(a, probe, shared_count);
+  set_status(XRMM_OK, "");
+  return rc ? 0 : xrmm::kv8_shared_workspace_bytes(a);
+}
+
+int xrmm_kv8_shared_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
+                              const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
+                              const void* shared_pages, int32_t shared_count, const void* block_table, const void* lengths,
+                              const void* starts, void* status, int64_t rows, int32_t max_new, int32_t batch,
+                              int32_t table_width, int64_t pages, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                              int32_t head_dim, float scale, int32_t causal, int32_t window, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  xrmm::KvAttnArgs a;
+  // a table of no columns, where all positions are shared ones, may have no address
+  if (int rc = attention_of(a, q, q_stride, output, dtype, k_cache, v_cache, k_scales, v_scales, cache_dtype,
+                            table_width == 0 ? lengths : block_table, lengths, starts, status, rows, max_new, batch, table_width,
+                            pages, page_size, q_heads, kv_heads, head_dim, scale, causal, window))
+    return rc;
+  if (int rc = shared_of(a, shared_pages, shared_count)) return rc;
+  if (rows > 0 && (!q || !output)) return fail("null tensor pointer");
+  if (!aligned(q, 2) || !aligned(output, 2)) return fail("kv8_shared_attention: q and the output must be aligned to their elements");
+  if (workspace != nullptr && !aligned(workspace, 256)) return fail("kv8_shared_attention: the workspace must be 256-byte aligned");
+  a.ws = workspace;
+  a.ws_bytes = workspace ? workspace_bytes : 0;
+  return done(xrmm::launch_kv8_shared_attention(a, static_cast<hipStream_t>(stream)), "kv8_shared_attention launch");
+}
+
 }  // extern "C"

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import math
 import os
 import warnings
 
@@ -930,3 +931,188 @@ def kv8_attention_kernel(T, q_heads, kv_heads, head_dim, *, batch, table_width, 
     if r is None:
         raise nat.XrmmInvalid(nat.last_error())
     return r.decode()
+
+
+def kv8_shared_attention(q, k_cache, v_cache, k_scales, v_scales, shared_pages, block_table, lengths, *, starts=None,
+                         max_new=None, scale=None, causal=True, window=0, out=None, workspace=None, status=None, stream=None):
+    """kv8_attention of a batch whose sequences share their first tokens.
+
+    Positions below ``len(shared_pages) * page_size`` of every sequence lie in the pages ``shared_pages`` (int32 ``[n]``),
+    whatever block_table's entries for them say; the others in block_table's (int32 ``[batch, width]``, the same as
+    kv8_append's: its first n columns belong to the shared positions). Everything else is as in ``kv8_attention``. The shared
+    tokens are read once for the rows of all sequences, on a workspace (``kv8_shared_attention_workspace_bytes``; under
+    graph capture give one, else each sequence reads them)."""
+    B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
+    if shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] >= 1 << 31:
+        raise nat.XrmmInvalid("shared_pages must be int32 [pages]")
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise nat.XrmmInvalid("q must be float16 or bfloat16")
+    if q.dim() != 3 or q.shape[1] == 0 or H == 0 or q.shape[1] % H != 0:
+        raise nat.XrmmInvalid("q must be [tokens, q_heads, head_dim] with q_heads a multiple of the cache's heads")
+    T, Hq, S = int(q.shape[0]), int(q.shape[1]), int(shared_pages.shape[0])
+    qs = _token_rows(q, Hq, D, "q")
+    _check_out(out, (T, Hq, D), q.dtype)
+    dev = _check_dev(k_cache, v_cache, k_scales, v_scales, shared_pages, block_table, lengths, starts, status, out)
+    _same_device(dev, q)
+    W, most, window = int(block_table.shape[1]), _i32(max_new or 0), _i32(window)
+    lib = nat.lib()
+    s = _stream(stream, dev)
+    need = int(lib.xrmm_kv8_shared_attention_workspace_bytes(T, most, int(starts is not None), B, S, W, page, Hq, H, D,
+                                                             int(causal), window))
+    ws, nws = _take_workspace(need, workspace, q, dev, s, stream)
+    if out is None:
+        out = _empty((T, Hq, D), q.dtype, q.device, stream)
+    nat.check(lib.xrmm_kv8_shared_attention(
+        _ptr(q), qs, _ptr(out), _LT[q.dtype], _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+        _CACHE[k_cache.dtype], _ptr(shared_pages), S, _ptr(block_table), _ptr(lengths), _ptr(starts), _ptr(status), T, most, B,
+        W, P, page, Hq, H, D, float(D ** -0.5 if scale is None else scale), int(causal), window, _ptr(ws), nws, s))
+    return out
+
+
+def kv8_shared_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batch, shared_pages, table_width, page_size,
+                                         max_new=0, ragged=False, causal=True, window=0):
+    """Bytes of the workspace of a kv8_shared_attention call (0: none); ``shared_pages``: how many, ``ragged``: the call has
+    ``starts``."""
+    return int(nat.lib().xrmm_kv8_shared_attention_workspace_bytes(
+        int(T), _i32(max_new), int(ragged), int(batch), _i32(shared_pages), int(table_width), int(page_size), int(q_heads),
+        int(kv_heads), int(head_dim), int(causal), _i32(window)))
+
+
+def rope_frequencies(rotary_dim, theta=10000.0, *, scaling=None, factor=1.0, original_length=None, low=1.0, high=None,
+                     device="cuda"):
+    """The float64 frequencies ``[rotary_dim / 2]`` of ``rope``, and the magnitude that belongs to them: ``(frequencies, magnitude)``.
+
+    ``theta ** (-2 i / rotary_dim)``, for contexts ``factor`` times those trained on changed by ``scaling``: ``"linear"`` divides all by
+    factor; ``"ntk"`` raises theta by ``factor ** (R / (R - 2))``, so that the slowest pair is divided by it and the fastest stays;
+    ``"bands"`` divides pairs that turn fewer than ``low`` times in ``original_length``, keeps those of more than ``high`` turns and
+    goes from one to the other in proportion to the turns between; ``"yarn"`` does so in proportion to the pair's index, and its
+    magnitude is ``0.1 ln(factor) + 1``. ``high``: 4 turns with bands, 32 with yarn, unless given. Other magnitudes are 1."""
+    R = int(rotary_dim)
+    if R <= 0 or R % 2:
+        raise nat.XrmmInvalid("rotary_dim must be even and positive")
+    if not (theta > 0 and factor > 0 and math.isfinite(theta) and math.isfinite(factor)):
+        raise nat.XrmmInvalid("theta and factor must be positive")
+    i = torch.arange(R // 2, dtype=torch.float64)
+    magnitude = 1.0
+    high = (32.0 if scaling == "yarn" else 4.0) if high is None else high
+    if scaling == "ntk":
+        if R == 2:
+            raise nat.XrmmInvalid("ntk scaling needs two pairs at least")
+        theta = theta * factor ** (R / (R - 2))
+    f = float(theta) ** (-2.0 * i / R)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling in ("bands", "yarn"):
+        if original_length is None or not original_length > 0 or not 0 < low < high:
+            raise nat.XrmmInvalid(f"{scaling} scaling needs original_length and 0 < low < high")
+        if scaling == "bands":
+            keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        else:
+            # the indices (not whole) whose pairs turn `high` and `low` times, and the ramp between the whole ones around them
+            at = lambda turns: R * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+            first, last = max(math.floor(at(high)), 0), min(math.ceil(at(low)), R - 1)
+            keep = 1 - ((i - first) / max(last - first, 1e-3)).clamp(0, 1)
+            magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        f = f * keep + f / factor * (1 - keep)
+    elif scaling not in (None, "ntk"):
+        raise nat.XrmmInvalid("scaling must be None, 'linear', 'ntk', 'bands' or 'yarn'")
+    return f.to(device), magnitude
+
+
+def rope(q, k=None, *, frequencies, positions=None, lengths=None, starts=None, magnitude=1.0, interleaved=False, inverse=False,
+         out=None, k_out=None, stream=None):
+    """Rotary positions of queries and keys: ``(q_out, k_out)``, or ``q_out`` without k.
+
+    q ``[T, q_heads, head_dim]`` and k ``[T, k_heads, head_dim]`` float32, float16 or bfloat16 (token stride free). Pair i of a
+    head, values ``(i, i + R / 2)`` with R twice the number of ``frequencies`` (float64, radians a position;
+    ``rope_frequencies``), or ``(2 i, 2 i + 1)`` if ``interleaved``, is turned by position * frequency and multiplied by
+    ``magnitude``; values behind R pass. Angles have 64 bits, the turn 32, rounded once. ``inverse`` turns back, with the same
+    magnitude: the gradient with regard to q and k of a loss whose gradient with regard to the outputs is given. Positions are
+    ``positions`` (int32 or int64 ``[T]``), or those of kv8_append's calls: the rows are each sequence's last tokens, of
+    ``lengths`` (int32 ``[batch]``) and ``starts`` as there; rows that starts leave out are not written. ``out`` and ``k_out``
+    may be q and k themselves (in place), or slices of a wider buffer."""
+    if q.dtype not in _LT or (k is not None and k.dtype != q.dtype):
+        raise nat.XrmmInvalid("q and k must both be float32, float16 or bfloat16")
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise nat.XrmmInvalid("q and k must be [tokens, heads, head_dim] with the same tokens and head_dim")
+    if frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise nat.XrmmInvalid("frequencies must be float64 [R / 2]")
+    T, Hq, D = (int(n) for n in q.shape)
+    Hk = 0 if k is None else int(k.shape[1])
+    if (positions is None) == (lengths is None):
+        raise nat.XrmmInvalid("give either positions or lengths")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (T,)):
+        raise nat.XrmmInvalid(f"positions must be int32 or int64 [{T}]")
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.dim() != 1):
+        raise nat.XrmmInvalid("lengths must be int32 [batch]")
+    if starts is not None and (lengths is None or starts.dtype != torch.int32 or tuple(starts.shape) != (lengths.shape[0] + 1,)):
+        raise nat.XrmmInvalid("starts must be int32 [batch + 1], with lengths")
+    if k is None and k_out is not None:
+        raise nat.XrmmInvalid("k_out without k")
+    qs, ks = _token_rows(q, Hq, D, "q"), 0 if k is None else _token_rows(k, Hk, D, "k")
+    _check_out(out, q.shape, q.dtype)
+    if k is not None:
+        _check_out(k_out, k.shape, q.dtype, "k_out")
+    dev = _check_dev(frequencies, positions, lengths, starts)
+    _same_device(dev, *(t for t in (q, k, out, k_out) if t is not None))
+    out = _empty(q.shape, q.dtype, q.device, stream) if out is None else out
+    if k is not None and k_out is None:
+        k_out = _empty(k.shape, k.dtype, k.device, stream)
+    os_, oks = _token_rows(out, Hq, D, "out"), 0 if k is None else _token_rows(k_out, Hk, D, "k_out")
+    nat.check(nat.lib().xrmm_rope(
+        _ptr(q), _ptr(k), _ptr(out), _ptr(k_out), qs, ks, os_, oks, _LT[q.dtype], _ptr(frequencies), 2 * int(frequencies.shape[0]),
+        float(magnitude), _ptr(positions), nat.I64 if positions is not None and positions.dtype == torch.int64 else nat.I32,
+        _ptr(lengths), _ptr(starts), T, 0 if lengths is None else int(lengths.shape[0]), Hq, Hk, D, int(interleaved), int(inverse),
+        _stream(stream, dev)))
+    return out if k is None else (out, k_out)
+
+
+def _setting(v, rows, dtype, name):
+    """A setting of ``sample``: ``(tensor or None, the number for all rows)``."""
+    if not torch.is_tensor(v):
+        return None, v
+    if v.dtype != dtype or tuple(v.shape) != (rows,):
+        raise nat.XrmmInvalid(f"{name} must be a number or {dtype} [{rows}], got {v.dtype} {tuple(v.shape)}")
+    return v, 0
+
+
+def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, workspace=None, stream=None):
+    """A token for each row of logits by the given numbers: ``(tokens, shares)``, int32 ``[rows]`` and float32 ``[rows]``.
+
+    logits ``[rows, vocab]`` float32, float16 or bfloat16 (row stride free), u float32 ``[rows]`` in [0, 1). In descending order of
+    the logits (of equal ones the lower index first) with weights ``exp((x - max) / temperature)``, kept are the first ``top_k``
+    (0: all), of those the shortest prefix with at least ``top_p`` of their weight (one token at least), of those the ones with
+    a weight of ``min_p`` or more. The token is the first, by index, at which the running sum of the kept weights exceeds u of
+    their sum; its share of that sum comes back as a logarithm. Temperature 0 takes the largest. Each setting is a number or a
+    tensor ``[rows]`` (float32; top_k int32). NaN and -infinity are never drawn: a row of nothing else gives token -1. Sums are of
+    whole numbers (a weight is one in units of 2^-46 of the largest at 2^16 tokens), so results do not depend on how a call is spread
+    over the device. Few rows are, on a workspace (``sample_workspace_bytes``; see ``matmul_nbits`` for whose it is and for
+    graph capture)."""
+    if logits.dtype not in _LT:
+        raise nat.XrmmInvalid("logits must be float32, float16 or bfloat16")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise nat.XrmmInvalid("logits must be [rows, vocab] with vocab positive")
+    rows, V = int(logits.shape[0]), int(logits.shape[1])
+    if rows and ((V > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < V)):
+        raise nat.XrmmInvalid("logits: a row must be contiguous, and rows must not overlap")
+    if u.dtype != torch.float32 or tuple(u.shape) != (rows,):
+        raise nat.XrmmInvalid(f"u must be float32 [{rows}]")
+    (tt, t), (pt, p), (mt, m) = (_setting(v, rows, torch.float32, n) for v, n in
+                                 ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p")))
+    kt, k = _setting(top_k, rows, torch.int32, "top_k")
+    dev = _check_dev(u, tt, pt, mt, kt)
+    _same_device(dev, logits)
+    lib = nat.lib()
+    s = _stream(stream, dev)
+    ws, nws = _take_workspace(int(lib.xrmm_sample_workspace_bytes(rows, V)), workspace, logits, dev, s, stream)
+    tokens = _empty((rows,), torch.int32, logits.device, stream)
+    shares = _empty((rows,), torch.float32, logits.device, stream)
+    nat.check(lib.xrmm_sample(
+        _ptr(logits), int(logits.stride(0)) if rows > 1 else V, _LT[logits.dtype], _ptr(u), _ptr(tt), _ptr(kt), _ptr(pt), _ptr(mt),
+        float(t), _i32(k), float(p), float(m), _ptr(tokens), _ptr(shares), rows, V, _ptr(ws), nws, s))
+    return tokens, shares
+
+
+def sample_workspace_bytes(rows, vocab):
+    """Bytes of the workspace of a sample call (0: none)."""
+    return int(nat.lib().xrmm_sample_workspace_bytes(int(rows), int(vocab)))
