@@ -16,8 +16,9 @@ namespace {
 constexpr int SB = 2048;      // bins
 constexpr float SB_NAT = 64.f;  // bins a nat
 constexpr int SLIST = 2048;   // tokens of the list; where more lie in the bins, the row itself is read in its place
-constexpr int ST = 1024;      // threads of a row
-constexpr int SW = ST / 64;
+constexpr int SNEAR = 256;    // of a list this short, each token counts those before it; of a longer one digits are counted
+constexpr int ST = 1024;      // threads of a row that one workgroup takes
+constexpr int SP = 256;       // threads of a part of a row
 
 struct Draw {       // a row's settings
   double c;         // log2(e) / temperature
@@ -144,19 +145,29 @@ struct RowOf {
 struct SampleLds {
   uint64_t mass[SB];
   uint32_t count[SB];
-  uint64_t list[SLIST];
+  uint64_t list[SLIST];   // composites
   uint64_t digits[256];
-  uint64_t part[SW];
+  uint64_t part[16];
   uint64_t a64, b64;
   uint32_t n, a32, b32;
+  int last;
 };
 
-// The first bin whose running sum reaches `need` (its index to s.a32, the sum before it to s.a64; SB where none does),
-// of masses or of counts. All threads.
-template <bool MASS>
-__device__ __forceinline__ void find_bin(SampleLds& s, uint64_t need) {
+// Bins that decide: top_k's threshold lies in bin kb, top_p's in lo .. hi (kb alone where there is no top_p); tokens before lo are
+// sure, those of neither dropped.
+struct Cut {
+  int lo, hi, kb;
+  uint64_t above;   // tokens before bin kb
+  uint64_t held_k;  // weight before bin kb; without top_k all of it
+  uint64_t held;    // weight before bin lo
+  __device__ __forceinline__ bool listed(int b) const { return (b >= lo && b <= hi) || b == kb; }
+};
+
+// The first bin whose running sum reaches `need`, of masses or of counts, and the sum before it; SB where none does. All threads.
+template <bool MASS, int NT>
+__device__ __forceinline__ int find_bin(SampleLds& s, uint64_t need, uint64_t* before_it) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int N = SB / ST;
+  constexpr int N = SB / NT;
   uint64_t v[N], sum = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -166,7 +177,10 @@ __device__ __forceinline__ void find_bin(SampleLds& s, uint64_t need) {
   const uint64_t inc = wave_scan64(sum, lane);
   __syncthreads();
   if (lane == 63) s.part[wave] = inc;
-  if (tid == 0) s.a32 = SB;
+  if (tid == 0) {
+    s.a32 = SB;
+    s.a64 = 0;
+  }
   __syncthreads();
   uint64_t before = inc - sum;
   for (int w = 0; w < wave; ++w) before += s.part[w];
@@ -179,11 +193,58 @@ __device__ __forceinline__ void find_bin(SampleLds& s, uint64_t need) {
     before += v[i];
   }
   __syncthreads();
+  *before_it = s.a64;
+  return static_cast<int>(s.a32);
+}
+
+// The sum of v over the workgroup, in all threads.
+template <int NT>
+__device__ __forceinline__ uint64_t block_sum64(SampleLds& s, uint64_t v) {
+  const int tid = threadIdx.x;
+  v = wave_sum64(v);
+  __syncthreads();
+  if ((tid & 63) == 0) s.part[tid >> 6] = v;
+  __syncthreads();
+  uint64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) all += s.part[w];
+  return all;
+}
+
+// From the histogram of a row. All threads.
+template <int NT>
+__device__ __forceinline__ Cut cut_of(SampleLds& s, const Draw& d) {
+  const int tid = threadIdx.x;
+  Cut c{0, -1, -1, 0, 0, 0};
+  if (d.k > 0) {
+    c.kb = find_bin<false, NT>(s, static_cast<uint64_t>(d.k), &c.above);
+    if (c.kb == SB) {  // fewer tokens than top_k: the last bin is all kept
+      uint64_t n = 0;
+      for (int i = tid; i < SB - 1; i += NT) n += s.count[i];
+      c.above = block_sum64<NT>(s, n);
+      c.kb = SB - 1;
+    }
+    c.lo = c.hi = c.kb;
+  }
+  if (d.p) {
+    const int end = d.k > 0 ? c.kb : SB;
+    uint64_t m = 0;
+    for (int i = tid; i < end; i += NT) m += s.mass[i];
+    c.held_k = block_sum64<NT>(s, m);
+    const uint64_t most = c.held_k + (d.k > 0 ? s.mass[c.kb] : 0);  // top_k's weight is from held_k to this
+    const int lo = find_bin<true, NT>(s, share_of(d.top_p, c.held_k), &c.held);
+    uint64_t unused;
+    const int hi = d.k > 0 ? find_bin<true, NT>(s, share_of(d.top_p, most), &unused) : lo;
+    c.lo = lo < SB ? lo : SB - 1;
+    c.hi = hi < SB ? hi : SB - 1;
+    if (d.k == 0) c.kb = c.lo;
+  }
+  __syncthreads();
+  return c;
 }
 
 // The composite at which a running sum over the candidates, in descending order, reaches `need` (>= 1): of their weights, or of their
-// number. `each(f)` calls f(composite, weight) for the candidates of each thread. 0 where all do not reach it; *rest: what is
-// missing to `need` before the found one.
+// number; 0 where all do not reach it. `each(f)` calls f(composite, weight) for the candidates of each thread. All threads.
 template <bool MASS, typename E>
 __device__ __forceinline__ uint64_t find_composite(SampleLds& s, uint64_t need, E&& each) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -222,50 +283,240 @@ __device__ __forceinline__ uint64_t find_composite(SampleLds& s, uint64_t need, 
   return prefix;
 }
 
-// One workgroup a row, all of it.
-template <typename T>
-__global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
-  typedef RowOf<T> R;
-  constexpr int VEC = R::VEC;
-  __shared__ SampleLds s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x;
-  const R r{static_cast<const T*>(a.x) + row * a.stride};
-  const Draw d = draw_of(a, row, F);
-  const int V = a.V;
-  const float ninf = -__builtin_inff();
+// The composite from which on a row's tokens are kept. `n` tokens are listed, in s.list if no more than SLIST. All threads.
+template <typename T, int NT>
+__device__ uint64_t threshold_of(SampleLds& s, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n) {
+  constexpr int VEC = RowOf<T>::VEC;
+  const int tid = threadIdx.x;
+  const float top = weigh.top;
+  // candidates: the listed tokens of bins from .. to whose composite is at least `least`
+  auto each_of = [&](int from, int to, uint64_t least, auto&& f) {
+    auto one = [&](uint64_t c) {
+      const float x = of_okey(static_cast<uint32_t>(c >> 32));
+      const int b = bin_of(x, top, d.s);
+      if (b >= from && b <= to && c >= least) f(c, Weigher::whole(weigh.units(x)));
+    };
+    if (n <= SLIST) {
+      for (uint32_t i = tid; i < n; i += NT) one(s.list[i]);
+    } else {
+#pragma unroll 1
+      for (int i = tid * VEC; i < V; i += NT * VEC) {
+        float x[VEC];
+        r.load(x, i, V);
+#pragma unroll 1
+        for (int e = 0; e < VEC; ++e)
+          if (x[e] > -__builtin_inff()) one(composite(x[e], i + e));
+      }
+    }
+  };
+  uint64_t threshold = 0;
+  if (n <= SNEAR) {
+    // Each token's number and weight of those before it. Weights go to s.mass, which the cut has left.
+    uint64_t c = 0, w = 0;
+    bool in_k = false, in_p = false;
+    __syncthreads();
+    if (tid < static_cast<int>(n)) {
+      c = s.list[tid];
+      const float x = of_okey(static_cast<uint32_t>(c >> 32));
+      const int b = bin_of(x, top, d.s);
+      w = Weigher::whole(weigh.units(x));
+      in_k = b == cut.kb;
+      in_p = b >= cut.lo && b <= cut.hi;
+      s.mass[tid] = w;
+      s.count[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
+    }
+    if (tid == 0) s.a64 = s.b64 = 0;
+    __syncthreads();
+    uint64_t before = 0, number = 0, k_weight = 0;
+    if (tid < static_cast<int>(n)) {
+      for (uint32_t j = 0; j < n; ++j) {
+        const bool first = s.list[j] > c;
+        const uint32_t of = s.count[j];
+        number += first && (of & 1) ? 1 : 0;
+        k_weight += first && (of & 1) ? s.mass[j] : 0;
+        before += first && (of & 2) ? s.mass[j] : 0;
+      }
+    }
+    uint64_t all = cut.held_k;
+    if (d.k > 0) {
+      const uint64_t want = static_cast<uint64_t>(d.k) - cut.above;
+      if (in_k && number + 1 == want) {
+        s.a64 = c;
+        s.b64 = k_weight + w;
+      }
+      __syncthreads();
+      threshold = s.a64;
+      if (d.p) {
+        uint64_t m = 0;
+        if (threshold == 0) m = block_sum64<NT>(s, in_k ? w : 0);  // all of them
+        all += threshold == 0 ? m : s.b64;
+      }
+    }
+    if (d.p) {
+      const uint64_t need = share_of(d.top_p, all), want = need > cut.held ? need - cut.held : 1;
+      __syncthreads();
+      if (tid == 0) s.a64 = 0;
+      __syncthreads();
+      if (in_p && w > 0 && before < want && before + w >= want) s.a64 = c;
+      __syncthreads();
+      threshold = s.a64 > threshold ? s.a64 : threshold;
+    }
+    __syncthreads();
+    return threshold;
+  }
+  if (d.k > 0)
+    threshold = find_composite<false>(s, static_cast<uint64_t>(d.k) - cut.above, [&](auto&& f) { each_of(cut.kb, cut.kb, 0, f); });
+  if (d.p) {
+    uint64_t all = cut.held_k;
+    if (d.k > 0) {
+      uint64_t mine = 0;
+      each_of(cut.kb, cut.kb, threshold, [&](uint64_t, uint64_t w) { mine += w; });
+      all += block_sum64<NT>(s, mine);
+    }
+    const uint64_t need = share_of(d.top_p, all);
+    const uint64_t c = find_composite<true>(s, need > cut.held ? need - cut.held : 1, [&](auto&& f) { each_of(cut.lo, cut.hi, 0, f); });
+    threshold = c > threshold ? c : threshold;
+  }
+  __syncthreads();
+  return threshold;
+}
 
-  // the largest logit, of the lowest index
-  uint64_t best = 0;
-  for (int i = tid * VEC; i < V; i += ST * VEC) {
-    float f[VEC];
-    r.load(f, i, V);
+// What a kept token weighs; 0 for one that is not.
+struct Keep {
+  Weigher weigh;
+  double least;
+  uint64_t threshold;
+  __device__ __forceinline__ uint64_t operator()(float x, uint32_t i) const {
+    if (!(x > -__builtin_inff()) || composite(x, i) < threshold) return 0;
+    const double u = weigh.units(x);
+    return u >= least ? Weigher::whole(u) : 0;
+  }
+};
+
+// The token at which the running sum of the kept weights over begin .. end - 1 passes `target`, narrowed to a wave's part at a time; `target_of`
+// turns the sum over all of it into the target (and may return what the caller knows). All threads.
+template <typename T, int NT, typename F>
+__device__ void draw_in(SampleLds& s, const RowOf<T>& r, int begin, int end, const Keep& keep, F&& target_of, int32_t* token, float* share) {
+  constexpr int VEC = RowOf<T>::VEC, NW = NT / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint64_t total = 0, target = 0;
+#pragma unroll 1
+  for (bool first = true;; first = false) {
+    const int per = ((end - begin + NW - 1) / NW + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
+    const int from = begin + wave * per, to = end - from < per ? end : from + per;
+    uint64_t mine = 0;
+#pragma unroll 1
+    for (int i = from + lane * VEC; i < to; i += 64 * VEC) {
+      float f[VEC];
+      r.load(f, i, to);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) mine += keep(f[e], static_cast<uint32_t>(i + e));
+    }
+    mine = wave_sum64(mine);
+    __syncthreads();
+    if (lane == 0) s.part[wave] = mine;
+    __syncthreads();
+    if (first) {
+      uint64_t all = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) all += s.part[w];
+      target = target_of(all, total);
+    }
+    int w = 0;
+    uint64_t before = 0;
+    while (w < NW - 1 && before + s.part[w] <= target) before += s.part[w++];
+    target -= before;
+    begin += w * per;
+    end = end - begin < per ? end : begin + per;
+    if (per == 64 * VEC) break;
+  }
+  if (wave != 0) return;
+  float f[VEC];
+  r.load(f, begin + lane * VEC, end);
+  uint64_t k[VEC], mine = 0;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) mine += k[e] = keep(f[e], static_cast<uint32_t>(begin + lane * VEC + e));
+  const uint64_t inc = wave_scan64(mine, lane);
+  uint64_t before = inc - mine;
+  if (before <= target && target < inc) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const uint64_t c = f[e] > ninf ? composite(f[e], i + e) : 0ull;
-      best = c > best ? c : best;
+      if (before <= target && target < before + k[e]) {
+        *token = begin + lane * VEC + e;
+        *share = static_cast<float>(log(keep.weigh.units(f[e]) / static_cast<double>(total)));
+      }
+      before += k[e];
     }
   }
+}
+
+// The largest composite of from .. to - 1, in all threads; 0 where there is none.
+template <typename T, int NT>
+__device__ __forceinline__ uint64_t best_of(SampleLds& s, const RowOf<T>& r, int from, int to) {
+  constexpr int VEC = RowOf<T>::VEC;
+  const int tid = threadIdx.x;
+  uint32_t key = 0, at = 0;  // the first of the largest: a thread's indexes ascend
+  for (int i = from + tid * VEC; i < to; i += NT * VEC) {
+    float f[VEC];
+    r.load(f, i, to);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const uint32_t k = f[e] > -__builtin_inff() ? okey(f[e]) : 0u;
+      at = k > key ? i + e : at;
+      key = k > key ? k : key;
+    }
+  }
+  uint64_t best = key == 0 ? 0 : static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - at);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const uint64_t c = shfl_xor64(best, o);
     best = c > best ? c : best;
   }
-  if (lane == 0) s.part[wave] = best;
+  if ((tid & 63) == 0) s.part[tid >> 6] = best;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < SW; ++w) best = s.part[w] > best ? s.part[w] : best;
+  for (int w = 0; w < NT / 64; ++w) best = s.part[w] > best ? s.part[w] : best;
+  return best;
+}
+
+// from .. to - 1 into the histogram.
+template <typename T, int NT>
+__device__ __forceinline__ void count_in(SampleLds& s, const RowOf<T>& r, int from, int to, const Draw& d, const Weigher& weigh) {
+  constexpr int VEC = RowOf<T>::VEC;
+  for (int i = from + static_cast<int>(threadIdx.x) * VEC; i < to; i += NT * VEC) {
+    float f[VEC];
+    r.load(f, i, to);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      if (!(f[e] > -__builtin_inff())) continue;
+      const int b = bin_of(f[e], weigh.top, d.s);
+      if (d.k > 0) atomicAdd(&s.count[b], 1u);
+      if (d.p) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), static_cast<unsigned long long>(Weigher::whole(weigh.units(f[e]))));
+    }
+  }
+}
+
+// One workgroup a row, all of it.
+template <typename T>
+__global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
+  constexpr int VEC = RowOf<T>::VEC;
+  __shared__ SampleLds s;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const Draw d = draw_of(a, row, F);
+  const int V = a.V;
+  const uint64_t best = best_of<T, ST>(s, r, 0, V);
   if (best == 0 || d.greedy) {
     if (tid == 0) {
       a.tokens[row] = best == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-      a.shares[row] = best == 0 ? ninf : 0.f;
+      a.shares[row] = best == 0 ? -__builtin_inff() : 0.f;
     }
     return;
   }
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
   const Weigher weigh{top, static_cast<double>(top), d.c, F};
-
-  uint64_t threshold = 0;  // composites from here on are kept
+  uint64_t threshold = 0;
   if (d.k > 0 || d.p) {
     for (int i = tid; i < SB; i += ST) {
       s.mass[i] = 0;
@@ -273,167 +524,295 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
     }
     if (tid == 0) s.n = 0;
     __syncthreads();
-    for (int i = tid * VEC; i < V; i += ST * VEC) {
-      float f[VEC];
-      r.load(f, i, V);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (!(f[e] > ninf)) continue;
-        const int b = bin_of(f[e], top, d.s);
-        if (d.k > 0) atomicAdd(&s.count[b], 1u);
-        if (d.p) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), static_cast<unsigned long long>(Weigher::whole(weigh.units(f[e]))));
-      }
-    }
+    count_in<T, ST>(s, r, 0, V, d, weigh);
     __syncthreads();
-    // bins lo .. hi hold the thresholds; `above` tokens and `held` weight lie in those before lo
-    int lo = 0, hi = SB - 1;
-    uint64_t held_k = 0;
-    if (d.k > 0) {
-      find_bin<false>(s, static_cast<uint64_t>(d.k));
-      hi = s.a32 < SB ? static_cast<int>(s.a32) : SB - 1;
-      lo = hi;
-    }
-    if (d.p) {
-      uint64_t all = 0;
-      if (d.k > 0) {  // the weight before bin hi: top_p of it, at least, is wanted
-        for (int i = lane; i < hi; i += 64) all += s.mass[i];
-      } else {
-        for (int i = lane; i < SB; i += 64) all += s.mass[i];
-      }
-      held_k = wave_sum64(all);
-      find_bin<true>(s, share_of(d.top_p, held_k));
-      const int b = s.a32 < SB ? static_cast<int>(s.a32) : SB - 1;
-      lo = d.k > 0 && b > hi ? hi : b;
-      if (d.k == 0) hi = lo;
-    }
-    uint64_t above = 0, held = 0;
-    for (int i = lane; i < lo; i += 64) {
-      above += s.count[i];
-      held += s.mass[i];
-    }
-    above = wave_sum64(above);
-    held = wave_sum64(held);
-    // the list
+    const Cut cut = cut_of<ST>(s, d);
     for (int i = tid * VEC; i < V; i += ST * VEC) {
       float f[VEC];
       r.load(f, i, V);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        if (!(f[e] > ninf)) continue;
-        const int b = bin_of(f[e], top, d.s);
-        if (b < lo || b > hi) continue;
+        if (!(f[e] > -__builtin_inff()) || !cut.listed(bin_of(f[e], top, d.s))) continue;
         const uint32_t at = atomicAdd(&s.n, 1u);
         if (at < SLIST) s.list[at] = composite(f[e], i + e);
       }
     }
     __syncthreads();
-    const uint32_t n = s.n;
-    auto each = [&](auto&& f) {
-      if (n <= SLIST) {
-        for (uint32_t i = tid; i < n; i += ST) {
-          const uint64_t c = s.list[i];
-          f(c, Weigher::whole(weigh.units(of_okey(static_cast<uint32_t>(c >> 32)))));
-        }
-      } else {
-        for (int i = tid * VEC; i < V; i += ST * VEC) {
-          float x[VEC];
-          r.load(x, i, V);
+    threshold = threshold_of<T, ST>(s, r, V, d, cut, weigh, s.n);
+  }
+  draw_in<T, ST>(s, r, 0, V, Keep{weigh, d.least, threshold},
+                 [&](uint64_t all, uint64_t& total) {
+                   total = all;
+                   return place_of(static_cast<double>(a.u[row]), all);
+                 },
+                 a.tokens + row, a.shares + row);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: parts of a row by workgroups, in launches that end where the whole row has to be known. k_sample_top: the largest logit.
+// k_sample_mass: the histogram, whose cut the last part to arrive takes; without top_k and top_p the parts' weights, and the draw.
+// k_sample_draw: the list and the sure tokens' weights by part; the last part to arrive finds the threshold, the part in which the
+// target falls, and the token in it. What parts leave for the last one goes past the L2 of its XCD.
+struct SampleRow {        // at the head of the workspace, zero between calls
+  uint64_t best;
+  uint32_t arrived, pad;
+};
+struct SampleShare {      // a row's, behind the head
+  uint64_t mass[SB];
+  uint64_t list[SLIST];
+  uint32_t count[SB];
+  Cut cut;
+  uint32_t n, pad[3];
+};                        // and its parts' weights
+constexpr int64_t SAMPLE_HEAD = 4096;
+constexpr int SAMPLE_ROWS = static_cast<int>(SAMPLE_HEAD / sizeof(SampleRow));
+
+struct SamplePlan {
+  int parts, size;        // of a row; size: logits of a part
+  __host__ __device__ int64_t row_bytes() const { return (static_cast<int64_t>(sizeof(SampleShare)) + parts * 8 + 255) / 256 * 256; }
+};
+
+template <typename U>
+__device__ __forceinline__ void put(U* p, U v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename U>
+__device__ __forceinline__ U get(const U* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+__device__ __forceinline__ SampleRow* row_of(const SampleArgs& a, int64_t row) { return static_cast<SampleRow*>(a.ws) + row; }
+__device__ __forceinline__ SampleShare* share_of_row(const SampleArgs& a, const SamplePlan& p, int64_t row) {
+  return reinterpret_cast<SampleShare*>(static_cast<uint8_t*>(a.ws) + SAMPLE_HEAD + row * p.row_bytes());
+}
+
+// Whether this workgroup is the last of its row's parts. What it put before is seen by that one. All threads.
+__device__ __forceinline__ bool last_part(SampleLds& s, SampleRow* w, int parts) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s.last = __hip_atomic_fetch_add(&w->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(parts) - 1u;
+    if (s.last) put(&w->arrived, 0u);
+  }
+  __syncthreads();
+  return s.last != 0;
+}
+
+template <typename T>
+__global__ __launch_bounds__(SP) void k_sample_top(SampleArgs a, SamplePlan p, int F) {
+  __shared__ SampleLds s;
+  const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
+  const int64_t row = blockIdx.y;
+  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
+  SampleShare* w = share_of_row(a, p, row);
+  for (int i = part * SP + tid; i < SB; i += p.parts * SP) {
+    w->mass[i] = 0;
+    w->count[i] = 0;
+  }
+  if (part == 0 && tid == 0) w->n = 0;
+  const uint64_t best = best_of<T, SP>(s, r, from, to);
+  if (tid == 0 && best != 0) __hip_atomic_fetch_max(&row_of(a, row)->best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The draw of a row whose parts' kept weights are known, by the last part to arrive.
+template <typename T>
+__device__ void draw_parts(SampleLds& s, const SampleArgs& a, const SamplePlan& p, int64_t row, const RowOf<T>& r, const Keep& keep,
+                           const uint64_t* weights, const uint64_t* more) {
+  // a wave's parts at a time are at most 64 * 4
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t v[4], sum = 0;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if (!(x[e] > ninf)) continue;
-            const int b = bin_of(x[e], top, d.s);
-            if (b >= lo && b <= hi) f(composite(x[e], i + e), Weigher::whole(weigh.units(x[e])));
-          }
-        }
+  for (int i = 0; i < 4; ++i) {
+    const int at = lane * 4 + i;
+    v[i] = at < p.parts ? get(weights + at) + (more ? more[at] : 0) : 0;
+    sum += v[i];
+  }
+  const uint64_t inc = wave_scan64(sum, lane);
+  const uint64_t total = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc >> 32), 63))) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc), 63));
+  const uint64_t target = place_of(static_cast<double>(a.u[row]), total);
+  uint64_t before = inc - sum;
+  __syncthreads();
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before <= target && target < before + v[i]) {
+        s.a32 = lane * 4 + i;
+        s.a64 = target - before;
       }
-    };
-    if (d.k > 0) threshold = find_composite<false>(s, static_cast<uint64_t>(d.k) - above, each);
-    if (d.p) {
-      uint64_t all = held_k;
-      if (d.k > 0) {  // top_k's weight: what is held before the list, and the list's part of it
-        __syncthreads();
-        if (tid == 0) s.a64 = 0;
-        __syncthreads();
-        uint64_t mine = 0;
-        each([&](uint64_t c, uint64_t w) { mine += c >= threshold ? w : 0ull; });
-        mine = wave_sum64(mine);
-        if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s.a64), static_cast<unsigned long long>(mine));
-        __syncthreads();
-        all = held + s.a64;
-      }
-      const uint64_t need = share_of(d.top_p, all);
-      const uint64_t c = find_composite<true>(s, need > held ? need - held : 1, each);
-      threshold = c > threshold ? c : threshold;
+      before += v[i];
     }
   }
+  __syncthreads();
+  const int from = static_cast<int>(s.a32) * p.size, to = a.V - from < p.size ? a.V : from + p.size;
+  const uint64_t rest = s.a64;
+  draw_in<T, SP>(s, r, from, to, keep,
+                 [&](uint64_t, uint64_t& t) {
+                   t = total;
+                   return rest;
+                 },
+                 a.tokens + row, a.shares + row);
+}
 
-  // the draw: the running sum of the kept weights by index, narrowed to a wave's part at a time
-  int begin = 0, end = V;
-  uint64_t total = 0, target = 0;
-  auto kept = [&](float x, uint32_t i) {
-    if (!(x > ninf) || composite(x, i) < threshold) return uint64_t{0};
-    const double u = weigh.units(x);
-    return u >= d.least ? Weigher::whole(u) : uint64_t{0};
-  };
-  for (bool firsts = true;; firsts = false) {
-    const int per = ((end - begin + SW - 1) / SW + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
-    const int64_t from = begin + static_cast<int64_t>(wave) * per, to = from + per < end ? from + per : end;
+template <typename T>
+__global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, int F) {
+  constexpr int VEC = RowOf<T>::VEC;
+  __shared__ SampleLds s;
+  const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
+  const int64_t row = blockIdx.y;
+  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
+  const Draw d = draw_of(a, row, F);
+  SampleRow* w = row_of(a, row);
+  SampleShare* sh = share_of_row(a, p, row);
+  uint64_t* weights = reinterpret_cast<uint64_t*>(sh + 1);
+  const uint64_t best = w->best;
+  if (best == 0 || d.greedy) {
+    if (!last_part(s, w, p.parts)) return;  // all parts have read `best`
+    if (tid == 0) {
+      a.tokens[row] = best == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
+      a.shares[row] = best == 0 ? -__builtin_inff() : 0.f;
+      put(&w->best, uint64_t{0});
+    }
+    return;
+  }
+  const float top = of_okey(static_cast<uint32_t>(best >> 32));
+  const Weigher weigh{top, static_cast<double>(top), d.c, F};
+  if (d.k == 0 && !d.p) {
+    const Keep keep{weigh, d.least, 0};
     uint64_t mine = 0;
-    for (int64_t i = from + lane * VEC; i < to; i += 64 * VEC) {
+    for (int i = from + tid * VEC; i < to; i += SP * VEC) {
       float f[VEC];
       r.load(f, i, to);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mine += kept(f[e], static_cast<uint32_t>(i + e));
+      for (int e = 0; e < VEC; ++e) mine += keep(f[e], static_cast<uint32_t>(i + e));
     }
-    mine = wave_sum64(mine);
-    __syncthreads();
-    if (lane == 0) s.part[wave] = mine;
-    __syncthreads();
-    uint64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < SW; ++w) all += s.part[w];
-    if (firsts) {
-      total = all;
-      target = place_of(static_cast<double>(a.u[row]), total);
-    }
-    int w = 0;
-    uint64_t before = 0;
-    while (w < SW - 1 && before + s.part[w] <= target) before += s.part[w++];
-    target -= before;
-    begin = begin + w * per;
-    end = begin + per < end ? begin + per : end;
-    if (per == 64 * VEC) break;
+    mine = block_sum64<SP>(s, mine);
+    if (tid == 0) put(weights + part, mine);
+    if (!last_part(s, w, p.parts)) return;
+    if (tid == 0) put(&w->best, uint64_t{0});
+    draw_parts(s, a, p, row, r, keep, weights, nullptr);
+    return;
   }
-  if (wave == 0) {
+  for (int i = tid; i < SB; i += SP) {
+    s.mass[i] = 0;
+    s.count[i] = 0;
+  }
+  __syncthreads();
+  count_in<T, SP>(s, r, from, to, d, weigh);
+  __syncthreads();
+  for (int i = tid; i < SB; i += SP) {
+    if (d.k > 0 && s.count[i] != 0) __hip_atomic_fetch_add(&sh->count[i], s.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (d.p && s.mass[i] != 0) __hip_atomic_fetch_add(&sh->mass[i], s.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (!last_part(s, w, p.parts)) return;
+  for (int i = tid; i < SB; i += SP) {
+    s.count[i] = d.k > 0 ? get(&sh->count[i]) : 0u;
+    s.mass[i] = d.p ? get(&sh->mass[i]) : 0u;
+  }
+  __syncthreads();
+  const Cut cut = cut_of<SP>(s, d);
+  if (tid == 0) sh->cut = cut;  // for the next launch
+}
+
+template <typename T>
+__global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, int F) {
+  constexpr int VEC = RowOf<T>::VEC;
+  __shared__ SampleLds s;
+  const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
+  const int64_t row = blockIdx.y;
+  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
+  const Draw d = draw_of(a, row, F);
+  SampleRow* w = row_of(a, row);
+  SampleShare* sh = share_of_row(a, p, row);
+  uint64_t* weights = reinterpret_cast<uint64_t*>(sh + 1);
+  const uint64_t best = w->best;
+  if (best == 0) return;  // drawn, or nothing to draw
+  const float top = of_okey(static_cast<uint32_t>(best >> 32));
+  const Weigher weigh{top, static_cast<double>(top), d.c, F};
+  const Cut cut = sh->cut;
+  uint64_t mine = 0;
+  for (int i = from + tid * VEC; i < to; i += SP * VEC) {
     float f[VEC];
-    r.load(f, begin + lane * VEC, end);
-    uint64_t k[VEC], mine = 0;
+    r.load(f, i, to);
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) mine += k[e] = kept(f[e], static_cast<uint32_t>(begin + lane * VEC + e));
-    const uint64_t inc = wave_scan64(mine, lane);
-    uint64_t before = inc - mine;
-    if (before <= target && target < inc) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (before <= target && target < before + k[e]) {
-          a.tokens[row] = begin + lane * VEC + e;
-          a.shares[row] = static_cast<float>(log(weigh.units(f[e]) / static_cast<double>(total)));
-        }
-        before += k[e];
+    for (int e = 0; e < VEC; ++e) {
+      if (!(f[e] > -__builtin_inff())) continue;
+      const int b = bin_of(f[e], top, d.s);
+      if (cut.listed(b)) {
+        const uint32_t at = __hip_atomic_fetch_add(&sh->n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (at < SLIST) put(&sh->list[at], composite(f[e], i + e));
+      } else if (b < cut.lo) {
+        const double u = weigh.units(f[e]);
+        mine += u >= d.least ? Weigher::whole(u) : 0;
       }
     }
   }
+  mine = block_sum64<SP>(s, mine);
+  if (tid == 0) put(weights + part, mine);
+  if (!last_part(s, w, p.parts)) return;
+  if (tid == 0) put(&w->best, uint64_t{0});
+  const uint32_t n = get(&sh->n);
+  for (uint32_t i = tid; i < n && i < SLIST; i += SP) s.list[i] = get(&sh->list[i]);
+  __syncthreads();
+  const uint64_t threshold = threshold_of<T, SP>(s, r, a.V, d, cut, weigh, n);
+  const Keep keep{weigh, d.least, threshold};
+  // the list's kept weights by part
+  for (int i = tid; i < p.parts; i += SP) s.mass[i] = 0;
+  __syncthreads();
+  auto add = [&](float x, uint32_t i) {
+    const uint64_t k = keep(x, i);
+    if (k != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[i / static_cast<uint32_t>(p.size)]), static_cast<unsigned long long>(k));
+  };
+  if (n <= SLIST) {
+    for (uint32_t i = tid; i < n; i += SP) {
+      const uint64_t c = s.list[i];
+      add(of_okey(static_cast<uint32_t>(c >> 32)), 0xFFFFFFFFu - static_cast<uint32_t>(c));
+    }
+  } else {
+#pragma unroll 1
+    for (int i = tid * VEC; i < a.V; i += SP * VEC) {
+      float f[VEC];
+      r.load(f, i, a.V);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (f[e] > -__builtin_inff() && cut.listed(bin_of(f[e], top, d.s))) add(f[e], static_cast<uint32_t>(i + e));
+    }
+  }
+  __syncthreads();
+  draw_parts(s, a, p, row, r, keep, weights, s.mass);
+}
+
+// Rows by parts where one workgroup a row would leave CUs idle and a row is long enough to pay for the launches.
+bool sample_split(int64_t rows, int64_t V, SamplePlan& p) {
+  if (rows < 1 || rows > SAMPLE_ROWS || rows > 128 || V < 8192) return false;
+  int64_t parts = 1024 / rows;
+  parts = parts < 64 ? parts : 64;
+  const int64_t most = (V + 2047) / 2048;
+  parts = parts < most ? parts : most;
+  p.size = static_cast<int>(((V + parts - 1) / parts + 2047) / 2048 * 2048);
+  p.parts = static_cast<int>((V + p.size - 1) / p.size);
+  return p.parts > 1;
 }
 
 template <typename T>
 hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
+  SamplePlan p;
+  if (a.ws != nullptr && sample_split(a.rows, a.V, p) && a.ws_bytes >= SAMPLE_HEAD + a.rows * p.row_bytes()) {
+    const dim3 grid(static_cast<uint32_t>(p.parts), static_cast<uint32_t>(a.rows));
+    k_sample_top<T><<<grid, SP, 0, st>>>(a, p, F);
+    k_sample_mass<T><<<grid, SP, 0, st>>>(a, p, F);
+    if (a.top_k != nullptr || a.top_p != nullptr || (a.top_k1 > 0 && a.top_k1 < a.V) || a.top_p1 < 1.0) k_sample_draw<T><<<grid, SP, 0, st>>>(a, p, F);
+    return hipGetLastError();
+  }
   k_sample_row<T><<<dim3(static_cast<uint32_t>(a.rows)), ST, 0, st>>>(a, F);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t sample_workspace_bytes(int64_t rows, int64_t V) { return 0; }
+int64_t sample_workspace_bytes(int64_t rows, int64_t V) {
+  SamplePlan p;
+  return sample_split(rows, V, p) ? SAMPLE_HEAD + rows * p.row_bytes() : 0;
+}
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
   if (a.rows == 0) return hipSuccess;

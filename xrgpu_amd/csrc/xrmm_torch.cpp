@@ -675,6 +675,187 @@ PyObject* bind_lowbit(PyObject*, PyObject* const* v, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------------------
+// Rotary positions, the draw of tokens, attention on a shared prefix
+
+using RopeFn = int (*)(const void*, const void*, void*, void*, int64_t, int64_t, int64_t, int64_t, int32_t, const void*, int32_t, double,
+                       const void*, int32_t, const void*, const void*, int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t,
+                       void*);
+using SampleWsFn = int64_t (*)(int64_t, int64_t);
+using SampleFn = int (*)(const void*, int64_t, int32_t, const void*, const void*, const void*, const void*, const void*, double, int32_t,
+                         double, double, void*, void*, int64_t, int64_t, void*, int64_t, void*);
+using SharedWsFn = int64_t (*)(int64_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t, int32_t);
+using SharedFn = int (*)(const void*, int64_t, void*, int32_t, const void*, const void*, const void*, const void*, int32_t, const void*,
+                         int32_t, const void*, const void*, const void*, void*, int64_t, int32_t, int32_t, int32_t, int64_t, int32_t,
+                         int32_t, int32_t, int32_t, float, int32_t, int32_t, void*, int64_t, void*);
+
+RopeFn g_rope;
+SampleWsFn g_sample_ws;
+SampleFn g_sample;
+SharedWsFn g_shared_ws;
+SharedFn g_shared;
+constexpr int I32 = 2, I64 = 7;  // xrmm_dtype
+
+bool real64(PyObject* o, double& v) {
+  int64_t i = 0;
+  if (PyFloat_CheckExact(o)) v = PyFloat_AS_DOUBLE(o);
+  else if (integer(o, i)) v = static_cast<double>(i);
+  else return false;
+  return true;
+}
+
+// (q, k, frequencies, positions, lengths, starts, magnitude, interleaved, inverse); the output, or both
+PyObject* rope(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    int dev = -1;
+    const at::Tensor *q, *k = nullptr, *f, *p = nullptr, *l = nullptr, *s = nullptr;
+    int64_t qs = 0, ks = 0, Hk = 0;
+    double magnitude;
+    void* st;
+    if (!plain(v[2], dev, f) || f->scalar_type() != at::kDouble || f->dim() != 1 || !THPVariable_CheckExact(v[0]) ||
+        THPVariable_Unpack(v[0]).dim() != 3 || none(v[3]) == none(v[4]) || !real64(v[6], magnitude) || !PyBool_Check(v[7]) ||
+        !PyBool_Check(v[8]))
+      Py_RETURN_NONE;
+    const at::Tensor& q0 = THPVariable_Unpack(v[0]);
+    const int64_t T = q0.size(0), Hq = q0.size(1), D = q0.size(2);
+    if (Hq == 0 || Hq > INT32_MAX || D == 0 || D > INT32_MAX || !token_rows(v[0], dev, Hq, D, q, qs) || lt(q->scalar_type()) < 0) Py_RETURN_NONE;
+    if (!none(v[1])) {
+      if (!THPVariable_CheckExact(v[1]) || THPVariable_Unpack(v[1]).dim() != 3) Py_RETURN_NONE;
+      Hk = THPVariable_Unpack(v[1]).size(1);
+      if (Hk == 0 || Hk > INT32_MAX || !token_rows(v[1], dev, Hk, D, k, ks) || k->size(0) != T || k->scalar_type() != q->scalar_type()) Py_RETURN_NONE;
+    }
+    if (!none(v[3]) && (!plain(v[3], dev, p) || !(p->scalar_type() == at::kInt || p->scalar_type() == at::kLong) || !shape(*p, {T}))) Py_RETURN_NONE;
+    if (!none(v[4]) && (!plain(v[4], dev, l) || l->scalar_type() != at::kInt || l->dim() != 1 || l->size(0) > INT32_MAX)) Py_RETURN_NONE;
+    if (!none(v[5]) && (l == nullptr || !plain(v[5], dev, s) || s->scalar_type() != at::kInt || !shape(*s, {l->size(0) + 1}))) Py_RETURN_NONE;
+    if (f->size(0) > INT32_MAX / 2 || !stream_of(dev, st)) Py_RETURN_NONE;
+    at::Tensor oq, ok;
+    int rc;
+    {
+      NoGil ng;
+      oq = at::empty(q->sizes(), q->options());
+      if (k) ok = at::empty(k->sizes(), k->options());
+      rc = g_rope(q->data_ptr(), k ? k->data_ptr() : nullptr, oq.data_ptr(), data_of(ok), qs, ks, Hq * D, Hk * D, lt(q->scalar_type()),
+                  f->data_ptr(), static_cast<int32_t>(2 * f->size(0)), magnitude, p ? p->data_ptr() : nullptr,
+                  p && p->scalar_type() == at::kLong ? I64 : I32, l ? l->data_ptr() : nullptr, s ? s->data_ptr() : nullptr, T,
+                  l ? static_cast<int32_t>(l->size(0)) : 0, static_cast<int32_t>(Hq), static_cast<int32_t>(Hk), static_cast<int32_t>(D),
+                  v[7] == Py_True, v[8] == Py_True, st);
+    }
+    if (!checked(rc)) return nullptr;
+    if (!k) return THPVariable_Wrap(oq);
+    PyObject *o0 = THPVariable_Wrap(oq), *o1 = THPVariable_Wrap(ok);
+    return Py_BuildValue("(NN)", o0, o1);
+  });
+}
+
+// (logits, u, temperature, top_k, top_p, min_p); an int: checked, needs a workspace of that many bytes
+PyObject* sample(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    int dev = -1;
+    const at::Tensor* u;
+    if (!plain(v[1], dev, u) || !THPVariable_CheckExact(v[0])) Py_RETURN_NONE;
+    const at::Tensor& x = THPVariable_Unpack(v[0]);
+    const auto keys = x.key_set();
+    if (!x.is_cuda() || x.layout() != at::kStrided || keys.has(c10::DispatchKey::Python) || keys.has_any(c10::functorch_transforms_ks) ||
+        x.is_conj() || x.is_neg() || x.get_device() != dev || x.dim() != 2 || lt(x.scalar_type()) < 0)
+      Py_RETURN_NONE;
+    const int64_t B = x.size(0), V = x.size(1);
+    if (B == 0 || V == 0 || (V > 1 && x.stride(1) != 1) || (B > 1 && x.stride(0) < V) || u->scalar_type() != at::kFloat || !shape(*u, {B}))
+      Py_RETURN_NONE;
+    double one[3] = {0, 0, 0};  // temperature, top_p, min_p
+    int32_t k = 0;
+    const void* by[4] = {nullptr, nullptr, nullptr, nullptr};  // temperature, top_p, min_p, top_k
+    for (int i = 0; i < 4; ++i) {
+      PyObject* o = v[i == 0 ? 2 : i == 1 ? 4 : i == 2 ? 5 : 3];
+      if (THPVariable_CheckExact(o)) {
+        const at::Tensor* t;
+        if (!plain(o, dev, t) || t->scalar_type() != (i == 3 ? at::kInt : at::kFloat) || !shape(*t, {B})) Py_RETURN_NONE;
+        by[i] = t->data_ptr();
+      } else if (i == 3 ? none(o) || !small(o, k) : !real64(o, one[i])) {
+        Py_RETURN_NONE;
+      }
+    }
+    void* st;
+    if (!stream_of(dev, st)) Py_RETURN_NONE;
+    const int64_t need = g_sample_ws(B, V);
+    at::Tensor tokens, shares, ws;
+    if (need > 0 && !kept_workspace(dev, st, need, ws)) return PyLong_FromLongLong(need);
+    int rc;
+    {
+      NoGil ng;
+      tokens = at::empty({B}, x.options().dtype(at::kInt));
+      shares = at::empty({B}, x.options().dtype(at::kFloat));
+      rc = g_sample(x.data_ptr(), B > 1 ? x.stride(0) : V, lt(x.scalar_type()), u->data_ptr(), by[0], by[3], by[1], by[2], one[0], k, one[1],
+                    one[2], tokens.data_ptr(), shares.data_ptr(), B, V, data_of(ws), bytes_of(ws), st);
+    }
+    if (!checked(rc)) return nullptr;
+    PyObject *o0 = THPVariable_Wrap(tokens), *o1 = THPVariable_Wrap(shares);
+    return Py_BuildValue("(NN)", o0, o1);
+  });
+}
+
+// (q, k_cache, v_cache, k_scales, v_scales, shared_pages, block_table, lengths, starts, max_new, scale, causal, window, status); an int:
+// checked, needs a workspace of that many bytes
+PyObject* kv8_shared_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  return guarded(n, 14, [&]() -> PyObject* {
+    int dev = -1;
+    Cache c;
+    const at::Tensor *q, *sp;
+    int64_t qs = 0;
+    int32_t most = 0, window = 0;
+    float scale;
+    void* st;
+    PyObject* const cache[6] = {v[1], v[2], v[3], v[4], v[6], v[7]};
+    if (!c.set(cache, v[8], v[13], dev) || !plain(v[5], dev, sp) || sp->scalar_type() != at::kInt || sp->dim() != 1 ||
+        sp->size(0) > INT32_MAX || !small(v[9], most) || !PyBool_Check(v[11]) || none(v[12]) || !small(v[12], window) ||
+        !THPVariable_CheckExact(v[0]) || THPVariable_Unpack(v[0]).dim() != 3)
+      Py_RETURN_NONE;
+    const int64_t Hq = THPVariable_Unpack(v[0]).size(1);
+    if (Hq == 0 || Hq > INT32_MAX || Hq % c.H != 0 || !token_rows(v[0], dev, Hq, c.D, q, qs) ||
+        !(q->scalar_type() == at::kHalf || q->scalar_type() == at::kBFloat16))
+      Py_RETURN_NONE;
+    if (none(v[10])) scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(c.D)));
+    else if (!real(v[10], scale)) Py_RETURN_NONE;
+    if (!stream_of(dev, st)) Py_RETURN_NONE;
+    const int32_t B = static_cast<int32_t>(c.B), W = static_cast<int32_t>(c.W), page = static_cast<int32_t>(c.page), S = static_cast<int32_t>(sp->size(0)),
+                  H = static_cast<int32_t>(c.H), D = static_cast<int32_t>(c.D), causal = v[11] == Py_True, heads = static_cast<int32_t>(Hq);
+    const int64_t need = g_shared_ws(q->size(0), most, c.starts != nullptr, B, S, W, page, heads, H, D, causal, window);
+    at::Tensor o, ws;
+    if (need > 0 && !kept_workspace(dev, st, need, ws)) return PyLong_FromLongLong(need);
+    int rc;
+    {
+      NoGil ng;
+      o = at::empty(q->sizes(), q->options());
+      rc = g_shared(q->data_ptr(), qs, o.data_ptr(), lt(q->scalar_type()), c.k->data_ptr(), c.v->data_ptr(), c.ks->data_ptr(), c.vs->data_ptr(),
+                    c.dt, sp->data_ptr(), S, c.table->data_ptr(), c.lengths->data_ptr(), c.starts, c.status, q->size(0), most, B, W, c.P, page,
+                    heads, H, D, scale, causal, window, data_of(ws), bytes_of(ws), st);
+    }
+    if (!checked(rc)) return nullptr;
+    return THPVariable_Wrap(o);
+  });
+}
+
+// (addresses of the five entry points)
+PyObject* bind_decode(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "bind_decode takes five addresses");
+    return nullptr;
+  }
+  void* f[5];
+  for (int i = 0; i < 5; ++i) {
+    f[i] = PyLong_AsVoidPtr(v[i]);
+    if (f[i] == nullptr) {
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null entry point");
+      return nullptr;
+    }
+  }
+  g_rope = reinterpret_cast<RopeFn>(f[0]);
+  g_sample_ws = reinterpret_cast<SampleWsFn>(f[1]);
+  g_sample = reinterpret_cast<SampleFn>(f[2]);
+  g_shared_ws = reinterpret_cast<SharedWsFn>(f[3]);
+  g_shared = reinterpret_cast<SharedFn>(f[4]);
+  Py_RETURN_NONE;
+}
+
 // (raw stream function, check function, addresses of the seven entry points)
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (n != 9) {
@@ -708,7 +889,8 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
 #define XRMM_FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {XRMM_FN(bind), XRMM_FN(matmul), XRMM_FN(qkv), XRMM_FN(mlp),
                           XRMM_FN(bnb4), XRMM_FN(gather), XRMM_FN(bind_lowbit), XRMM_FN(mx4_quantize),
-                          XRMM_FN(matmul_mx4), XRMM_FN(kv8_append), XRMM_FN(kv8_attention), {nullptr, nullptr, 0, nullptr}};
+                          XRMM_FN(matmul_mx4), XRMM_FN(kv8_append), XRMM_FN(kv8_attention), XRMM_FN(bind_decode),
+                          XRMM_FN(rope), XRMM_FN(sample), XRMM_FN(kv8_shared_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_xrmm_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -77,6 +77,9 @@ def _load_front():
         ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
             "xrmm_mx4_quantize", "xrmm_matmul_mx4_workspace_bytes", "xrmm_matmul_mx4", "xrmm_kv8_append",
             "xrmm_kv8_attention_workspace_bytes", "xrmm_kv8_attention")))
+    mod.bind_decode(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in (
+        "xrmm_rope", "xrmm_sample_workspace_bytes", "xrmm_sample", "xrmm_kv8_shared_attention_workspace_bytes",
+        "xrmm_kv8_shared_attention")))
     return mod
 
 
@@ -942,6 +945,11 @@ def kv8_shared_attention(q, k_cache, v_cache, k_scales, v_scales, shared_pages, 
     kv8_append's: its first n columns belong to the shared positions). Everything else is as in ``kv8_attention``. The shared
     tokens are read once for the rows of all sequences, on a workspace (``kv8_shared_attention_workspace_bytes``; under
     graph capture give one, else each sequence reads them)."""
+    if out is None and workspace is None and stream is None and _front():
+        r = _FRONT.kv8_shared_attention(q, k_cache, v_cache, k_scales, v_scales, shared_pages, block_table, lengths, starts,
+                                        max_new, scale, causal, window, status)
+        if r is not None and type(r) is not int:
+            return r
     B, P, H, page, D = _check_cache(k_cache, v_cache, k_scales, v_scales, block_table, lengths, starts, status)
     if shared_pages.dtype != torch.int32 or shared_pages.dim() != 1 or shared_pages.shape[0] >= 1 << 31:
         raise nat.XrmmInvalid("shared_pages must be int32 [pages]")
@@ -1031,6 +1039,10 @@ def rope(q, k=None, *, frequencies, positions=None, lengths=None, starts=None, m
     ``positions`` (int32 or int64 ``[T]``), or those of kv8_append's calls: the rows are each sequence's last tokens, of
     ``lengths`` (int32 ``[batch]``) and ``starts`` as there; rows that starts leave out are not written. ``out`` and ``k_out``
     may be q and k themselves (in place), or slices of a wider buffer."""
+    if out is None and k_out is None and stream is None and _front():
+        r = _FRONT.rope(q, k, frequencies, positions, lengths, starts, magnitude, interleaved, inverse)
+        if r is not None:
+            return r
     if q.dtype not in _LT or (k is not None and k.dtype != q.dtype):
         raise nat.XrmmInvalid("q and k must both be float32, float16 or bfloat16")
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
@@ -1088,6 +1100,10 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, workspa
     whole numbers (a weight is one in units of 2^-46 of the largest at 2^16 tokens), so results do not depend on how a call is spread
     over the device. Few rows are, on a workspace (``sample_workspace_bytes``; see ``matmul_nbits`` for whose it is and for
     graph capture)."""
+    if workspace is None and stream is None and _front():
+        r = _FRONT.sample(logits, u, temperature, top_k, top_p, min_p)
+        if r is not None and type(r) is not int:
+            return r
     if logits.dtype not in _LT:
         raise nat.XrmmInvalid("logits must be float32, float16 or bfloat16")
     if logits.dim() != 2 or logits.shape[1] == 0:
