@@ -521,6 +521,12 @@ int xrmm_kv8_attention(const void* q, int64_t q_stride, void* output, int32_t dt
 int64_t xrmm_kv8_shared_attention_workspace_bytes(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t shared_count,
                                                   int32_t table_width, int32_t page_size, int32_t q_heads, int32_t kv_heads,
                                                   int32_t head_dim, int32_t causal, int32_t window);
+/* How xrmm_kv8_shared_attention goes about it with a workspace: "kv8_walk" (each sequence over all of its tokens),
+ * "kv8_prefix_tile" or "kv8_prefix_rows" (the shared tokens once, in tiles of 128 rows or of 16), NULL for an invalid geometry.
+ * No device work. */
+const char* xrmm_kv8_shared_attention_kernel(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t shared_count,
+                                             int32_t table_width, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                                             int32_t head_dim, int32_t causal, int32_t window);
 int xrmm_kv8_shared_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
                               const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
                               const void* shared_pages, int32_t shared_count, const void* block_table, const void* lengths,

@@ -90,6 +90,7 @@ def _sig(lib):
     s("xrmm_kv8_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32,
       _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
     s("xrmm_kv8_shared_attention_workspace_bytes", _i64, _i64, *[_i32] * 11)
+    s("xrmm_kv8_shared_attention_kernel", ctypes.c_char_p, _i64, *[_i32] * 11)
     s("xrmm_kv8_shared_attention", ctypes.c_int, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp,
       _i64, _i32, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _vp, _i64, _vp)
     s("xrmm_rope", ctypes.c_int, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i32, _f64, _vp, _i32, _vp, _vp, _i64,

@@ -199,7 +199,12 @@ const char* kv8_kernel_name(const KvAttnArgs& a) {
   return a.c.B > 0 && a.max_new > 0 && attention_plan(a, true).tile ? "kv8_tile" : "kv8_rows";
 }
 
-hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st) { return attention_launch<KV_PLAIN>(a, st); }
+hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st) {
+  if (a.c.B == 0 || a.max_new == 0) return hipSuccess;
+  KvPlan p = attention_plan(a, a.ws != nullptr);
+  if (p.ws_bytes > a.ws_bytes) p = attention_plan(a, false);
+  return attention_with<KV_PLAIN>(a, p, st);
+}
 
 hipError_t launch_kv8_append(const KvAppendArgs& a, hipStream_t st) {
   if (a.c.B == 0 || a.max_new == 0) return hipSuccess;

@@ -9,6 +9,14 @@ namespace xrmm {
 
 int device_cus();
 
+// How a launch is laid out; see kind_plan.
+struct KvPlan {
+  bool tile;  // k_kv8_tile, else k_kv8_rows
+  int waves;  // of k_kv8_rows
+  int64_t row_tiles, splits, chunk, ws_bytes;
+  double time;
+};
+
 namespace {
 
 __device__ __forceinline__ float two(int e) { return __builtin_bit_cast(float, static_cast<uint32_t>(e + 127) << 23); }
@@ -29,13 +37,81 @@ __device__ __forceinline__ float two(int e) { return __builtin_bit_cast(float, s
 
 constexpr int KVT = 32;      // tokens of a step
 
-// What a launch walks over: each sequence's own table, or a table whose first pages are the batch's.
-enum KvMode { KV_PLAIN, KV_WALK };
+// What a launch walks over. KV_PLAIN: each sequence's table. With shared pages: KV_WALK, a sequence's rows over the shared pages and its
+// own; KV_PREFIX, the rows of all sequences, as of one, over the shared pages; KV_OWN, a sequence's rows over its own pages
+// alone. The last two leave parts in the workspace, which k_kv8_join joins.
+enum KvMode { KV_PLAIN, KV_WALK, KV_PREFIX, KV_OWN };
+
+constexpr bool kv_parts(KvMode m) { return m == KV_PREFIX || m == KV_OWN; }
 
 // Pages that a sequence's tokens can lie in.
 template <KvMode MODE>
 __device__ __forceinline__ int kv_span(const KvAttnArgs& a) {
   return MODE == KV_PLAIN || a.c.width > a.shared_pages ? a.c.width : a.shared_pages;
+}
+
+// A row's part: unnormalised outputs [D] and (maximum, sum), by part, key head and row of the head.
+template <int D>
+struct KvPart {
+  float* o;
+  f32x2* ml;
+  int64_t row0;  // of the key head
+  __device__ __forceinline__ KvPart(const KvAttnArgs& a, int part, int h) {
+    const int64_t rows = a.c.rows * a.Hq;
+    float* base = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + a.parts_at);
+    row0 = static_cast<int64_t>(h) * (a.c.rows * (a.Hq / a.c.Hkv));
+    o = base + (part * rows + row0) * D;
+    ml = reinterpret_cast<f32x2*>(base + a.parts * rows * D) + part * rows + row0;
+  }
+};
+
+// Sequence and position of a row of the call's tensors: false where `starts` puts it in none. By halving, as few calls need it.
+__device__ __forceinline__ bool kv_position(const KvAttnArgs& a, int row, int& b, int& pos) {
+  const KvCache& c = a.c;
+  if (c.starts == nullptr) b = row / c.each;
+  else {
+    int lo = 0, hi = c.B;  // the first sequence that ends behind the row
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (c.starts[mid + 1] <= row) lo = mid + 1;
+      else hi = mid;
+    }
+    b = lo;
+    if (b >= c.B) return false;
+  }
+  int first, count;
+  if (!kv_rows(c, b, a.max_new, first, count) || row < first || row >= first + count) return false;
+  const int all = c.lengths[b] > 0 ? c.lengths[b] : 0;
+  pos = all - count + (row - first);
+  return true;
+}
+
+// The shared tokens that a row sees.
+struct KvSeen {
+  int lo, hi;
+};
+__device__ __forceinline__ KvSeen kv_shared_seen(const KvAttnArgs& a, int tokens, int row) {
+  int b, pos;
+  if (!kv_position(a, row, b, pos)) return {0, 0};
+  const int len = a.c.lengths[b] < tokens ? (a.c.lengths[b] > 0 ? a.c.lengths[b] : 0) : tokens;
+  KvSeen s;
+  s.hi = a.causal && pos + 1 < len ? (pos + 1 > 0 ? pos + 1 : 0) : len;
+  s.lo = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
+  if (s.lo >= s.hi) s.lo = s.hi = 0;
+  return s;
+}
+
+// Whether all rows of all sequences see all of the shared tokens, as they do unless a sequence ends among them or a window begins
+// there. All threads of the workgroup.
+__device__ __forceinline__ bool kv_all_seen(const KvAttnArgs& a, int tokens) {
+  int ok = 1;
+  for (int b = threadIdx.x; b < a.c.B; b += blockDim.x) {
+    int first, count;
+    if (!kv_rows(a.c, b, a.max_new, first, count) || count == 0) continue;
+    const int len = a.c.lengths[b];
+    if (len < tokens || (a.causal && static_cast<int64_t>(len) - count + 1 < tokens) || (a.window > 0 && len > a.window)) ok = 0;
+  }
+  return __syncthreads_and(ok) != 0;
 }
 
 template <KvMode MODE>
@@ -151,27 +227,67 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   const uint32_t bh = unit / row_tiles;
   const int h = static_cast<int>(bh % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(bh / static_cast<uint32_t>(c.Hkv));
   const int G = a.Hq / c.Hkv;
-  int first, count;
-  if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  int first, count, past, len;
+  const int tokens = a.shared_pages << c.page_log2;  // the shared ones
+  bool whole = true;                                 // KV_PREFIX: all rows see all of them
+  if constexpr (MODE == KV_PREFIX) {
+    first = 0;
+    count = static_cast<int>(c.rows);
+    past = len = tokens;
+    whole = kv_all_seen(a, tokens);
+  } else {
+    if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  }
   const int nrows = count * G, r0 = tile * 16;
   if (r0 >= nrows) return;
-  // positions past the table are left out: the walk over tokens ends with the table
-  const int span = kv_span<MODE>(a) << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0, past = all - count;
-  const int len = all < span ? all : span;
-  if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  if constexpr (MODE != KV_PREFIX) {
+    // positions past the table are left out: the walk over tokens ends with the table
+    const int span = kv_span<MODE>(a) << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0;
+    past = all - count;
+    len = all < span ? all : span;
+    if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  }
 
   // the tokens that any of the rows sees, and those that all of them see
   const int last = r0 + 16 < nrows ? r0 + 15 : nrows - 1, i0 = r0 / G, i1 = last / G;
-  auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
-  auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
-  const int hi_all = row_hi(i1), lo_all = (row_lo(i0) < hi_all ? row_lo(i0) : hi_all) / KVT * KVT, full_lo = row_lo(i1), full_hi = row_hi(i0);
+  auto row_hi = [&](int i) { return MODE == KV_PREFIX ? tokens : a.causal && past + i + 1 < len ? past + i + 1 : len; };
+  auto row_lo = [&](int i) {  // no difference below -2^31
+    const int lo = MODE != KV_PREFIX && a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0;
+    return MODE == KV_OWN && lo < tokens ? tokens : lo;
+  };
+  int hi_all = row_hi(i1), low = row_lo(i0), full_lo = row_lo(i1), full_hi = row_hi(i0);
+  KvSeen sees{0, tokens};
+  if constexpr (MODE == KV_PREFIX) {
+    if (!whole) {
+      sees = kv_shared_seen(a, tokens, (r0 + col < nrows ? r0 + col : nrows - 1) / G);
+      int top = sees.hi, bottom = sees.hi > 0 ? sees.lo : tokens, most = sees.lo, least = sees.hi;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        top = max(top, __shfl_xor(top, o, 64));
+        bottom = min(bottom, __shfl_xor(bottom, o, 64));
+        most = max(most, __shfl_xor(most, o, 64));
+        least = min(least, __shfl_xor(least, o, 64));
+      }
+      hi_all = __builtin_amdgcn_readfirstlane(top);
+      low = __builtin_amdgcn_readfirstlane(bottom);
+      full_lo = __builtin_amdgcn_readfirstlane(most);
+      full_hi = __builtin_amdgcn_readfirstlane(least);
+    }
+  }
+  const int lo_all = (low < hi_all ? low : hi_all) / KVT * KVT;
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;  // at most `splits`
-  if (split >= parts) return;
+  if (split >= parts) {
+    if constexpr (kv_parts(MODE)) {
+      const KvPart<D> part(a, a.part0 + static_cast<int>(split), h);
+      if (tid < 16 && r0 + tid < nrows) part.ml[static_cast<int64_t>(first) * G + r0 + tid] = f32x2{-__builtin_inff(), 0.f};
+    }
+    return;
+  }
   const int tlo = lo_all + static_cast<int>(split * chunk);
   const int thi = splits > 1 && split + 1 < parts ? tlo + static_cast<int>(chunk) : hi_all;
 
   // the first token that a row sees: pages wholly before it may be gone (no branch around the lookup: it would be waited for)
-  const int seen = row_lo(i0);
+  const int seen = low;
   auto find = [&](uint32_t t0, int32_t (&pg)[2]) {
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
@@ -210,8 +326,8 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
     const bool ok = r < nrows;
     const int rr = ok ? r : nrows - 1, i = rr / G, hq = h * G + rr % G;
     const int64_t at = (first + i) * a.q_stride + static_cast<int64_t>(hq) * D + g * KD;
-    hi = ok ? row_hi(i) : 0;
-    lo = row_lo(i);
+    hi = !ok ? 0 : MODE == KV_PREFIX ? sees.hi : row_hi(i);
+    lo = MODE == KV_PREFIX ? sees.lo : row_lo(i);
     // at any element's address; rows past the last read its row and see nothing
     typedef f16x8 f16x8_2 __attribute__((aligned(2)));
     const f16* src = static_cast<const f16*>(a.q) + at;
@@ -396,6 +512,15 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   }
   __syncthreads();
   const int rows = nrows - r0 < 16 ? nrows - r0 : 16, pieces = rows * (D / 4);  // pieces of four values
+  if constexpr (kv_parts(MODE)) {
+    const KvPart<D> part(a, a.part0 + static_cast<int>(split), h);
+    const int64_t at = static_cast<int64_t>(first) * G + r0;
+#pragma unroll 1
+    for (int p = tid; p < pieces; p += 64 * W)
+      reinterpret_cast<f32x4*>(part.o + at * D)[p] = *reinterpret_cast<const f32x4*>(&row[p / (D / 4)][p % (D / 4) * 4]);
+    if (tid < rows) part.ml[at + tid] = f32x2{rm[tid], rl[tid]};
+    return;
+  }
   auto put = [&](int p, f32x4 v, float lsum) {
     const int r = r0 + p / (D / 4);
     const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
@@ -530,31 +655,84 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   const KvCache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t nbh = static_cast<uint32_t>(c.Hkv) * static_cast<uint32_t>(c.B), bh = blockIdx.x % nbh, rest = blockIdx.x / nbh;
+  const uint32_t nbh = MODE == KV_PREFIX ? static_cast<uint32_t>(c.Hkv) : static_cast<uint32_t>(c.Hkv) * static_cast<uint32_t>(c.B), bh = blockIdx.x % nbh, rest = blockIdx.x / nbh;
   const uint32_t split = rest % splits;
   const int tile = static_cast<int>(row_tiles - 1 - rest / splits);
   const uint32_t unit = bh * row_tiles + static_cast<uint32_t>(tile);
   const int h = static_cast<int>(bh % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(bh / static_cast<uint32_t>(c.Hkv));
   const int G = a.Hq / c.Hkv;
-  int first, count;
-  if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  int first, count, past, len;
+  const int tokens = a.shared_pages << c.page_log2;  // the shared ones
+  bool whole = true;                                 // KV_PREFIX: all rows see all of them
+  if constexpr (MODE == KV_PREFIX) {
+    first = 0;
+    count = static_cast<int>(c.rows);
+    past = len = tokens;
+    whole = kv_all_seen(a, tokens);
+  } else {
+    if (!kv_rows(c, b, a.max_new, first, count) && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  }
   const int nrows = count * G, r0 = tile * KVM_ROWS;
   if (r0 >= nrows) return;
-  const int span = kv_span<MODE>(a) << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0, past = all - count;
-  const int len = all < span ? all : span;
-  if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
-  auto row_hi = [&](int i) { return a.causal && past + i + 1 < len ? past + i + 1 : len; };
-  auto row_lo = [&](int i) { return a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0; };  // no difference below -2^31
+  if constexpr (MODE != KV_PREFIX) {
+    const int span = kv_span<MODE>(a) << c.page_log2, all = c.lengths[b] > 0 ? c.lengths[b] : 0;
+    past = all - count;
+    len = all < span ? all : span;
+    if (all > span && tid == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
+  }
+  auto row_hi = [&](int i) { return MODE == KV_PREFIX ? tokens : a.causal && past + i + 1 < len ? past + i + 1 : len; };
+  auto row_lo = [&](int i) {  // no difference below -2^31
+    const int lo = MODE != KV_PREFIX && a.window > 0 && past + i + 1 > a.window ? past + i + 1 - a.window : 0;
+    return MODE == KV_OWN && lo < tokens ? tokens : lo;
+  };
   auto query = [&](int r) { return (r < nrows ? r : nrows - 1) / G; };  // of a row, the last one's past the end
-  const int hi_all = row_hi(query(r0 + KVM_ROWS - 1)), lo_all = (row_lo(query(r0)) < hi_all ? row_lo(query(r0)) : hi_all) / TT * TT;
+  int hi_all = row_hi(query(r0 + KVM_ROWS - 1)), low = row_lo(query(r0));
+  const int w0 = r0 + 32 * wave;  // this wave's first row
+  KvSeen sees{0, tokens};
+  int w_top = tokens, w_bottom = 0, w_most = 0, w_least = tokens;  // KV_PREFIX: the largest and least hi and lo of the wave's rows
+  if constexpr (MODE == KV_PREFIX) {
+    if (!whole) {
+      int top = 0, bottom = tokens;
+#pragma unroll 1
+      for (int e = 0; e < KVM_ROWS; e += 64) {
+        const KvSeen s = kv_shared_seen(a, tokens, query(r0 + e + lane));
+        top = max(top, s.hi);
+        bottom = min(bottom, s.hi > 0 ? s.lo : tokens);
+      }
+      sees = kv_shared_seen(a, tokens, query(w0 + col));
+      int wt = sees.hi, wb = sees.hi > 0 ? sees.lo : tokens, wm = sees.lo, wl = sees.hi;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        top = max(top, __shfl_xor(top, o, 64));
+        bottom = min(bottom, __shfl_xor(bottom, o, 64));
+        wt = max(wt, __shfl_xor(wt, o, 64));
+        wb = min(wb, __shfl_xor(wb, o, 64));
+        wm = max(wm, __shfl_xor(wm, o, 64));
+        wl = min(wl, __shfl_xor(wl, o, 64));
+      }
+      hi_all = __builtin_amdgcn_readfirstlane(top);
+      low = __builtin_amdgcn_readfirstlane(bottom);
+      w_top = __builtin_amdgcn_readfirstlane(wt);
+      w_bottom = __builtin_amdgcn_readfirstlane(wb);
+      w_most = __builtin_amdgcn_readfirstlane(wm);
+      w_least = __builtin_amdgcn_readfirstlane(wl);
+    }
+  }
+  const int lo_all = (low < hi_all ? low : hi_all) / TT * TT;
   const uint32_t parts = hi_all > lo_all ? (static_cast<uint32_t>(hi_all - lo_all) + chunk - 1) / chunk : 1u;
-  if (split >= parts) return;
+  if (split >= parts) {
+    if constexpr (kv_parts(MODE)) {
+      const KvPart<D> part(a, a.part0 + static_cast<int>(split), h);
+      if (tid < KVM_ROWS && r0 + tid < nrows) part.ml[static_cast<int64_t>(first) * G + r0 + tid] = f32x2{-__builtin_inff(), 0.f};
+    }
+    return;
+  }
   const int tlo = lo_all + static_cast<int>(split * chunk);
   const int thi = splits > 1 && split + 1 < parts ? tlo + static_cast<int>(chunk) : hi_all;
   // this wave's rows: the tokens that any sees, and those that all see
-  const int w0 = r0 + 32 * wave;
-  const bool live = w0 < nrows;
-  const int wlo = row_lo(query(w0)), whi = live ? row_hi(query(w0 + 31)) : 0, full_lo = row_lo(query(w0 + 31)), full_hi = row_hi(query(w0));
+  const bool live = w0 < nrows, pre = MODE == KV_PREFIX;
+  const int wlo = pre ? w_bottom : row_lo(query(w0)), whi = !live ? 0 : pre ? w_top : row_hi(query(w0 + 31));
+  const int full_lo = pre ? w_most : row_lo(query(w0 + 31)), full_hi = pre ? w_least : row_hi(query(w0));
 
   // ---- moving a tile: K pieces of 16 codes of a token, V pieces of four tokens by eight d
   // Everything of a tile is loaded together, from pages looked up a tile before. Lane l looks up the page of the 16 tokens
@@ -564,7 +742,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   float scn;                   // this lane's scale of the loaded tile
   uint32_t none_n = 0;         // the loaded tile's 16-token groups in no page, a bit each
   bool bad = false;
-  const int lg = lane & (GR - 1), seen = row_lo(query(r0));  // the first token that a row sees: pages wholly before it may be gone
+  const int lg = lane & (GR - 1), seen = low;  // the first token that a row sees: pages wholly before it may be gone
   auto find = [&](int t0) {
     const int t = t0 + 16 * lg;
     const int32_t p = kv_page_of<MODE>(a, b, t);
@@ -665,8 +843,8 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     const int i = query(r), hq = h * G + (ok ? r % G : 0);
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (first + i) * a.q_stride + static_cast<int64_t>(hq) * D + 8 * hf;
     const bool whole = ((reinterpret_cast<uintptr_t>(a.q) | static_cast<uintptr_t>(a.q_stride * 2)) & 15u) == 0;
-    hi = ok ? row_hi(i) : 0;
-    lo = row_lo(i);
+    hi = !ok ? 0 : MODE == KV_PREFIX ? sees.hi : row_hi(i);
+    lo = MODE == KV_PREFIX ? sees.lo : row_lo(i);
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) {
       u32x4 v = {0u, 0u, 0u, 0u};
@@ -904,6 +1082,21 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   if (__any(bad) && lane == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   l += __shfl_xor(l, 32, 64);
+  if constexpr (kv_parts(MODE)) {
+    const KvPart<D> part(a, a.part0 + static_cast<int>(split), h);
+    const int64_t at = static_cast<int64_t>(first) * G + r;
+    if (r < nrows) {
+      f32x4* to = reinterpret_cast<f32x4*>(part.o + at * D + 4 * hf);
+#pragma unroll
+      for (int j = 0; j < JT; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          to[8 * j + 2 * y] = f32x4{kv_shift(o[j][4 * y], ve - KV_PE), kv_shift(o[j][4 * y + 1], ve - KV_PE), kv_shift(o[j][4 * y + 2], ve - KV_PE),
+                                    kv_shift(o[j][4 * y + 3], ve - KV_PE)};
+      if (hf == 0) part.ml[at] = f32x2{m, l};
+    }
+    return;
+  }
   if (parts > 1) {
     constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
     constexpr uint32_t PART = static_cast<uint32_t>(Ti::PART), ML = KVM_ROWS * D * 4;
@@ -1003,13 +1196,6 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
 //         waves in use; a join 3 and 2 a part (its parts of 128 rows are read one after the other)
 // 8 to 32 new tokens on 30000 with four heads a group: 41 to 79 us by rows, 89 to 184 by tiles; 32 sequences with 16 and 32 on 1000:
 // 89 and 172 by rows, 43 and 56 by tiles.
-struct KvPlan {
-  bool tile;  // k_kv8_tile, else k_kv8_rows
-  int waves;  // of k_kv8_rows
-  int64_t row_tiles, splits, chunk, ws_bytes;
-  double time;
-};
-
 KvPlan kind_plan(const KvAttnArgs& a, bool have_ws, bool tile) {
   const int64_t nrows = static_cast<int64_t>(a.max_new) * (a.Hq / a.c.Hkv), cus = device_cus() > 0 ? device_cus() : 256;
   const int64_t rows = tile ? KVM_ROWS : 16;
@@ -1057,7 +1243,7 @@ KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
 
 template <int D, bool FP8, KvMode MODE>
 hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
-  const int64_t n = p.row_tiles * p.splits * a.c.Hkv * a.c.B;
+  const int64_t n = p.row_tiles * p.splits * a.c.Hkv * (MODE == KV_PREFIX ? 1 : a.c.B);
   if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
   const uint32_t rt = static_cast<uint32_t>(p.row_tiles), sp = static_cast<uint32_t>(p.splits), ch = static_cast<uint32_t>(p.chunk);
@@ -1084,10 +1270,7 @@ hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
 }
 
 template <KvMode MODE>
-hipError_t attention_launch(const KvAttnArgs& a, hipStream_t st) {
-  if (a.c.B == 0 || a.max_new == 0) return hipSuccess;
-  KvPlan p = attention_plan(a, a.ws != nullptr);
-  if (p.ws_bytes > a.ws_bytes) p = attention_plan(a, false);
+hipError_t attention_with(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
   switch (a.c.D * 2 + (a.c.fp8 ? 1 : 0)) {
     case 128: return attention_for<64, false, MODE>(a, p, st);
     case 129: return attention_for<64, true, MODE>(a, p, st);

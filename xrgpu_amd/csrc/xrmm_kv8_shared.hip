@@ -3,10 +3,152 @@
 
 namespace xrmm {
 
-int64_t kv8_shared_workspace_bytes(const KvAttnArgs& a) {
-  return a.c.B == 0 || a.max_new == 0 ? 0 : attention_plan(a, true).ws_bytes;
+hipError_t launch_kv8_walk(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
+hipError_t launch_kv8_prefix(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
+hipError_t launch_kv8_own(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
+
+namespace {
+
+// The parts of a row: weights exp2(maximum - the largest maximum), outputs added in the parts' order, divided by the sum. A thread has
+// four values of a row, and the loads of eight parts in flight. Rows that `starts` leaves out are not written.
+constexpr int KVJ_T = 256;
+
+template <int D>
+__global__ __launch_bounds__(KVJ_T) void k_kv8_join(KvAttnArgs a) {
+  const int64_t rows = a.c.rows * a.Hq, piece = static_cast<int64_t>(blockIdx.x) * KVJ_T + threadIdx.x;
+  const int64_t out = piece / (D / 4);  // [row][head]
+  const int d = static_cast<int>(piece % (D / 4)) * 4;
+  if (out >= rows) return;
+  const int row = static_cast<int>(out / a.Hq), hq = static_cast<int>(out % a.Hq), G = a.Hq / a.c.Hkv, h = hq / G;
+  int b, pos;
+  if (!kv_position(a, row, b, pos)) return;
+  const int64_t at = static_cast<int64_t>(row) * G + hq % G;
+  const KvPart<D> part(a, 0, h);
+  float m = -__builtin_inff(), l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 8;
+#pragma unroll 1
+  for (int p0 = 0; p0 < a.parts; p0 += N) {
+    f32x4 x[N];
+    f32x2 ml[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int64_t p = (p0 + i < a.parts ? p0 + i : p0) * rows + at;
+      ml[i] = part.ml[p];
+      x[i] = *reinterpret_cast<const f32x4*>(part.o + p * D + d);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (p0 + i >= a.parts || ml[i][0] == -__builtin_inff()) continue;  // no such part, or one that saw nothing and left no outputs
+      const float mn = fmaxf(m, ml[i][0]), f0 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[i][0] - mn);
+      o = o * f0 + x[i] * f1;
+      l = l * f0 + ml[i][1] * f1;
+      m = mn;
+    }
+  }
+  o *= l != 0.f ? 1.f / l : 0.f;
+  typedef u32x2 u32x2_2 __attribute__((aligned(2)));
+  *reinterpret_cast<u32x2_2*>(static_cast<uint16_t*>(a.o) + out * D + d) =
+      a.dtype == LT_F16 ? __builtin_bit_cast(u32x2, __builtin_convertvector(o, f16x4)) : __builtin_bit_cast(u32x2, __builtin_convertvector(o, bf16x4));
 }
 
-hipError_t launch_kv8_shared_attention(const KvAttnArgs& a, hipStream_t st) { return attention_launch<KV_WALK>(a, st); }
+hipError_t launch_join(const KvAttnArgs& a, hipStream_t st) {
+  const int64_t n = (a.c.rows * a.Hq * (a.c.D / 4) + KVJ_T - 1) / KVJ_T;
+  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<uint32_t>(n));
+  switch (a.c.D) {
+    case 64: k_kv8_join<64><<<grid, KVJ_T, 0, st>>>(a); break;
+    case 96: k_kv8_join<96><<<grid, KVJ_T, 0, st>>>(a); break;
+    case 128: k_kv8_join<128><<<grid, KVJ_T, 0, st>>>(a); break;
+    default: k_kv8_join<256><<<grid, KVJ_T, 0, st>>>(a);
+  }
+  return hipGetLastError();
+}
+
+// A launch that leaves parts: nrows rows of each of `seqs` sequences over `span` tokens, by the times of kind_plan and the bytes of its parts,
+// written and read at 4 TB/s.
+KvPlan part_plan(const KvAttnArgs& a, int64_t nrows, int64_t seqs, int64_t span, bool tile) {
+  const int64_t cus = device_cus() > 0 ? device_cus() : 256, rows = tile ? KVM_ROWS : 16;
+  KvPlan p{};
+  p.tile = tile;
+  p.row_tiles = (nrows + rows - 1) / rows;
+  const int64_t units = p.row_tiles * a.c.Hkv * seqs, room = tile && a.c.D <= 128 ? 2 * cus : cus;
+  const int live = nrows < KVM_ROWS ? static_cast<int>((nrows + 31) / 32) : 4;
+  static constexpr double kTile[5] = {0, 36, 28, 24, 18};
+  const double rate = tile ? kTile[live] : 75.0, start = tile ? 10.0 : 7.0, wide = a.c.D > 128 ? 2.0 : 1.0;
+  const double part = 2.0 * static_cast<double>(nrows * seqs * a.c.Hkv) * (a.c.D + 2) * 4 / 4e6;  // us
+  span = span > 0 ? span : 1;
+  int64_t most = units < room ? room / units : 1;
+  most = most < 64 ? most : 64;
+  for (int64_t want = 1; want <= most; ++want) {
+    const int64_t chunk = want > 1 ? ((span + want - 1) / want + KVR_PASS - 1) / KVR_PASS * KVR_PASS : (span + KVR_PASS - 1) / KVR_PASS * KVR_PASS;
+    const int64_t parts = (span + chunk - 1) / chunk;
+    const double time = static_cast<double>((units * parts + room - 1) / room) * (start + wide * static_cast<double>(chunk) / rate) + part * static_cast<double>(parts);
+    if (p.splits == 0 || time < p.time) {
+      p.splits = parts;
+      p.chunk = chunk;
+      p.time = time;
+    }
+  }
+  p.waves = p.chunk <= 2 * KVT ? 2 : p.chunk <= 8 * KVT || (p.chunk <= 2048 && units * p.splits > cus) ? 4 : 8;
+  return p;
+}
+
+struct SharedPlan {
+  bool walk;  // the sequences one by one, over all of their tokens
+  KvPlan all, prefix, own;
+  int64_t ws_bytes;
+};
+
+SharedPlan shared_plan(const KvAttnArgs& a, bool have_ws) {
+  SharedPlan s{};
+  const int64_t G = a.Hq / a.c.Hkv, tokens = static_cast<int64_t>(a.shared_pages) << a.c.page_log2;
+  // the walk begins at a multiple of a tile's tokens before the sequences' own
+  const int64_t own = 64 + (a.c.width > a.shared_pages ? static_cast<int64_t>(a.c.width - a.shared_pages) << a.c.page_log2 : 0);
+  s.walk = true;
+  s.all = attention_plan(a, have_ws);
+  s.ws_bytes = s.all.ws_bytes;
+  if (!have_ws || tokens == 0 || a.c.B < 2 || a.c.rows * G > 0x7FFFFFF0) return s;
+  auto least = [&](int64_t nrows, int64_t seqs, int64_t span) {
+    const KvPlan x = part_plan(a, nrows, seqs, span, false);
+    if (nrows <= 16) return x;
+    const KvPlan y = part_plan(a, nrows, seqs, span, true);
+    return y.time < x.time ? y : x;
+  };
+  s.prefix = least(a.c.rows * G, 1, tokens);
+  s.own = least(static_cast<int64_t>(a.max_new) * G, a.c.B, own);
+  if (s.prefix.time + s.own.time + 4.0 < s.all.time) {
+    s.walk = false;
+    s.ws_bytes = KV_COUNTERS + (s.prefix.splits + s.own.splits) * a.c.rows * a.Hq * (a.c.D + 2) * 4;
+  }
+  return s;
+}
+
+}  // namespace
+
+int64_t kv8_shared_workspace_bytes(const KvAttnArgs& a) {
+  return a.c.B == 0 || a.max_new == 0 ? 0 : shared_plan(a, true).ws_bytes;
+}
+
+const char* kv8_shared_kernel_name(const KvAttnArgs& a) {
+  if (a.c.B == 0 || a.max_new == 0) return "kv8_walk";
+  const SharedPlan p = shared_plan(a, true);
+  return p.walk ? "kv8_walk" : p.prefix.tile ? "kv8_prefix_tile" : "kv8_prefix_rows";
+}
+
+hipError_t launch_kv8_shared_attention(const KvAttnArgs& a, hipStream_t st) {
+  if (a.c.B == 0 || a.max_new == 0) return hipSuccess;
+  SharedPlan p = shared_plan(a, a.ws != nullptr);
+  if (p.ws_bytes > a.ws_bytes) p = shared_plan(a, false);
+  if (p.walk) return launch_kv8_walk(a, p.all, st);
+  KvAttnArgs x = a;
+  x.parts = static_cast<int32_t>(p.prefix.splits + p.own.splits);
+  x.parts_at = KV_COUNTERS;
+  x.part0 = 0;
+  hipError_t e = launch_kv8_prefix(x, p.prefix, st);
+  x.part0 = static_cast<int32_t>(p.prefix.splits);
+  if (e == hipSuccess) e = launch_kv8_own(x, p.own, st);
+  return e == hipSuccess ? launch_join(x, st) : e;
+}
 
 }  // namespace xrmm

@@ -76,6 +76,8 @@ struct KvAttnArgs {
   int dtype;                   // LT_F16 / LT_BF16
   const int32_t* shared;       // pages of every sequence's first tokens (kv8_shared_attention), else null
   int32_t shared_pages;
+  int32_t parts, part0;        // parts of a row in the workspace, and the first of a launch's own
+  int64_t parts_at;            // where they begin
 };
 
 hipError_t launch_kv8_append(const KvAppendArgs& a, hipStream_t st);
@@ -84,6 +86,7 @@ int64_t kv8_workspace_bytes(const KvAttnArgs& a);
 const char* kv8_kernel_name(const KvAttnArgs& a);
 hipError_t launch_kv8_shared_attention(const KvAttnArgs& a, hipStream_t st);
 int64_t kv8_shared_workspace_bytes(const KvAttnArgs& a);
+const char* kv8_shared_kernel_name(const KvAttnArgs& a);
 
 hipError_t launch_mx4_quantize(const MxQuantArgs& a, hipStream_t st);
 hipError_t launch_matmul_mx4(const MxArgs& a, hipStream_t st);

@@ -287,6 +287,18 @@ int64_t xrmm_kv8_shared_attention_workspace_bytes(int64_t rows, int32_t max_new,
   return rc ? 0 : xrmm::kv8_shared_workspace_bytes(a);
 }
 
+const char* xrmm_kv8_shared_attention_kernel(int64_t rows, int32_t max_new, int32_t ragged, int32_t batch, int32_t shared_count,
+                                             int32_t table_width, int32_t page_size, int32_t q_heads, int32_t kv_heads,
+                                             int32_t head_dim, int32_t causal, int32_t window) {
+  static const int32_t probe[1] = {};
+  xrmm::KvAttnArgs a;
+  if (attention_geometry(a, rows, max_new, ragged, batch, table_width, page_size, q_heads, kv_heads, head_dim, causal, window) ||
+      shared_of(a, probe, shared_count))
+    return nullptr;
+  set_status(XRMM_OK, "");
+  return xrmm::kv8_shared_kernel_name(a);
+}
+
 int xrmm_kv8_shared_attention(const void* q, int64_t q_stride, void* output, int32_t dtype, const void* k_cache,
                               const void* v_cache, const void* k_scales, const void* v_scales, int32_t cache_dtype,
                               const void* shared_pages, int32_t shared_count, const void* block_table, const void* lengths,

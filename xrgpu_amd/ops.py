@@ -986,6 +986,18 @@ def kv8_shared_attention_workspace_bytes(T, q_heads, kv_heads, head_dim, *, batc
         int(kv_heads), int(head_dim), int(causal), _i32(window)))
 
 
+def kv8_shared_attention_kernel(T, q_heads, kv_heads, head_dim, *, batch, shared_pages, table_width, page_size, max_new=0,
+                                ragged=False, causal=True, window=0) -> str:
+    """How a kv8_shared_attention call goes with a workspace: "kv8_walk" (each sequence over all of its tokens),
+    "kv8_prefix_tile" or "kv8_prefix_rows" (the shared tokens once)."""
+    r = nat.lib().xrmm_kv8_shared_attention_kernel(
+        int(T), _i32(max_new), int(ragged), int(batch), _i32(shared_pages), int(table_width), int(page_size), int(q_heads),
+        int(kv_heads), int(head_dim), int(causal), _i32(window))
+    if r is None:
+        raise nat.XrmmInvalid(nat.last_error())
+    return r.decode()
+
+
 def rope_frequencies(rotary_dim, theta=10000.0, *, scaling=None, factor=1.0, original_length=None, low=1.0, high=None,
                      device="cuda"):
     """The float64 frequencies ``[rotary_dim / 2]`` of ``rope``, and the magnitude that belongs to them: ``(frequencies, magnitude)``.
