@@ -925,6 +925,105 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
       __syncthreads();
       continue;
     }
+    auto of = [&](float x, int u) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), u)); };
+    if constexpr (MODE != KV_PLAIN) {
+      // Tiles that all rows of the wave see, with factors of the usual kind, as nearly all of a long shared part: the steps below without
+      // their masks and choices, in one piece of code that the products and the softmax's instructions share.
+      const bool all_usual = (__ballot(!((lane & GR) != 0 ? scl >= 0x1p-60f && scl < 0x1p60f : scl >= 0.f && a.scale >= 0.f)) & ((1u << (2 * GR)) - 1u)) == 0;
+      if (__builtin_amdgcn_readfirstlane(static_cast<int>(all_usual && none == 0 && t0 >= full_lo && t0 + TT <= full_hi))) {
+        const float sc = scl;
+        int top_e = KV_NONE, low_e = -KV_NONE;
+        {
+          const int el = kv_scale_exp(sc);
+#pragma unroll
+          for (int u = 0; u < GR; ++u) {
+            const int e = __builtin_amdgcn_readlane(el, GR + u);
+            top_e = e > top_e ? e : top_e;
+            low_e = e < low_e ? e : low_e;
+          }
+        }
+        if (low_e + 19 > (top_e > most ? top_e : most)) {  // factors from 2^-8 of the largest on, as `usual` below
+          const int was = ve;
+          if (top_e > least) {
+            ve = top_e > ve ? top_e : ve;
+            least = top_e;
+            most = top_e > most ? top_e : most;
+            up = static_cast<float>(most - ve);
+            down = kv_shift(1.f, ve - most);
+          }
+          f32x16 s[TT / 32];
+          constexpr int KA = D > 128 ? 4 : 2;
+          auto kfrag = [&](int x, int u) { return *reinterpret_cast<const f16x8*>(ks + (32 * u + col) * Ti::KP + kv_kslot(col, 2 * x + hf) * 16); };
+          f16x8 kf[KA][TT / 32];
+#pragma unroll
+          for (int x = 0; x < KA; ++x)
+#pragma unroll
+            for (int u = 0; u < TT / 32; ++u) kf[x][u] = kfrag(x, u);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int x = 0; x < D / 16; ++x) {
+#pragma unroll
+            for (int u = 0; u < TT / 32; ++u) {
+              s[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[x % KA][u], q[x], x == 0 ? f32x16{} : s[u], 0, 0, 0);
+              if (x + KA < D / 16) kf[x % KA][u] = kfrag(x + KA, u);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          const float wl = kv_shift(sc, KV_PE - most), lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
+          move();
+          float top = -__builtin_inff();
+#pragma unroll
+          for (int u = 0; u < GR; ++u) {
+            float x = s[u / 2][8 * (u & 1)];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) x = fmaxf(x, s[u / 2][8 * (u & 1) + e]);
+            top = fmaxf(top, x * (qs * of(sc, u)));
+          }
+          {
+            const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, top), false, false);
+            top = fmaxf(__builtin_bit_cast(float, both[0]), __builtin_bit_cast(float, both[1]));
+          }
+          if (__any(top > m + KV_LAG || was < ve)) {
+            const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - base);
+            m = mn;
+            l *= f;
+            const float fo = kv_shift(f, was - ve);
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[j][e] *= fo;
+          }
+          const float rise = up - (m == -__builtin_inff() ? 0.f : m);
+          float sums = 0.f;
+#pragma unroll
+          for (int gu = 0; gu < GR; ++gu) {
+            f16x8 pf;
+            const float kfac = qs * of(sc, gu), lw = of(lwl, GR + gu) + rise;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[gu / 2][8 * (gu & 1) + e], kfac, lw));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[gu / 2][8 * (gu & 1) + e + 1], kfac, lw));
+              sum += p0 + p1;
+              const f16x2 h2 = __builtin_convertvector((f32x2{p0, p1}), f16x2);
+              pf[e] = h2[0];
+              pf[e + 1] = h2[1];
+            }
+            sums += sum * of(rwl, GR + gu);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) {
+              const int d = 32 * j + col;
+              const f16x8 vf = *reinterpret_cast<const f16x8*>(vs + d * Ti::VP + kv_vslot<D>(d, gu * 2 + hf) * 16);
+              o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
+            }
+          }
+          l += sums * down;
+          __syncthreads();
+          continue;
+        }
+      }
+    }
     const uint32_t no = none;
     const float sc = scl;
     const int was = ve;
@@ -984,8 +1083,7 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
     const float wl = kv_shift(sc, KV_PE - most), lwl = __builtin_amdgcn_logf(wl), rwl = __builtin_amdgcn_rcpf(wl);
     // factors of the usual kind, no masks: see below
     const bool usual = (lane & GR) != 0 ? wl >= 0x1p-8f && wl < 0x1p11f : sc >= 0.f && a.scale >= 0.f;
-    const bool plain = (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && open;
-    auto of = [&](float x, int u) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), u)); };
+    const bool plain = MODE == KV_PLAIN && (__ballot(!usual) & ((1u << (2 * GR)) - 1u)) == 0 && open;
     move();
     {
       float top = -__builtin_inff();
