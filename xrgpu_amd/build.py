@@ -62,6 +62,7 @@ UNITS = [
     ("xrmm_kv8_shared_mode.hip", ["-DXRMM_KV_MODE=1"], "kv8_walk.o"),
     ("xrmm_kv8_shared_mode.hip", ["-DXRMM_KV_MODE=2"], "kv8_prefix.o"),
     ("xrmm_kv8_shared_mode.hip", ["-DXRMM_KV_MODE=3"], "kv8_own.o"),
+    ("xrmm_kv8_shared_mode.hip", ["-DXRMM_KV_MODE=4"], "kv8_both.o"),
     ("xrmm_rope.hip", [], "rope.o"),
     ("xrmm_sample.hip", [], "sample.o"),
     ("xrmm_lowbit_api.cpp", [], "lowbit_api.o"),

@@ -216,13 +216,22 @@ struct KvStep {
   KvBytes<D / 16> v[8];
 };
 
+template <int D, int W>
+struct KvRowsLds {  // where the waves' parts meet
+  static constexpr int JT = D / 16 < 8 ? D / 16 : 8;  // output tiles of a round
+  f32x4 red[W][JT][64];
+  float row[16][D];
+  float wm[W][16], wl[W][16], rm[16], rl[16];
+  int last;
+};
+
 template <int D, bool FP8, int W, bool TWO, KvMode MODE>
-__global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+__device__ __forceinline__ void kv8_rows(const KvAttnArgs& a, uint32_t row_tiles, uint32_t splits, uint32_t chunk, uint32_t block, KvRowsLds<D, W>& lds) {
   constexpr int KD = D / 4, VD = D / 16;  // codes of a token that a lane holds
   const KvCache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t split = blockIdx.x % splits, unit = blockIdx.x / splits;
+  const uint32_t split = block % splits, unit = block / splits;
   const int tile = static_cast<int>(unit % row_tiles);
   const uint32_t bh = unit / row_tiles;
   const int h = static_cast<int>(bh % static_cast<uint32_t>(c.Hkv)), b = static_cast<int>(bh / static_cast<uint32_t>(c.Hkv));
@@ -467,10 +476,10 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   if (bad && lane == 0 && c.status != nullptr) atomicMax(c.status, KV_BAD);
 
   // The waves' parts meet in LDS. Sums of rows: over the four lanes of a column, then the waves.
-  constexpr int JT = VD < 8 ? VD : 8;  // output tiles of a round
-  __shared__ float wm[W][16], wl[W][16];
-  __shared__ f32x4 red[W][JT][64];
-  __shared__ float row[16][D];
+  constexpr int JT = KvRowsLds<D, W>::JT;
+  auto &wm = lds.wm, &wl = lds.wl;
+  auto& red = lds.red;
+  auto& row = lds.row;
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (g == 0) {
@@ -505,7 +514,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
     }
   }
   // sums of this workgroup's tokens: the rows' outputs in `row`, maxima and sums where wave is 0 and g is 0
-  __shared__ float rm[16], rl[16];
+  auto &rm = lds.rm, &rl = lds.rl;
   if (tid < 16) {
     rm[tid] = top;
     rl[tid] = sum;
@@ -537,7 +546,7 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   }
   constexpr int COHERENT = 1 | 16;  // sc0 sc1: past the L2 of the XCD
   constexpr uint32_t PART = static_cast<uint32_t>(kv_part_bytes<D>());
-  __shared__ int s_last;
+  int& s_last = lds.last;
   uint32_t* cnt = static_cast<uint32_t*>(a.ws);
   const rsrc_t rW = mk_rsrc(static_cast<uint8_t*>(a.ws) + KV_COUNTERS + static_cast<int64_t>(unit) * splits * PART, splits * PART);
 #pragma unroll 1
@@ -607,6 +616,12 @@ __global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(
   }
 }
 
+template <int D, bool FP8, int W, bool TWO, KvMode MODE>
+__global__ __launch_bounds__(64 * W, D > 128 || W == 8 ? 2 : 3) void k_kv8_rows(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+  __shared__ KvRowsLds<D, W> lds;
+  kv8_rows<D, FP8, W, TWO, MODE>(a, row_tiles, splits, chunk, blockIdx.x, lds);
+}
+
 // ---------------------------------------------------------------------------
 // Many rows: products bound the call. A workgroup takes 128 rows (32 a wave) of one sequence and key head and walks over
 // tiles of TT tokens: their codes become binary16 in LDS once for all rows, K as it lies (tokens by d), V transposed (d
@@ -648,14 +663,13 @@ __device__ __forceinline__ int kv_vslot(int d, int piece) {
 }
 
 template <int D, bool FP8, KvMode MODE>
-__global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+__device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles, uint32_t splits, uint32_t chunk, uint32_t block, unsigned char* smem) {
   typedef KvTile<D> Ti;
   constexpr int TT = Ti::TT, KN = Ti::KN, VN = Ti::VN, JT = D / 32, GR = TT / 16;
-  extern __shared__ __align__(16) unsigned char smem[];
   const KvCache& c = a.c;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hf = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t nbh = MODE == KV_PREFIX ? static_cast<uint32_t>(c.Hkv) : static_cast<uint32_t>(c.Hkv) * static_cast<uint32_t>(c.B), bh = blockIdx.x % nbh, rest = blockIdx.x / nbh;
+  const uint32_t nbh = MODE == KV_PREFIX ? static_cast<uint32_t>(c.Hkv) : static_cast<uint32_t>(c.Hkv) * static_cast<uint32_t>(c.B), bh = block % nbh, rest = block / nbh;
   const uint32_t split = rest % splits;
   const int tile = static_cast<int>(row_tiles - 1 - rest / splits);
   const uint32_t unit = bh * row_tiles + static_cast<uint32_t>(tile);
@@ -1285,6 +1299,18 @@ __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs 
   }
 }
 
+template <int D, bool FP8, KvMode MODE>
+__global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  kv8_tile<D, FP8, MODE>(a, row_tiles, splits, chunk, blockIdx.x, smem);
+}
+
+template <int D>
+constexpr int kv8_tile_lds() {
+  constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16);
+  return 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
+}
+
 // Tokens are split only as far as the card has room for more workgroups at once: a start, a join and the code's own fetch
 // cost more than even shares gain (one sequence of 65000: 129 us in shares of 256 tokens, 83 of 512, 57 of 1024, 39 of 2048,
 // one a CU; 48 of up to 8000: 227 us in shares of 1024, 170 of 2048, 108 unsplit; 8 of 4000: 35 of 512, 25 of 1024, 32 of 2048).
@@ -1357,7 +1383,7 @@ hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
     else rows(std::false_type{});
     return hipGetLastError();
   }
-  constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16), lds = 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
+  constexpr int lds = kv8_tile_lds<D>();
   static std::atomic<int> done[kMaxDevices];
   if (lds > 65536) {
     const hipError_t e = raise_lds_cap(reinterpret_cast<const void*>(k_kv8_tile<D, FP8, MODE>), lds, done);

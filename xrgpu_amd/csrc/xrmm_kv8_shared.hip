@@ -6,46 +6,61 @@ namespace xrmm {
 hipError_t launch_kv8_walk(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
 hipError_t launch_kv8_prefix(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
 hipError_t launch_kv8_own(const KvAttnArgs& a, const KvPlan& p, hipStream_t st);
+hipError_t launch_kv8_both(const KvAttnArgs& a, const KvPlan& prefix, const KvPlan& own, hipStream_t st);
 
 namespace {
 
-// The parts of a row: weights exp2(maximum - the largest maximum), outputs added in the parts' order, divided by the sum. A thread has
-// four values of a row, and the loads of eight parts in flight. Rows that `starts` leaves out are not written.
+// The parts of a row: weights exp2(maximum - the largest maximum), outputs added in a fixed order, divided by the sum. A thread has four
+// values of a row and every fourth part, a wave's groups of 16 threads the four shares, and their loads in flight together; the shares meet across
+// the wave. Rows that `starts` leaves out are not written.
 constexpr int KVJ_T = 256;
 
 template <int D>
 __global__ __launch_bounds__(KVJ_T) void k_kv8_join(KvAttnArgs a) {
-  const int64_t rows = a.c.rows * a.Hq, piece = static_cast<int64_t>(blockIdx.x) * KVJ_T + threadIdx.x;
-  const int64_t out = piece / (D / 4);  // [row][head]
+  const int lane = threadIdx.x & 63, share = lane >> 4;
+  const int64_t rows = a.c.rows * a.Hq, piece = (static_cast<int64_t>(blockIdx.x) * (KVJ_T / 64) + (threadIdx.x >> 6)) * 16 + (lane & 15);
+  const int64_t out = piece / (D / 4);  // [row][head]; the same in a wave's shares
   const int d = static_cast<int>(piece % (D / 4)) * 4;
-  if (out >= rows) return;
-  const int row = static_cast<int>(out / a.Hq), hq = static_cast<int>(out % a.Hq), G = a.Hq / a.c.Hkv, h = hq / G;
-  int b, pos;
-  if (!kv_position(a, row, b, pos)) return;
+  const bool in = out < rows;
+  const int row = in ? static_cast<int>(out / a.Hq) : 0, hq = in ? static_cast<int>(out % a.Hq) : 0, G = a.Hq / a.c.Hkv, h = hq / G;
   const int64_t at = static_cast<int64_t>(row) * G + hq % G;
   const KvPart<D> part(a, 0, h);
   float m = -__builtin_inff(), l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   constexpr int N = 8;
 #pragma unroll 1
-  for (int p0 = 0; p0 < a.parts; p0 += N) {
+  for (int p0 = share; p0 < a.parts; p0 += 4 * N) {
     f32x4 x[N];
     f32x2 ml[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int64_t p = (p0 + i < a.parts ? p0 + i : p0) * rows + at;
+      const int64_t p = (p0 + 4 * i < a.parts ? p0 + 4 * i : p0) * rows + at;
       ml[i] = part.ml[p];
       x[i] = *reinterpret_cast<const f32x4*>(part.o + p * D + d);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (p0 + i >= a.parts || ml[i][0] == -__builtin_inff()) continue;  // no such part, or one that saw nothing and left no outputs
+      if (p0 + 4 * i >= a.parts || ml[i][0] == -__builtin_inff()) continue;  // no such part, or one that saw nothing and left no outputs
       const float mn = fmaxf(m, ml[i][0]), f0 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[i][0] - mn);
       o = o * f0 + x[i] * f1;
       l = l * f0 + ml[i][1] * f1;
       m = mn;
     }
   }
+#pragma unroll
+  for (int s = 16; s <= 32; s <<= 1) {
+    const float m1 = __shfl_xor(m, s, 64), l1 = __shfl_xor(l, s, 64);
+    const f32x4 o1 = {__shfl_xor(o[0], s, 64), __shfl_xor(o[1], s, 64), __shfl_xor(o[2], s, 64), __shfl_xor(o[3], s, 64)};
+    // the same operands in the same order in both lanes
+    const bool low = (lane & s) == 0;
+    const float ma = low ? m : m1, mb = low ? m1 : m, mn = fmaxf(ma, mb);
+    const float fa = ma == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ma - mn), fb = mb == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mb - mn);
+    o = (low ? o : o1) * fa + (low ? o1 : o) * fb;
+    l = (low ? l : l1) * fa + (low ? l1 : l) * fb;
+    m = mn;
+  }
+  int b, pos;
+  if (!in || share != 0 || !kv_position(a, row, b, pos)) return;
   o *= l != 0.f ? 1.f / l : 0.f;
   typedef u32x2 u32x2_2 __attribute__((aligned(2)));
   *reinterpret_cast<u32x2_2*>(static_cast<uint16_t*>(a.o) + out * D + d) =
@@ -53,7 +68,7 @@ __global__ __launch_bounds__(KVJ_T) void k_kv8_join(KvAttnArgs a) {
 }
 
 hipError_t launch_join(const KvAttnArgs& a, hipStream_t st) {
-  const int64_t n = (a.c.rows * a.Hq * (a.c.D / 4) + KVJ_T - 1) / KVJ_T;
+  const int64_t n = (a.c.rows * a.Hq * (a.c.D / 4) + KVJ_T / 4 - 1) / (KVJ_T / 4);
   if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
   switch (a.c.D) {
@@ -145,6 +160,10 @@ hipError_t launch_kv8_shared_attention(const KvAttnArgs& a, hipStream_t st) {
   x.parts = static_cast<int32_t>(p.prefix.splits + p.own.splits);
   x.parts_at = KV_COUNTERS;
   x.part0 = 0;
+  if (p.prefix.tile && !p.own.tile && p.own.row_tiles == 1 && a.c.D <= 128) {
+    const hipError_t e = launch_kv8_both(x, p.prefix, p.own, st);
+    return e == hipSuccess ? launch_join(x, st) : e;
+  }
   hipError_t e = launch_kv8_prefix(x, p.prefix, st);
   x.part0 = static_cast<int32_t>(p.prefix.splits);
   if (e == hipSuccess) e = launch_kv8_own(x, p.own, st);
