@@ -11,18 +11,26 @@ namespace {
 // tells apart, and weights below 2^-46 of it (31 nats) are 0: such tokens are not drawn.
 //
 // Order: by logit, of equal ones (0 and -0 are) the lower index first: the composite (ordered bits of x, ~index), unique in a row. top_k, top_p
-// and min_p each keep a prefix of that order. A row's thresholds come from a histogram over the distance to the maximum (64 bins a nat): the bins
-// in which they can fall give a short list, and among its tokens each is found digit by digit of the composite.
+// and min_p each keep a prefix of that order. A row is read four times:
+//   its largest logit
+//   a histogram over the distance to it (64 bins a nat), which tells the few bins in which each threshold lies: of counts for top_k, of
+//     weights by float32's exponential for top_p, whose error is bounded and widens the bins
+//   those bins' tokens into a list, and the exact weight of all before and behind them: a 64-bit exponential a token, which is what bounds
+//     rows with top_p
+//   the part in which the number falls.
+// For top_k up to a quarter of the threads, the threads' own largest logits are counted in place of all: no fewer than top_k tokens reach
+// the top_k-th of them, and hardly more, so the list holds all that may be kept.
 constexpr int SB = 2048;      // bins
 constexpr float SB_NAT = 64.f;  // bins a nat
 constexpr int SLIST = 2048;   // tokens of the list; where more lie in the bins, the row itself is read in its place
 constexpr int SNEAR = 256;    // of a list this short, each token counts those before it; of a longer one digits are counted
 constexpr int ST = 1024;      // threads of a row that one workgroup takes
 constexpr int SP = 256;       // threads of a part of a row
+constexpr int SAPPROX = 30;   // the histogram's weights are in units of 2^-30
 
 struct Draw {       // a row's settings
   double c;         // log2(e) / temperature
-  float s;          // bins a unit of logit
+  float s;          // bins a two of logits
   double top_p, least;  // least: in units of weights, or 0
   int k;            // 0: all
   bool greedy, p;
@@ -36,7 +44,7 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs& a, int64_t row, int F)
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   d.greedy = !(t > 0.0);
   d.c = 1.44269504088896340736 / (d.greedy ? 1.0 : t);
-  d.s = SB_NAT / static_cast<float>(d.greedy ? 1.0 : t);
+  d.s = 2.f * SB_NAT / static_cast<float>(d.greedy ? 1.0 : t);
   d.k = k > 0 && k < a.V ? k : 0;
   d.p = p < 1.0;
   d.top_p = p > 0.0 ? p : 0.0;
@@ -85,8 +93,11 @@ struct Weigher {
   }
 };
 
+// Half of top - x: no finite logits' overflows.
+__device__ __forceinline__ float half_below(float x, float top) { return __builtin_fmaf(x, -0.5f, 0.5f * top); }
+
 __device__ __forceinline__ int bin_of(float x, float top, float s) {
-  return x == top ? 0 : static_cast<int>(fminf((top - x) * s, static_cast<float>(SB - 1)));
+  return x == top ? 0 : static_cast<int>(fminf(half_below(x, top) * s, static_cast<float>(SB - 1)));
 }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
@@ -127,7 +138,7 @@ struct RowOf {
   static constexpr int VEC = 16 / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   const T* x;
-  // VEC values from i on; -infinity past `end` and for NaN
+  // VEC values from i on; -infinity past `end`
   __device__ __forceinline__ void load(float (&f)[VEC], int64_t i, int64_t end) const {
     if (i + VEC <= end) {
       const vec v = *reinterpret_cast<const vec*>(x + i);
@@ -137,41 +148,61 @@ struct RowOf {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = i + e < end ? static_cast<float>(x[i + e]) : -__builtin_inff();
     }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = f[e] == f[e] ? f[e] : -__builtin_inff();
   }
 };
 
-struct SampleLds {
+struct HistLds {
   uint64_t mass[SB];
   uint32_t count[SB];
-  uint64_t list[SLIST];   // composites
-  uint64_t digits[256];
+};
+
+struct ListLds {
+  uint64_t list[SLIST];    // composites
+  uint64_t digits[256];    // also the weights of a short list
+  uint64_t weight[256];    // of the row's parts
+  uint32_t kind[SNEAR];
+};
+
+struct BlockLds {
   uint64_t part[16];
   uint64_t a64, b64;
   uint32_t n, a32, b32;
   int last;
 };
 
-// Bins that decide: top_k's threshold lies in bin kb, top_p's in lo .. hi (kb alone where there is no top_p); tokens before lo are
-// sure, those of neither dropped.
+// Bins that decide: top_k's threshold lies in klo .. khi, with `above` tokens before klo; top_p's in plo .. phi. Both ranges are listed; tokens
+// before `sure` are kept by both.
 struct Cut {
-  int lo, hi, kb;
-  uint64_t above;   // tokens before bin kb
-  uint64_t held_k;  // weight before bin kb; without top_k all of it
-  uint64_t held;    // weight before bin lo
-  __device__ __forceinline__ bool listed(int b) const { return (b >= lo && b <= hi) || b == kb; }
+  int klo, khi, plo, phi, sure;
+  uint32_t above;
+  __device__ __forceinline__ bool listed(int b) const { return (b >= klo && b <= khi) || (b >= plo && b <= phi); }
 };
+
+__device__ __forceinline__ bool few(const Draw& d, int threads) { return d.k > 0 && d.k <= threads / 4; }
+
+// The sum of v over the workgroup, in all threads.
+template <int NT>
+__device__ __forceinline__ uint64_t block_sum64(BlockLds& s, uint64_t v) {
+  const int tid = threadIdx.x;
+  v = wave_sum64(v);
+  __syncthreads();
+  if ((tid & 63) == 0) s.part[tid >> 6] = v;
+  __syncthreads();
+  uint64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) all += s.part[w];
+  return all;
+}
 
 // The first bin whose running sum reaches `need`, of masses or of counts, and the sum before it; SB where none does. All threads.
 template <bool MASS, int NT>
-__device__ __forceinline__ int find_bin(SampleLds& s, uint64_t need, uint64_t* before_it) {
+__device__ __forceinline__ int find_bin(BlockLds& s, const HistLds& hist, uint64_t need, uint64_t* before_it) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int N = SB / NT;
   uint64_t v[N], sum = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    v[i] = MASS ? s.mass[tid * N + i] : s.count[tid * N + i];
+    v[i] = MASS ? hist.mass[tid * N + i] : hist.count[tid * N + i];
     sum += v[i];
   }
   const uint64_t inc = wave_scan64(sum, lane);
@@ -197,47 +228,44 @@ __device__ __forceinline__ int find_bin(SampleLds& s, uint64_t need, uint64_t* b
   return static_cast<int>(s.a32);
 }
 
-// The sum of v over the workgroup, in all threads.
+// From the histogram of a row with top_k or top_p. All threads.
 template <int NT>
-__device__ __forceinline__ uint64_t block_sum64(SampleLds& s, uint64_t v) {
+__device__ __forceinline__ Cut cut_of(BlockLds& s, const HistLds& hist, const Draw& d, int V, int threads) {
   const int tid = threadIdx.x;
-  v = wave_sum64(v);
-  __syncthreads();
-  if ((tid & 63) == 0) s.part[tid >> 6] = v;
-  __syncthreads();
-  uint64_t all = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) all += s.part[w];
-  return all;
-}
-
-// From the histogram of a row. All threads.
-template <int NT>
-__device__ __forceinline__ Cut cut_of(SampleLds& s, const Draw& d) {
-  const int tid = threadIdx.x;
-  Cut c{0, -1, -1, 0, 0, 0};
+  Cut c{0, -1, 0, -1, 0, 0};
+  uint64_t before;
+  if (few(d, threads)) {
+    const int b = find_bin<false, NT>(s, hist, static_cast<uint64_t>(d.k), &before);
+    c.khi = b < SB ? b : SB - 1;
+    c.phi = d.p ? c.khi : -1;
+    return c;
+  }
   if (d.k > 0) {
-    c.kb = find_bin<false, NT>(s, static_cast<uint64_t>(d.k), &c.above);
-    if (c.kb == SB) {  // fewer tokens than top_k: the last bin is all kept
+    const int b = find_bin<false, NT>(s, hist, static_cast<uint64_t>(d.k), &before);
+    if (b == SB) {  // fewer tokens than top_k: all are kept
       uint64_t n = 0;
-      for (int i = tid; i < SB - 1; i += NT) n += s.count[i];
-      c.above = block_sum64<NT>(s, n);
-      c.kb = SB - 1;
+      for (int i = tid; i < SB - 1; i += NT) n += hist.count[i];
+      before = block_sum64<NT>(s, n);
     }
-    c.lo = c.hi = c.kb;
+    c.klo = c.khi = c.sure = b < SB ? b : SB - 1;
+    c.above = static_cast<uint32_t>(before);
   }
   if (d.p) {
-    const int end = d.k > 0 ? c.kb : SB;
+    // top_k's weight is from that before its bin to that with it. A bin's weights are off by 2^-17 of themselves (float32's exponential,
+    // of arguments up to 48) and half a unit each.
+    const int end = d.k > 0 ? c.klo : SB;
     uint64_t m = 0;
-    for (int i = tid; i < end; i += NT) m += s.mass[i];
-    c.held_k = block_sum64<NT>(s, m);
-    const uint64_t most = c.held_k + (d.k > 0 ? s.mass[c.kb] : 0);  // top_k's weight is from held_k to this
-    const int lo = find_bin<true, NT>(s, share_of(d.top_p, c.held_k), &c.held);
-    uint64_t unused;
-    const int hi = d.k > 0 ? find_bin<true, NT>(s, share_of(d.top_p, most), &unused) : lo;
-    c.lo = lo < SB ? lo : SB - 1;
-    c.hi = hi < SB ? hi : SB - 1;
-    if (d.k == 0) c.kb = c.lo;
+    for (int i = tid; i < end; i += NT) m += hist.mass[i];
+    m = block_sum64<NT>(s, m);
+    const double least = d.top_p * static_cast<double>(m), most = d.top_p * static_cast<double>(m + (d.k > 0 ? hist.mass[c.klo] : 0));
+    const double off = static_cast<double>(V) + 1.0;
+    const double lo = least * (1.0 - 0x1p-16) - 2.0 * off, hi = most * (1.0 + 0x1p-16) + 2.0 * off;
+    const int l = find_bin<true, NT>(s, hist, lo < 1.0 ? 1 : static_cast<uint64_t>(lo), &before);
+    const int h = find_bin<true, NT>(s, hist, static_cast<uint64_t>(hi) + 1, &before);
+    c.phi = d.k > 0 ? (h < c.klo ? h : c.klo) : (h < SB ? h : SB - 1);
+    c.plo = l < c.phi ? l : c.phi;
+    c.sure = c.plo;
+    if (d.k == 0) c.klo = SB;
   }
   __syncthreads();
   return c;
@@ -246,24 +274,24 @@ __device__ __forceinline__ Cut cut_of(SampleLds& s, const Draw& d) {
 // The composite at which a running sum over the candidates, in descending order, reaches `need` (>= 1): of their weights, or of their
 // number; 0 where all do not reach it. `each(f)` calls f(composite, weight) for the candidates of each thread. All threads.
 template <bool MASS, typename E>
-__device__ __forceinline__ uint64_t find_composite(SampleLds& s, uint64_t need, E&& each) {
+__device__ __forceinline__ uint64_t find_composite(BlockLds& s, ListLds& t, uint64_t need, E&& each) {
   const int tid = threadIdx.x, lane = tid & 63;
   uint64_t prefix = 0;
 #pragma unroll 1
   for (int shift = 56; shift >= 0; shift -= 8) {
     __syncthreads();
-    if (tid < 256) s.digits[tid] = 0;
+    if (tid < 256) t.digits[tid] = 0;
     if (tid == 0) s.b32 = 256;
     __syncthreads();
     each([&](uint64_t comp, uint64_t w) {
       if (shift == 56 || comp >> (shift + 8) == prefix)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.digits[comp >> shift & 255]), static_cast<unsigned long long>(MASS ? w : 1));
+        atomicAdd(reinterpret_cast<unsigned long long*>(&t.digits[comp >> shift & 255]), static_cast<unsigned long long>(MASS ? w : 1));
     });
     __syncthreads();
     if (tid < 64) {  // digits 255 - 4 lane .. - 3, descending
       uint64_t v[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += v[i] = s.digits[255 - 4 * lane - i];
+      for (int i = 0; i < 4; ++i) sum += v[i] = t.digits[255 - 4 * lane - i];
       uint64_t before = wave_scan64(sum, lane) - sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -283,21 +311,68 @@ __device__ __forceinline__ uint64_t find_composite(SampleLds& s, uint64_t need, 
   return prefix;
 }
 
-// The composite from which on a row's tokens are kept. `n` tokens are listed, in s.list if no more than SLIST. All threads.
+// The composite from which on a row's tokens are kept. `n` tokens are listed, in t.list if no more than SLIST; `held` is the exact weight of the
+// sure ones, `mid` of what top_k keeps behind top_p's bins for certain. All threads.
 template <typename T, int NT>
-__device__ uint64_t threshold_of(SampleLds& s, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n) {
+__device__ uint64_t threshold_of(BlockLds& s, ListLds& t, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n,
+                                 uint64_t held, uint64_t mid) {
   constexpr int VEC = RowOf<T>::VEC;
   const int tid = threadIdx.x;
   const float top = weigh.top;
-  // candidates: the listed tokens of bins from .. to whose composite is at least `least`
-  auto each_of = [&](int from, int to, uint64_t least, auto&& f) {
+  uint64_t threshold = 0;
+  if (n <= SNEAR) {
+    // Each token's number and weight of those before it.
+    uint64_t c = 0, w = 0;
+    bool in_k = false, in_p = false, before_k = false;
+    __syncthreads();
+    if (tid < static_cast<int>(n)) {
+      c = t.list[tid];
+      const float x = of_okey(static_cast<uint32_t>(c >> 32));
+      const int b = bin_of(x, top, d.s);
+      w = Weigher::whole(weigh.units(x));
+      in_k = b >= cut.klo && b <= cut.khi;
+      in_p = b >= cut.plo && b <= cut.phi;
+      before_k = b < cut.klo;
+      t.digits[tid] = w;
+      t.kind[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
+    }
+    if (tid == 0) s.a64 = s.b64 = 0;
+    __syncthreads();
+    uint64_t before = 0;
+    uint32_t number = 0;
+    if (tid < static_cast<int>(n)) {
+      for (uint32_t j = 0; j < n; ++j) {
+        const bool first = t.list[j] > c;
+        const uint32_t of = t.kind[j];
+        number += first ? of & 1u : 0u;
+        before += first && (of & 2u) ? t.digits[j] : 0;
+      }
+    }
+    if (d.k > 0) {
+      if (in_k && number + 1 == static_cast<uint32_t>(d.k) - cut.above) s.a64 = c;
+      __syncthreads();
+      threshold = s.a64;
+    }
+    if (d.p) {
+      const uint64_t all = held + mid + block_sum64<NT>(s, before_k || c >= threshold ? w : 0);
+      const uint64_t need = share_of(d.top_p, all), want = need > held ? need - held : 1;
+      if (in_p && before < want && before + w >= want) s.b64 = c;
+      __syncthreads();
+      threshold = s.b64 > threshold ? s.b64 : threshold;
+    }
+    __syncthreads();
+    return threshold;
+  }
+  // f(composite, weight, bin) for the listed tokens of bins from .. to; for the others' sake
+  auto each_of = [&](int from, int to, auto&& f) {
     auto one = [&](uint64_t c) {
       const float x = of_okey(static_cast<uint32_t>(c >> 32));
       const int b = bin_of(x, top, d.s);
-      if (b >= from && b <= to && c >= least) f(c, Weigher::whole(weigh.units(x)));
+      if (b >= from && b <= to && cut.listed(b)) f(c, Weigher::whole(weigh.units(x)), b);
     };
     if (n <= SLIST) {
-      for (uint32_t i = tid; i < n; i += NT) one(s.list[i]);
+#pragma unroll 1
+      for (uint32_t i = tid; i < n; i += NT) one(t.list[i]);
     } else {
 #pragma unroll 1
       for (int i = tid * VEC; i < V; i += NT * VEC) {
@@ -309,72 +384,17 @@ __device__ uint64_t threshold_of(SampleLds& s, const RowOf<T>& r, int V, const D
       }
     }
   };
-  uint64_t threshold = 0;
-  if (n <= SNEAR) {
-    // Each token's number and weight of those before it. Weights go to s.mass, which the cut has left.
-    uint64_t c = 0, w = 0;
-    bool in_k = false, in_p = false;
-    __syncthreads();
-    if (tid < static_cast<int>(n)) {
-      c = s.list[tid];
-      const float x = of_okey(static_cast<uint32_t>(c >> 32));
-      const int b = bin_of(x, top, d.s);
-      w = Weigher::whole(weigh.units(x));
-      in_k = b == cut.kb;
-      in_p = b >= cut.lo && b <= cut.hi;
-      s.mass[tid] = w;
-      s.count[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
-    }
-    if (tid == 0) s.a64 = s.b64 = 0;
-    __syncthreads();
-    uint64_t before = 0, number = 0, k_weight = 0;
-    if (tid < static_cast<int>(n)) {
-      for (uint32_t j = 0; j < n; ++j) {
-        const bool first = s.list[j] > c;
-        const uint32_t of = s.count[j];
-        number += first && (of & 1) ? 1 : 0;
-        k_weight += first && (of & 1) ? s.mass[j] : 0;
-        before += first && (of & 2) ? s.mass[j] : 0;
-      }
-    }
-    uint64_t all = cut.held_k;
-    if (d.k > 0) {
-      const uint64_t want = static_cast<uint64_t>(d.k) - cut.above;
-      if (in_k && number + 1 == want) {
-        s.a64 = c;
-        s.b64 = k_weight + w;
-      }
-      __syncthreads();
-      threshold = s.a64;
-      if (d.p) {
-        uint64_t m = 0;
-        if (threshold == 0) m = block_sum64<NT>(s, in_k ? w : 0);  // all of them
-        all += threshold == 0 ? m : s.b64;
-      }
-    }
-    if (d.p) {
-      const uint64_t need = share_of(d.top_p, all), want = need > cut.held ? need - cut.held : 1;
-      __syncthreads();
-      if (tid == 0) s.a64 = 0;
-      __syncthreads();
-      if (in_p && w > 0 && before < want && before + w >= want) s.a64 = c;
-      __syncthreads();
-      threshold = s.a64 > threshold ? s.a64 : threshold;
-    }
-    __syncthreads();
-    return threshold;
-  }
   if (d.k > 0)
-    threshold = find_composite<false>(s, static_cast<uint64_t>(d.k) - cut.above, [&](auto&& f) { each_of(cut.kb, cut.kb, 0, f); });
+    threshold = find_composite<false>(s, t, static_cast<uint64_t>(d.k) - cut.above, [&](auto&& f) {
+      each_of(cut.klo, cut.khi, [&](uint64_t c, uint64_t w, int) { f(c, w); });
+    });
   if (d.p) {
-    uint64_t all = cut.held_k;
-    if (d.k > 0) {
-      uint64_t mine = 0;
-      each_of(cut.kb, cut.kb, threshold, [&](uint64_t, uint64_t w) { mine += w; });
-      all += block_sum64<NT>(s, mine);
-    }
-    const uint64_t need = share_of(d.top_p, all);
-    const uint64_t c = find_composite<true>(s, need > cut.held ? need - cut.held : 1, [&](auto&& f) { each_of(cut.lo, cut.hi, 0, f); });
+    uint64_t mine = 0;
+    each_of(0, SB, [&](uint64_t c, uint64_t w, int b) { mine += b < cut.klo || c >= threshold ? w : 0; });
+    const uint64_t all = held + mid + block_sum64<NT>(s, mine), need = share_of(d.top_p, all);
+    const uint64_t c = find_composite<true>(s, t, need > held ? need - held : 1, [&](auto&& f) {
+      each_of(cut.plo, cut.phi, [&](uint64_t k, uint64_t w, int) { f(k, w); });
+    });
     threshold = c > threshold ? c : threshold;
   }
   __syncthreads();
@@ -393,96 +413,153 @@ struct Keep {
   }
 };
 
-// The token at which the running sum of the kept weights over begin .. end - 1 passes `target`, narrowed to a wave's part at a time; `target_of`
-// turns the sum over all of it into the target (and may return what the caller knows). All threads.
-template <typename T, int NT, typename F>
-__device__ void draw_in(SampleLds& s, const RowOf<T>& r, int begin, int end, const Keep& keep, F&& target_of, int32_t* token, float* share) {
+// The token at which the running sum of the kept weights over begin .. end - 1 passes `target`, narrowed to a wave's part at a time. All threads.
+template <typename T, int NT>
+__device__ void draw_in(BlockLds& s, const RowOf<T>& r, int begin, int end, const Keep& keep, uint64_t target, uint64_t total, int32_t* token,
+                        float* share) {
   constexpr int VEC = RowOf<T>::VEC, NW = NT / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  uint64_t total = 0, target = 0;
 #pragma unroll 1
-  for (bool first = true;; first = false) {
+  while (true) {
     const int per = ((end - begin + NW - 1) / NW + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
     const int from = begin + wave * per, to = end - from < per ? end : from + per;
-    uint64_t mine = 0;
+    float f[VEC];
+    uint64_t k[VEC], mine = 0;
 #pragma unroll 1
-    for (int i = from + lane * VEC; i < to; i += 64 * VEC) {
-      float f[VEC];
+    for (int i = from + lane * VEC; i < from + per; i += 64 * VEC) {
       r.load(f, i, to);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mine += keep(f[e], static_cast<uint32_t>(i + e));
+      for (int e = 0; e < VEC; ++e) mine += k[e] = keep(f[e], static_cast<uint32_t>(i + e));
     }
-    mine = wave_sum64(mine);
+    const uint64_t sum = wave_sum64(mine);
     __syncthreads();
-    if (lane == 0) s.part[wave] = mine;
+    if (lane == 0) s.part[wave] = sum;
     __syncthreads();
-    if (first) {
-      uint64_t all = 0;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) all += s.part[w];
-      target = target_of(all, total);
-    }
     int w = 0;
     uint64_t before = 0;
     while (w < NW - 1 && before + s.part[w] <= target) before += s.part[w++];
     target -= before;
-    begin += w * per;
-    end = end - begin < per ? end : begin + per;
-    if (per == 64 * VEC) break;
-  }
-  if (wave != 0) return;
-  float f[VEC];
-  r.load(f, begin + lane * VEC, end);
-  uint64_t k[VEC], mine = 0;
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) mine += k[e] = keep(f[e], static_cast<uint32_t>(begin + lane * VEC + e));
-  const uint64_t inc = wave_scan64(mine, lane);
-  uint64_t before = inc - mine;
-  if (before <= target && target < inc) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (before <= target && target < before + k[e]) {
-        *token = begin + lane * VEC + e;
-        *share = static_cast<float>(log(keep.weigh.units(f[e]) / static_cast<double>(total)));
-      }
-      before += k[e];
+    if (per > 64 * VEC) {
+      begin += w * per;
+      end = end - begin < per ? end : begin + per;
+      continue;
     }
+    if (w != wave) return;  // one load a lane, still in its registers
+    const uint64_t inc = wave_scan64(mine, lane);
+    before = inc - mine;
+    if (before <= target && target < inc) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        if (before <= target && target < before + k[e]) {
+          *token = from + lane * VEC + e;
+          *share = static_cast<float>(log(keep.weigh.units(f[e]) / static_cast<double>(total)));
+        }
+        before += k[e];
+      }
+    }
+    return;
   }
 }
 
-// The largest composite of from .. to - 1, in all threads; 0 where there is none.
+// The draw of a row from the kept weights of its parts (at most 256, in t.weight): the part, then the token in it. All threads.
 template <typename T, int NT>
-__device__ __forceinline__ uint64_t best_of(SampleLds& s, const RowOf<T>& r, int from, int to) {
+__device__ void draw_parts(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t row, const RowOf<T>& r, const Keep& keep, int parts, int size) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t v[4], sum = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum += v[i] = lane * 4 + i < parts ? t.weight[lane * 4 + i] : 0;
+  const uint64_t inc = wave_scan64(sum, lane);
+  const uint64_t total = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc >> 32), 63))) << 32 |
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc), 63));
+  const uint64_t target = place_of(static_cast<double>(a.u[row]), total);
+  uint64_t before = inc - sum;
+  if (tid < 64) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (before <= target && target < before + v[i]) {
+        s.a32 = lane * 4 + i;
+        s.a64 = target - before;
+      }
+      before += v[i];
+    }
+  }
+  __syncthreads();
+  const int from = static_cast<int>(s.a32) * size, to = a.V - from < size ? a.V : from + size;
+  draw_in<T, NT>(s, r, from, to, keep, s.a64, total, a.tokens + row, a.shares + row);
+}
+
+// The listed tokens' kept weights to t.weight, by part. All threads.
+template <typename T, int NT>
+__device__ __forceinline__ void add_list(ListLds& t, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Keep& keep, uint32_t n, int size) {
   constexpr int VEC = RowOf<T>::VEC;
   const int tid = threadIdx.x;
-  uint32_t key = 0, at = 0;  // the first of the largest: a thread's indexes ascend
-  for (int i = from + tid * VEC; i < to; i += NT * VEC) {
+  auto add = [&](float x, uint32_t i) {
+    const uint64_t k = keep(x, i);
+    if (k != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&t.weight[i / static_cast<uint32_t>(size)]), static_cast<unsigned long long>(k));
+  };
+  if (n <= SLIST) {
+#pragma unroll 1
+    for (uint32_t i = tid; i < n; i += NT) {
+      const uint64_t c = t.list[i];
+      add(of_okey(static_cast<uint32_t>(c >> 32)), 0xFFFFFFFFu - static_cast<uint32_t>(c));
+    }
+    return;
+  }
+#pragma unroll 1
+  for (int i = tid * VEC; i < V; i += NT * VEC) {
+    float f[VEC];
+    r.load(f, i, V);
+#pragma unroll 1
+    for (int e = 0; e < VEC; ++e)
+      if (f[e] > -__builtin_inff() && cut.listed(bin_of(f[e], keep.weigh.top, d.s))) add(f[e], static_cast<uint32_t>(i + e));
+  }
+}
+
+// This thread's largest logit of from .. to - 1 and the first index that has it (a thread's ascend); -infinity where there is none.
+template <typename T, int NT>
+__device__ __forceinline__ float thread_best(const RowOf<T>& r, int from, int to, uint32_t& at) {
+  constexpr int VEC = RowOf<T>::VEC;
+  float best = -__builtin_inff();
+  at = 0;
+  for (int i = from + static_cast<int>(threadIdx.x) * VEC; i < to; i += NT * VEC) {
     float f[VEC];
     r.load(f, i, to);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const uint32_t k = f[e] > -__builtin_inff() ? okey(f[e]) : 0u;
-      at = k > key ? i + e : at;
-      key = k > key ? k : key;
+      at = f[e] > best ? i + e : at;
+      best = f[e] > best ? f[e] : best;
     }
   }
-  uint64_t best = key == 0 ? 0 : static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - at);
+  return best;
+}
+
+// The workgroup's largest composite, in all threads; 0 where there is none.
+template <int NT>
+__device__ __forceinline__ uint64_t block_best(BlockLds& s, float x, uint32_t at) {
+  uint64_t best = x > -__builtin_inff() ? composite(x, at) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const uint64_t c = shfl_xor64(best, o);
     best = c > best ? c : best;
   }
-  if ((tid & 63) == 0) s.part[tid >> 6] = best;
+  if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = best;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) best = s.part[w] > best ? s.part[w] : best;
   return best;
 }
 
-// from .. to - 1 into the histogram.
+// from .. to - 1 into the histogram: counts of all of them (or of the threads' largest ones, `mine`), and weights by float32's exponential.
 template <typename T, int NT>
-__device__ __forceinline__ void count_in(SampleLds& s, const RowOf<T>& r, int from, int to, const Draw& d, const Weigher& weigh) {
+__device__ __forceinline__ void count_in(HistLds& hist, const RowOf<T>& r, int from, int to, const Draw& d, const Weigher& weigh, bool few_k, float mine) {
   constexpr int VEC = RowOf<T>::VEC;
+  if (few_k) {
+    if (mine > -__builtin_inff()) atomicAdd(&hist.count[bin_of(mine, weigh.top, d.s)], 1u);
+    return;
+  }
+  const float c = static_cast<float>(-2.0 * d.c);
+#pragma unroll 1
   for (int i = from + static_cast<int>(threadIdx.x) * VEC; i < to; i += NT * VEC) {
     float f[VEC];
     r.load(f, i, to);
@@ -490,23 +567,64 @@ __device__ __forceinline__ void count_in(SampleLds& s, const RowOf<T>& r, int fr
     for (int e = 0; e < VEC; ++e) {
       if (!(f[e] > -__builtin_inff())) continue;
       const int b = bin_of(f[e], weigh.top, d.s);
-      if (d.k > 0) atomicAdd(&s.count[b], 1u);
-      if (d.p) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), static_cast<unsigned long long>(Weigher::whole(weigh.units(f[e]))));
+      if (d.k > 0) atomicAdd(&hist.count[b], 1u);
+      if (d.p) {
+        const float y = f[e] == weigh.top ? 0.f : half_below(f[e], weigh.top) * c;
+        const uint32_t w = static_cast<uint32_t>(__builtin_rintf(__builtin_amdgcn_exp2f(y + static_cast<float>(SAPPROX))));
+        if (w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&hist.mass[b]), static_cast<unsigned long long>(w));
+      }
     }
   }
 }
 
-// One workgroup a row, all of it.
+// from .. to - 1: listed tokens through `list(composite)`, and this thread's exact weights: of the sure ones, of those of them that min_p
+// keeps, and of what lies behind top_p's bins and is top_k's for certain. `step`: threads that take a stretch together, `first` this one's place.
+template <typename T, typename L>
+__device__ __forceinline__ void split_in(const RowOf<T>& r, int from, int to, int first, int step, const Draw& d, const Cut& cut, const Weigher& weigh,
+                                         uint64_t& held, uint64_t& kept, uint64_t& mid, L&& list) {
+  constexpr int VEC = RowOf<T>::VEC;
+#pragma unroll 1
+  for (int i = from + first * VEC; i < to; i += step * VEC) {
+    float f[VEC];
+    r.load(f, i, to);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const int b = f[e] > -__builtin_inff() ? bin_of(f[e], weigh.top, d.s) : SB;
+      if (b < SB && cut.listed(b)) list(composite(f[e], i + e));
+      const bool sure = b < cut.sure, behind = d.p && b > cut.phi && b < cut.klo && b < SB;
+      if (sure || behind) {
+        const double u = weigh.units(f[e]);
+        const uint64_t w = Weigher::whole(u);
+        held += sure ? w : 0;
+        kept += sure && u >= d.least ? w : 0;
+        mid += behind ? w : 0;
+      }
+    }
+  }
+}
+
+// One workgroup a row, all of it; a wave's part is a stretch of the row.
 template <typename T>
 __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
   constexpr int VEC = RowOf<T>::VEC;
-  __shared__ SampleLds s;
-  const int tid = threadIdx.x;
+  __shared__ BlockLds s;
+  __shared__ HistLds hist;
+  __shared__ ListLds t;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
   const Draw d = draw_of(a, row, F);
   const int V = a.V;
-  const uint64_t best = best_of<T, ST>(s, r, 0, V);
+  const bool filter = d.k > 0 || d.p;
+  if (filter && !d.greedy)
+    for (int i = tid; i < SB; i += ST) {
+      hist.mass[i] = 0;
+      hist.count[i] = 0;
+    }
+  if (tid == 0) s.n = 0;
+  uint32_t at;
+  const float mine = thread_best<T, ST>(r, 0, V, at);
+  const uint64_t best = block_best<ST>(s, mine, at);
   if (best == 0 || d.greedy) {
     if (tid == 0) {
       a.tokens[row] = best == 0 ? -1 : static_cast<int32_t>(0xFFFFFFFFu - static_cast<uint32_t>(best));
@@ -516,43 +634,50 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
   }
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
   const Weigher weigh{top, static_cast<double>(top), d.c, F};
-  uint64_t threshold = 0;
-  if (d.k > 0 || d.p) {
-    for (int i = tid; i < SB; i += ST) {
-      s.mass[i] = 0;
-      s.count[i] = 0;
-    }
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    count_in<T, ST>(s, r, 0, V, d, weigh);
-    __syncthreads();
-    const Cut cut = cut_of<ST>(s, d);
-    for (int i = tid * VEC; i < V; i += ST * VEC) {
+  Keep keep{weigh, d.least, 0};
+  constexpr int parts = ST / 64;
+  const int size = ((V + parts - 1) / parts + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
+  const int from = wave * size < V ? wave * size : V, to = V - from < size ? V : from + size;
+  if (!filter) {
+    uint64_t kept = 0;
+#pragma unroll 1
+    for (int i = from + lane * VEC; i < to; i += 64 * VEC) {
       float f[VEC];
-      r.load(f, i, V);
+      r.load(f, i, to);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        if (!(f[e] > -__builtin_inff()) || !cut.listed(bin_of(f[e], top, d.s))) continue;
-        const uint32_t at = atomicAdd(&s.n, 1u);
-        if (at < SLIST) s.list[at] = composite(f[e], i + e);
-      }
+      for (int e = 0; e < VEC; ++e) kept += keep(f[e], static_cast<uint32_t>(i + e));
     }
-    __syncthreads();
-    threshold = threshold_of<T, ST>(s, r, V, d, cut, weigh, s.n);
+    kept = wave_sum64(kept);
+    if (lane == 0) t.weight[wave] = kept;
+    draw_parts<T, ST>(s, t, a, row, r, keep, parts, size);
+    return;
   }
-  draw_in<T, ST>(s, r, 0, V, Keep{weigh, d.least, threshold},
-                 [&](uint64_t all, uint64_t& total) {
-                   total = all;
-                   return place_of(static_cast<double>(a.u[row]), all);
-                 },
-                 a.tokens + row, a.shares + row);
+  count_in<T, ST>(hist, r, 0, V, d, weigh, few(d, ST), mine);
+  __syncthreads();
+  const Cut cut = cut_of<ST>(s, hist, d, V, ST);
+  uint64_t held = 0, kept = 0, mid = 0;
+  split_in<T>(r, from, to, lane, 64, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
+    const uint32_t n = atomicAdd(&s.n, 1u);
+    if (n < SLIST) t.list[n] = c;
+  });
+  kept = wave_sum64(kept);
+  if (lane == 0) t.weight[wave] = kept;
+  if (d.p) {
+    held = block_sum64<ST>(s, held);
+    mid = block_sum64<ST>(s, mid);
+  }
+  __syncthreads();
+  const uint32_t n = s.n;
+  keep.threshold = threshold_of<T, ST>(s, t, r, V, d, cut, weigh, n, held, mid);
+  add_list<T, ST>(t, r, V, d, cut, keep, n, size);
+  draw_parts<T, ST>(s, t, a, row, r, keep, parts, size);
 }
 
 // ---------------------------------------------------------------------------
 // Few rows: parts of a row by workgroups, in launches that end where the whole row has to be known. k_sample_top: the largest logit.
 // k_sample_mass: the histogram, whose cut the last part to arrive takes; without top_k and top_p the parts' weights, and the draw.
-// k_sample_draw: the list and the sure tokens' weights by part; the last part to arrive finds the threshold, the part in which the
-// target falls, and the token in it. What parts leave for the last one goes past the L2 of its XCD.
+// k_sample_draw: the list and the exact weights by part; the last part to arrive finds the threshold, the part in which the number
+// falls, and the token in it. What parts leave for the last one goes past the L2 of its XCD.
 struct SampleRow {        // at the head of the workspace, zero between calls
   uint64_t best;
   uint32_t arrived, pad;
@@ -562,14 +687,15 @@ struct SampleShare {      // a row's, behind the head
   uint64_t list[SLIST];
   uint32_t count[SB];
   Cut cut;
-  uint32_t n, pad[3];
-};                        // and its parts' weights
+  uint32_t n, pad;
+};                        // and three weights of each part: kept, held, mid
 constexpr int64_t SAMPLE_HEAD = 4096;
 constexpr int SAMPLE_ROWS = static_cast<int>(SAMPLE_HEAD / sizeof(SampleRow));
+static_assert(sizeof(SampleShare) % 8 == 0);
 
 struct SamplePlan {
   int parts, size;        // of a row; size: logits of a part
-  __host__ __device__ int64_t row_bytes() const { return (static_cast<int64_t>(sizeof(SampleShare)) + parts * 8 + 255) / 256 * 256; }
+  __host__ __device__ int64_t row_bytes() const { return (static_cast<int64_t>(sizeof(SampleShare)) + parts * 24 + 255) / 256 * 256; }
 };
 
 template <typename U>
@@ -583,7 +709,7 @@ __device__ __forceinline__ SampleShare* share_of_row(const SampleArgs& a, const 
 }
 
 // Whether this workgroup is the last of its row's parts. What it put before is seen by that one. All threads.
-__device__ __forceinline__ bool last_part(SampleLds& s, SampleRow* w, int parts) {
+__device__ __forceinline__ bool last_part(BlockLds& s, SampleRow* w, int parts) {
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -596,7 +722,7 @@ __device__ __forceinline__ bool last_part(SampleLds& s, SampleRow* w, int parts)
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_top(SampleArgs a, SamplePlan p, int F) {
-  __shared__ SampleLds s;
+  __shared__ BlockLds s;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
   const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
@@ -607,54 +733,20 @@ __global__ __launch_bounds__(SP) void k_sample_top(SampleArgs a, SamplePlan p, i
     w->count[i] = 0;
   }
   if (part == 0 && tid == 0) w->n = 0;
-  const uint64_t best = best_of<T, SP>(s, r, from, to);
+  uint32_t at;
+  const float mine = thread_best<T, SP>(r, from, to, at);
+  const uint64_t best = block_best<SP>(s, mine, at);
   if (tid == 0 && best != 0) __hip_atomic_fetch_max(&row_of(a, row)->best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// The draw of a row whose parts' kept weights are known, by the last part to arrive.
-template <typename T>
-__device__ void draw_parts(SampleLds& s, const SampleArgs& a, const SamplePlan& p, int64_t row, const RowOf<T>& r, const Keep& keep,
-                           const uint64_t* weights, const uint64_t* more) {
-  // a wave's parts at a time are at most 64 * 4
-  const int tid = threadIdx.x, lane = tid & 63;
-  uint64_t v[4], sum = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = lane * 4 + i;
-    v[i] = at < p.parts ? get(weights + at) + (more ? more[at] : 0) : 0;
-    sum += v[i];
-  }
-  const uint64_t inc = wave_scan64(sum, lane);
-  const uint64_t total = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc >> 32), 63))) << 32 |
-                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc), 63));
-  const uint64_t target = place_of(static_cast<double>(a.u[row]), total);
-  uint64_t before = inc - sum;
-  __syncthreads();
-  if (tid < 64) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (before <= target && target < before + v[i]) {
-        s.a32 = lane * 4 + i;
-        s.a64 = target - before;
-      }
-      before += v[i];
-    }
-  }
-  __syncthreads();
-  const int from = static_cast<int>(s.a32) * p.size, to = a.V - from < p.size ? a.V : from + p.size;
-  const uint64_t rest = s.a64;
-  draw_in<T, SP>(s, r, from, to, keep,
-                 [&](uint64_t, uint64_t& t) {
-                   t = total;
-                   return rest;
-                 },
-                 a.tokens + row, a.shares + row);
 }
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, int F) {
   constexpr int VEC = RowOf<T>::VEC;
-  __shared__ SampleLds s;
+  __shared__ BlockLds s;
+  __shared__ union {
+    HistLds hist;
+    ListLds list;
+  } u;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
   const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
@@ -678,6 +770,7 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
   if (d.k == 0 && !d.p) {
     const Keep keep{weigh, d.least, 0};
     uint64_t mine = 0;
+#pragma unroll 1
     for (int i = from + tid * VEC; i < to; i += SP * VEC) {
       float f[VEC];
       r.load(f, i, to);
@@ -688,34 +781,42 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
     if (tid == 0) put(weights + part, mine);
     if (!last_part(s, w, p.parts)) return;
     if (tid == 0) put(&w->best, uint64_t{0});
-    draw_parts(s, a, p, row, r, keep, weights, nullptr);
+    if (tid < p.parts) u.list.weight[tid] = get(weights + tid);
+    draw_parts<T, SP>(s, u.list, a, row, r, keep, p.parts, p.size);
     return;
   }
+  const int threads = p.parts * SP;
+  const bool few_k = few(d, threads);
   for (int i = tid; i < SB; i += SP) {
-    s.mass[i] = 0;
-    s.count[i] = 0;
+    u.hist.mass[i] = 0;
+    u.hist.count[i] = 0;
+  }
+  float mine = 0.f;
+  if (few_k) {
+    uint32_t at;
+    mine = thread_best<T, SP>(r, from, to, at);
   }
   __syncthreads();
-  count_in<T, SP>(s, r, from, to, d, weigh);
+  count_in<T, SP>(u.hist, r, from, to, d, weigh, few_k, mine);
   __syncthreads();
   for (int i = tid; i < SB; i += SP) {
-    if (d.k > 0 && s.count[i] != 0) __hip_atomic_fetch_add(&sh->count[i], s.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (d.p && s.mass[i] != 0) __hip_atomic_fetch_add(&sh->mass[i], s.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (u.hist.count[i] != 0) __hip_atomic_fetch_add(&sh->count[i], u.hist.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (u.hist.mass[i] != 0) __hip_atomic_fetch_add(&sh->mass[i], u.hist.mass[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!last_part(s, w, p.parts)) return;
   for (int i = tid; i < SB; i += SP) {
-    s.count[i] = d.k > 0 ? get(&sh->count[i]) : 0u;
-    s.mass[i] = d.p ? get(&sh->mass[i]) : 0u;
+    u.hist.count[i] = d.k > 0 ? get(&sh->count[i]) : 0u;
+    u.hist.mass[i] = d.p && !few_k ? get(&sh->mass[i]) : 0u;
   }
   __syncthreads();
-  const Cut cut = cut_of<SP>(s, d);
+  const Cut cut = cut_of<SP>(s, u.hist, d, a.V, threads);
   if (tid == 0) sh->cut = cut;  // for the next launch
 }
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, int F) {
-  constexpr int VEC = RowOf<T>::VEC;
-  __shared__ SampleLds s;
+  __shared__ BlockLds s;
+  __shared__ ListLds t;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
   const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
@@ -729,56 +830,34 @@ __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, 
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
   const Weigher weigh{top, static_cast<double>(top), d.c, F};
   const Cut cut = sh->cut;
-  uint64_t mine = 0;
-  for (int i = from + tid * VEC; i < to; i += SP * VEC) {
-    float f[VEC];
-    r.load(f, i, to);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      if (!(f[e] > -__builtin_inff())) continue;
-      const int b = bin_of(f[e], top, d.s);
-      if (cut.listed(b)) {
-        const uint32_t at = __hip_atomic_fetch_add(&sh->n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (at < SLIST) put(&sh->list[at], composite(f[e], i + e));
-      } else if (b < cut.lo) {
-        const double u = weigh.units(f[e]);
-        mine += u >= d.least ? Weigher::whole(u) : 0;
-      }
+  uint64_t held = 0, kept = 0, mid = 0;
+  split_in<T>(r, from, to, tid, SP, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
+    const uint32_t at = __hip_atomic_fetch_add(&sh->n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (at < SLIST) put(&sh->list[at], c);
+  });
+  kept = block_sum64<SP>(s, kept);
+  if (tid == 0) put(weights + part, kept);
+  if (d.p) {
+    held = block_sum64<SP>(s, held);
+    mid = block_sum64<SP>(s, mid);
+    if (tid == 0) {
+      put(weights + p.parts + part, held);
+      put(weights + 2 * p.parts + part, mid);
     }
   }
-  mine = block_sum64<SP>(s, mine);
-  if (tid == 0) put(weights + part, mine);
   if (!last_part(s, w, p.parts)) return;
   if (tid == 0) put(&w->best, uint64_t{0});
   const uint32_t n = get(&sh->n);
-  for (uint32_t i = tid; i < n && i < SLIST; i += SP) s.list[i] = get(&sh->list[i]);
-  __syncthreads();
-  const uint64_t threshold = threshold_of<T, SP>(s, r, a.V, d, cut, weigh, n);
-  const Keep keep{weigh, d.least, threshold};
-  // the list's kept weights by part
-  for (int i = tid; i < p.parts; i += SP) s.mass[i] = 0;
-  __syncthreads();
-  auto add = [&](float x, uint32_t i) {
-    const uint64_t k = keep(x, i);
-    if (k != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[i / static_cast<uint32_t>(p.size)]), static_cast<unsigned long long>(k));
-  };
-  if (n <= SLIST) {
-    for (uint32_t i = tid; i < n; i += SP) {
-      const uint64_t c = s.list[i];
-      add(of_okey(static_cast<uint32_t>(c >> 32)), 0xFFFFFFFFu - static_cast<uint32_t>(c));
-    }
-  } else {
-#pragma unroll 1
-    for (int i = tid * VEC; i < a.V; i += SP * VEC) {
-      float f[VEC];
-      r.load(f, i, a.V);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (f[e] > -__builtin_inff() && cut.listed(bin_of(f[e], top, d.s))) add(f[e], static_cast<uint32_t>(i + e));
-    }
+  for (uint32_t i = tid; i < n && i < SLIST; i += SP) t.list[i] = get(&sh->list[i]);
+  if (tid < p.parts) t.weight[tid] = get(weights + tid);
+  if (d.p) {
+    held = block_sum64<SP>(s, tid < p.parts ? get(weights + p.parts + tid) : 0);
+    mid = block_sum64<SP>(s, tid < p.parts ? get(weights + 2 * p.parts + tid) : 0);
   }
   __syncthreads();
-  draw_parts(s, a, p, row, r, keep, weights, s.mass);
+  const Keep keep{weigh, d.least, threshold_of<T, SP>(s, t, r, a.V, d, cut, weigh, n, held, mid)};
+  add_list<T, SP>(t, r, a.V, d, cut, keep, n, p.size);
+  draw_parts<T, SP>(s, t, a, row, r, keep, p.parts, p.size);
 }
 
 // Rows by parts where one workgroup a row would leave CUs idle and a row is long enough to pay for the launches.
