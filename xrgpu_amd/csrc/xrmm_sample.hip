@@ -43,7 +43,7 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs& a, int64_t row, int F)
   const double m = a.min_p ? static_cast<double>(a.min_p[row]) : a.min_p1;
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   d.greedy = !(t > 0.0);
-  d.c = 1.44269504088896340736 / (d.greedy ? 1.0 : t);
+  d.c = 1.44269504088896340736 / (d.greedy ? 1.0 : t < 1e300 ? t : 1e300);  // not 0: an infinity's distance stays one
   d.s = 2.f * SB_NAT / static_cast<float>(d.greedy ? 1.0 : t);
   d.k = k > 0 && k < a.V ? k : 0;
   d.p = p < 1.0;
@@ -61,32 +61,30 @@ __device__ __forceinline__ float of_okey(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t composite(float x, uint32_t i) { return static_cast<uint64_t>(okey(x)) << 32 | (0xFFFFFFFFu - i); }
 
-// 2^y in units of 2^-F, y <= 0: 2^n 2^f by the Taylor series of 2^f, |f| <= 1/2, whose rest after f^11 is 6 10^-15.
-__device__ __forceinline__ double exp2_units(double y, int F) {
-  const double n = __builtin_rint(y), r = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = __builtin_fma(p, r, 1.0 / 3628800.0);
-  p = __builtin_fma(p, r, 1.0 / 362880.0);
-  p = __builtin_fma(p, r, 1.0 / 40320.0);
-  p = __builtin_fma(p, r, 1.0 / 5040.0);
-  p = __builtin_fma(p, r, 1.0 / 720.0);
-  p = __builtin_fma(p, r, 1.0 / 120.0);
-  p = __builtin_fma(p, r, 1.0 / 24.0);
-  p = __builtin_fma(p, r, 1.0 / 6.0);
-  p = __builtin_fma(p, r, 0.5);
-  p = __builtin_fma(p, r, 1.0);
-  p = __builtin_fma(p, r, 1.0);
-  return __builtin_ldexp(p, static_cast<int>(n) + F);
-}
-
+// What a logit weighs, in units of 2^-F of the largest, not yet rounded: 2^n 2^r for y = n + r, |r| <= 1/2, by the Taylor series of 2^r
+// up to r^11, whose rest is 6 10^-15. Without branches: a NaN is an infinite logit less itself (others are no logits here), and a weight
+// of far below half a unit rounds to none.
 struct Weigher {
   float top;   // the row's largest logit
   double topd, c;
   int F;
-  __device__ __forceinline__ double units(float x) const {  // not yet rounded
-    const double y = (static_cast<double>(x) - topd) * c;
-    // a NaN is infinity less itself or times 0; the test keeps it and what rounds to 0 away
-    return x == top ? __builtin_ldexp(1.0, F) : y > -static_cast<double>(F + 2) ? exp2_units(y, F) : 0.0;
+  __device__ __forceinline__ double units(float x) const {
+    const double y = __builtin_fmax(__builtin_fmin((static_cast<double>(x) - topd) * c, 0.0), -1000.0);
+    const double n = __builtin_rint(y), r = y - n;
+    // ln(2)^k / k!
+    double p = 4.44553827187081e-10;
+    p = __builtin_fma(p, r, 7.054911620801121e-09);
+    p = __builtin_fma(p, r, 1.0178086009239696e-07);
+    p = __builtin_fma(p, r, 1.3215486790144305e-06);
+    p = __builtin_fma(p, r, 1.5252733804059838e-05);
+    p = __builtin_fma(p, r, 0.00015403530393381606);
+    p = __builtin_fma(p, r, 0.0013333558146428441);
+    p = __builtin_fma(p, r, 0.009618129107628477);
+    p = __builtin_fma(p, r, 0.055504108664821576);
+    p = __builtin_fma(p, r, 0.2402265069591007);
+    p = __builtin_fma(p, r, 0.6931471805599453);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_ldexp(p, static_cast<int>(n) + F);
   }
   __device__ __forceinline__ static uint64_t whole(double u) {  // to nearest; u <= 2^51
     return __builtin_bit_cast(uint64_t, u + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
@@ -96,8 +94,9 @@ struct Weigher {
 // Half of top - x: no finite logits' overflows.
 __device__ __forceinline__ float half_below(float x, float top) { return __builtin_fmaf(x, -0.5f, 0.5f * top); }
 
+// A NaN, an infinity less itself, comes to 0.
 __device__ __forceinline__ int bin_of(float x, float top, float s) {
-  return x == top ? 0 : static_cast<int>(fminf(half_below(x, top) * s, static_cast<float>(SB - 1)));
+  return static_cast<int>(__builtin_amdgcn_fmed3f(half_below(x, top) * s, 0.f, static_cast<float>(SB - 1)));
 }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
@@ -133,21 +132,51 @@ __device__ __forceinline__ uint64_t share_of(double p, uint64_t s) {
   return n < 1 ? 1 : n > s ? s : n;
 }
 
-template <typename T>
+template <typename T, int N>
 struct RowOf {
-  static constexpr int VEC = 16 / sizeof(T);
+  static constexpr int VEC = N;
   typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   const T* x;
-  // VEC values from i on; -infinity past `end`
-  __device__ __forceinline__ void load(float (&f)[VEC], int64_t i, int64_t end) const {
-    if (i + VEC <= end) {
-      const vec v = *reinterpret_cast<const vec*>(x + i);
+  __device__ __forceinline__ static float value(T v) {  // NaN is -infinity
+    const float f = static_cast<float>(v);
+    return f == f ? f : -__builtin_inff();
+  }
+  // f(VEC values, index of the first) for `step` threads' vectors of from .. to - 1, this thread the `first` of them; AHEAD loads in flight.
+  // The last vector ends with the stretch: what it repeats is -infinity. A row has VEC logits at least.
+  template <int AHEAD, typename F>
+  __device__ __forceinline__ void each(int from, int to, int first, int step, F&& f) const {
+    const int stride = step * VEC, last = to - VEC;
+    int i = from + first * VEC;
+    vec v[AHEAD];
+    auto load = [&](int at) {
+      at = at < last ? at : last;
+      return *reinterpret_cast<const vec*>(x + (at > 0 ? at : 0));
+    };
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = static_cast<float>(v[e]);
-    } else {
+    for (int n = 0; n < AHEAD; ++n) v[n] = load(i + n * stride);
+#pragma unroll 1
+    while (i < to) {
+      const vec now = v[0];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = i + e < end ? static_cast<float>(x[i + e]) : -__builtin_inff();
+      for (int n = 0; n + 1 < AHEAD; ++n) v[n] = v[n + 1];
+      v[AHEAD - 1] = load(i + AHEAD * stride);
+      float a[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) a[e] = value(now[e]);
+      const int at = i < last ? i : last;
+      if (__builtin_expect(at != i, 0)) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) a[e] = at + e >= i ? a[e] : -__builtin_inff();
+      }
+      f(a, at);
+      i += stride;
     }
+  }
+  // f(logit, index), one by one in a short loop, for what few rows come to
+  template <typename F>
+  __device__ __forceinline__ void slowly(int to, int first, int step, F&& f) const {
+#pragma unroll 1
+    for (int i = first; i < to; i += step) f(value(x[i]), i);
   }
 };
 
@@ -234,14 +263,13 @@ __device__ __forceinline__ Cut cut_of(BlockLds& s, const HistLds& hist, const Dr
   const int tid = threadIdx.x;
   Cut c{0, -1, 0, -1, 0, 0};
   uint64_t before;
-  if (few(d, threads)) {
-    const int b = find_bin<false, NT>(s, hist, static_cast<uint64_t>(d.k), &before);
-    c.khi = b < SB ? b : SB - 1;
-    c.phi = d.p ? c.khi : -1;
-    return c;
-  }
   if (d.k > 0) {
     const int b = find_bin<false, NT>(s, hist, static_cast<uint64_t>(d.k), &before);
+    if (few(d, threads)) {
+      c.khi = b < SB ? b : SB - 1;
+      c.phi = d.p ? c.khi : -1;
+      return c;
+    }
     if (b == SB) {  // fewer tokens than top_k: all are kept
       uint64_t n = 0;
       for (int i = tid; i < SB - 1; i += NT) n += hist.count[i];
@@ -260,8 +288,12 @@ __device__ __forceinline__ Cut cut_of(BlockLds& s, const HistLds& hist, const Dr
     const double least = d.top_p * static_cast<double>(m), most = d.top_p * static_cast<double>(m + (d.k > 0 ? hist.mass[c.klo] : 0));
     const double off = static_cast<double>(V) + 1.0;
     const double lo = least * (1.0 - 0x1p-16) - 2.0 * off, hi = most * (1.0 + 0x1p-16) + 2.0 * off;
-    const int l = find_bin<true, NT>(s, hist, lo < 1.0 ? 1 : static_cast<uint64_t>(lo), &before);
-    const int h = find_bin<true, NT>(s, hist, static_cast<uint64_t>(hi) + 1, &before);
+    int l = 0, h = 0;
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      l = h;
+      h = find_bin<true, NT>(s, hist, i != 0 ? static_cast<uint64_t>(hi) + 1 : lo < 1.0 ? 1 : static_cast<uint64_t>(lo), &before);
+    }
     c.phi = d.k > 0 ? (h < c.klo ? h : c.klo) : (h < SB ? h : SB - 1);
     c.plo = l < c.phi ? l : c.phi;
     c.sure = c.plo;
@@ -313,77 +345,78 @@ __device__ __forceinline__ uint64_t find_composite(BlockLds& s, ListLds& t, uint
 
 // The composite from which on a row's tokens are kept. `n` tokens are listed, in t.list if no more than SLIST; `held` is the exact weight of the
 // sure ones, `mid` of what top_k keeps behind top_p's bins for certain. All threads.
-template <typename T, int NT>
-__device__ uint64_t threshold_of(BlockLds& s, ListLds& t, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n,
-                                 uint64_t held, uint64_t mid) {
-  constexpr int VEC = RowOf<T>::VEC;
+//
+// Of a short list: each token's number and weight of those before it.
+template <int NT>
+__device__ __forceinline__ uint64_t threshold_near(BlockLds& s, ListLds& t, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n, uint64_t held,
+                                                   uint64_t mid) {
   const int tid = threadIdx.x;
-  const float top = weigh.top;
-  uint64_t threshold = 0;
-  if (n <= SNEAR) {
-    // Each token's number and weight of those before it.
-    uint64_t c = 0, w = 0;
-    bool in_k = false, in_p = false, before_k = false;
-    __syncthreads();
-    if (tid < static_cast<int>(n)) {
-      c = t.list[tid];
-      const float x = of_okey(static_cast<uint32_t>(c >> 32));
-      const int b = bin_of(x, top, d.s);
-      w = Weigher::whole(weigh.units(x));
-      in_k = b >= cut.klo && b <= cut.khi;
-      in_p = b >= cut.plo && b <= cut.phi;
-      before_k = b < cut.klo;
-      t.digits[tid] = w;
-      t.kind[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
-    }
-    if (tid == 0) s.a64 = s.b64 = 0;
-    __syncthreads();
-    uint64_t before = 0;
-    uint32_t number = 0;
-    if (tid < static_cast<int>(n)) {
-      for (uint32_t j = 0; j < n; ++j) {
-        const bool first = t.list[j] > c;
-        const uint32_t of = t.kind[j];
-        number += first ? of & 1u : 0u;
-        before += first && (of & 2u) ? t.digits[j] : 0;
-      }
-    }
-    if (d.k > 0) {
-      if (in_k && number + 1 == static_cast<uint32_t>(d.k) - cut.above) s.a64 = c;
-      __syncthreads();
-      threshold = s.a64;
-    }
-    if (d.p) {
-      const uint64_t all = held + mid + block_sum64<NT>(s, before_k || c >= threshold ? w : 0);
-      const uint64_t need = share_of(d.top_p, all), want = need > held ? need - held : 1;
-      if (in_p && before < want && before + w >= want) s.b64 = c;
-      __syncthreads();
-      threshold = s.b64 > threshold ? s.b64 : threshold;
-    }
-    __syncthreads();
-    return threshold;
+  uint64_t c = 0, w = 0, threshold = 0;
+  bool in_k = false, in_p = false, before_k = false;
+  if (tid < static_cast<int>(n)) {
+    c = t.list[tid];
+    const float x = of_okey(static_cast<uint32_t>(c >> 32));
+    const int b = bin_of(x, weigh.top, d.s);
+    w = Weigher::whole(weigh.units(x));
+    in_k = b >= cut.klo && b <= cut.khi;
+    in_p = b >= cut.plo && b <= cut.phi;
+    before_k = b < cut.klo;
+    t.digits[tid] = w;
+    t.kind[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
   }
-  // f(composite, weight, bin) for the listed tokens of bins from .. to; for the others' sake
+  if (tid == 0) s.a64 = s.b64 = 0;
+  __syncthreads();
+  uint64_t before = 0;
+  uint32_t number = 0;
+  if (tid < static_cast<int>(n)) {
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) {
+      const bool first = t.list[j] > c;
+      const uint32_t of = t.kind[j];
+      number += first ? of & 1u : 0u;
+      before += first && (of & 2u) ? t.digits[j] : 0;
+    }
+  }
+  if (d.k > 0) {
+    if (in_k && number + 1 == static_cast<uint32_t>(d.k) - cut.above) s.a64 = c;
+    __syncthreads();
+    threshold = s.a64;
+  }
+  if (d.p) {
+    const uint64_t all = held + mid + block_sum64<NT>(s, before_k || c >= threshold ? w : 0);
+    const uint64_t need = share_of(d.top_p, all), want = need > held ? need - held : 1;
+    if (in_p && before < want && before + w >= want) s.b64 = c;
+    __syncthreads();
+    threshold = s.b64 > threshold ? s.b64 : threshold;
+  }
+  __syncthreads();
+  return threshold;
+}
+
+// Of a longer one, or of the row where the list holds less than all: digit by digit. Apart, so that the other rows' code is short.
+template <typename R, int NT>
+__device__ __attribute__((noinline)) uint64_t threshold_far(BlockLds* sp, ListLds* tp, const R r, int V, const Draw d, const Cut cut, const Weigher weigh,
+                                                            uint32_t n, uint64_t held, uint64_t mid) {
+  BlockLds& s = *sp;
+  ListLds& t = *tp;
+  const int tid = threadIdx.x;
+  // f(composite, weight, bin) for the listed tokens of bins from .. to
   auto each_of = [&](int from, int to, auto&& f) {
     auto one = [&](uint64_t c) {
       const float x = of_okey(static_cast<uint32_t>(c >> 32));
-      const int b = bin_of(x, top, d.s);
+      const int b = bin_of(x, weigh.top, d.s);
       if (b >= from && b <= to && cut.listed(b)) f(c, Weigher::whole(weigh.units(x)), b);
     };
     if (n <= SLIST) {
 #pragma unroll 1
       for (uint32_t i = tid; i < n; i += NT) one(t.list[i]);
     } else {
-#pragma unroll 1
-      for (int i = tid * VEC; i < V; i += NT * VEC) {
-        float x[VEC];
-        r.load(x, i, V);
-#pragma unroll 1
-        for (int e = 0; e < VEC; ++e)
-          if (x[e] > -__builtin_inff()) one(composite(x[e], i + e));
-      }
+      r.slowly(V, tid, NT, [&](float x, int i) {
+        if (x > -__builtin_inff()) one(composite(x, static_cast<uint32_t>(i)));
+      });
     }
   };
+  uint64_t threshold = 0;
   if (d.k > 0)
     threshold = find_composite<false>(s, t, static_cast<uint64_t>(d.k) - cut.above, [&](auto&& f) {
       each_of(cut.klo, cut.khi, [&](uint64_t c, uint64_t w, int) { f(c, w); });
@@ -401,6 +434,12 @@ __device__ uint64_t threshold_of(BlockLds& s, ListLds& t, const RowOf<T>& r, int
   return threshold;
 }
 
+template <typename R, int NT>
+__device__ __forceinline__ uint64_t threshold_of(BlockLds& s, ListLds& t, const R& r, int V, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n,
+                                                 uint64_t held, uint64_t mid) {
+  return n <= SNEAR ? threshold_near<NT>(s, t, d, cut, weigh, n, held, mid) : threshold_far<R, NT>(&s, &t, r, V, d, cut, weigh, n, held, mid);
+}
+
 // What a kept token weighs; 0 for one that is not.
 struct Keep {
   Weigher weigh;
@@ -413,11 +452,22 @@ struct Keep {
   }
 };
 
+// The thread that has a row's token writes it; one logarithm in a kernel's code.
+struct Found {
+  float x;
+  int token;  // -1: another thread's
+  uint64_t total;
+  __device__ __forceinline__ void write(const SampleArgs& a, int64_t row, const Weigher& weigh) const {
+    if (token < 0) return;
+    a.tokens[row] = token;
+    a.shares[row] = static_cast<float>(log(weigh.units(x) / static_cast<double>(total)));
+  }
+};
+
 // The token at which the running sum of the kept weights over begin .. end - 1 passes `target`, narrowed to a wave's part at a time. All threads.
-template <typename T, int NT>
-__device__ void draw_in(BlockLds& s, const RowOf<T>& r, int begin, int end, const Keep& keep, uint64_t target, uint64_t total, int32_t* token,
-                        float* share) {
-  constexpr int VEC = RowOf<T>::VEC, NW = NT / 64;
+template <typename R, int NT>
+__device__ __forceinline__ Found draw_in(BlockLds& s, const R& r, int begin, int end, const Keep& keep, uint64_t target, uint64_t total) {
+  constexpr int VEC = R::VEC, NW = NT / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
 #pragma unroll 1
   while (true) {
@@ -425,12 +475,20 @@ __device__ void draw_in(BlockLds& s, const RowOf<T>& r, int begin, int end, cons
     const int from = begin + wave * per, to = end - from < per ? end : from + per;
     float f[VEC];
     uint64_t k[VEC], mine = 0;
-#pragma unroll 1
-    for (int i = from + lane * VEC; i < from + per; i += 64 * VEC) {
-      r.load(f, i, to);
+    int at = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mine += k[e] = keep(f[e], static_cast<uint32_t>(i + e));
+    for (int e = 0; e < VEC; ++e) {
+      f[e] = 0.f;
+      k[e] = 0;
     }
+    r.template each<1>(from, to, lane, 64, [&](const float (&x)[VEC], int i) {
+      at = i;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        f[e] = x[e];
+        mine += k[e] = keep(x[e], static_cast<uint32_t>(i + e));
+      }
+    });
     const uint64_t sum = wave_sum64(mine);
     __syncthreads();
     if (lane == 0) s.part[wave] = sum;
@@ -444,26 +502,27 @@ __device__ void draw_in(BlockLds& s, const RowOf<T>& r, int begin, int end, cons
       end = end - begin < per ? end : begin + per;
       continue;
     }
-    if (w != wave) return;  // one load a lane, still in its registers
+    Found found{0.f, -1, total};
+    if (w != wave) return found;  // one load a lane, still in its registers
     const uint64_t inc = wave_scan64(mine, lane);
     before = inc - mine;
     if (before <= target && target < inc) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         if (before <= target && target < before + k[e]) {
-          *token = from + lane * VEC + e;
-          *share = static_cast<float>(log(keep.weigh.units(f[e]) / static_cast<double>(total)));
+          found.token = at + e;
+          found.x = f[e];
         }
         before += k[e];
       }
     }
-    return;
+    return found;
   }
 }
 
 // The draw of a row from the kept weights of its parts (at most 256, in t.weight): the part, then the token in it. All threads.
-template <typename T, int NT>
-__device__ void draw_parts(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t row, const RowOf<T>& r, const Keep& keep, int parts, int size) {
+template <typename R, int NT>
+__device__ __forceinline__ Found draw_parts(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t row, const R& r, const Keep& keep, int parts, int size) {
   const int tid = threadIdx.x, lane = tid & 63;
   uint64_t v[4], sum = 0;
   __syncthreads();
@@ -486,13 +545,12 @@ __device__ void draw_parts(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t
   }
   __syncthreads();
   const int from = static_cast<int>(s.a32) * size, to = a.V - from < size ? a.V : from + size;
-  draw_in<T, NT>(s, r, from, to, keep, s.a64, total, a.tokens + row, a.shares + row);
+  return draw_in<R, NT>(s, r, from, to, keep, s.a64, total);
 }
 
 // The listed tokens' kept weights to t.weight, by part. All threads.
-template <typename T, int NT>
-__device__ __forceinline__ void add_list(ListLds& t, const RowOf<T>& r, int V, const Draw& d, const Cut& cut, const Keep& keep, uint32_t n, int size) {
-  constexpr int VEC = RowOf<T>::VEC;
+template <typename R, int NT>
+__device__ __forceinline__ void add_list(ListLds& t, const R& r, int V, const Draw& d, const Cut& cut, const Keep& keep, uint32_t n, int size) {
   const int tid = threadIdx.x;
   auto add = [&](float x, uint32_t i) {
     const uint64_t k = keep(x, i);
@@ -506,31 +564,47 @@ __device__ __forceinline__ void add_list(ListLds& t, const RowOf<T>& r, int V, c
     }
     return;
   }
-#pragma unroll 1
-  for (int i = tid * VEC; i < V; i += NT * VEC) {
-    float f[VEC];
-    r.load(f, i, V);
-#pragma unroll 1
-    for (int e = 0; e < VEC; ++e)
-      if (f[e] > -__builtin_inff() && cut.listed(bin_of(f[e], keep.weigh.top, d.s))) add(f[e], static_cast<uint32_t>(i + e));
+  r.slowly(V, tid, NT, [&](float x, int i) {
+    if (x > -__builtin_inff() && cut.listed(bin_of(x, keep.weigh.top, d.s))) add(x, static_cast<uint32_t>(i));
+  });
+}
+
+// The draw of a row whose kept tokens are all in a short list. All threads.
+template <int NT>
+__device__ __forceinline__ Found draw_list(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t row, const Keep& keep, uint32_t n) {
+  const int tid = threadIdx.x;
+  const bool mine = tid < static_cast<int>(n);
+  uint64_t c = 0, k = 0;
+  float x = 0.f;
+  if (mine) {
+    c = t.list[tid];
+    x = of_okey(static_cast<uint32_t>(c >> 32));
+    k = keep(x, 0xFFFFFFFFu - static_cast<uint32_t>(c));
+    t.digits[tid] = k;
   }
+  const uint64_t total = block_sum64<NT>(s, k), target = place_of(static_cast<double>(a.u[row]), total);
+  Found found{x, -1, total};
+  if (k == 0) return found;
+  uint64_t before = 0;
+#pragma unroll 4
+  for (uint32_t j = 0; j < n; ++j) before += static_cast<uint32_t>(t.list[j]) > static_cast<uint32_t>(c) ? t.digits[j] : 0;  // of a lower index
+  if (before <= target && target < before + k) found.token = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(c));
+  return found;
 }
 
 // This thread's largest logit of from .. to - 1 and the first index that has it (a thread's ascend); -infinity where there is none.
-template <typename T, int NT>
-__device__ __forceinline__ float thread_best(const RowOf<T>& r, int from, int to, uint32_t& at) {
-  constexpr int VEC = RowOf<T>::VEC;
+template <typename R, int NT>
+__device__ __forceinline__ float thread_best(const R& r, int from, int to, uint32_t& at) {
+  constexpr int VEC = R::VEC;
   float best = -__builtin_inff();
   at = 0;
-  for (int i = from + static_cast<int>(threadIdx.x) * VEC; i < to; i += NT * VEC) {
-    float f[VEC];
-    r.load(f, i, to);
+  r.template each<4>(from, to, static_cast<int>(threadIdx.x), NT, [&](const float (&f)[VEC], int i) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       at = f[e] > best ? i + e : at;
       best = f[e] > best ? f[e] : best;
     }
-  }
+  });
   return best;
 }
 
@@ -551,68 +625,88 @@ __device__ __forceinline__ uint64_t block_best(BlockLds& s, float x, uint32_t at
 }
 
 // from .. to - 1 into the histogram: counts of all of them (or of the threads' largest ones, `mine`), and weights by float32's exponential.
-template <typename T, int NT>
-__device__ __forceinline__ void count_in(HistLds& hist, const RowOf<T>& r, int from, int to, const Draw& d, const Weigher& weigh, bool few_k, float mine) {
-  constexpr int VEC = RowOf<T>::VEC;
+template <typename R, int NT>
+__device__ __forceinline__ void count_in(HistLds& hist, const R& r, int from, int to, const Draw& d, const Weigher& weigh, bool few_k, float mine) {
+  constexpr int VEC = R::VEC;
   if (few_k) {
     if (mine > -__builtin_inff()) atomicAdd(&hist.count[bin_of(mine, weigh.top, d.s)], 1u);
     return;
   }
   const float c = static_cast<float>(-2.0 * d.c);
-#pragma unroll 1
-  for (int i = from + static_cast<int>(threadIdx.x) * VEC; i < to; i += NT * VEC) {
-    float f[VEC];
-    r.load(f, i, to);
+  r.template each<1>(from, to, static_cast<int>(threadIdx.x), NT, [&](const float (&f)[VEC], int) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      if (!(f[e] > -__builtin_inff())) continue;
+      if (!(f[e] > -__builtin_inff())) continue;  // rows that a grammar masks would meet in one bin
       const int b = bin_of(f[e], weigh.top, d.s);
       if (d.k > 0) atomicAdd(&hist.count[b], 1u);
       if (d.p) {
-        const float y = f[e] == weigh.top ? 0.f : half_below(f[e], weigh.top) * c;
-        const uint32_t w = static_cast<uint32_t>(__builtin_rintf(__builtin_amdgcn_exp2f(y + static_cast<float>(SAPPROX))));
-        if (w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&hist.mass[b]), static_cast<unsigned long long>(w));
+        const float y = __builtin_fminf(half_below(f[e], weigh.top) * c, 0.f);
+        atomicAdd(reinterpret_cast<unsigned long long*>(&hist.mass[b]),
+                  static_cast<unsigned long long>(static_cast<uint32_t>(__builtin_amdgcn_exp2f(y + static_cast<float>(SAPPROX)))));
       }
     }
-  }
+  });
 }
 
 // from .. to - 1: listed tokens through `list(composite)`, and this thread's exact weights: of the sure ones, of those of them that min_p
 // keeps, and of what lies behind top_p's bins and is top_k's for certain. `step`: threads that take a stretch together, `first` this one's place.
-template <typename T, typename L>
-__device__ __forceinline__ void split_in(const RowOf<T>& r, int from, int to, int first, int step, const Draw& d, const Cut& cut, const Weigher& weigh,
+template <typename R, typename L>
+__device__ __forceinline__ void split_in(const R& r, int from, int to, int first, int step, const Draw& d, const Cut& cut, const Weigher& weigh,
                                          uint64_t& held, uint64_t& kept, uint64_t& mid, L&& list) {
-  constexpr int VEC = RowOf<T>::VEC;
-#pragma unroll 1
-  for (int i = from + first * VEC; i < to; i += step * VEC) {
-    float f[VEC];
-    r.load(f, i, to);
+  constexpr int VEC = R::VEC;
+  if (d.k == 0) {  // top_p alone: every token's weight counts
+    uint64_t all = 0, sure = 0, listed = 0;
+    r.template each<1>(from, to, first, step, [&](const float (&f)[VEC], int i) {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const int b = bin_of(f[e], weigh.top, d.s);
+        const double u = weigh.units(f[e]);
+        const uint64_t w = Weigher::whole(u), ws = b < cut.sure ? w : 0;
+        all += w;
+        sure += ws;
+        if (d.least > 0.0) kept += u >= d.least ? ws : 0;
+        if (b >= cut.plo && b <= cut.phi && f[e] > -__builtin_inff()) {
+          listed += w;
+          list(composite(f[e], i + e));
+        }
+      }
+    });
+    held = sure;
+    if (!(d.least > 0.0)) kept = sure;
+    mid = all - sure - listed;
+    return;
+  }
+  r.template each<1>(from, to, first, step, [&](const float (&f)[VEC], int i) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int b = f[e] > -__builtin_inff() ? bin_of(f[e], weigh.top, d.s) : SB;
-      if (b < SB && cut.listed(b)) list(composite(f[e], i + e));
-      const bool sure = b < cut.sure, behind = d.p && b > cut.phi && b < cut.klo && b < SB;
-      if (sure || behind) {
+      const int b = bin_of(f[e], weigh.top, d.s);
+      if (b > cut.khi || !(f[e] > -__builtin_inff())) continue;  // nearly all
+      if (cut.listed(b)) list(composite(f[e], i + e));
+      else {
         const double u = weigh.units(f[e]);
         const uint64_t w = Weigher::whole(u);
-        held += sure ? w : 0;
-        kept += sure && u >= d.least ? w : 0;
-        mid += behind ? w : 0;
+        if (b < cut.sure) {
+          held += w;
+          kept += u >= d.least ? w : 0;
+        } else {
+          mid += w;
+        }
       }
     }
-  }
+  });
 }
 
 // One workgroup a row, all of it; a wave's part is a stretch of the row.
-template <typename T>
+template <typename T, int N>
 __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
-  constexpr int VEC = RowOf<T>::VEC;
+  typedef RowOf<T, N> R;
+  constexpr int VEC = R::VEC;
   __shared__ BlockLds s;
   __shared__ HistLds hist;
   __shared__ ListLds t;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
-  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const R r{static_cast<const T*>(a.x) + row * a.stride};
   const Draw d = draw_of(a, row, F);
   const int V = a.V;
   const bool filter = d.k > 0 || d.p;
@@ -623,7 +717,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
     }
   if (tid == 0) s.n = 0;
   uint32_t at;
-  const float mine = thread_best<T, ST>(r, 0, V, at);
+  const float mine = thread_best<R, ST>(r, 0, V, at);
   const uint64_t best = block_best<ST>(s, mine, at);
   if (best == 0 || d.greedy) {
     if (tid == 0) {
@@ -640,23 +734,23 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
   const int from = wave * size < V ? wave * size : V, to = V - from < size ? V : from + size;
   if (!filter) {
     uint64_t kept = 0;
-#pragma unroll 1
-    for (int i = from + lane * VEC; i < to; i += 64 * VEC) {
-      float f[VEC];
-      r.load(f, i, to);
+    r.template each<1>(from, to, lane, 64, [&](const float (&f)[VEC], int) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) kept += keep(f[e], static_cast<uint32_t>(i + e));
-    }
+      for (int e = 0; e < VEC; ++e) {
+        const double u = weigh.units(f[e]);
+        kept += u >= d.least ? Weigher::whole(u) : 0;
+      }
+    });
     kept = wave_sum64(kept);
     if (lane == 0) t.weight[wave] = kept;
-    draw_parts<T, ST>(s, t, a, row, r, keep, parts, size);
+    draw_parts<R, ST>(s, t, a, row, r, keep, parts, size).write(a, row, weigh);
     return;
   }
-  count_in<T, ST>(hist, r, 0, V, d, weigh, few(d, ST), mine);
+  count_in<R, ST>(hist, r, 0, V, d, weigh, few(d, ST), mine);
   __syncthreads();
   const Cut cut = cut_of<ST>(s, hist, d, V, ST);
   uint64_t held = 0, kept = 0, mid = 0;
-  split_in<T>(r, from, to, lane, 64, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
+  split_in(r, from, to, lane, 64, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
     const uint32_t n = atomicAdd(&s.n, 1u);
     if (n < SLIST) t.list[n] = c;
   });
@@ -668,9 +762,14 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
   }
   __syncthreads();
   const uint32_t n = s.n;
-  keep.threshold = threshold_of<T, ST>(s, t, r, V, d, cut, weigh, n, held, mid);
-  add_list<T, ST>(t, r, V, d, cut, keep, n, size);
-  draw_parts<T, ST>(s, t, a, row, r, keep, parts, size);
+  keep.threshold = threshold_of<R, ST>(s, t, r, V, d, cut, weigh, n, held, mid);
+  Found found;
+  if (cut.sure == 0 && n <= SNEAR) found = draw_list<ST>(s, t, a, row, keep, n);
+  else {
+    add_list<R, ST>(t, r, V, d, cut, keep, n, size);
+    found = draw_parts<R, ST>(s, t, a, row, r, keep, parts, size);
+  }
+  found.write(a, row, weigh);
 }
 
 // ---------------------------------------------------------------------------
@@ -722,10 +821,11 @@ __device__ __forceinline__ bool last_part(BlockLds& s, SampleRow* w, int parts) 
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_top(SampleArgs a, SamplePlan p, int F) {
+  typedef RowOf<T, 16 / sizeof(T)> R;
   __shared__ BlockLds s;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
-  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const R r{static_cast<const T*>(a.x) + row * a.stride};
   const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
   SampleShare* w = share_of_row(a, p, row);
   for (int i = part * SP + tid; i < SB; i += p.parts * SP) {
@@ -734,14 +834,15 @@ __global__ __launch_bounds__(SP) void k_sample_top(SampleArgs a, SamplePlan p, i
   }
   if (part == 0 && tid == 0) w->n = 0;
   uint32_t at;
-  const float mine = thread_best<T, SP>(r, from, to, at);
+  const float mine = thread_best<R, SP>(r, from, to, at);
   const uint64_t best = block_best<SP>(s, mine, at);
   if (tid == 0 && best != 0) __hip_atomic_fetch_max(&row_of(a, row)->best, best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, int F) {
-  constexpr int VEC = RowOf<T>::VEC;
+  typedef RowOf<T, 16 / sizeof(T)> R;
+  constexpr int VEC = R::VEC;
   __shared__ BlockLds s;
   __shared__ union {
     HistLds hist;
@@ -749,7 +850,7 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
   } u;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
-  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const R r{static_cast<const T*>(a.x) + row * a.stride};
   const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
   const Draw d = draw_of(a, row, F);
   SampleRow* w = row_of(a, row);
@@ -770,19 +871,19 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
   if (d.k == 0 && !d.p) {
     const Keep keep{weigh, d.least, 0};
     uint64_t mine = 0;
-#pragma unroll 1
-    for (int i = from + tid * VEC; i < to; i += SP * VEC) {
-      float f[VEC];
-      r.load(f, i, to);
+    r.template each<1>(from, to, tid, SP, [&](const float (&f)[VEC], int) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mine += keep(f[e], static_cast<uint32_t>(i + e));
-    }
+      for (int e = 0; e < VEC; ++e) {
+        const double u = weigh.units(f[e]);
+        mine += u >= d.least ? Weigher::whole(u) : 0;
+      }
+    });
     mine = block_sum64<SP>(s, mine);
     if (tid == 0) put(weights + part, mine);
     if (!last_part(s, w, p.parts)) return;
     if (tid == 0) put(&w->best, uint64_t{0});
     if (tid < p.parts) u.list.weight[tid] = get(weights + tid);
-    draw_parts<T, SP>(s, u.list, a, row, r, keep, p.parts, p.size);
+    draw_parts<R, SP>(s, u.list, a, row, r, keep, p.parts, p.size).write(a, row, weigh);
     return;
   }
   const int threads = p.parts * SP;
@@ -794,10 +895,10 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
   float mine = 0.f;
   if (few_k) {
     uint32_t at;
-    mine = thread_best<T, SP>(r, from, to, at);
+    mine = thread_best<R, SP>(r, from, to, at);
   }
   __syncthreads();
-  count_in<T, SP>(u.hist, r, from, to, d, weigh, few_k, mine);
+  count_in<R, SP>(u.hist, r, from, to, d, weigh, few_k, mine);
   __syncthreads();
   for (int i = tid; i < SB; i += SP) {
     if (u.hist.count[i] != 0) __hip_atomic_fetch_add(&sh->count[i], u.hist.count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -815,11 +916,12 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
 
 template <typename T>
 __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, int F) {
+  typedef RowOf<T, 16 / sizeof(T)> R;
   __shared__ BlockLds s;
   __shared__ ListLds t;
   const int tid = threadIdx.x, part = static_cast<int>(blockIdx.x);
   const int64_t row = blockIdx.y;
-  const RowOf<T> r{static_cast<const T*>(a.x) + row * a.stride};
+  const R r{static_cast<const T*>(a.x) + row * a.stride};
   const int from = part * p.size, to = a.V - from < p.size ? a.V : from + p.size;
   const Draw d = draw_of(a, row, F);
   SampleRow* w = row_of(a, row);
@@ -831,9 +933,11 @@ __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, 
   const Weigher weigh{top, static_cast<double>(top), d.c, F};
   const Cut cut = sh->cut;
   uint64_t held = 0, kept = 0, mid = 0;
-  split_in<T>(r, from, to, tid, SP, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
-    const uint32_t at = __hip_atomic_fetch_add(&sh->n, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (at < SLIST) put(&sh->list[at], c);
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+  split_in(r, from, to, tid, SP, d, cut, weigh, held, kept, mid, [&](uint64_t c) {
+    const uint32_t n = atomicAdd(&s.n, 1u);
+    if (n < SLIST) t.list[n] = c;
   });
   kept = block_sum64<SP>(s, kept);
   if (tid == 0) put(weights + part, kept);
@@ -845,19 +949,35 @@ __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, 
       put(weights + 2 * p.parts + part, mid);
     }
   }
+  const uint32_t own = s.n;  // behind a barrier of the sums
+  if (own > 0) {
+    __syncthreads();
+    if (tid == 0) s.a32 = __hip_atomic_fetch_add(&sh->n, own, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const uint32_t base = s.a32;
+    for (uint32_t i = tid; i < own && i < SLIST && base + i < SLIST; i += SP) put(&sh->list[base + i], t.list[i]);
+  }
   if (!last_part(s, w, p.parts)) return;
   if (tid == 0) put(&w->best, uint64_t{0});
+  // all that the parts left, in flight together
   const uint32_t n = get(&sh->n);
-  for (uint32_t i = tid; i < n && i < SLIST; i += SP) t.list[i] = get(&sh->list[i]);
-  if (tid < p.parts) t.weight[tid] = get(weights + tid);
-  if (d.p) {
-    held = block_sum64<SP>(s, tid < p.parts ? get(weights + p.parts + tid) : 0);
-    mid = block_sum64<SP>(s, tid < p.parts ? get(weights + 2 * p.parts + tid) : 0);
-  }
+  const uint64_t head = get(&sh->list[tid]);
+  const uint64_t w0 = tid < p.parts ? get(weights + tid) : 0, w1 = d.p && tid < p.parts ? get(weights + p.parts + tid) : 0,
+                 w2 = d.p && tid < p.parts ? get(weights + 2 * p.parts + tid) : 0;
+  t.list[tid] = head;
+  for (uint32_t i = SP + tid; i < n && i < SLIST; i += SP) t.list[i] = get(&sh->list[i]);
+  if (tid < p.parts) t.weight[tid] = w0;
+  held = block_sum64<SP>(s, w1);
+  mid = block_sum64<SP>(s, w2);
   __syncthreads();
-  const Keep keep{weigh, d.least, threshold_of<T, SP>(s, t, r, a.V, d, cut, weigh, n, held, mid)};
-  add_list<T, SP>(t, r, a.V, d, cut, keep, n, p.size);
-  draw_parts<T, SP>(s, t, a, row, r, keep, p.parts, p.size);
+  const Keep keep{weigh, d.least, threshold_of<R, SP>(s, t, r, a.V, d, cut, weigh, n, held, mid)};
+  Found found;
+  if (cut.sure == 0 && n <= SNEAR) found = draw_list<SP>(s, t, a, row, keep, n);
+  else {
+    add_list<R, SP>(t, r, a.V, d, cut, keep, n, p.size);
+    found = draw_parts<R, SP>(s, t, a, row, r, keep, p.parts, p.size);
+  }
+  found.write(a, row, weigh);
 }
 
 // Rows by parts where one workgroup a row would leave CUs idle and a row is long enough to pay for the launches.
@@ -882,7 +1002,9 @@ hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
     if (a.top_k != nullptr || a.top_p != nullptr || (a.top_k1 > 0 && a.top_k1 < a.V) || a.top_p1 < 1.0) k_sample_draw<T><<<grid, SP, 0, st>>>(a, p, F);
     return hipGetLastError();
   }
-  k_sample_row<T><<<dim3(static_cast<uint32_t>(a.rows)), ST, 0, st>>>(a, F);
+  const dim3 grid(static_cast<uint32_t>(a.rows));
+  if (a.V >= static_cast<int>(16 / sizeof(T))) k_sample_row<T, 16 / sizeof(T)><<<grid, ST, 0, st>>>(a, F);
+  else k_sample_row<T, 1><<<grid, ST, 0, st>>>(a, F);
   return hipGetLastError();
 }
 
