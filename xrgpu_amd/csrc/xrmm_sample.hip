@@ -43,8 +43,9 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs& a, int64_t row, int F)
   const double m = a.min_p ? static_cast<double>(a.min_p[row]) : a.min_p1;
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   d.greedy = !(t > 0.0);
-  d.c = 1.44269504088896340736 / (d.greedy ? 1.0 : t < 1e300 ? t : 1e300);  // not 0: an infinity's distance stays one
-  d.s = 2.f * SB_NAT / static_cast<float>(d.greedy ? 1.0 : t);
+  const double heat = d.greedy ? 1.0 : t < 1e300 ? t : 1e300;  // an infinity's distance stays one
+  d.c = 1.44269504088896340736 / heat;
+  d.s = 2.f * SB_NAT / static_cast<float>(heat);
   d.k = k > 0 && k < a.V ? k : 0;
   d.p = p < 1.0;
   d.top_p = p > 0.0 ? p : 0.0;
@@ -62,15 +63,18 @@ __device__ __forceinline__ float of_okey(uint32_t k) {
 __device__ __forceinline__ uint64_t composite(float x, uint32_t i) { return static_cast<uint64_t>(okey(x)) << 32 | (0xFFFFFFFFu - i); }
 
 // What a logit weighs, in units of 2^-F of the largest, not yet rounded: 2^n 2^r for y = n + r, |r| <= 1/2, by the Taylor series of 2^r
-// up to r^11, whose rest is 6 10^-15. Without branches: a NaN is an infinite logit less itself (others are no logits here), and a weight
-// of far below half a unit rounds to none.
+// up to r^11, whose rest is 6 10^-15. Without branches, roundings to whole numbers by addition and powers of two by the exponent's bits
+// (a row with top_p 22 -> 12 us a pass of 50001, beside min, max, rint, ldexp and conversions of 64 bits). Below 2^-1000, -infinity among
+// them, is 2^-1000, which rounds to none.
 struct Weigher {
   float top;   // the row's largest logit
   double topd, c;
   int F;
+  __device__ __forceinline__ Weigher(float t, double factor, int f) : top(t), topd(t), c(factor), F(f) {}
   __device__ __forceinline__ double units(float x) const {
-    const double y = __builtin_fmax(__builtin_fmin((static_cast<double>(x) - topd) * c, 0.0), -1000.0);
-    const double n = __builtin_rint(y), r = y - n;
+    if (top == __builtin_inff()) return x == top ? __builtin_ldexp(1.0, F) : 0.0;  // the same for all
+    const double y = __builtin_fmax((static_cast<double>(x) - topd) * c, -1000.0);
+    const double whole = y + 6755399441055744.0, r = y - (whole - 6755399441055744.0);  // 1.5 2^52: its low bits are the whole number
     // ln(2)^k / k!
     double p = 4.44553827187081e-10;
     p = __builtin_fma(p, r, 7.054911620801121e-09);
@@ -84,7 +88,8 @@ struct Weigher {
     p = __builtin_fma(p, r, 0.2402265069591007);
     p = __builtin_fma(p, r, 0.6931471805599453);
     p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p, static_cast<int>(n) + F);
+    const u32x2 bits = __builtin_bit_cast(u32x2, p);
+    return __builtin_bit_cast(double, u32x2{bits[0], bits[1] + ((__builtin_bit_cast(u32x2, whole)[0] + static_cast<uint32_t>(F)) << 20)});
   }
   __device__ __forceinline__ static uint64_t whole(double u) {  // to nearest; u <= 2^51
     return __builtin_bit_cast(uint64_t, u + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
@@ -99,26 +104,41 @@ __device__ __forceinline__ int bin_of(float x, float top, float s) {
   return static_cast<int>(__builtin_amdgcn_fmed3f(half_below(x, top) * s, 0.f, static_cast<float>(SB - 1)));
 }
 
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int o) {
-  return static_cast<uint64_t>(static_cast<uint32_t>(__shfl_up(static_cast<int>(v >> 32), o, 64))) << 32 |
-         static_cast<uint32_t>(__shfl_up(static_cast<int>(v), o, 64));
+// A lane's value of another lane by the data path of its row (CTRL), 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, false));
+  return static_cast<uint64_t>(hi) << 32 | lo;
 }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  return static_cast<uint64_t>(static_cast<uint32_t>(__shfl_xor(static_cast<int>(v >> 32), o, 64))) << 32 |
-         static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64));
+__device__ __forceinline__ uint64_t last_lane(uint64_t v) {
+  return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63))) << 32 |
+         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += shfl_xor64(v, o);
-  return v;
+__device__ __forceinline__ uint64_t wave_scan64(uint64_t v) {  // inclusive
+  v += dpp64<0x111, 0xF>(v);  // from 1, 2, 4 and 8 lanes before, in a row of 16
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  v += dpp64<0x118, 0xF>(v);
+  v += dpp64<0x142, 0xA>(v);  // the row's last lane to the next row
+  return v + dpp64<0x143, 0xC>(v);  // lane 31 to the upper half
 }
-__device__ __forceinline__ uint64_t wave_scan64(uint64_t v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t u = shfl_up64(v, o);
-    if (lane >= o) v += u;
-  }
-  return v;
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) { return last_lane(wave_scan64(v)); }
+__device__ __forceinline__ uint64_t wave_max64(uint64_t v) {
+  auto with = [&](uint64_t u) { v = u > v ? u : v; };
+  with(dpp64<0x111, 0xF>(v));
+  with(dpp64<0x112, 0xF>(v));
+  with(dpp64<0x114, 0xF>(v));
+  with(dpp64<0x118, 0xF>(v));
+  with(dpp64<0x142, 0xA>(v));
+  with(dpp64<0x143, 0xC>(v));
+  return last_lane(v);
+}
+__device__ __forceinline__ uint64_t row_sum64(uint64_t v) {  // of 16 lanes, in the last of them
+  v += dpp64<0x111, 0xF>(v);
+  v += dpp64<0x112, 0xF>(v);
+  v += dpp64<0x114, 0xF>(v);
+  return v + dpp64<0x118, 0xF>(v);
 }
 
 // The number u's place in a sum s, rounded down: running sums of whole numbers pass u s where they pass it.
@@ -189,6 +209,7 @@ struct ListLds {
   uint64_t list[SLIST];    // composites
   uint64_t digits[256];    // also the weights of a short list
   uint64_t weight[256];    // of the row's parts
+  uint64_t before[SNEAR];
   uint32_t kind[SNEAR];
 };
 
@@ -234,7 +255,7 @@ __device__ __forceinline__ int find_bin(BlockLds& s, const HistLds& hist, uint64
     v[i] = MASS ? hist.mass[tid * N + i] : hist.count[tid * N + i];
     sum += v[i];
   }
-  const uint64_t inc = wave_scan64(sum, lane);
+  const uint64_t inc = wave_scan64(sum);
   __syncthreads();
   if (lane == 63) s.part[wave] = inc;
   if (tid == 0) {
@@ -324,7 +345,7 @@ __device__ __forceinline__ uint64_t find_composite(BlockLds& s, ListLds& t, uint
       uint64_t v[4], sum = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum += v[i] = t.digits[255 - 4 * lane - i];
-      uint64_t before = wave_scan64(sum, lane) - sum;
+      uint64_t before = wave_scan64(sum) - sum;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (before < need && before + v[i] >= need) {
@@ -346,7 +367,31 @@ __device__ __forceinline__ uint64_t find_composite(BlockLds& s, ListLds& t, uint
 // The composite from which on a row's tokens are kept. `n` tokens are listed, in t.list if no more than SLIST; `held` is the exact weight of the
 // sure ones, `mid` of what top_k keeps behind top_p's bins for certain. All threads.
 //
-// Of a short list: each token's number and weight of those before it.
+// Of a short list: each token's number and weight of those before it, by 16 lanes a token (158 tokens 14.8 -> 0.7 us beside a thread for each).
+// f(i, number, weight) in one lane for each token i; of j, `first` says whether it comes before i, t.kind[j] & 1 counts it and
+// t.digits[j] is what it adds.
+template <int NT, typename P, typename F>
+__device__ __forceinline__ void each_before(const ListLds& t, uint32_t n, P&& first, F&& f) {
+  const uint32_t lane = threadIdx.x & 15;
+#pragma unroll 1
+  for (uint32_t i0 = 0; i0 < n; i0 += NT / 16) {
+    const uint32_t i = i0 + (threadIdx.x >> 4);
+    const uint64_t c = t.list[i < n ? i : 0];
+    uint64_t number = 0, weight = 0;
+#pragma unroll 4
+    for (uint32_t j = lane; j < n; j += 16) {
+      const uint64_t cj = t.list[j], w = t.digits[j];
+      const uint32_t k = t.kind[j];
+      const bool is = first(cj, c);
+      number += is ? k & 1u : 0u;
+      weight += is ? w : 0;
+    }
+    number = row_sum64(number);
+    weight = row_sum64(weight);
+    if (lane == 15 && i < n) f(i, static_cast<uint32_t>(number), weight);
+  }
+}
+
 template <int NT>
 __device__ __forceinline__ uint64_t threshold_near(BlockLds& s, ListLds& t, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n, uint64_t held,
                                                    uint64_t mid) {
@@ -361,31 +406,25 @@ __device__ __forceinline__ uint64_t threshold_near(BlockLds& s, ListLds& t, cons
     in_k = b >= cut.klo && b <= cut.khi;
     in_p = b >= cut.plo && b <= cut.phi;
     before_k = b < cut.klo;
-    t.digits[tid] = w;
-    t.kind[tid] = (in_k ? 1 : 0) | (in_p ? 2 : 0);
+    t.digits[tid] = in_p ? w : 0;
+    t.kind[tid] = in_k ? 1 : 0;
   }
   if (tid == 0) s.a64 = s.b64 = 0;
   __syncthreads();
-  uint64_t before = 0;
-  uint32_t number = 0;
-  if (tid < static_cast<int>(n)) {
-#pragma unroll 4
-    for (uint32_t j = 0; j < n; ++j) {
-      const bool first = t.list[j] > c;
-      const uint32_t of = t.kind[j];
-      number += first ? of & 1u : 0u;
-      before += first && (of & 2u) ? t.digits[j] : 0;
-    }
-  }
-  if (d.k > 0) {
-    if (in_k && number + 1 == static_cast<uint32_t>(d.k) - cut.above) s.a64 = c;
-    __syncthreads();
-    threshold = s.a64;
-  }
+  const uint32_t want_k = static_cast<uint32_t>(d.k) - cut.above;
+  each_before<NT>(t, n, [](uint64_t x, uint64_t y) { return x > y; }, [&](uint32_t i, uint32_t number, uint64_t weight) {
+    if (d.k > 0 && (t.kind[i] & 1u) != 0 && number + 1 == want_k) s.a64 = t.list[i];
+    t.before[i] = weight;
+  });
+  __syncthreads();
+  threshold = s.a64;  // 0 without top_k
   if (d.p) {
     const uint64_t all = held + mid + block_sum64<NT>(s, before_k || c >= threshold ? w : 0);
     const uint64_t need = share_of(d.top_p, all), want = need > held ? need - held : 1;
-    if (in_p && before < want && before + w >= want) s.b64 = c;
+    if (in_p) {
+      const uint64_t before = t.before[tid];
+      if (before < want && before + w >= want) s.b64 = c;
+    }
     __syncthreads();
     threshold = s.b64 > threshold ? s.b64 : threshold;
   }
@@ -504,7 +543,7 @@ __device__ __forceinline__ Found draw_in(BlockLds& s, const R& r, int begin, int
     }
     Found found{0.f, -1, total};
     if (w != wave) return found;  // one load a lane, still in its registers
-    const uint64_t inc = wave_scan64(mine, lane);
+    const uint64_t inc = wave_scan64(mine);
     before = inc - mine;
     if (before <= target && target < inc) {
 #pragma unroll
@@ -528,9 +567,8 @@ __device__ __forceinline__ Found draw_parts(BlockLds& s, ListLds& t, const Sampl
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) sum += v[i] = lane * 4 + i < parts ? t.weight[lane * 4 + i] : 0;
-  const uint64_t inc = wave_scan64(sum, lane);
-  const uint64_t total = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc >> 32), 63))) << 32 |
-                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inc), 63));
+  const uint64_t inc = wave_scan64(sum);
+  const uint64_t total = last_lane(inc);
   const uint64_t target = place_of(static_cast<double>(a.u[row]), total);
   uint64_t before = inc - sum;
   if (tid < 64) {
@@ -573,22 +611,22 @@ __device__ __forceinline__ void add_list(ListLds& t, const R& r, int V, const Dr
 template <int NT>
 __device__ __forceinline__ Found draw_list(BlockLds& s, ListLds& t, const SampleArgs& a, int64_t row, const Keep& keep, uint32_t n) {
   const int tid = threadIdx.x;
-  const bool mine = tid < static_cast<int>(n);
-  uint64_t c = 0, k = 0;
-  float x = 0.f;
-  if (mine) {
-    c = t.list[tid];
-    x = of_okey(static_cast<uint32_t>(c >> 32));
-    k = keep(x, 0xFFFFFFFFu - static_cast<uint32_t>(c));
+  uint64_t k = 0;
+  if (tid < static_cast<int>(n)) {
+    const uint64_t c = t.list[tid];
+    k = keep(of_okey(static_cast<uint32_t>(c >> 32)), 0xFFFFFFFFu - static_cast<uint32_t>(c));
     t.digits[tid] = k;
   }
   const uint64_t total = block_sum64<NT>(s, k), target = place_of(static_cast<double>(a.u[row]), total);
-  Found found{x, -1, total};
-  if (k == 0) return found;
-  uint64_t before = 0;
-#pragma unroll 4
-  for (uint32_t j = 0; j < n; ++j) before += static_cast<uint32_t>(t.list[j]) > static_cast<uint32_t>(c) ? t.digits[j] : 0;  // of a lower index
-  if (before <= target && target < before + k) found.token = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(c));
+  Found found{0.f, -1, total};
+  each_before<NT>(t, n, [](uint64_t x, uint64_t y) { return static_cast<uint32_t>(x) > static_cast<uint32_t>(y); },  // a lower index
+                  [&](uint32_t i, uint32_t, uint64_t before) {
+                    if (before <= target && target < before + t.digits[i]) {
+                      const uint64_t c = t.list[i];
+                      found.token = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(c));
+                      found.x = of_okey(static_cast<uint32_t>(c >> 32));
+                    }
+                  });
   return found;
 }
 
@@ -612,11 +650,7 @@ __device__ __forceinline__ float thread_best(const R& r, int from, int to, uint3
 template <int NT>
 __device__ __forceinline__ uint64_t block_best(BlockLds& s, float x, uint32_t at) {
   uint64_t best = x > -__builtin_inff() ? composite(x, at) : 0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t c = shfl_xor64(best, o);
-    best = c > best ? c : best;
-  }
+  best = wave_max64(best);
   if ((threadIdx.x & 63) == 0) s.part[threadIdx.x >> 6] = best;
   __syncthreads();
 #pragma unroll
@@ -727,7 +761,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
     return;
   }
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
-  const Weigher weigh{top, static_cast<double>(top), d.c, F};
+  const Weigher weigh(top, d.c, F);
   Keep keep{weigh, d.least, 0};
   constexpr int parts = ST / 64;
   const int size = ((V + parts - 1) / parts + 64 * VEC - 1) / (64 * VEC) * (64 * VEC);
@@ -867,7 +901,7 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
     return;
   }
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
-  const Weigher weigh{top, static_cast<double>(top), d.c, F};
+  const Weigher weigh(top, d.c, F);
   if (d.k == 0 && !d.p) {
     const Keep keep{weigh, d.least, 0};
     uint64_t mine = 0;
@@ -930,7 +964,7 @@ __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, 
   const uint64_t best = w->best;
   if (best == 0) return;  // drawn, or nothing to draw
   const float top = of_okey(static_cast<uint32_t>(best >> 32));
-  const Weigher weigh{top, static_cast<double>(top), d.c, F};
+  const Weigher weigh(top, d.c, F);
   const Cut cut = sh->cut;
   uint64_t held = 0, kept = 0, mid = 0;
   if (tid == 0) s.n = 0;
