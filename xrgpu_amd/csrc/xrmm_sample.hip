@@ -43,7 +43,7 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs& a, int64_t row, int F)
   const double m = a.min_p ? static_cast<double>(a.min_p[row]) : a.min_p1;
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   d.greedy = !(t > 0.0);
-  const double heat = d.greedy ? 1.0 : t < 1e300 ? t : 1e300;  // an infinity's distance stays one
+  const double heat = d.greedy ? 1.0 : t < 1e30 ? t : 1e30;  // the largest float32, which stands for infinity, stays far from others
   d.c = 1.44269504088896340736 / heat;
   d.s = 2.f * SB_NAT / static_cast<float>(heat);
   d.k = k > 0 && k < a.V ? k : 0;
@@ -62,31 +62,36 @@ __device__ __forceinline__ float of_okey(uint32_t k) {
 }
 __device__ __forceinline__ uint64_t composite(float x, uint32_t i) { return static_cast<uint64_t>(okey(x)) << 32 | (0xFFFFFFFFu - i); }
 
+// p r + c with c in scalar registers: the compiler's own choice copies c to vector registers for each product.
+__device__ __forceinline__ double fma_s(double p, double r, double c) {
+  double o;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(o) : "v"(p), "v"(r), "s"(c));
+  return o;
+}
+
 // What a logit weighs, in units of 2^-F of the largest, not yet rounded: 2^n 2^r for y = n + r, |r| <= 1/2, by the Taylor series of 2^r
-// up to r^11, whose rest is 6 10^-15. Without branches, roundings to whole numbers by addition and powers of two by the exponent's bits
-// (a row with top_p 22 -> 12 us a pass of 50001, beside min, max, rint, ldexp and conversions of 64 bits). Below 2^-1000, -infinity among
-// them, is 2^-1000, which rounds to none.
+// up to r^11, whose rest is 6 10^-15. Without branches, roundings to whole numbers by addition and powers of two by the exponent's bits.
+// Below 2^-1000, -infinity among them, is 2^-1000, which rounds to none.
 struct Weigher {
   float top;   // the row's largest logit
   double topd, c;
   int F;
   __device__ __forceinline__ Weigher(float t, double factor, int f) : top(t), topd(t), c(factor), F(f) {}
   __device__ __forceinline__ double units(float x) const {
-    if (top == __builtin_inff()) return x == top ? __builtin_ldexp(1.0, F) : 0.0;  // the same for all
     const double y = __builtin_fmax((static_cast<double>(x) - topd) * c, -1000.0);
     const double whole = y + 6755399441055744.0, r = y - (whole - 6755399441055744.0);  // 1.5 2^52: its low bits are the whole number
     // ln(2)^k / k!
     double p = 4.44553827187081e-10;
-    p = __builtin_fma(p, r, 7.054911620801121e-09);
-    p = __builtin_fma(p, r, 1.0178086009239696e-07);
-    p = __builtin_fma(p, r, 1.3215486790144305e-06);
-    p = __builtin_fma(p, r, 1.5252733804059838e-05);
-    p = __builtin_fma(p, r, 0.00015403530393381606);
-    p = __builtin_fma(p, r, 0.0013333558146428441);
-    p = __builtin_fma(p, r, 0.009618129107628477);
-    p = __builtin_fma(p, r, 0.055504108664821576);
-    p = __builtin_fma(p, r, 0.2402265069591007);
-    p = __builtin_fma(p, r, 0.6931471805599453);
+    p = fma_s(p, r, 7.054911620801121e-09);
+    p = fma_s(p, r, 1.0178086009239696e-07);
+    p = fma_s(p, r, 1.3215486790144305e-06);
+    p = fma_s(p, r, 1.5252733804059838e-05);
+    p = fma_s(p, r, 0.00015403530393381606);
+    p = fma_s(p, r, 0.0013333558146428441);
+    p = fma_s(p, r, 0.009618129107628477);
+    p = fma_s(p, r, 0.055504108664821576);
+    p = fma_s(p, r, 0.2402265069591007);
+    p = fma_s(p, r, 0.6931471805599453);
     p = __builtin_fma(p, r, 1.0);
     const u32x2 bits = __builtin_bit_cast(u32x2, p);
     return __builtin_bit_cast(double, u32x2{bits[0], bits[1] + ((__builtin_bit_cast(u32x2, whole)[0] + static_cast<uint32_t>(F)) << 20)});
@@ -99,7 +104,6 @@ struct Weigher {
 // Half of top - x: no finite logits' overflows.
 __device__ __forceinline__ float half_below(float x, float top) { return __builtin_fmaf(x, -0.5f, 0.5f * top); }
 
-// A NaN, an infinity less itself, comes to 0.
 __device__ __forceinline__ int bin_of(float x, float top, float s) {
   return static_cast<int>(__builtin_amdgcn_fmed3f(half_below(x, top) * s, 0.f, static_cast<float>(SB - 1)));
 }
@@ -157,9 +161,10 @@ struct RowOf {
   static constexpr int VEC = N;
   typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   const T* x;
-  __device__ __forceinline__ static float value(T v) {  // NaN is -infinity
-    const float f = static_cast<float>(v);
-    return f == f ? f : -__builtin_inff();
+  // NaN is -infinity, infinity the largest float32
+  __device__ __forceinline__ static float value(T v) {
+    const float x = static_cast<float>(v);
+    return x == x ? fminf(x, 3.4028234663852886e38f) : -__builtin_inff();
   }
   // f(VEC values, index of the first) for `step` threads' vectors of from .. to - 1, this thread the `first` of them; AHEAD loads in flight.
   // The last vector ends with the stretch: what it repeats is -infinity. A row has VEC logits at least.
@@ -667,14 +672,14 @@ __device__ __forceinline__ void count_in(HistLds& hist, const R& r, int from, in
     return;
   }
   const float c = static_cast<float>(-2.0 * d.c);
-  r.template each<1>(from, to, static_cast<int>(threadIdx.x), NT, [&](const float (&f)[VEC], int) {
+  r.template each<4>(from, to, static_cast<int>(threadIdx.x), NT, [&](const float (&f)[VEC], int) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       if (!(f[e] > -__builtin_inff())) continue;  // rows that a grammar masks would meet in one bin
       const int b = bin_of(f[e], weigh.top, d.s);
       if (d.k > 0) atomicAdd(&hist.count[b], 1u);
       if (d.p) {
-        const float y = __builtin_fminf(half_below(f[e], weigh.top) * c, 0.f);
+        const float y = half_below(f[e], weigh.top) * c;
         atomicAdd(reinterpret_cast<unsigned long long*>(&hist.mass[b]),
                   static_cast<unsigned long long>(static_cast<uint32_t>(__builtin_amdgcn_exp2f(y + static_cast<float>(SAPPROX)))));
       }
@@ -690,18 +695,28 @@ __device__ __forceinline__ void split_in(const R& r, int from, int to, int first
   constexpr int VEC = R::VEC;
   if (d.k == 0) {  // top_p alone: every token's weight counts
     uint64_t all = 0, sure = 0, listed = 0;
-    r.template each<1>(from, to, first, step, [&](const float (&f)[VEC], int i) {
+    r.template each<4>(from, to, first, step, [&](const float (&f)[VEC], int i) {
+      bool any = false;
+      uint64_t w[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const int b = bin_of(f[e], weigh.top, d.s);
         const double u = weigh.units(f[e]);
-        const uint64_t w = Weigher::whole(u), ws = b < cut.sure ? w : 0;
-        all += w;
+        w[e] = Weigher::whole(u);
+        const uint64_t ws = b < cut.sure ? w[e] : 0;
+        all += w[e];
         sure += ws;
         if (d.least > 0.0) kept += u >= d.least ? ws : 0;
-        if (b >= cut.plo && b <= cut.phi && f[e] > -__builtin_inff()) {
-          listed += w;
-          list(composite(f[e], i + e));
+        any |= b >= cut.plo && b <= cut.phi;
+      }
+      if (any) {  // few vectors
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const int b = bin_of(f[e], weigh.top, d.s);
+          if (b >= cut.plo && b <= cut.phi && f[e] > -__builtin_inff()) {
+            listed += w[e];
+            list(composite(f[e], i + e));
+          }
         }
       }
     });
@@ -710,7 +725,7 @@ __device__ __forceinline__ void split_in(const R& r, int from, int to, int first
     mid = all - sure - listed;
     return;
   }
-  r.template each<1>(from, to, first, step, [&](const float (&f)[VEC], int i) {
+  r.template each<4>(from, to, first, step, [&](const float (&f)[VEC], int i) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       const int b = bin_of(f[e], weigh.top, d.s);
@@ -768,7 +783,7 @@ __global__ __launch_bounds__(ST) void k_sample_row(SampleArgs a, int F) {
   const int from = wave * size < V ? wave * size : V, to = V - from < size ? V : from + size;
   if (!filter) {
     uint64_t kept = 0;
-    r.template each<1>(from, to, lane, 64, [&](const float (&f)[VEC], int) {
+    r.template each<4>(from, to, lane, 64, [&](const float (&f)[VEC], int) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const double u = weigh.units(f[e]);
@@ -905,7 +920,7 @@ __global__ __launch_bounds__(SP) void k_sample_mass(SampleArgs a, SamplePlan p, 
   if (d.k == 0 && !d.p) {
     const Keep keep{weigh, d.least, 0};
     uint64_t mine = 0;
-    r.template each<1>(from, to, tid, SP, [&](const float (&f)[VEC], int) {
+    r.template each<4>(from, to, tid, SP, [&](const float (&f)[VEC], int) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const double u = weigh.units(f[e]);
