@@ -1029,10 +1029,26 @@ __global__ __launch_bounds__(SP) void k_sample_draw(SampleArgs a, SamplePlan p, 
   found.write(a, row, weigh);
 }
 
-// Rows by parts where one workgroup a row would leave CUs idle and a row is long enough to pay for the launches.
-bool sample_split(int64_t rows, int64_t V, SamplePlan& p) {
-  if (rows < 1 || rows > SAMPLE_ROWS || rows > 128 || V < 8192) return false;
-  int64_t parts = 1024 / rows;
+// What a call's rows ask for: the numbers of estimated times below.
+enum Kind { NO_FILTER, TOP_K, TOP_P };
+
+Kind kind_of(const SampleArgs& a) {
+  if (a.top_p != nullptr || a.top_p1 < 1.0) return TOP_P;
+  return a.top_k != nullptr || (a.top_k1 > 0 && a.top_k1 < a.V) ? TOP_K : NO_FILTER;
+}
+
+// Rows by parts where that is estimated faster (us, measured on float32 logits, no filter / top_k 50 / top_p 0.95):
+//   a workgroup a row: 7 + V / 2950, 10.5 + V / 5400, 12 + V / 1500 for each round of 256 (32000 logits: 16.6, 16.8, 33; 128000: 50, 34, 98)
+//   by parts: 10.5, 22, 28 and the logits at 330, 500 and 170 thousand a us (1 x 128000: 11, 23, 34; 64 x 128000: 36, 38, 75)
+// 64 parts a row and 512 workgroups at most, 1024 from 32 rows on (16 x 128000 with top_p 48 in 32 parts, 58 in 64; 64 x 128000 75
+// in 16, 77 in 8).
+bool sample_split(int64_t rows, int64_t V, Kind kind, SamplePlan& p) {
+  static constexpr double kRow[3] = {7.0, 10.5, 12.0}, kRowRate[3] = {2950, 5400, 1500}, kStart[3] = {10.5, 22.0, 28.0}, kRate[3] = {330e3, 500e3, 170e3};
+  if (rows < 1 || rows > SAMPLE_ROWS || V < 4096) return false;
+  const double whole = kRow[kind] + static_cast<double>(V) / kRowRate[kind];
+  const double parted = kStart[kind] + (kind == TOP_P && rows > 1 ? 6.0 : 0.0) + static_cast<double>(rows) * static_cast<double>(V) / kRate[kind];
+  if (whole <= parted) return false;
+  int64_t parts = (rows < 32 ? 512 : 1024) / rows;
   parts = parts < 64 ? parts : 64;
   const int64_t most = (V + 2047) / 2048;
   parts = parts < most ? parts : most;
@@ -1044,11 +1060,11 @@ bool sample_split(int64_t rows, int64_t V, SamplePlan& p) {
 template <typename T>
 hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
   SamplePlan p;
-  if (a.ws != nullptr && sample_split(a.rows, a.V, p) && a.ws_bytes >= SAMPLE_HEAD + a.rows * p.row_bytes()) {
+  if (a.ws != nullptr && sample_split(a.rows, a.V, kind_of(a), p) && a.ws_bytes >= SAMPLE_HEAD + a.rows * p.row_bytes()) {
     const dim3 grid(static_cast<uint32_t>(p.parts), static_cast<uint32_t>(a.rows));
     k_sample_top<T><<<grid, SP, 0, st>>>(a, p, F);
     k_sample_mass<T><<<grid, SP, 0, st>>>(a, p, F);
-    if (a.top_k != nullptr || a.top_p != nullptr || (a.top_k1 > 0 && a.top_k1 < a.V) || a.top_p1 < 1.0) k_sample_draw<T><<<grid, SP, 0, st>>>(a, p, F);
+    if (kind_of(a) != NO_FILTER) k_sample_draw<T><<<grid, SP, 0, st>>>(a, p, F);
     return hipGetLastError();
   }
   const dim3 grid(static_cast<uint32_t>(a.rows));
@@ -1059,9 +1075,15 @@ hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
 
 }  // namespace
 
-int64_t sample_workspace_bytes(int64_t rows, int64_t V) {
-  SamplePlan p;
-  return sample_split(rows, V, p) ? SAMPLE_HEAD + rows * p.row_bytes() : 0;
+int64_t sample_workspace_bytes(int64_t rows, int64_t V) {  // whatever the call's settings
+  int64_t most = 0;
+  for (const Kind kind : {NO_FILTER, TOP_K, TOP_P}) {
+    SamplePlan p;
+    if (!sample_split(rows, V, kind, p)) continue;
+    const int64_t n = SAMPLE_HEAD + rows * p.row_bytes();
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st) {
