@@ -13,6 +13,14 @@ def ops():
     return _ops
 
 
+@pytest.fixture(params=["", "kv8_walk", "kv8_prefix_rows", "kv8_prefix_tile"], autouse=True)
+def way(request, monkeypatch):
+    """Every test by each way that a call can go, beside the one that is estimated fastest."""
+    if request.param:
+        monkeypatch.setenv("XRMM_KV8_SHARED", request.param)
+    return request.param
+
+
 def shared_cache(kind, shared, lens, H, D, page, **kw):
     """A cache whose sequences have ``lens`` tokens, the first ``shared`` pages common to all: the oracle's table names them, the
     device's holds what must not be read there."""
@@ -232,3 +240,35 @@ def test_streams_workspaces_graphs_and_repeats(gpu, B, n):
             # another order of the sums, and weights of eleven bits: within their rounding of the eager call's
             e = ops().kv8_shared_attention(q, **d)
             assert (got.float() - e.float()).abs().max() <= 2.0 ** -7 * float(e.float().abs().max())
+
+
+def test_the_named_way_is_taken(gpu, way):
+    kw = dict(batch=40, shared_pages=4, table_width=6, page_size=16)
+    name = ops().kv8_shared_attention_kernel(40, 8, 2, 64, **kw)
+    assert name == way if way else name in ("kv8_walk", "kv8_prefix_rows", "kv8_prefix_tile")
+
+
+@pytest.mark.parametrize("D,G,page", [(128, 4, 64), (64, 8, 16), (256, 4, 128), (96, 1, 32)])
+def test_sequences_that_end_among_the_shared_tokens_of_many(gpu, D, G, page):
+    """Rows of one tile whose sequences see all, some and none of the shared tokens, in no order, with and without windows."""
+    S = 600 // page
+    lens = [(S * page + 40, 17, S * page, 0, S * page + 1, 300, S * page - 1, 64)[b % 8] for b in range(45)]
+    c, d = shared_cache("int8", S, lens, 1, D, page, seed=D, scales="any")
+    q = torch.randn(45, G, D, generator=torch.Generator().manual_seed(D)).half().cuda()
+    for kw in (dict(), dict(window=100), dict(causal=False), dict(causal=False, window=90)):
+        check(c, d, q, [1] * 45, **kw)
+    counts = [min(n, (1, 3, 0, 2)[b % 4]) for b, n in enumerate(lens)]
+    q = torch.randn(sum(counts), G, D, generator=torch.Generator().manual_seed(D)).half().cuda()
+    for kw in (dict(), dict(window=100)):
+        check(c, d, q, counts, **kw)
+
+
+@pytest.mark.parametrize("kind,dt,D,n", [("int8", "f16", 128, 60), ("e4m3", "bf16", 64, 130), ("int8", "bf16", 256, 40)])
+def test_long_shared_parts_are_split(gpu, kind, dt, D, n):
+    """Shared tokens in several parts, own tokens of many rows; value scales far apart in the parts."""
+    c, d = shared_cache(kind, 24, [24 * 64 + n + 7, 24 * 64 + n], 1, D, 64, seed=D)
+    pages = d["shared_pages"].cpu().numpy()
+    c.vs[pages[5:9]] *= np.float32(64.0)
+    d["v_scales"] = torch.from_numpy(c.vs.copy()).cuda()
+    q = torch.randn(2 * n, 8, D, generator=torch.Generator().manual_seed(D)).to(DT[dt]).cuda()
+    check(c, d, q, [n, n])

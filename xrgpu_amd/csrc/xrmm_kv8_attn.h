@@ -993,10 +993,7 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
             for (int e = 1; e < 8; ++e) x = fmaxf(x, s[u / 2][8 * (u & 1) + e]);
             top = fmaxf(top, x * (qs * of(sc, u)));
           }
-          {
-            const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, top), false, false);
-            top = fmaxf(__builtin_bit_cast(float, both[0]), __builtin_bit_cast(float, both[1]));
-          }
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
           if (__any(top > m + KV_LAG || was < ve)) {
             const float mn = fmaxf(m, top), base = mn == -__builtin_inff() ? 0.f : mn;
             const float f = __builtin_amdgcn_exp2f(m - base);

@@ -1,4 +1,7 @@
 // Attention of a batch whose sequences' first tokens lie in the same pages of the 8-bit cache.
+#include <cstdlib>
+#include <cstring>
+
 #include "xrmm_kv8_attn.h"
 
 namespace xrmm {
@@ -40,7 +43,8 @@ __global__ __launch_bounds__(KVJ_T) void k_kv8_join(KvAttnArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (p0 + 4 * i >= a.parts || ml[i][0] == -__builtin_inff()) continue;  // no such part, or one that saw nothing and left no outputs
+      // no such part, or one that saw nothing and left no outputs; a query that is no number has a sum that is none
+      if (p0 + 4 * i >= a.parts || (ml[i][0] == -__builtin_inff() && ml[i][1] == 0.f)) continue;
       const float mn = fmaxf(m, ml[i][0]), f0 = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[i][0] - mn);
       o = o * f0 + x[i] * f1;
       l = l * f0 + ml[i][1] * f1;
@@ -115,7 +119,11 @@ struct SharedPlan {
   int64_t ws_bytes;
 };
 
+// XRMM_KV8_SHARED names a way (as xrmm_kv8_shared_attention_kernel does) to take instead of the fastest one, where a call can go it.
 SharedPlan shared_plan(const KvAttnArgs& a, bool have_ws) {
+  const char* way = std::getenv("XRMM_KV8_SHARED");
+  const bool walk = way != nullptr && std::strcmp(way, "kv8_walk") == 0, rows = way != nullptr && std::strcmp(way, "kv8_prefix_rows") == 0,
+             tile = way != nullptr && std::strcmp(way, "kv8_prefix_tile") == 0;
   SharedPlan s{};
   const int64_t G = a.Hq / a.c.Hkv, tokens = static_cast<int64_t>(a.shared_pages) << a.c.page_log2;
   // the walk begins at a multiple of a tile's tokens before the sequences' own
@@ -123,18 +131,19 @@ SharedPlan shared_plan(const KvAttnArgs& a, bool have_ws) {
   s.walk = true;
   s.all = attention_plan(a, have_ws);
   s.ws_bytes = s.all.ws_bytes;
-  if (!have_ws || tokens == 0 || a.c.B < 2 || a.c.rows * G > 0x7FFFFFF0) return s;
+  if (!have_ws || tokens == 0 || a.c.B < 2 || a.c.rows * G > 0x7FFFFFF0 || walk) return s;
   auto least = [&](int64_t nrows, int64_t seqs, int64_t span) {
     const KvPlan x = part_plan(a, nrows, seqs, span, false);
     if (nrows <= 16) return x;
     const KvPlan y = part_plan(a, nrows, seqs, span, true);
     return y.time < x.time ? y : x;
   };
-  s.prefix = least(a.c.rows * G, 1, tokens);
+  s.prefix = rows || tile ? part_plan(a, a.c.rows * G, 1, tokens, tile) : least(a.c.rows * G, 1, tokens);
   s.own = least(static_cast<int64_t>(a.max_new) * G, a.c.B, own);
-  if (s.prefix.time + s.own.time + 4.0 < s.all.time) {
+  const int64_t bytes = KV_COUNTERS + (s.prefix.splits + s.own.splits) * a.c.rows * a.Hq * (a.c.D + 2) * 4;
+  if ((rows || tile || s.prefix.time + s.own.time + 4.0 < s.all.time) && bytes <= int64_t{1} << 28) {
     s.walk = false;
-    s.ws_bytes = KV_COUNTERS + (s.prefix.splits + s.own.splits) * a.c.rows * a.Hq * (a.c.D + 2) * 4;
+    s.ws_bytes = bytes;
   }
   return s;
 }
