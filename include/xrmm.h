@@ -558,8 +558,8 @@ int xrmm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_
  * top_p >= 1: all); of those the ones with w >= min_p. The token is the first, by index, at
  * which the running sum of the kept weights exceeds uniforms[row] (float32, [0, 1)) of their sum: tokens int32, shares
  * float32: the logarithm of its part of that sum. Temperature 0 takes the largest. NaN and
- * -infinity are never drawn; a row of nothing else gives token -1 and share -infinity. An infinity
- * leaves only infinities. Weights are whole multiples of 2^-F of the largest, F = min(51, 62 -
+ * -infinity are never drawn; a row of nothing else gives token -1 and share -infinity. Infinity counts
+ * as the largest float32, and temperatures as ones from 10^-30 to 10^30. Weights are whole multiples of 2^-F of the largest, F = min(51, 62 -
  * ceil(log2 vocab)): sums are exact, and a token of less than half a unit is not drawn. Arrays by row take the place
  * of the one setting where not NULL (float32; top_k int32); in them a temperature not above 0 or NaN
  * is 0, top_k below 1 is all, a NaN top_p or min_p is off, and others are clamped to [0, 1]. The

@@ -113,3 +113,22 @@ def test_shared_front_refuses():
     for x, msg in ((q.float(), "q must be"), (z(2, 3, 64), "multiple"), (z(2, 2, 96), r"\[tokens, 2, 64\]")):
         with pytest.raises(nat.XrmmInvalid, match=msg):
             ops.kv8_shared_attention(x, shared_pages=P, **cache())
+
+
+def test_shared_attention_names_its_way(monkeypatch):
+    f = lambda T, B, S, W, **kw: ops.kv8_shared_attention_kernel(T, 32, 8, 128, batch=B, shared_pages=S, table_width=W, page_size=64, **kw)
+    size = lambda T, B, S, W: ops.kv8_shared_attention_workspace_bytes(T, 32, 8, 128, batch=B, shared_pages=S, table_width=W, page_size=64)
+    assert f(64, 64, 128, 138) == "kv8_prefix_tile" and f(1, 1, 128, 138) == "kv8_walk" and f(64, 64, 0, 138) == "kv8_walk"
+    assert size(64, 64, 128, 138) > size(64, 64, 0, 138)
+    monkeypatch.setenv("XRMM_KV8_SHARED", "kv8_prefix_rows")
+    assert f(64, 64, 128, 138) == "kv8_prefix_rows" and f(1, 1, 128, 138) == "kv8_walk"
+    monkeypatch.setenv("XRMM_KV8_SHARED", "kv8_walk")
+    assert f(64, 64, 128, 138) == "kv8_walk"
+    with pytest.raises(nat.XrmmInvalid, match="head size"):
+        ops.kv8_shared_attention_kernel(1, 8, 2, 80, batch=1, shared_pages=1, table_width=1, page_size=64)
+
+
+def test_sample_workspaces():
+    """None where a workgroup a row is estimated fastest whatever is asked for."""
+    assert ops.sample_workspace_bytes(1, 128000) > 4096 and ops.sample_workspace_bytes(1, 2000) == 0 and ops.sample_workspace_bytes(500, 128000) == 0
+    assert ops.sample_workspace_bytes(0, 128000) == 0 and ops.sample_workspace_bytes(4, 0) == 0

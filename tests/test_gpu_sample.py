@@ -208,3 +208,15 @@ def test_one_workspace_serves_different_calls_in_turn(gpu):
     for _ in range(2):
         for (x, n, kw), w in zip(calls, want):
             assert all(torch.equal(a, b) for a, b in zip(o.sample(x, n, **kw), w))
+
+
+@pytest.mark.parametrize("B,V", [(260, 5000), (3, 100000)])
+def test_more_ties_than_the_list_holds(gpu, B, V):
+    """By a workgroup a row and by parts: thousands of equal logits where the thresholds lie."""
+    x = torch.zeros(B, V, device="cuda")
+    x[:, 7::V // 3] = 2.0  # three or four larger ones
+    u = torch.rand(B, generator=torch.Generator().manual_seed(B)).cuda()
+    for kw in (dict(top_k=V // 2), dict(top_p=0.5003), dict(top_k=V // 2, top_p=0.7123), dict(top_k=V // 2, top_p=0.7123, min_p=0.01)):
+        t, s = ops().sample(x, u, **kw)
+        rows = [0, B // 2, B - 1]
+        check(x[rows], u[rows], got=(t[rows], s[rows]), **kw)

@@ -43,7 +43,8 @@ __device__ __forceinline__ Draw draw_of(const SampleArgs& a, int64_t row, int F)
   const double m = a.min_p ? static_cast<double>(a.min_p[row]) : a.min_p1;
   const int k = a.top_k ? a.top_k[row] : a.top_k1;
   d.greedy = !(t > 0.0);
-  const double heat = d.greedy ? 1.0 : t < 1e30 ? t : 1e30;  // the largest float32, which stands for infinity, stays far from others
+  // 10^-30 to 10^30: the factors stay finite, and the largest float32, which stands for infinity, far from other logits
+  const double heat = d.greedy ? 1.0 : t < 1e-30 ? 1e-30 : t < 1e30 ? t : 1e30;
   d.c = 1.44269504088896340736 / heat;
   d.s = 2.f * SB_NAT / static_cast<float>(heat);
   d.k = k > 0 && k < a.V ? k : 0;
