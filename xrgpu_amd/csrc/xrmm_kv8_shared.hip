@@ -15,7 +15,8 @@ namespace {
 
 // The parts of a row: weights exp2(maximum - the largest maximum), outputs added in a fixed order, divided by the sum. A thread has four
 // values of a row and every fourth part, a wave's groups of 16 threads the four shares, and their loads in flight together; the shares meet across
-// the wave. Rows that `starts` leaves out are not written.
+// the wave. The parts' bytes and the start bound it: 11 us for 64 sequences of 32 heads of 128 in 33 parts (35 MB), 9.6 for 128 in 17 (36 MB), which
+// is why part_plan counts the parts' bytes. Rows that `starts` leaves out are not written.
 constexpr int KVJ_T = 256;
 
 template <int D>

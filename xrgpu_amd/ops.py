@@ -1108,10 +1108,10 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, workspa
     (0: all), of those the shortest prefix with at least ``top_p`` of their weight (one token at least), of those the ones with
     a weight of ``min_p`` or more. The token is the first, by index, at which the running sum of the kept weights exceeds u of
     their sum; its share of that sum comes back as a logarithm. Temperature 0 takes the largest. Each setting is a number or a
-    tensor ``[rows]`` (float32; top_k int32). NaN and -infinity are never drawn: a row of nothing else gives token -1. Sums are of
-    whole numbers (a weight is one in units of 2^-46 of the largest at 2^16 tokens), so results do not depend on how a call is spread
-    over the device. Few rows are, on a workspace (``sample_workspace_bytes``; see ``matmul_nbits`` for whose it is and for
-    graph capture)."""
+    tensor ``[rows]`` (float32; top_k int32). NaN and -infinity are never drawn: a row of nothing else gives token -1. Infinity counts
+    as the largest float32, temperatures outside 1e-30 .. 1e30 as these. Sums are of whole numbers (a weight is one in units of
+    2^-46 of the largest at 2^16 tokens), so results do not depend on how a call is spread over the device. Few rows are, on
+    a workspace (``sample_workspace_bytes``; see ``matmul_nbits`` for whose it is and for graph capture)."""
     if workspace is None and stream is None and _front():
         r = _FRONT.sample(logits, u, temperature, top_k, top_p, min_p)
         if r is not None and type(r) is not int:
