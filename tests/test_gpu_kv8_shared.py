@@ -272,3 +272,24 @@ def test_long_shared_parts_are_split(gpu, kind, dt, D, n):
     d["v_scales"] = torch.from_numpy(c.vs.copy()).cuda()
     q = torch.randn(2 * n, 8, D, generator=torch.Generator().manual_seed(D)).to(DT[dt]).cuda()
     check(c, d, q, [n, n])
+
+
+def test_sequences_of_more_rows_than_max_new(gpu, way):
+    """They count as wrong: their rows stay as they are, the others' are right."""
+    B, shared, page, D = 40, 12, 64, 128
+    counts = [1 + b % 2 for b in range(B)]
+    counts[3] = 5
+    c, d = shared_cache("int8", shared, [shared * page + 7 + 3 * b for b in range(B)], 1, D, page, seed=21)
+    q = torch.randn(sum(counts), 4, D, generator=torch.Generator().manual_seed(21)).half().cuda()
+    want = ops().kv8_shared_attention(q, **d, starts=starts_of(counts), max_new=5)
+    out, status = torch.full_like(q, 7.0), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops().kv8_shared_attention(q, **d, starts=starts_of(counts), max_new=2, out=out, status=status)
+    first = sum(counts[:3])
+    assert int(status.item()) == 55 and (out[first:first + 5] == 7).all()
+    # either call: weights rounded to binary16 (half a step, 2^-11) and the outputs too; scores as float32 sums of D products
+    keep = torch.ones(len(q), dtype=torch.bool, device="cuda")
+    keep[first:first + 5] = False
+    top_k, top_v = 128 * float(c.ks.max()), 128 * float(c.vs.max())
+    scores = D * 2.0 ** -24 * float(q.float().abs().sum(-1).max()) * top_k / D ** 0.5
+    o, w = out[keep].double(), want[keep].double()
+    assert ((o - w).abs() <= 2 * top_v * (2.0 ** -11 + 2 * scores) + (o.abs() + w.abs()) * 2.0 ** -11).all()
