@@ -114,6 +114,9 @@ KvPlan part_plan(const KvAttnArgs& a, int64_t nrows, int64_t seqs, int64_t span,
   return p;
 }
 
+// Whether own rows go into one launch with tiles of the shared tokens.
+bool together(const KvAttnArgs& a, const KvPlan& own) { return !own.tile && own.row_tiles == 1 && a.c.D <= 128; }
+
 struct SharedPlan {
   bool walk;  // the sequences one by one, over all of their tokens
   KvPlan all, prefix, own;
@@ -133,16 +136,18 @@ SharedPlan shared_plan(const KvAttnArgs& a, bool have_ws) {
   s.all = attention_plan(a, have_ws);
   s.ws_bytes = s.all.ws_bytes;
   if (!have_ws || tokens == 0 || a.c.B < 2 || a.c.rows * G > 0x7FFFFFF0 || walk) return s;
-  auto least = [&](int64_t nrows, int64_t seqs, int64_t span) {
-    const KvPlan x = part_plan(a, nrows, seqs, span, false);
-    if (nrows <= 16) return x;
-    const KvPlan y = part_plan(a, nrows, seqs, span, true);
-    return y.time < x.time ? y : x;
-  };
-  s.prefix = rows || tile ? part_plan(a, a.c.rows * G, 1, tokens, tile) : least(a.c.rows * G, 1, tokens);
-  s.own = least(static_cast<int64_t>(a.max_new) * G, a.c.B, own);
+  const int64_t nrows = static_cast<int64_t>(a.max_new) * G;
+  auto faster = [](const KvPlan& x, const KvPlan& y, double more) { return y.time + more < x.time ? y : x; };
+  s.own = part_plan(a, nrows, a.c.B, own, false);
+  if (nrows > 16) s.own = faster(s.own, part_plan(a, nrows, a.c.B, own, true), 0.0);
+  // Beside tiles the own rows cost about half of their time: with that counted, 64 rows a key head on 6400 shared tokens (8 heads of 128) go by
+  // tiles, 23 us for 29 by rows.
+  const double beside = together(a, s.own) ? 0.5 * s.own.time : s.own.time;
+  s.prefix = part_plan(a, a.c.rows * G, 1, tokens, tile);
+  if (!rows && !tile && a.c.rows * G > 16) s.prefix = faster(s.prefix, part_plan(a, a.c.rows * G, 1, tokens, true), beside - s.own.time);
+  const double time = s.prefix.time + (s.prefix.tile ? beside : s.own.time) + 4.0;
   const int64_t bytes = KV_COUNTERS + (s.prefix.splits + s.own.splits) * a.c.rows * a.Hq * (a.c.D + 2) * 4;
-  if ((rows || tile || s.prefix.time + s.own.time + 4.0 < s.all.time) && bytes <= int64_t{1} << 28) {
+  if ((rows || tile || time < s.all.time) && bytes <= int64_t{1} << 28) {
     s.walk = false;
     s.ws_bytes = bytes;
   }
@@ -170,7 +175,7 @@ hipError_t launch_kv8_shared_attention(const KvAttnArgs& a, hipStream_t st) {
   x.parts = static_cast<int32_t>(p.prefix.splits + p.own.splits);
   x.parts_at = KV_COUNTERS;
   x.part0 = 0;
-  if (p.prefix.tile && !p.own.tile && p.own.row_tiles == 1 && a.c.D <= 128) {
+  if (p.prefix.tile && together(a, p.own)) {
     const hipError_t e = launch_kv8_both(x, p.prefix, p.own, st);
     return e == hipSuccess ? launch_join(x, st) : e;
   }
