@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from oracle import lowbit as LB
 from tests.test_gpu_kv8 import DT, Cache, check_attention, starts_of
 
 pytestmark = pytest.mark.gpu
@@ -293,3 +294,39 @@ def test_sequences_of_more_rows_than_max_new(gpu, way):
     scores = D * 2.0 ** -24 * float(q.float().abs().sum(-1).max()) * top_k / D ** 0.5
     o, w = out[keep].double(), want[keep].double()
     assert ((o - w).abs() <= 2 * top_v * (2.0 ** -11 + 2 * scores) + (o.abs() + w.abs()) * 2.0 ** -11).all()
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,G,n", [(64, 8, 1), (96, 4, 2), (128, 4, 1), (128, 16, 1), (256, 4, 1), (256, 5, 3)])
+def test_weights_of_few_rows_have_two_terms_by_every_way(gpu, kind, D, G, n):
+    """Up to 16 rows of a sequence and key head keep 22 bits of a weight, of shared tokens too, as kv8_attention's do.
+
+    Queries of eight small integers and key factors that are powers of two: sums of products are exact. In powers of two, of which ln 2 times as much
+    is a weight's relative error, a score is off by 2^-24 of the largest five times (log2 e, the product with it, the difference of two), and an exponent
+    of up to 16 by three roundings. With the exponentials' 2^-22 that counts in numerator and denominator; then the second terms' own rounding, 2^-22, and
+    float32 sums over the tokens, 2^-24 each: all of sum p |v| / sum p. At last an output's own rounding. Weights of eleven bits are off by up to 2^-12 each, some
+    2^-16 of that sum in the mean of 64, as many of these outputs would show."""
+    B, page, S = 40, 16, 4
+    lens = [S * page + n + b % 4 for b in range(B)]
+    lens[5], lens[17] = 50, 64  # among the shared tokens, and at their end
+    c, d = shared_cache(kind, S, lens, 1, D, page, seed=D + G)
+    g = np.random.default_rng(D + G)
+    c.ks[:] = 2.0 ** -7 if kind == "int8" else 2.0 ** -8
+    d["k_scales"] = torch.from_numpy(c.ks.copy()).cuda()
+    q = np.zeros((B * n, G, D))
+    for row in q.reshape(-1, D):
+        row[g.choice(D, 8, replace=False)] = g.integers(1, 4, 8) * g.choice((-1, 1), 8)
+    o = ops().kv8_shared_attention(torch.from_numpy(q).half().cuda(), **d, scale=2.0 ** -2).double().cpu().numpy()
+    for b, L in enumerate(lens):
+        pages = c.table[b, : -(-L // page)]
+        k, v = (LB.decode8(x[pages, 0].reshape(-1, D)[:L], kind) * np.repeat(s[pages, 0].astype(np.float64), page)[:L, None] for x, s in ((c.k, c.ks), (c.v, c.vs)))
+        for i in range(n):
+            seen = L - n + i + 1
+            z = q[b * n + i] @ k[:seen].T / 4
+            p = np.exp(z - z.max(1, keepdims=True))
+            p /= p.sum(1, keepdims=True)
+            want, size = p @ v[:seen], p @ np.abs(v[:seen])
+            top = np.abs(z).max() * np.log2(np.e)
+            assert top < 64
+            off = 2 * (np.log(2) * 2.0 ** -24 * (5 * top + 3 * 16) + 2.0 ** -22) + 2.0 ** -22 + seen * 2.0 ** -24
+            assert (np.abs(o[b * n + i] - want) <= size * off + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()

@@ -128,11 +128,14 @@ __device__ __forceinline__ int32_t kv_page_of(const KvAttnArgs& a, int b, uint32
 // above every value scale that the row has seen so far in magnitude: 2^KV_PE at most, so that small weights stay normal. A page
 // that a row's mask hides does not count for it, so what the row cannot see does not change it. Only
 // exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
-// the codes are exact in. Where a key head's rows of a sequence are one tile of 16, as in calls of single tokens, a weight is the sum of two
-// binary16 terms (22 bits): the cache's bytes bound these calls, and the second term costs them 0 to 2 % (48 sequences of up to 8000 95.2 -> 96.4 us).
-// Elsewhere instructions do, and a second term would cost 5 to 6 % by rows (32 tokens on 30000 71.6 -> 76.3) and 23 % by tiles (two chunks of
-// 2000 on 4000 272 -> 335): a weight keeps eleven bits, which raises the error of float16 outputs against 64 bits from 2.1e-4 with
-// float32 weights to 2.6e-4 (3.1e-4 in windows of few tokens), of bfloat16 ones not at all. The denominator sums the weights before they are rounded.
+// exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
+// the codes are exact in. Where a sequence's rows of a key head are at most 16, as in calls of single tokens, a weight is the sum of two
+// binary16 terms (22 bits), of shared tokens too, whose rows of all sequences make larger tiles: one call's precision does not depend on the way it goes.
+// Bytes bound the calls by rows of one tile, and the second term costs them 0 to 2 % (48 sequences of up to 8000 95.2 -> 96.4 us); shared tokens by tiles pay
+// more (64 sequences on 8192 of them 49 -> 51 us, 128 on 32768 138 -> 159) and gain in error of float16 outputs against 64 bits 2.4e-4 -> 2.1e-4, that of
+// float32 weights. Elsewhere instructions bound the call, and a second term would cost 5 to 6 % by rows (32 tokens on 30000 71.6 -> 76.3) and 23 % by tiles
+// (two chunks of 2000 on 4000 272 -> 335): a weight keeps eleven bits, which raises the error of float16 outputs from 2.1e-4 with float32 weights to
+// 2.6e-4 (3.1e-4 in windows of few tokens), of bfloat16 ones not at all. The denominator sums the weights before they are rounded.
 constexpr int KV_PE = 11;
 constexpr int KV_NONE = -1000;  // e before any scale
 
@@ -662,7 +665,7 @@ __device__ __forceinline__ int kv_vslot(int d, int piece) {
   return KvTile<D>::TT == 64 ? piece ^ ((d ^ (d >> 3)) & 7) : piece ^ (((d >> 1) ^ (d >> 3)) & 3);
 }
 
-template <int D, bool FP8, KvMode MODE>
+template <int D, bool FP8, bool TWO, KvMode MODE>
 __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles, uint32_t splits, uint32_t chunk, uint32_t block, unsigned char* smem) {
   typedef KvTile<D> Ti;
   constexpr int TT = Ti::TT, KN = Ti::KN, VN = Ti::VN, JT = D / 32, GR = TT / 16;
@@ -1009,7 +1012,7 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
           float sums = 0.f;
 #pragma unroll
           for (int gu = 0; gu < GR; ++gu) {
-            f16x8 pf;
+            f16x8 pf, pl;  // the weights; TWO: what binary16 leaves of them
             const float kfac = qs * of(sc, gu), lw = of(lwl, GR + gu) + rise;
             float sum = 0.f;
 #pragma unroll
@@ -1020,12 +1023,18 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
               const f16x2 h2 = __builtin_convertvector((f32x2{p0, p1}), f16x2);
               pf[e] = h2[0];
               pf[e + 1] = h2[1];
+              if constexpr (TWO) {
+                const f16x2 l2 = __builtin_convertvector((f32x2{p0 - static_cast<float>(h2[0]), p1 - static_cast<float>(h2[1])}), f16x2);
+                pl[e] = l2[0];
+                pl[e + 1] = l2[1];
+              }
             }
             sums += sum * of(rwl, GR + gu);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
               const int d = 32 * j + col;
               const f16x8 vf = *reinterpret_cast<const f16x8*>(vs + d * Ti::VP + kv_vslot<D>(d, gu * 2 + hf) * 16);
+              if constexpr (TWO) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[j], 0, 0, 0);
               o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
             }
           }
@@ -1138,8 +1147,8 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
 #pragma unroll
         for (int sl = 0; sl < 2; ++sl) {
           const int gu = 2 * u + sl;
-          f16x8 pf;
-          if (plain) {
+          f16x8 pf, pl;
+          if (plain) {  // KV_PLAIN alone, and never TWO
             // the exponential with the value's factor in its exponent: one multiply-add and one exponential a weight
             const float kf = qs * of(sc, gu), lw = of(lwl, GR + gu) + rise;
             float sum = 0.f;
@@ -1160,7 +1169,9 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
               const float v = s[u][8 * sl + e], p = __builtin_amdgcn_exp2f(v - base);
               l += p;
               // a masked token's weight is 0 whatever its page's scale holds
-              pf[e] = static_cast<f16>(v == -__builtin_inff() ? 0.f : p * w);
+              const float x = v == -__builtin_inff() ? 0.f : p * w;
+              pf[e] = static_cast<f16>(x);
+              if constexpr (TWO) pl[e] = static_cast<f16>(x - static_cast<float>(pf[e]));
             }
           }
           auto vfrag = [&](int j) {
@@ -1175,13 +1186,18 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < JT; ++j) {
+              if constexpr (TWO) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j % VA], pl, o[j], 0, 0, 0);
               o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j % VA], pf, o[j], 0, 0, 0);
               if (j + VA < JT) vf[j % VA] = vfrag(j + VA);
               __builtin_amdgcn_sched_barrier(0);
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < JT; ++j) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vfrag(j), pf, o[j], 0, 0, 0);
+            for (int j = 0; j < JT; ++j) {
+              const f16x8 vf = vfrag(j);
+              if constexpr (TWO) o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl, o[j], 0, 0, 0);
+              o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf, o[j], 0, 0, 0);
+            }
           }
         }
       l += sums * down;
@@ -1296,10 +1312,11 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
   }
 }
 
-template <int D, bool FP8, KvMode MODE>
+template <int D, bool FP8, bool TWO, KvMode MODE>
 __global__ __launch_bounds__(KVM_T, D > 128 ? 1 : 2) void k_kv8_tile(KvAttnArgs a, uint32_t row_tiles, uint32_t splits, uint32_t chunk) {
+  static_assert(MODE == KV_PREFIX || !TWO);
   extern __shared__ __align__(16) unsigned char smem[];
-  kv8_tile<D, FP8, MODE>(a, row_tiles, splits, chunk, blockIdx.x, smem);
+  kv8_tile<D, FP8, TWO, MODE>(a, row_tiles, splits, chunk, blockIdx.x, smem);
 }
 
 template <int D>
@@ -1307,6 +1324,9 @@ constexpr int kv8_tile_lds() {
   constexpr int strips = KVM_WAVES * 32 * (D * 2 + 16);
   return 2 * KvTile<D>::STAGE > strips ? 2 * KvTile<D>::STAGE : strips;
 }
+
+// Whether a weight is the sum of two binary16 terms; see KV_PE.
+bool kv_two(const KvAttnArgs& a) { return static_cast<int64_t>(a.max_new) * (a.Hq / a.c.Hkv) <= 16; }
 
 // Tokens are split only as far as the card has room for more workgroups at once: a start, a join and the code's own fetch
 // cost more than even shares gain (one sequence of 65000: 129 us in shares of 256 tokens, 83 of 512, 57 of 1024, 39 of 2048,
@@ -1357,7 +1377,7 @@ KvPlan kind_plan(const KvAttnArgs& a, bool have_ws, bool tile) {
 
 KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
   const KvPlan rows = kind_plan(a, have_ws, false);
-  if (static_cast<int64_t>(a.max_new) * (a.Hq / a.c.Hkv) <= 16) return rows;
+  if (kv_two(a)) return rows;
   const KvPlan tile = kind_plan(a, have_ws, true);
   return tile.time < rows.time ? tile : rows;
 }
@@ -1376,18 +1396,25 @@ hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
         default: k_kv8_rows<D, FP8, 8, decltype(two)::value, MODE><<<grid, 512, 0, st>>>(a, rt, sp, ch);
       }
     };
-    if (p.row_tiles == 1) rows(std::true_type{});
+    if (kv_two(a)) rows(std::true_type{});
     else rows(std::false_type{});
     return hipGetLastError();
   }
-  constexpr int lds = kv8_tile_lds<D>();
-  static std::atomic<int> done[kMaxDevices];
-  if (lds > 65536) {
-    const hipError_t e = raise_lds_cap(reinterpret_cast<const void*>(k_kv8_tile<D, FP8, MODE>), lds, done);
-    if (e != hipSuccess) return e;
+  auto tile = [&](auto two) {
+    constexpr bool TWO = decltype(two)::value;
+    constexpr int lds = kv8_tile_lds<D>();
+    static std::atomic<int> done[kMaxDevices];
+    if (lds > 65536) {
+      const hipError_t e = raise_lds_cap(reinterpret_cast<const void*>(k_kv8_tile<D, FP8, TWO, MODE>), lds, done);
+      if (e != hipSuccess) return e;
+    }
+    k_kv8_tile<D, FP8, TWO, MODE><<<grid, KVM_T, lds, st>>>(a, rt, sp, ch);
+    return hipGetLastError();
+  };
+  if constexpr (MODE == KV_PREFIX) {
+    if (kv_two(a)) return tile(std::true_type{});
   }
-  k_kv8_tile<D, FP8, MODE><<<grid, KVM_T, lds, st>>>(a, rt, sp, ch);
-  return hipGetLastError();
+  return tile(std::false_type{});
 }
 
 template <KvMode MODE>

@@ -95,7 +95,8 @@ KvPlan part_plan(const KvAttnArgs& a, int64_t nrows, int64_t seqs, int64_t span,
   const int64_t units = p.row_tiles * a.c.Hkv * seqs, room = tile && a.c.D <= 128 ? 2 * cus : cus;
   const int live = nrows < KVM_ROWS ? static_cast<int>((nrows + 31) / 32) : 4;
   static constexpr double kTile[5] = {0, 36, 28, 24, 18};
-  const double rate = tile ? kTile[live] : 75.0, start = tile ? 10.0 : 7.0, wide = a.c.D > 128 ? 2.0 : 1.0;
+  const double two = kv_two(a) && nrows > 16 ? tile ? 0.87 : 0.95 : 1.0;  // a weight's second term beside products, not beside bytes
+  const double rate = (tile ? kTile[live] : 75.0) * two, start = tile ? 10.0 : 7.0, wide = a.c.D > 128 ? 2.0 : 1.0;
   const double part = 2.0 * static_cast<double>(nrows * seqs * a.c.Hkv) * (a.c.D + 2) * 4 / 4e6;  // us
   span = span > 0 ? span : 1;
   int64_t most = units < room ? room / units : 1;

@@ -13,9 +13,9 @@ hipError_t launch_kv8_prefix(const KvAttnArgs& a, const KvPlan& p, hipStream_t s
 namespace {
 
 // Tiles over the shared tokens and single rows over the sequences' own, which need nothing of each other: the first are bound by instructions, the
-// second by the cache's bytes. The short own workgroups come first, so that the long tiles fill the CUs behind them: 42 us for 64 sequences with
-// 8192 shared tokens and 600 of their own (32 heads on 8 of 128, e4m3), 146 for 128 with 32768 and 301 (int8). With the kinds in turns by eights the
-// last tiles begin late (46, 197). Heads of 256 leave no LDS for it.
+// second by the cache's bytes. The short own workgroups come first, so that the long tiles fill the CUs behind them: 44 us for 64 sequences with
+// 8192 shared tokens and 600 of their own (32 heads on 8 of 128, e4m3), 164 for 128 with 32768 and 301 (int8); weights of two terms (KV_PE), as rows of
+// one tile have. With the kinds in turns by eights the last tiles begin late (4 us more, and 50). Heads of 256 leave no LDS for it.
 template <int D, bool FP8>
 __global__ __launch_bounds__(KVM_T, 2) void k_kv8_shared(KvAttnArgs a, uint32_t prefix_tiles, uint32_t prefix_splits, uint32_t prefix_chunk,
                                                          uint32_t prefix_blocks, uint32_t own_tiles, uint32_t own_splits, uint32_t own_chunk) {
@@ -24,7 +24,7 @@ __global__ __launch_bounds__(KVM_T, 2) void k_kv8_shared(KvAttnArgs a, uint32_t 
   const uint32_t own_blocks = gridDim.x - prefix_blocks;
   const bool prefix = blockIdx.x >= own_blocks;
   const uint32_t block = prefix ? blockIdx.x - own_blocks : blockIdx.x;
-  if (prefix) kv8_tile<D, FP8, KV_PREFIX>(a, prefix_tiles, prefix_splits, prefix_chunk, block, smem);
+  if (prefix) kv8_tile<D, FP8, true, KV_PREFIX>(a, prefix_tiles, prefix_splits, prefix_chunk, block, smem);
   else {
     KvAttnArgs x = a;
     x.part0 = static_cast<int32_t>(prefix_splits);
