@@ -189,3 +189,17 @@ def test_frequencies(gpu):
         g, r = g.cpu(), (g / f).cpu()
         assert (r[turns > 40] == 1).all() and torch.allclose(r[turns < 0.8], torch.tensor(0.125, dtype=torch.float64), rtol=1e-14)
         assert (r.diff() <= 0).all() and m == (0.1 * np.log(8.0) + 1 if s == "yarn" else 1.0)
+
+
+def test_more_rows_than_a_grid_has_threads(gpu):
+    """A workgroup a row: 2^24 rows are 2^32 threads, of which a launch's count has 32 bits."""
+    T = (1 << 24) + 5
+    q = torch.arange(T, dtype=torch.int32, device="cuda").remainder_(251).half().view(T, 1, 1).expand(T, 1, 2).contiguous()
+    f = torch.tensor([0.37], dtype=torch.float64, device="cuda")
+    for kw in (dict(positions=torch.arange(T, dtype=torch.int32, device="cuda").remainder_(997)), dict(lengths=torch.tensor([T], dtype=torch.int32, device="cuda"))):
+        got = ops().rope(q, frequencies=f, **kw)
+        step = 1 << 21
+        for at in range(0, T, step):  # the same rows in calls of their own
+            end = min(T, at + step)
+            one = dict(positions=kw["positions"][at:end]) if "positions" in kw else dict(lengths=torch.tensor([end], dtype=torch.int32, device="cuda"))
+            assert torch.equal(got[at:end], ops().rope(q[at:end], frequencies=f, **one)), at

@@ -14,7 +14,7 @@ struct RopeArgs {
   const int32_t* lengths;    // [B]
   const int32_t* starts;     // [B + 1], or null: `each` rows a sequence
   double magnitude;
-  int64_t rows;
+  int64_t rows, row0;        // row0: the first of a launch
   int32_t B, each, Hq, Hk, D, R;
   int dtype;                 // LT
   bool wide_positions, interleaved, inverse;
@@ -36,6 +36,9 @@ struct SampleArgs {
   int32_t V;
   int dtype;                 // LT
 };
+
+// A launch's threads along x are counted in 32 bits; a grid of more runs in part, without an error. Calls of many rows are launched in pieces.
+constexpr int64_t kLaunchThreads = int64_t{1} << 31;
 
 hipError_t launch_rope(const RopeArgs& a, hipStream_t st);
 hipError_t launch_sample(const SampleArgs& a, hipStream_t st);

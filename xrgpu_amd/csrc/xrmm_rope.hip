@@ -47,7 +47,7 @@ __global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a) {
   extern __shared__ __align__(8) unsigned char smem[];
   f32x2* cs = reinterpret_cast<f32x2*>(smem);  // [R / 2]
   const int tid = threadIdx.x, half = a.R / 2, heads = a.Hq + a.Hk;
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.row0 + blockIdx.x;
   const bool moved = a.q != a.oq || (a.Hk > 0 && a.k != a.ok);  // else what passes is in place already
 
   // this thread's piece of a head, and the first of the heads that it visits
@@ -157,11 +157,17 @@ __global__ __launch_bounds__(ROPE_T) void k_rope(RopeArgs a) {
 
 template <typename T, int V>
 hipError_t rope_layout(const RopeArgs& a, hipStream_t st) {
-  const dim3 grid(static_cast<uint32_t>(a.rows));
   const size_t lds = static_cast<size_t>(a.R / 2) * sizeof(f32x2);
-  if (!a.interleaved) k_rope<T, V, false><<<grid, ROPE_T, lds, st>>>(a);
-  else if constexpr (V > 1) k_rope<T, V, true><<<grid, ROPE_T, lds, st>>>(a);
-  return hipGetLastError();
+  RopeArgs x = a;
+  for (; x.row0 < a.rows; x.row0 += kLaunchThreads / ROPE_T) {
+    const int64_t left = a.rows - x.row0;
+    const dim3 grid(static_cast<uint32_t>(left < kLaunchThreads / ROPE_T ? left : kLaunchThreads / ROPE_T));
+    if (!a.interleaved) k_rope<T, V, false><<<grid, ROPE_T, lds, st>>>(x);
+    else if constexpr (V > 1) k_rope<T, V, true><<<grid, ROPE_T, lds, st>>>(x);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <typename T>
@@ -169,7 +175,6 @@ hipError_t rope_type(const RopeArgs& a, hipStream_t st) {
   int v = 16 / static_cast<int>(sizeof(T));
   const int of = a.interleaved ? a.R : a.R / 2;
   while (of % v != 0) v /= 2;
-  if (a.rows > 0x7FFFFFFF) return hipErrorInvalidValue;
   switch (v) {
     case 8:
       if constexpr (sizeof(T) == 2) return rope_layout<T, 8>(a, st);
