@@ -220,3 +220,20 @@ def test_more_ties_than_the_list_holds(gpu, B, V):
         t, s = ops().sample(x, u, **kw)
         rows = [0, B // 2, B - 1]
         check(x[rows], u[rows], got=(t[rows], s[rows]), **kw)
+
+
+@pytest.mark.parametrize("V", [3, 8])
+def test_more_rows_than_a_grid_has_threads(gpu, V):
+    """A workgroup of 1024 a row: 2^22 rows are 2^32 threads, of which a launch's count has 32 bits."""
+    B = (1 << 22) + 5
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x, u = torch.randn(B, V, generator=g, device="cuda").half(), torch.rand(B, generator=g, device="cuda")
+    by_row = dict(temperature=torch.rand(B, generator=g, device="cuda"), top_k=torch.randint(0, 3, (B,), generator=g, device="cuda").int(),
+                  top_p=0.3 + torch.rand(B, generator=g, device="cuda"), min_p=torch.rand(B, generator=g, device="cuda") * 0.2)
+    for kw in (dict(temperature=0.8), by_row):
+        t, s = ops().sample(x, u, **kw)
+        step = 1 << 20
+        for at in range(0, B, step):  # the same rows in calls of their own
+            part = slice(at, min(B, at + step))
+            t1, s1 = ops().sample(x[part], u[part], **{n: v[part] if torch.is_tensor(v) else v for n, v in kw.items()})
+            assert torch.equal(t[part], t1) and torch.equal(s[part], s1), at

@@ -1059,7 +1059,7 @@ bool sample_split(int64_t rows, int64_t V, Kind kind, SamplePlan& p) {
 }
 
 template <typename T>
-hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
+hipError_t sample_type(SampleArgs a, int F, hipStream_t st) {
   SamplePlan p;
   if (a.ws != nullptr && sample_split(a.rows, a.V, kind_of(a), p) && a.ws_bytes >= SAMPLE_HEAD + a.rows * p.row_bytes()) {
     const dim3 grid(static_cast<uint32_t>(p.parts), static_cast<uint32_t>(a.rows));
@@ -1068,10 +1068,23 @@ hipError_t sample_type(const SampleArgs& a, int F, hipStream_t st) {
     if (kind_of(a) != NO_FILTER) k_sample_draw<T><<<grid, SP, 0, st>>>(a, p, F);
     return hipGetLastError();
   }
-  const dim3 grid(static_cast<uint32_t>(a.rows));
-  if (a.V >= static_cast<int>(16 / sizeof(T))) k_sample_row<T, 16 / sizeof(T)><<<grid, ST, 0, st>>>(a, F);
-  else k_sample_row<T, 1><<<grid, ST, 0, st>>>(a, F);
-  return hipGetLastError();
+  constexpr int64_t most = kLaunchThreads / ST;
+  while (true) {
+    const dim3 grid(static_cast<uint32_t>(a.rows < most ? a.rows : most));
+    if (a.V >= static_cast<int>(16 / sizeof(T))) k_sample_row<T, 16 / sizeof(T)><<<grid, ST, 0, st>>>(a, F);
+    else k_sample_row<T, 1><<<grid, ST, 0, st>>>(a, F);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.rows <= most) return e;
+    a.rows -= most;
+    a.x = static_cast<const T*>(a.x) + most * a.stride;
+    a.u += most;
+    a.tokens += most;
+    a.shares += most;
+    if (a.temperature) a.temperature += most;
+    if (a.top_p) a.top_p += most;
+    if (a.min_p) a.min_p += most;
+    if (a.top_k) a.top_k += most;
+  }
 }
 
 }  // namespace
