@@ -222,6 +222,67 @@ def test_more_ties_than_the_list_holds(gpu, B, V):
         check(x[rows], u[rows], got=(t[rows], s[rows]), **kw)
 
 
+@pytest.mark.parametrize("dt,B,V", [("f32", 8, 60000), ("bf16", 8, 60000), ("f16", 64, 128000)])
+def test_settings_by_row_in_parts(gpu, dt, B, V):
+    """Greedy, empty, masked and unfiltered rows beside ones of small and large top_k and of top_p, in one call that is split over the device: rows
+    leave its launches at different places."""
+    o = ops()
+    g = torch.Generator().manual_seed(B + V)
+    wide = torch.zeros(B, V + 3, dtype=DT[dt], device="cuda")
+    x = wide[:, 1:1 + V]
+    x.copy_(logits(B, V, dt, seed=9))
+    wide[:, 0], wide[:, 1 + V:] = 100.0, 100.0
+    x[3], x[5] = -float("inf"), float("nan")
+    x[6, torch.rand(V, generator=g).cuda() > 0.03] = -float("inf")
+    of = lambda values, dtype: torch.tensor([values[b % len(values)] for b in range(B)], dtype=dtype, device="cuda")
+    kw = dict(temperature=of([0.7, 1.3, 0.0, 1.0, 1.5, 1.0, 0.9, 1.1], torch.float32), top_k=of([0, 5, 0, 20000, 0, 3, 50, 20000, 0, 1], torch.int32),
+              top_p=of([1.0, 0.9, 0.95], torch.float32), min_p=of([0.0, 0.0, 0.02, 0.0, 0.0], torch.float32))
+    u = torch.rand(B, generator=g).cuda()
+    need = o.sample_workspace_bytes(B, V)
+    assert need > 4096
+    ws = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+    ws[:4096] = 0
+    t, s = o.sample(x, u, workspace=ws, **kw)
+    assert not ws[:4096].any()
+    assert t[3] == t[5] == -1 and s[3] == s[5] == -float("inf")
+    rows = list(range(0, B, max(1, B // 16)))
+    check(x[rows], u[rows], got=(t[rows], s[rows]), **{n: v[rows] for n, v in kw.items()})
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(o.sample(x, u, workspace=ws, **kw), (t, s)))
+    many = 320  # a workgroup a row
+    assert o.sample_workspace_bytes(many, V) == 0
+    again = torch.arange(many, device="cuda") % B
+    if V * many <= 320 * 60000:
+        other = o.sample(x[again], u[again], **{n: v[again] for n, v in kw.items()})
+        assert torch.equal(other[0], t[again]) and torch.equal(other[1], s[again])
+    one = {n: v[:1].clone() for n, v in kw.items()}  # a row by itself, all of its launches for kinds that it does not have
+    for b in range(0, B, 3):
+        for n, v in kw.items():
+            one[n].copy_(v[b:b + 1])
+        t1, s1 = o.sample(x[b:b + 1], u[b:b + 1], **one)
+        assert torch.equal(t1, t[b:b + 1]) and torch.equal(s1, s[b:b + 1])
+
+
+@pytest.mark.parametrize("V", [3000, 60000])
+@pytest.mark.parametrize("t", [1e-45, 1e-38, 1e-31, 1e-30])
+def test_small_temperatures_are_not_none(gpu, V, t):
+    """They draw among equal largest logits, which temperature 0 does not; as a number and as a tensor, subnormal ones too."""
+    n, u = 7, [0.0, 0.35, 0.5, 0.99]
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(V)).clamp(max=5.0).cuda()
+    at = torch.arange(n, device="cuda") * (V // n) + 11
+    x[:, at] = 9.0
+    u = torch.tensor(u, device="cuda")
+    want = at[(u.double() * n).floor().long()].int()
+    for setting in (t, torch.full((4,), t, dtype=torch.float32, device="cuda")):
+        for kw in ({}, dict(top_k=n), dict(top_p=0.9999), dict(top_k=100, top_p=0.9999)):
+            tokens, shares = ops().sample(x, u, temperature=setting, **kw)
+            assert torch.equal(tokens, want), (setting, kw)
+            # the 64-bit logarithm, rounded to float32
+            assert (shares.double() + np.log(n)).abs().max() <= 2.0 ** -24 * np.log(n)
+    tokens, shares = ops().sample(x, u, temperature=0.0)
+    assert (tokens == at[0]).all() and (shares == 0).all()
+
+
 @pytest.mark.parametrize("V", [3, 8])
 def test_more_rows_than_a_grid_has_threads(gpu, V):
     """A workgroup of 1024 a row: 2^22 rows are 2^32 threads, of which a launch's count has 32 bits."""
