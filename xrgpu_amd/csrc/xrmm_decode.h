@@ -37,7 +37,7 @@ struct SampleArgs {
   int dtype;                 // LT
 };
 
-// A launch's threads along x are counted in 32 bits; a grid of more runs in part, without an error. Calls of many rows are launched in pieces.
+// Threads of a launch of a call that takes several (see grid_counts).
 constexpr int64_t kLaunchThreads = int64_t{1} << 31;
 
 hipError_t launch_rope(const RopeArgs& a, hipStream_t st);

@@ -211,7 +211,7 @@ hipError_t launch_kv8_append(const KvAppendArgs& a, hipStream_t st) {
   // pages that a sequence's new tokens can lie in
   const int64_t touched = (a.max_new + a.c.page - 2) / a.c.page + 1;
   const int64_t grid = touched * a.c.B * a.c.Hkv * 2;
-  if (grid > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_counts(grid, KVA_T)) return hipErrorInvalidValue;
   const dim3 g(static_cast<uint32_t>(grid));
   const uint32_t t = static_cast<uint32_t>(touched);
   if (a.c.fp8) {

@@ -1385,7 +1385,7 @@ KvPlan attention_plan(const KvAttnArgs& a, bool have_ws) {
 template <int D, bool FP8, KvMode MODE>
 hipError_t attention_for(const KvAttnArgs& a, const KvPlan& p, hipStream_t st) {
   const int64_t n = p.row_tiles * p.splits * a.c.Hkv * (MODE == KV_PREFIX ? 1 : a.c.B);
-  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_counts(n, p.tile ? KVM_T : 64 * p.waves)) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
   const uint32_t rt = static_cast<uint32_t>(p.row_tiles), sp = static_cast<uint32_t>(p.splits), ch = static_cast<uint32_t>(p.chunk);
   if (!p.tile) {

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(KVJ_T) void k_kv8_join(KvAttnArgs a) {
 
 hipError_t launch_join(const KvAttnArgs& a, hipStream_t st) {
   const int64_t n = (a.c.rows * a.Hq * (a.c.D / 4) + KVJ_T / 4 - 1) / (KVJ_T / 4);
-  if (n > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_counts(n, KVJ_T)) return hipErrorInvalidValue;
   const dim3 grid(static_cast<uint32_t>(n));
   switch (a.c.D) {
     case 64: k_kv8_join<64><<<grid, KVJ_T, 0, st>>>(a); break;

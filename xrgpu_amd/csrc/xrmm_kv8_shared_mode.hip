@@ -35,7 +35,7 @@ __global__ __launch_bounds__(KVM_T, 2) void k_kv8_shared(KvAttnArgs a, uint32_t 
 template <int D, bool FP8>
 hipError_t shared_for(const KvAttnArgs& a, const KvPlan& p, const KvPlan& o, hipStream_t st) {
   const int64_t np = p.row_tiles * p.splits * a.c.Hkv, no = o.row_tiles * o.splits * a.c.Hkv * a.c.B;
-  if (np + no > 0x7FFFFFFF) return hipErrorInvalidValue;
+  if (!grid_counts(np + no, KVM_T)) return hipErrorInvalidValue;
   constexpr int lds = kv8_tile_lds<D>();
   static std::atomic<int> done[kMaxDevices];
   if (lds > 65536) {

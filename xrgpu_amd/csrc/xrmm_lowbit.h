@@ -80,6 +80,9 @@ struct KvAttnArgs {
   int64_t parts_at;            // where they begin
 };
 
+// A launch's threads along x are counted in 32 bits; a grid of more runs in part, without an error.
+inline bool grid_counts(int64_t workgroups, int64_t threads) { return workgroups <= 0xFFFFFFFFll / threads; }
+
 hipError_t launch_kv8_append(const KvAppendArgs& a, hipStream_t st);
 hipError_t launch_kv8_attention(const KvAttnArgs& a, hipStream_t st);
 int64_t kv8_workspace_bytes(const KvAttnArgs& a);
