@@ -132,3 +132,24 @@ def test_sample_workspaces():
     """None where a workgroup a row is estimated fastest whatever is asked for."""
     assert ops.sample_workspace_bytes(1, 128000) > 4096 and ops.sample_workspace_bytes(1, 2000) == 0 and ops.sample_workspace_bytes(500, 128000) == 0
     assert ops.sample_workspace_bytes(0, 128000) == 0 and ops.sample_workspace_bytes(4, 0) == 0
+
+
+BIG = (1 << 63) - 1
+
+
+def test_rope_strides_that_are_of_no_use_are_not_read():
+    """Of one row, and of no heads: what they hold decides nothing, whether memory overlaps above all."""
+    for rows, kw in ((1, {}), (0, {}), (1, dict(Hk=1, k=PTR + 1024, ok=PTR + 1024))):
+        for stride in (BIG, -BIG, 0, 1 << 62):
+            assert rope(rows=rows, oq=PTR + 2, qs=stride, ks=stride, oqs=stride, oks=stride, **kw) == (nat.XRMM_EINVAL if rows else nat.XRMM_OK)
+            assert rows == 0 or "overlap" in nat.last_error()
+    for stride in (BIG, -BIG, 1 << 62):
+        assert rope(rows=2, oq=PTR + 2, ks=stride, oks=stride) == nat.XRMM_EINVAL and "overlap" in nat.last_error()
+
+
+@pytest.mark.parametrize("name", ["qs", "ks", "oqs", "oks"])
+def test_rope_refuses_strides_whose_ranges_no_memory_has(name):
+    # 2^62 elements of 2 bytes are 2^63 bytes: they wrap to a range that overlaps nothing
+    for stride in (BIG, 1 << 62, 1 << 61):
+        assert rope(**{**dict(rows=3, Hk=1, k=PTR, ok=PTR), name: stride}) == nat.XRMM_EINVAL
+        assert "past any memory" in nat.last_error(), nat.last_error()

@@ -80,6 +80,10 @@ int xrmm_rope(const void* q, const void* k, void* q_out, void* k_out, int64_t q_
   const int64_t size = dtype == XRMM_F32 ? 4 : 2, qw = static_cast<int64_t>(q_heads) * head_dim, kw = static_cast<int64_t>(k_heads) * head_dim;
   if (rows > 1 && ((q_heads > 0 && (q_stride < qw || q_out_stride < qw)) || (k_heads > 0 && (k_stride < kw || k_out_stride < kw))))
     return fail("rope: token strides below heads * head_dim");
+  if (rows <= 1 || q_heads == 0) q_stride = q_out_stride = qw;  // of no use
+  if (rows <= 1 || k_heads == 0) k_stride = k_out_stride = kw;
+  for (const int64_t stride : {q_stride, k_stride, q_out_stride, k_out_stride})
+    if (rows > 1 && stride > INT64_MAX / 8 / rows) return fail("rope: token strides past any memory");  // ranges stay below 2^63 bytes
   if (rows > 0 && ((q_heads > 0 && (!q || !q_out)) || (k_heads > 0 && (!k || !k_out)) || !frequencies)) return fail("null tensor pointer");
   if (!aligned(q, size) || !aligned(k, size) || !aligned(q_out, size) || !aligned(k_out, size)) return fail("rope: tensors must be aligned to their elements");
   if (!aligned(frequencies, 8) || !aligned(positions, positions_dtype == XRMM_I64 ? 8 : 4) || !aligned(lengths, 4) || !aligned(starts, 4))
