@@ -153,3 +153,25 @@ def test_rope_refuses_strides_whose_ranges_no_memory_has(name):
     for stride in (BIG, 1 << 62, 1 << 61):
         assert rope(**{**dict(rows=3, Hk=1, k=PTR, ok=PTR), name: stride}) == nat.XRMM_EINVAL
         assert "past any memory" in nat.last_error(), nat.last_error()
+
+
+INF = float("inf")
+
+
+@pytest.mark.parametrize("kw,msg", [
+    (dict(theta=1.0, scaling="yarn", original_length=4096, factor=4.0), "theta above 1"), (dict(theta=0.5, scaling="yarn", original_length=4096, factor=4.0), "theta above 1"),
+    *[({**dict(scaling=s, original_length=4096, factor=4.0), **kw}, "finite") for s in ("yarn", "bands")
+      for kw in (dict(original_length=INF), dict(original_length=float("nan")), dict(high=INF), dict(low=float("nan")), dict(low=INF, high=INF))],
+    (dict(scaling="ntk", factor=1e300), "finite theta"), (dict(theta=1e308, scaling="ntk", factor=10.0), "finite theta"),
+])
+def test_rope_frequencies_refuse_numbers_that_give_none(kw, msg):
+    """A division by the logarithm of 1, floors of infinities and powers past float64 raised Python's own errors, or none."""
+    with pytest.raises(nat.XrmmInvalid, match=msg):
+        ops.rope_frequencies(8, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(theta=1.0), dict(theta=0.5, scaling="linear", factor=2.0), dict(theta=0.5, scaling="bands", original_length=100, factor=4.0),
+                                dict(theta=1.0, scaling="bands", original_length=100, factor=4.0), dict(theta=1.0 + 2.0 ** -40, scaling="yarn", original_length=4096, factor=4.0)])
+def test_rope_frequencies_take_the_others(kw):
+    f, m = ops.rope_frequencies(8, device="cpu", **kw)
+    assert f.shape == (4,) and f.isfinite().all() and m >= 1.0

@@ -1018,13 +1018,20 @@ def rope_frequencies(rotary_dim, theta=10000.0, *, scaling=None, factor=1.0, ori
     if scaling == "ntk":
         if R == 2:
             raise nat.XrmmInvalid("ntk scaling needs two pairs at least")
-        theta = theta * factor ** (R / (R - 2))
+        try:
+            theta = theta * factor ** (R / (R - 2))
+        except OverflowError:
+            theta = math.inf
+        if not math.isfinite(theta):
+            raise nat.XrmmInvalid("ntk scaling by this factor leaves no finite theta")
     f = float(theta) ** (-2.0 * i / R)
     if scaling == "linear":
         f = f / factor
     elif scaling in ("bands", "yarn"):
-        if original_length is None or not original_length > 0 or not 0 < low < high:
-            raise nat.XrmmInvalid(f"{scaling} scaling needs original_length and 0 < low < high")
+        if original_length is None or not 0 < original_length < math.inf or not 0 < low < high < math.inf:
+            raise nat.XrmmInvalid(f"{scaling} scaling needs original_length and 0 < low < high, all finite")
+        if scaling == "yarn" and not theta > 1:
+            raise nat.XrmmInvalid("yarn scaling needs theta above 1, so that turns fall with the index")
         if scaling == "bands":
             keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
         else:
