@@ -128,7 +128,6 @@ __device__ __forceinline__ int32_t kv_page_of(const KvAttnArgs& a, int b, uint32
 // above every value scale that the row has seen so far in magnitude: 2^KV_PE at most, so that small weights stay normal. A page
 // that a row's mask hides does not count for it, so what the row cannot see does not change it. Only
 // exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
-// exponents are compared and shifted, so scales may be negative, and as small or as large as a float32 is. Binary16 is what
 // the codes are exact in. Where a sequence's rows of a key head are at most 16, as in calls of single tokens, a weight is the sum of two
 // binary16 terms (22 bits), of shared tokens too, whose rows of all sequences make larger tiles: one call's precision does not depend on the way it goes.
 // Bytes bound the calls by rows of one tile, and the second term costs them 0 to 2 % (48 sequences of up to 8000 95.2 -> 96.4 us); shared tokens by tiles pay
@@ -143,6 +142,11 @@ constexpr int KV_NONE = -1000;  // e before any scale
 __device__ __forceinline__ int kv_scale_exp(float scale) {
   const uint32_t m = __builtin_bit_cast(uint32_t, scale) & 0x7FFFFFFFu;
   return m - 1u < 0x7F7FFFFFu ? __builtin_amdgcn_frexp_expf(scale) : KV_NONE;
+}
+
+// x y + z in one rounding. Where sums of two products are written without it, the compiler rounds either of the two, by the code around.
+__device__ __forceinline__ f32x4 kv_fma(f32x4 x, float y, f32x4 z) {
+  return f32x4{__builtin_fmaf(x[0], y, z[0]), __builtin_fmaf(x[1], y, z[1]), __builtin_fmaf(x[2], y, z[2]), __builtin_fmaf(x[3], y, z[3])};
 }
 
 __device__ __forceinline__ float kv_shift(float x, int e) { return __builtin_ldexpf(x, e); }
@@ -591,8 +595,8 @@ __device__ __forceinline__ void kv8_rows(const KvAttnArgs& a, uint32_t row_tiles
           if (s + i * groups >= parts) break;
           const float pm = ml[i][0], mn = fmaxf(vm, pm), bs = mn == -__builtin_inff() ? 0.f : mn;
           const float f0 = __builtin_amdgcn_exp2f(vm - bs), f1 = __builtin_amdgcn_exp2f(pm - bs);
-          v = v * f0 + __builtin_bit_cast(f32x4, x[i]) * f1;
-          vl = vl * f0 + ml[i][1] * f1;
+          v = kv_fma(v, f0, __builtin_bit_cast(f32x4, x[i]) * f1);
+          vl = __builtin_fmaf(vl, f0, ml[i][1] * f1);
           vm = mn;
         }
       }
@@ -1265,16 +1269,16 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
         const float pm = x[0], mn = fmaxf(m, pm), base = mn == -__builtin_inff() ? 0.f : mn;
         const float f0 = __builtin_amdgcn_exp2f(m - base), f1 = __builtin_amdgcn_exp2f(pm - base);
         m = mn;
-        l = l * f0 + x[1] * f1;
+        l = __builtin_fmaf(l, f0, x[1] * f1);
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const f32x4 x4 = v[j][y];  // elements by name: this compiler may fold v[e >> 2][e & 3] over an array of vectors to element 0
-            o[j][4 * y] = o[j][4 * y] * f0 + x4.x * f1;
-            o[j][4 * y + 1] = o[j][4 * y + 1] * f0 + x4.y * f1;
-            o[j][4 * y + 2] = o[j][4 * y + 2] * f0 + x4.z * f1;
-            o[j][4 * y + 3] = o[j][4 * y + 3] * f0 + x4.w * f1;
+            o[j][4 * y] = __builtin_fmaf(x4.x, f1, o[j][4 * y] * f0);
+            o[j][4 * y + 1] = __builtin_fmaf(x4.y, f1, o[j][4 * y + 1] * f0);
+            o[j][4 * y + 2] = __builtin_fmaf(x4.z, f1, o[j][4 * y + 2] * f0);
+            o[j][4 * y + 3] = __builtin_fmaf(x4.w, f1, o[j][4 * y + 3] * f0);
           }
       }
     }
