@@ -330,3 +330,16 @@ def test_weights_of_few_rows_have_two_terms_by_every_way(gpu, kind, D, G, n):
             assert top < 64
             off = 2 * (np.log(2) * 2.0 ** -24 * (5 * top + 3 * 16) + 2.0 ** -22) + 2.0 ** -22 + seen * 2.0 ** -24
             assert (np.abs(o[b * n + i] - want) <= size * off + np.abs(want) * 2.0 ** -11 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("n,G", [(1, 8), (4, 4), (1, 1)])
+def test_the_walk_is_kv8_attention_bit_for_bit(gpu, monkeypatch, D, n, G):
+    """The same kernel by another page lookup, split over workgroups and joined: the same roundings, whatever the compiler makes of either."""
+    monkeypatch.setenv("XRMM_KV8_SHARED", "kv8_walk")
+    c, d = shared_cache("int8", 40, [2700, 2600], 2, D, 64, seed=D, scales="any")
+    q = torch.randn(2 * n, 2 * G, D, generator=torch.Generator().manual_seed(D + n)).half().cuda()
+    kw = dict(batch=2, table_width=c.table.shape[1], page_size=64)
+    assert ops().kv8_attention_workspace_bytes(2 * n, 2 * G, 2, D, **kw) > 4096  # split
+    walked = ops().kv8_shared_attention(q, **d)
+    assert torch.equal(walked, ops().kv8_attention(q, **c.dev()))

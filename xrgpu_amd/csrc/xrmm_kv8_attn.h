@@ -1274,7 +1274,8 @@ __device__ __forceinline__ void kv8_tile(const KvAttnArgs& a, uint32_t row_tiles
         for (int j = 0; j < JT; ++j)
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            const f32x4 x4 = v[j][y];  // elements by name: this compiler may fold v[e >> 2][e & 3] over an array of vectors to element 0
+            const f32x4 x4 = v[j][y];  // elements by name: this compiler may fold v[e >> 2][e & 3] over an array of vectors to element 0,
+            // and takes element 0 for __builtin_bit_cast of a vector's element (cast the vector, or pass the element by value)
             o[j][4 * y] = __builtin_fmaf(x4.x, f1, o[j][4 * y] * f0);
             o[j][4 * y + 1] = __builtin_fmaf(x4.y, f1, o[j][4 * y + 1] * f0);
             o[j][4 * y + 2] = __builtin_fmaf(x4.z, f1, o[j][4 * y + 2] * f0);

@@ -13,13 +13,20 @@ namespace {
 // Order: by logit, of equal ones (0 and -0 are) the lower index first: the composite (ordered bits of x, ~index), unique in a row. top_k, top_p
 // and min_p each keep a prefix of that order. A row is read four times:
 //   its largest logit
-//   a histogram over the distance to it (64 bins a nat), which tells the few bins in which each threshold lies: of counts for top_k, of
+//   a histogram over the distance to it (64 bins a nat), which tells the bins in which each threshold lies: of counts for top_k, of
 //     weights by float32's exponential for top_p, whose error is bounded and widens the bins
-//   those bins' tokens into a list, and the exact weight of all before and behind them: a 64-bit exponential a token, which is what bounds
-//     rows with top_p
+//   those bins' tokens into a list, and the exact weight of all before and behind them
 //   the part in which the number falls.
 // For top_k up to a quarter of the threads, the threads' own largest logits are counted in place of all: no fewer than top_k tokens reach
 // the top_k-th of them, and hardly more, so the list holds all that may be kept.
+//
+// Vector instructions bound rows with top_p: 116 a token (256 rows of 50001), of which the 64-bit exponential is about 20; the others clean
+// the logits, take their bins again in each pass, and choose and add whole weights.
+//
+// The histogram's bound on its error is two units of 2^-30 a token, so top_p's bins grow with the vocabulary. From 50000 logits on, the more the flatter,
+// most rows with top_p of 0.95 or more list over SNEAR tokens (one row of 152000 24 -> 36 to 50 us), and from about 260000 some list over SLIST, with which
+// a workgroup reads the row itself about ten times, a logit a thread (one row of 260000 with top_p 0.99 at temperature 1 2550 us for 44 at 1.5, 49 rows 4040 for
+// 105): right, and slower than torch's elementary operations (310, 2960).
 constexpr int SB = 2048;      // bins
 constexpr float SB_NAT = 64.f;  // bins a nat
 constexpr int SLIST = 2048;   // tokens of the list; where more lie in the bins, the row itself is read in its place
@@ -198,7 +205,7 @@ struct RowOf {
       i += stride;
     }
   }
-  // f(logit, index), one by one in a short loop, for what few rows come to
+  // f(logit, index), one by one in a short loop: for rows that list more than SLIST tokens
   template <typename F>
   __device__ __forceinline__ void slowly(int to, int first, int step, F&& f) const {
 #pragma unroll 1
@@ -370,9 +377,6 @@ __device__ __forceinline__ uint64_t find_composite(BlockLds& s, ListLds& t, uint
   return prefix;
 }
 
-// The composite from which on a row's tokens are kept. `n` tokens are listed, in t.list if no more than SLIST; `held` is the exact weight of the
-// sure ones, `mid` of what top_k keeps behind top_p's bins for certain. All threads.
-//
 // Of a short list: each token's number and weight of those before it, by 16 lanes a token (158 tokens 14.8 -> 0.7 us beside a thread for each).
 // f(i, number, weight) in one lane for each token i; of j, `first` says whether it comes before i, t.kind[j] & 1 counts it and
 // t.digits[j] is what it adds.
@@ -398,6 +402,8 @@ __device__ __forceinline__ void each_before(const ListLds& t, uint32_t n, P&& fi
   }
 }
 
+// The composite from which on a row's tokens are kept. `n` tokens are listed, in t.list if no more than SLIST; `held` is the exact weight of the
+// sure ones, `mid` of what top_k keeps behind top_p's bins for certain. All threads. Here of a short list.
 template <int NT>
 __device__ __forceinline__ uint64_t threshold_near(BlockLds& s, ListLds& t, const Draw& d, const Cut& cut, const Weigher& weigh, uint32_t n, uint64_t held,
                                                    uint64_t mid) {
