@@ -1005,7 +1005,7 @@ def rope_frequencies(rotary_dim, theta=10000.0, *, scaling=None, factor=1.0, ori
     ``theta ** (-2 i / rotary_dim)``, for contexts ``factor`` times those trained on changed by ``scaling``: ``"linear"`` divides all by
     factor; ``"ntk"`` raises theta by ``factor ** (R / (R - 2))``, so that the slowest pair is divided by it and the fastest stays;
     ``"bands"`` divides pairs that turn fewer than ``low`` times in ``original_length``, keeps those of more than ``high`` turns and
-    goes from one to the other in proportion to the turns between; ``"yarn"`` does so in proportion to the pair's index, and its
+    goes from one to the other in proportion to the turns between; ``"yarn"`` does so in proportion to the pair's index (theta above 1), and its
     magnitude is ``0.1 ln(factor) + 1``. ``high``: 4 turns with bands, 32 with yarn, unless given. Other magnitudes are 1."""
     R = int(rotary_dim)
     if R <= 0 or R % 2:
